@@ -9,7 +9,17 @@ and the coordinate joins.  All computation runs in
 libejhip.so (HIP kernels behind a C ABI, include/einjax_hip.h).
 """
 
-from .autodiff import sparse_einsum, sparse_einsum_raw, sparse_einsum_raw_vjp
+from .autodiff import (
+    combine_experts,
+    combine_experts_vjp,
+    grouped_matmul,
+    grouped_matmul_vjp,
+    route_experts,
+    route_experts_vjp,
+    sparse_einsum,
+    sparse_einsum_raw,
+    sparse_einsum_raw_vjp,
+)
 from .execution.engine import ExecutionEngine, build_dependency_graph, topological_sort
 from .execution.sparse_dispatch import (
     coordinate_join,
@@ -19,12 +29,16 @@ from .execution.sparse_dispatch import (
     segment_sum,
 )
 from .kernels import (
+    ExpertRouting,
     KernelInfo,
     KernelRegistry,
     block_sparse_matmul,
     block_sparse_matmul_generic,
     coordinate_join_hash,
     coordinate_join_sorted,
+    group_by_expert,
+    int8_matmul,
+    quantize_rows,
 )
 from .tensor import (
     CaseAssignment,
@@ -68,4 +82,7 @@ __all__ = [
     "KernelInfo", "block_sparse_matmul", "block_sparse_matmul_generic", "coordinate_join_hash",
     "coordinate_join_sorted", "sparse_einsum", "sparse_einsum_raw", "sparse_einsum_raw_vjp",
     "ExecutionEngine", "build_dependency_graph", "topological_sort",
+    "ExpertRouting", "route_experts", "route_experts_vjp", "group_by_expert", "grouped_matmul",
+    "grouped_matmul_vjp", "combine_experts", "combine_experts_vjp", "quantize_rows",
+    "int8_matmul",
 ]

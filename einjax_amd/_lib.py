@@ -31,6 +31,10 @@ EJ_F64 = 2
 EJ_I32 = 3
 EJ_I64 = 4
 EJ_F16 = 5
+EJ_I8 = 6
+
+EJ_W_KN = 0
+EJ_W_NK = 1
 
 EJ_ORDER_PROBE = 0
 EJ_ORDER_SORTED = 1
@@ -60,6 +64,16 @@ class EinsumDesc(ctypes.Structure):
         ("b_sb", _i64), ("b_sk", _i64), ("b_sn", _i64),
         ("c_sb", _i64), ("c_sm", _i64), ("c_sn", _i64),
         ("out_dtype", _i32), ("reserved", _i32),
+    ]
+
+
+class GroupedDesc(ctypes.Structure):
+    """Mirror of ej_grouped_desc."""
+
+    _fields_ = [
+        ("dtype", _i32), ("out_dtype", _i32), ("w_order", _i32), ("n_groups", _i32),
+        ("k", _i32), ("n", _i32), ("n_slots", _i64), ("n_rows", _i64), ("x_stride", _i64),
+        ("w_group", _i64), ("w_stride", _i64), ("out_stride", _i64),
     ]
 
 
@@ -138,6 +152,18 @@ SIGNATURES = {
     "ej_pair_einsum_vjp": (_i32, [ctypes.c_char_p, _P_i64, _i32, _P_i64, _i32, _i32, _vp, _i64,
                                   _vp, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _sz,
                                   _vp]),
+    "ej_expert_route_workspace_size": (_i32, [_i64, _i32, _P_sz]),
+    "ej_expert_route": (_i32, [_vp, _i32, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp,
+                               _vp, _sz, _vp]),
+    "ej_expert_group": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ej_expert_route_vjp": (_i32, [_vp, _i32, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "ej_expert_combine": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _vp]),
+    "ej_expert_combine_vjp": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
+                                     _vp, _i64, _vp, _vp, _vp]),
+    "ej_quantize_rows": (_i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "ej_grouped_gemm": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                               _vp]),
+    "ej_grouped_gemm_dw": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,302 @@
+// The weighted sum of each token's expert results, its gradients, and rows in
+// 8-bit integers with a scale each.
+//
+// All three are bound by memory: every row is read once (the second pass of
+// the quantization over a row comes from the cache) and written once, sixteen
+// bytes a lane where the rows are aligned.
+#include "ej_internal.h"
+
+#include <type_traits>
+
+namespace ej {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPicks = 16;
+constexpr int kZeroBlocks = 256;  // workgroups that zero the rows no pair holds
+// HIP launches hold fewer than 2^32 threads.
+constexpr int64_t kMaxBlocks = ((int64_t{1} << 32) - 1) / kThreads;
+
+template <class T>
+__device__ inline float widen(T v) {
+  return static_cast<float>(v);
+}
+
+// N consecutive elements (16 bytes when VEC), widened.
+template <class T, bool VEC>
+struct Piece {
+  static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  float v[N];
+  __device__ inline void load(const T *p) {
+    if constexpr (VEC) {
+      struct alignas(16) { T e[N]; } w = *reinterpret_cast<const decltype(w) *>(p);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = widen(w.e[i]);
+    } else {
+      v[0] = widen(*p);
+    }
+  }
+  __device__ inline void store(T *p) const {
+    if constexpr (VEC) {
+      struct alignas(16) { T e[N]; } w;
+#pragma unroll
+      for (int i = 0; i < N; ++i) w.e[i] = static_cast<T>(v[i]);
+      *reinterpret_cast<decltype(w) *>(p) = w;
+    } else {
+      *p = static_cast<T>(v[0]);
+    }
+  }
+};
+
+struct CombineArgs {
+  const void *y;
+  int64_t ld_y, ld_out;
+  int64_t n_slots, n_tokens;
+  int32_t k, n;
+  const float *weights;    // null: every weight is 1
+  const int32_t *slots;
+  const int32_t *offsets;  // gradient: offsets[n_groups] = live slots
+  int32_t n_groups;
+  void *out;
+};
+
+// out[t] = sum_j weights[t, j] y[slots[t, j]]: summed in fp32 in the order of
+// the picks, rounded once.  One workgroup a token and stretch of columns.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsigned col_blocks) {
+  constexpr int N = Piece<T, VEC>::N;
+  const int64_t t = blockIdx.x / col_blocks;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x % col_blocks) * kThreads + threadIdx.x) * N;
+  if (col >= a.n) return;
+  float sum[N] = {};
+  for (int j = 0; j < a.k; ++j) {
+    const int64_t s = a.slots[t * a.k + j];
+    if (s < 0 || s >= a.n_slots) continue;
+    const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
+    Piece<T, VEC> y;
+    y.load(static_cast<const T *>(a.y) + s * a.ld_y + col);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] += w * y.v[i];
+  }
+  Piece<T, VEC> o;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o.v[i] = sum[i];
+  o.store(static_cast<T *>(a.out) + t * a.ld_out + col);
+}
+
+// grad_y[slots[t, j]] = weights[t, j] grad[t]; grad_w[t, j] = grad[t] . y[slots[t, j]].
+// One workgroup a token, so every dot product is summed in a fixed order;
+// workgroups past the tokens zero grad_y's rows that no pair holds.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, const void *grad,
+                                                               int64_t ld_grad, void *grad_y,
+                                                               float *grad_w) {
+  constexpr int N = Piece<T, VEC>::N, W = kThreads / 64;
+  if (blockIdx.x >= a.n_tokens) {
+    if (!grad_y) return;
+    int64_t live = a.offsets[a.n_groups];
+    live = live < 0 ? 0 : live;
+    for (int64_t s = live + (blockIdx.x - a.n_tokens); s < a.n_slots;
+         s += gridDim.x - a.n_tokens)
+      for (int64_t col = threadIdx.x; col < a.n; col += kThreads)
+        static_cast<T *>(grad_y)[s * a.n + col] = static_cast<T>(0.f);
+    return;
+  }
+  __shared__ float part[W][kMaxPicks];
+  const int64_t t = blockIdx.x;
+  const T *g = static_cast<const T *>(grad) + t * ld_grad;
+  for (int j = 0; j < a.k; ++j) {
+    const int64_t s = a.slots[t * a.k + j];
+    float dot = 0.f;
+    if (s >= 0 && s < a.n_slots) {
+      const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
+      const T *y = static_cast<const T *>(a.y) + s * a.ld_y;
+      T *d = static_cast<T *>(grad_y) + s * a.n;
+      for (int64_t col = threadIdx.x * N; col < a.n; col += kThreads * N) {
+        Piece<T, VEC> gv;
+        gv.load(g + col);
+        if (grad_w) {
+          Piece<T, VEC> yv;
+          yv.load(y + col);
+#pragma unroll
+          for (int i = 0; i < N; ++i) dot += gv.v[i] * yv.v[i];
+        }
+        if (grad_y) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) gv.v[i] *= w;
+          gv.store(d + col);
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][j] = dot;
+  }
+  __syncthreads();
+  if (grad_w && threadIdx.x < a.k) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += part[w][threadIdx.x];
+    grad_w[t * a.k + threadIdx.x] = sum;
+  }
+}
+
+// q = round(x / scale), scale = max |x| / 127 (as max |x| times the nearest
+// fp32 to 1/127); ties to even.  A row of zeros has scale 0 and zeros; a row
+// with a NaN or an infinity has scale NaN and zeros, so that whatever is
+// computed with it is NaN.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t ld, int32_t n,
+                                                            int8_t *q, float *scale) {
+  constexpr int N = Piece<T, VEC>::N, W = kThreads / 64;
+  __shared__ float part[W];
+  const int64_t r = blockIdx.x;
+  const T *row = x + r * ld;
+  float most = 0.f;
+  bool bad = false;
+  for (int64_t col = threadIdx.x * N; col < n; col += kThreads * N) {
+    Piece<T, VEC> v;
+    v.load(row + col);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float m = fabsf(v.v[i]);
+      bad |= !(m <= 3.402823466e38f);
+      most = fmaxf(most, m);
+    }
+  }
+  if (bad) most = INFINITY;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) most = fmaxf(most, part[w]);
+  float s = most * static_cast<float>(1.0 / 127.0);
+  const bool plain = s > 0.f && most < INFINITY;
+  if (threadIdx.x == 0) scale[r] = most < INFINITY ? s : __uint_as_float(0x7fc00000u);
+  for (int64_t col = threadIdx.x * N; col < n; col += kThreads * N) {
+    Piece<T, VEC> v;
+    v.load(row + col);
+    struct alignas(N) { int8_t e[N]; } o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float f = plain ? rintf(v.v[i] / s) : 0.f;
+      // a subnormal scale may round so far down that a quotient passes 127
+      o.e[i] = static_cast<int8_t>(fminf(fmaxf(f, -127.f), 127.f));
+    }
+    *reinterpret_cast<decltype(o) *>(q + r * n + col) = o;
+  }
+}
+
+template <class F>
+int by_type(int32_t dtype, F f) {
+  if (dtype == EJ_F32) return f(static_cast<float *>(nullptr));
+  if (dtype == EJ_BF16) return f(static_cast<__bf16 *>(nullptr));
+  if (dtype == EJ_F16) return f(static_cast<_Float16 *>(nullptr));
+  set_error("values of dtype %d: expected EJ_F32, EJ_BF16 or EJ_F16", dtype);
+  return EJ_E_INVAL;
+}
+
+bool aligned16(const void *p, int64_t ld, int size) {
+  return reinterpret_cast<size_t>(p) % 16 == 0 && ld * size % 16 == 0;
+}
+
+int check_combine(int64_t n_slots, int64_t n_tokens, int32_t k, int32_t n) {
+  EJ_CHECK_ARG(n_slots >= 0 && n_tokens >= 0 && n >= 0, "negative size");
+  EJ_CHECK_ARG(k >= 1, "k = %d, expected at least 1", k);
+  if (k > kMaxPicks || n_tokens > kMaxBlocks - kZeroBlocks || n_slots >= (int64_t{1} << 31)) {
+    set_error("%lld tokens of %d picks: at most %lld of %d are supported", (long long)n_tokens, k,
+              (long long)(kMaxBlocks - kZeroBlocks), kMaxPicks);
+    return EJ_E_UNSUPPORTED;
+  }
+  return EJ_OK;
+}
+
+}  // namespace
+}  // namespace ej
+
+using namespace ej;
+
+extern "C" int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
+                                 const float *weights, const int32_t *slots, int64_t n_tokens,
+                                 int32_t k, int32_t n, void *out, ej_stream_t stream) {
+  EJ_TRY(check_combine(n_slots, n_tokens, k, n));
+  return by_type(dtype, [&](auto *tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    if (n_tokens == 0 || n == 0) return EJ_OK;
+    EJ_CHECK_ARG(slots && out && (y || n_slots == 0), "null argument");
+    EJ_CHECK_ARG(ld_y >= n, "row stride %lld below n = %d", (long long)ld_y, n);
+    CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, nullptr, 0, out};
+    const bool vec = aligned16(y, ld_y, sizeof(T)) && aligned16(out, n, sizeof(T));
+    const int64_t cols =
+        ceil_div(n, static_cast<int64_t>(kThreads) * (vec ? 16 / sizeof(T) : 1));
+    if (n_tokens * cols > kMaxBlocks) {
+      set_error("%lld rows of %d: too many for one launch", (long long)n_tokens, n);
+      return EJ_E_UNSUPPORTED;
+    }
+    const dim3 grid(static_cast<unsigned>(n_tokens * cols));
+    if (vec)
+      hipLaunchKernelGGL((combine_kernel<T, true>), grid, dim3(kThreads), 0, as_stream(stream), a,
+                         static_cast<unsigned>(cols));
+    else
+      hipLaunchKernelGGL((combine_kernel<T, false>), grid, dim3(kThreads), 0, as_stream(stream),
+                         a, static_cast<unsigned>(cols));
+    EJ_LAUNCH_CHECK();
+    return EJ_OK;
+  });
+}
+
+extern "C" int ej_expert_combine_vjp(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
+                                     const float *weights, const int32_t *slots,
+                                     const int32_t *offsets, int32_t n_groups, int64_t n_tokens,
+                                     int32_t k, int32_t n, const void *grad, int64_t ld_grad,
+                                     void *grad_y, float *grad_weights, ej_stream_t stream) {
+  EJ_TRY(check_combine(n_slots, n_tokens, k, n));
+  EJ_CHECK_ARG(n_groups >= 0, "negative n_groups");
+  return by_type(dtype, [&](auto *tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    if (!grad_y && !grad_weights) return EJ_OK;
+    if (n_slots == 0 && n_tokens == 0) return EJ_OK;
+    EJ_CHECK_ARG(offsets && (n_tokens == 0 || (slots && (grad || n == 0))), "null argument");
+    EJ_CHECK_ARG(ld_y >= n && ld_grad >= n, "row stride below n = %d", n);
+    CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, offsets, n_groups, nullptr};
+    const bool vec = aligned16(y, ld_y, sizeof(T)) && aligned16(grad, ld_grad, sizeof(T)) &&
+                     aligned16(grad_y, n, sizeof(T));
+    const dim3 grid(static_cast<unsigned>(n_tokens + kZeroBlocks));
+    if (vec)
+      hipLaunchKernelGGL((combine_vjp_kernel<T, true>), grid, dim3(kThreads), 0,
+                         as_stream(stream), a, grad, ld_grad, grad_y, grad_weights);
+    else
+      hipLaunchKernelGGL((combine_vjp_kernel<T, false>), grid, dim3(kThreads), 0,
+                         as_stream(stream), a, grad, ld_grad, grad_y, grad_weights);
+    EJ_LAUNCH_CHECK();
+    return EJ_OK;
+  });
+}
+
+extern "C" int ej_quantize_rows(const void *x, int32_t dtype, int64_t n_rows, int64_t ld,
+                                int32_t n, int8_t *q, float *scale, ej_stream_t stream) {
+  EJ_CHECK_ARG(n_rows >= 0 && n >= 0, "negative size");
+  return by_type(dtype, [&](auto *tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    if (n_rows == 0) return EJ_OK;
+    EJ_CHECK_ARG(scale && (n == 0 || (x && q)), "null argument");
+    EJ_CHECK_ARG(ld >= n, "row stride %lld below n = %d", (long long)ld, n);
+    if (n_rows > kMaxBlocks) {
+      set_error("%lld rows: too many for one launch", (long long)n_rows);
+      return EJ_E_UNSUPPORTED;
+    }
+    constexpr int N = 16 / sizeof(T);
+    const bool vec = aligned16(x, ld, sizeof(T)) && n % N == 0 &&
+                     reinterpret_cast<size_t>(q) % N == 0;
+    const dim3 grid(static_cast<unsigned>(n_rows));
+    if (vec)
+      hipLaunchKernelGGL((quantize_kernel<T, true>), grid, dim3(kThreads), 0, as_stream(stream),
+                         static_cast<const T *>(x), ld, n, q, scale);
+    else
+      hipLaunchKernelGGL((quantize_kernel<T, false>), grid, dim3(kThreads), 0, as_stream(stream),
+                         static_cast<const T *>(x), ld, n, q, scale);
+    EJ_LAUNCH_CHECK();
+    return EJ_OK;
+  });
+}

@@ -1,0 +1,144 @@
+// Products grouped by expert: argument checks and the choice of kernel.
+#include "ej_grouped.h"
+
+#include "ej_grouped_launch.h"
+
+namespace ej {
+namespace {
+
+bool aligned16(const void *p, int64_t a, int64_t b, int size) {
+  return reinterpret_cast<size_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
+}
+
+int elem_size(int32_t dtype) { return dtype == EJ_F32 ? 4 : dtype == EJ_I8 ? 1 : 2; }
+
+int check_desc(const ej_grouped_desc *d) {
+  EJ_CHECK_ARG(d, "null descriptor");
+  EJ_CHECK_ARG(d->dtype == EJ_F32 || d->dtype == EJ_BF16 || d->dtype == EJ_F16 ||
+                   d->dtype == EJ_I8,
+               "operands of dtype %d: expected EJ_F32, EJ_BF16, EJ_F16 or EJ_I8", d->dtype);
+  EJ_CHECK_ARG(d->w_order == EJ_W_KN || d->w_order == EJ_W_NK, "w_order = %d", d->w_order);
+  EJ_CHECK_ARG(d->n_groups >= 0 && d->k >= 0 && d->n >= 0 && d->n_slots >= 0 && d->n_rows >= 0,
+               "negative size");
+  const int64_t w_row = d->w_order == EJ_W_KN ? d->n : d->k;
+  const int64_t w_rows = d->w_order == EJ_W_KN ? d->k : d->n;
+  EJ_CHECK_ARG(d->x_stride >= d->k && d->out_stride >= d->n && d->w_stride >= w_row,
+               "a row stride is below its row's length");
+  EJ_CHECK_ARG(d->n_groups <= 1 || d->w_group >= w_rows * d->w_stride || w_rows * w_row == 0,
+               "groups of w overlap: stride %lld for %lld rows of %lld", (long long)d->w_group,
+               (long long)w_rows, (long long)d->w_stride);
+  if (d->n_slots >= (int64_t{1} << 31) || d->n_rows >= (int64_t{1} << 31)) {
+    set_error("%lld slots of %lld rows: fewer than 2^31 are supported", (long long)d->n_slots,
+              (long long)d->n_rows);
+    return EJ_E_UNSUPPORTED;
+  }
+  return EJ_OK;
+}
+
+}  // namespace
+}  // namespace ej
+
+using namespace ej;
+
+extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const int32_t *rows,
+                               const int32_t *offsets, const void *w, const float *x_scale,
+                               const float *w_scale, void *out, ej_stream_t stream) {
+  EJ_TRY(check_desc(d));
+  const bool i8 = d->dtype == EJ_I8;
+  EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype ||
+                   (i8 && (d->out_dtype == EJ_BF16 || d->out_dtype == EJ_F16)),
+               "result of dtype %d from operands of dtype %d", d->out_dtype, d->dtype);
+  EJ_CHECK_ARG(d->out_dtype != EJ_I8, "8-bit results are not products");
+  if (i8) {
+    EJ_CHECK_ARG(d->w_order == EJ_W_NK, "8-bit weights are k-contiguous (EJ_W_NK)");
+    // |sum| <= 128 * 128 * k
+    EJ_CHECK_ARG(d->k < (1 << 17), "k = %d: the 32-bit sum of 8-bit products holds k < 131072",
+                 d->k);
+  }
+  if (d->n_slots == 0 || d->n == 0) return EJ_OK;
+  EJ_CHECK_ARG(out, "null result");
+  EJ_CHECK_ARG(offsets || d->n_groups == 1, "null offsets of %d groups", d->n_groups);
+  EJ_CHECK_ARG(rows || d->n_rows >= d->n_slots, "%lld rows for %lld slots without a row index",
+               (long long)d->n_rows, (long long)d->n_slots);
+  EJ_CHECK_ARG(d->n_groups == 0 || d->n_rows > 0, "%lld slots of no rows",
+               (long long)d->n_slots);
+  EJ_CHECK_ARG(d->k == 0 || d->n_groups == 0 || (x && w), "null operand");
+  EJ_CHECK_ARG(!i8 || d->n_groups == 0 || (x_scale && w_scale), "null scale");
+
+  const int size = elem_size(d->dtype);
+  GroupedArgs g = {};
+  g.a = static_cast<const char *>(x);
+  g.b = static_cast<const char *>(w);
+  g.c = out;
+  g.a_rows = rows;
+  g.offsets = offsets;
+  g.a_scale = x_scale;
+  g.b_scale = w_scale;
+  g.lda = d->x_stride;
+  g.ldb = d->w_stride;
+  g.ldc = d->out_stride;
+  g.b_group = d->w_group;
+  g.n_a = d->n_rows;
+  g.slots = d->n_slots;
+  g.n_groups = d->n_groups;
+  g.n = d->n;
+  g.k = d->k;
+  g.out = d->out_dtype;
+  // 16-byte loads need whole, aligned chunks in every row
+  const int chunk = 16 / size;
+  const bool direct = d->k % chunk == 0 && aligned16(x, d->x_stride, 0, size) &&
+                      aligned16(w, d->w_stride, d->w_group, size) &&
+                      (d->w_order == EJ_W_NK || d->n % chunk == 0);
+  const GroupedRows r{g, d->w_order == EJ_W_NK, direct};
+  switch (d->dtype) {
+    case EJ_BF16: return grouped_rows_bf16(r, as_stream(stream));
+    case EJ_F16: return grouped_rows_f16(r, as_stream(stream));
+    case EJ_I8: return grouped_rows_i8(r, as_stream(stream));
+    default: return grouped_rows_f32(r, as_stream(stream));
+  }
+}
+
+extern "C" int ej_grouped_gemm_dw(const ej_grouped_desc *d, const void *x, const int32_t *rows,
+                                  const int32_t *offsets, const void *grad, void *grad_w,
+                                  ej_stream_t stream) {
+  EJ_TRY(check_desc(d));
+  EJ_CHECK_ARG(d->dtype != EJ_I8, "8-bit products have no gradient");
+  EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype,
+               "gradient of dtype %d from operands of dtype %d", d->out_dtype, d->dtype);
+  if (d->n_groups == 0 || d->k == 0 || d->n == 0) return EJ_OK;
+  EJ_CHECK_ARG(grad_w, "null result");
+  EJ_CHECK_ARG(offsets || d->n_groups == 1, "null offsets of %d groups", d->n_groups);
+  EJ_CHECK_ARG(rows || d->n_rows >= d->n_slots, "%lld rows for %lld slots without a row index",
+               (long long)d->n_rows, (long long)d->n_slots);
+  EJ_CHECK_ARG(d->n_slots == 0 || (d->n_rows > 0 && x && grad), "null operand");
+  const int size = elem_size(d->dtype), chunk = 16 / size;
+  GroupedArgs g = {};
+  g.offsets = offsets;
+  g.c = grad_w;
+  g.c_group = d->w_group;
+  g.ldc = d->w_stride;
+  g.slots = d->n_slots;
+  g.n_groups = d->n_groups;
+  g.out = d->out_dtype;
+  // the rows of D are k for [k][n] weights and n for [n][k]
+  const bool kn = d->w_order == EJ_W_KN;
+  const char *xp = static_cast<const char *>(x), *gp = static_cast<const char *>(grad);
+  g.a = kn ? xp : gp;
+  g.a_rows = kn ? rows : nullptr;
+  g.lda = kn ? d->x_stride : d->out_stride;
+  g.n_a = kn ? d->n_rows : d->n_slots;
+  g.m = kn ? d->k : d->n;
+  g.b = kn ? gp : xp;
+  g.b_rows = kn ? nullptr : rows;
+  g.ldb = kn ? d->out_stride : d->x_stride;
+  g.n_b = kn ? d->n_slots : d->n_rows;
+  g.n = kn ? d->n : d->k;
+  const bool direct = d->k % chunk == 0 && d->n % chunk == 0 &&
+                      aligned16(x, d->x_stride, 0, size) &&
+                      aligned16(grad, d->out_stride, 0, size);
+  switch (d->dtype) {
+    case EJ_BF16: return grouped_wgrad_bf16(g, direct, as_stream(stream));
+    case EJ_F16: return grouped_wgrad_f16(g, direct, as_stream(stream));
+    default: return grouped_wgrad_f32(g, direct, as_stream(stream));
+  }
+}

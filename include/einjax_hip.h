@@ -90,7 +90,8 @@ extern "C" {
 #define EJ_F64 2 /* tiling, COO ingest, to_dense and ej_segment_sum */
 #define EJ_I32 3 /* integer tile einsums (ej_pair_einsum, ej_segment_einsum) and ej_segment_sum */
 #define EJ_I64 4 /* ej_segment_sum */
-#define EJ_F16 5 /* ej_segment_sum */
+#define EJ_F16 5 /* ej_segment_sum and the expert operators */
+#define EJ_I8 6  /* ej_grouped_gemm with scales */
 
 /* Pair orders of the join.  With n_keys == 0 both give the cross product in
  * lhs-major order (sparse_dispatch.py:53-59, pallas_gather.py:50-54). */
@@ -643,6 +644,104 @@ int ej_pair_einsum_vjp(const char *kernel_string, const int64_t *lhs_tile, int32
 int ej_relation_to_dense(const int32_t *coords, const void *values, int64_t n_tiles,
                          int32_t dtype, int32_t ndim, const int64_t *shape,
                          const int64_t *tile_shape, void *dense, ej_stream_t stream);
+
+/* ---- expert operators -------------------------------------------------------
+ * A mixture of experts is a relation between tokens and experts that is made
+ * anew on every call: routing makes it, products grouped by expert contract
+ * over it, and a weighted sum takes their rows back to the tokens.  The
+ * reference has no such operators; these follow this library's conventions.
+ *
+ * n_tokens tokens pick k experts each; a (token, expert) pair is a slot.  The
+ * slots are grouped by expert, those of one expert in token order:
+ *   offsets int32 [n_experts + 1]   slots [offsets[e], offsets[e + 1]) are e's
+ *   slots   int32 [n_tokens, k]     slot of each pair, -1 where it has none
+ *   rows    int32 [n_tokens * k]    token of each slot, 0 past the last one
+ * Sizes of groups stay on the device.  Values are EJ_F32, EJ_BF16 or EJ_F16;
+ * sums are formed in fp32 and rounded once.  All calls are asynchronous. */
+
+/* Routing.  Of each token's logits (row stride ld elements) the k largest are
+ * its picks, equal ones in the order of their experts; NaN counts as larger
+ * than anything, and a logit of -inf excludes its expert.  weights float32
+ * [n_tokens, k]: the softmax over all logits at the picks, or with
+ * renormalize != 0 the softmax over the picks.  A token with fewer than k
+ * experts left has experts -1, weights 0 and slots -1 for the rest.
+ * At most 1024 experts and 16 picks.  The workspace may be NULL where its size
+ * is 0.  ej_expert_group groups picks that the caller made (int32
+ * [n_tokens, k]; a value outside [0, n_experts) has no slot). */
+int ej_expert_route_workspace_size(int64_t n_tokens, int32_t n_experts, size_t *bytes);
+int ej_expert_route(const void *logits, int32_t dtype, int64_t n_tokens, int32_t n_experts,
+                    int64_t ld, int32_t k, int32_t renormalize, float *weights, int32_t *experts,
+                    int32_t *offsets, int32_t *rows, int32_t *slots, void *workspace,
+                    size_t workspace_bytes, ej_stream_t stream);
+int ej_expert_group(const int32_t *experts, int64_t n_tokens, int32_t k, int32_t n_experts,
+                    int32_t *offsets, int32_t *rows, int32_t *slots, void *workspace,
+                    size_t workspace_bytes, ej_stream_t stream);
+
+/* Gradient of the routing's weights to the logits: grad_logits [n_tokens,
+ * n_experts] (contiguous, of the logits' dtype), fully written; the picks are
+ * constants. */
+int ej_expert_route_vjp(const void *logits, int32_t dtype, int64_t n_tokens, int32_t n_experts,
+                        int64_t ld, int32_t k, int32_t renormalize, const int32_t *experts,
+                        const float *grad_weights, void *grad_logits, ej_stream_t stream);
+
+/* out[t] = sum over j of weights[t, j] y[slots[t, j]] (weights NULL: 1), pairs
+ * without a slot left out; out [n_tokens, n] contiguous. */
+int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
+                      const float *weights, const int32_t *slots, int64_t n_tokens, int32_t k,
+                      int32_t n, void *out, ej_stream_t stream);
+
+/* Its gradients: grad_y [n_slots, n] contiguous, zero in the rows from
+ * offsets[n_groups] on, and grad_weights [n_tokens, k]; either may be NULL.
+ * Every slot below offsets[n_groups] must be held by exactly one pair, as
+ * ej_expert_route makes them. */
+int ej_expert_combine_vjp(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
+                          const float *weights, const int32_t *slots, const int32_t *offsets,
+                          int32_t n_groups, int64_t n_tokens, int32_t k, int32_t n,
+                          const void *grad, int64_t ld_grad, void *grad_y, float *grad_weights,
+                          ej_stream_t stream);
+
+/* Rows in 8-bit integers: scale[r] = max |x[r]| times fp32(1/127), q = x / scale
+ * rounded to nearest even; a row of zeros has scale 0, one with a NaN or an
+ * infinity scale NaN (and q = 0). q [n_rows, n] contiguous. */
+int ej_quantize_rows(const void *x, int32_t dtype, int64_t n_rows, int64_t ld, int32_t n,
+                     int8_t *q, float *scale, ej_stream_t stream);
+
+/* Products grouped by expert.  w_order EJ_W_KN: W [n_groups][k][n], n
+ * contiguous; EJ_W_NK: [n_groups][n][k], k contiguous; strides in elements. */
+#define EJ_W_KN 0
+#define EJ_W_NK 1
+typedef struct ej_grouped_desc {
+  int32_t dtype;      /* of x and w: EJ_F32, EJ_BF16, EJ_F16, or EJ_I8 (EJ_W_NK, k < 2^17) */
+  int32_t out_dtype;  /* of the result: EJ_F32, or the 16-bit dtype (EJ_I8: any) */
+  int32_t w_order;
+  int32_t n_groups;
+  int32_t k, n;
+  int64_t n_slots;    /* rows of the result; below 2^31 */
+  int64_t n_rows;     /* rows of x */
+  int64_t x_stride;   /* between rows of x */
+  int64_t w_group;    /* between groups of w */
+  int64_t w_stride;   /* between rows of w */
+  int64_t out_stride; /* between rows of the result (of grad for the gradient) */
+} ej_grouped_desc;
+
+/* out[s] = x[rows[s]] W_e for the slots s of group e; rows NULL: x[s] (then
+ * n_rows >= n_slots).  Rows of out that no group covers are zero.  offsets is
+ * read as non-decreasing values in [0, n_slots]; others give undefined rows,
+ * never an access outside the operands; NULL with n_groups == 1: one group of
+ * every slot.  EJ_I8: x_scale [n_rows] and w_scale
+ * [n_groups][n], out = x_scale w_scale (exact integer sum); NULL otherwise. */
+int ej_grouped_gemm(const ej_grouped_desc *desc, const void *x, const int32_t *rows,
+                    const int32_t *offsets, const void *w, const float *x_scale,
+                    const float *w_scale, void *out, ej_stream_t stream);
+
+/* Gradient to the weights: grad_w_e = sum over the slots s of group e of
+ * x[rows[s]]^T grad[s], in the order and strides that the descriptor gives
+ * w (a group without slots gets zeros).  The gradient to x is ej_grouped_gemm
+ * of grad and W with k and n, and EJ_W_KN and EJ_W_NK, exchanged, followed by
+ * ej_expert_combine without weights where rows were gathered. */
+int ej_grouped_gemm_dw(const ej_grouped_desc *desc, const void *x, const int32_t *rows,
+                       const int32_t *offsets, const void *grad, void *grad_w,
+                       ej_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,616 @@
+"""Expert operators against their definitions in 64 bits.
+
+Bounds are those of the arithmetic: a sum of n products formed in fp32 is off
+by at most about n 2^-24 times the sum of the products' magnitudes (twice that
+is allowed, for sums formed in another order and of products rounded before
+they are added), and one rounding to the result's type by its unit roundoff.
+"""
+
+import pytest
+import torch
+
+import einjax_amd as ej
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+UNIT = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+TINY = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}
+
+
+def rng(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def assert_within(got, want, bound):
+    assert got.shape == want.shape
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} off, worst "
+                           f"{float((err / bound.clamp(min=1e-300)).max()):.3g} times the bound")
+
+
+def sum_bound(want, magnitudes, n, dtype):
+    return UNIT[dtype] * want.abs() + 2 * (n + 2) * 2.0 ** -24 * magnitudes + TINY[dtype]
+
+
+def make_picks(t, k, e, seed, kind="even"):
+    """Distinct experts of each token: even, skewed, all on the first ones,
+    with padded tokens, with single missing picks, or none at all."""
+    g = rng(seed)
+    score = torch.rand(t, e, generator=g, device="cuda")
+    if kind == "skew":
+        score = score * torch.exp(2 * torch.randn(e, generator=g, device="cuda"))
+    if kind == "first":
+        score = -torch.arange(e, device="cuda").float().expand(t, e)
+    picks = torch.sort(score, dim=1, descending=True).indices[:, :k].contiguous()
+    if kind == "padded" and t:
+        picks[torch.rand(t, generator=g, device="cuda") < 0.3] = -1
+    if kind == "holes" and t:
+        picks[torch.rand(t, k, generator=g, device="cuda") < 0.3] = -1
+    if kind == "none":
+        picks.fill_(-1)
+    return picks
+
+
+def plain_grouping(picks, e):
+    t, k = picks.shape
+    flat = picks.reshape(-1).tolist()
+    order = sorted((p for p in range(t * k) if 0 <= flat[p] < e), key=lambda p: flat[p])
+    offsets, rows, slots = [0] * (e + 1), [0] * (t * k), [-1] * (t * k)
+    for s, p in enumerate(order):
+        rows[s], slots[p] = p // k, s
+        offsets[flat[p] + 1] += 1
+    for i in range(e):
+        offsets[i + 1] += offsets[i]
+    return offsets, rows, [slots[i * k:(i + 1) * k] for i in range(t)]
+
+
+# ---- routing ------------------------------------------------------------------
+
+ROUTES = [(0, 4, 2), (1, 1, 1), (1, 64, 4), (3, 7, 7), (17, 16, 16), (255, 33, 3), (256, 8, 2),
+          (257, 8, 2), (300, 128, 8), (1000, 200, 5), (4097, 60, 6), (700, 257, 9),
+          (90, 1024, 16), (500, 1000, 4)]
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k", ROUTES)
+def test_route(gpu, t, e, k, dtype, renorm):
+    g = rng(t + e)
+    logits = randn(g, t, e, dtype=dtype, scale=2.0)
+    if t > 4 and e > 8:
+        logits[1] = 0.5                     # all equal: the lowest experts
+        logits[2, ::2] = -float("inf")      # half excluded
+        logits[3] = -float("inf")           # a padding token
+        logits[4] = torch.finfo(dtype).min  # all of the lowest value
+        logits[0, :3] = -0.0
+        logits[0, 3:6] = 0.0
+    r = ej.route_experts(logits, k, renormalize=renorm)
+    l64 = logits.double()
+    order = torch.sort(l64, dim=1, descending=True, stable=True)
+    picks = order.indices[:, :k].clone()
+    held = order.values[:, :k] > -float("inf")
+    picks[~held] = -1
+    assert torch.equal(r.experts.long(), picks)
+    offsets, rows, slots = plain_grouping(picks, e)
+    assert r.offsets.tolist() == offsets
+    assert r.rows.tolist() == rows
+    assert r.slots.tolist() == slots
+    top = torch.where(held, order.values[:, :k], -float("inf"))
+    want = torch.softmax(top, 1) if renorm else torch.softmax(l64, 1).gather(
+        1, order.indices[:, :k])
+    want = torch.where(held, want, torch.zeros_like(want))
+    # exp within 2 ulp, of an argument rounded once; a sum of e terms; a division
+    arg = 40.0 if t > 4 and e > 8 else 20.0
+    assert_within(r.weights, want, (arg + e + 8) * 2.0 ** -24 * want + 1e-37)
+
+
+def test_route_nan_and_infinity(gpu):
+    logits = torch.zeros(4, 6, device="cuda")
+    logits[1, 4] = float("nan")
+    logits[2, 3] = float("inf")
+    logits[3, 1] = 1.0
+    r = ej.route_experts(logits, 2)
+    assert r.experts.tolist() == [[0, 1], [4, 0], [3, 0], [1, 0]]
+    w = r.weights.cpu()
+    assert torch.isnan(w[1]).all() and torch.isnan(w[2]).all()
+    assert torch.isfinite(w[0]).all() and torch.isfinite(w[3]).all()
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k", [r for r in ROUTES if r[0] > 0])
+def test_route_gradient(gpu, t, e, k, dtype, renorm):
+    g = rng(t * e)
+    logits = randn(g, t, e, dtype=dtype, scale=1.5)
+    if t > 4 and e > 8:
+        logits[2, ::2] = -float("inf")
+        logits[3] = -float("inf")
+    leaf = logits.clone().requires_grad_()
+    r = ej.route_experts(leaf, k, renormalize=renorm)
+    cot = randn(g, t, k)
+    (got,) = torch.autograd.grad(r.weights, leaf, cot)
+    assert got.dtype == dtype
+    l64 = logits.double()
+    picks = r.experts.long().clamp(min=0)
+    held = (r.experts >= 0)
+    p = torch.exp(l64 - torch.clamp(l64.amax(1, keepdim=True), min=-1e30))
+    if renorm:
+        p = torch.zeros_like(p).scatter_add(1, picks, p.gather(1, picks) * held)
+    p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
+    full = torch.zeros_like(p).scatter_add(1, picks, cot.double() * held)
+    dot = (p * full).sum(1, keepdim=True)
+    want = p * (full - dot)
+    mag = p * (full.abs() + (p * full.abs()).sum(1, keepdim=True))
+    assert_within(got, want, UNIT[dtype] * want.abs() + (60 + 2 * e) * 2.0 ** -24 * mag
+                  + TINY[dtype])
+
+
+def test_route_gradient_against_differences(gpu):
+    g = rng(5)
+    logits = randn(g, 12, 10)
+    cot = randn(g, 12, 3)
+    for renorm in (True, False):
+        r = ej.route_experts(logits, 3, renormalize=renorm)
+        grad = ej.route_experts_vjp(logits, r.experts, cot, renormalize=renorm)
+        d = randn(g, 12, 10)
+        h = 2.0 ** -7
+        up = ej.route_experts(logits + h * d, 3, renormalize=renorm)
+        down = ej.route_experts(logits - h * d, 3, renormalize=renorm)
+        same = (up.experts == r.experts).all(1) & (down.experts == r.experts).all(1)
+        assert int(same.sum()) >= 6
+        num = ((up.weights - down.weights).double() * cot).sum(1) / (2 * h)
+        want = (grad.double() * d).sum(1)
+        # central differences: h^2 times third derivatives of a softmax along d
+        # (at most |d|^3 |cot|), and rounding 2^-22 / h
+        room = (h * h * d.norm(dim=1) ** 3 + 2.0 ** -22 / h * 4) * cot.norm(dim=1)
+        assert (((num - want).abs() <= room) | ~same).all()
+
+
+def test_route_takes_strided_logits(gpu):
+    g = rng(9)
+    wide = randn(g, 40, 50)
+    for logits in (wide[:, 3:19], wide[::2, :20], wide.t()[:30]):
+        a = ej.route_experts(logits, 4)
+        b = ej.route_experts(logits.contiguous(), 4)
+        assert torch.equal(a.experts, b.experts) and torch.equal(a.weights, b.weights)
+        ga = ej.route_experts_vjp(logits, a.experts, a.weights)
+        gb = ej.route_experts_vjp(logits.contiguous(), a.experts, a.weights)
+        assert torch.equal(ga, gb)
+
+
+@pytest.mark.parametrize("kind", ["even", "skew", "first", "padded", "holes", "none"])
+@pytest.mark.parametrize("t,e,k", [(0, 3, 2), (1, 5, 1), (200, 9, 3), (256, 300, 16), (1500, 9, 3),
+                                   (3000, 1024, 7)])
+def test_group_by_expert(gpu, t, e, k, kind):
+    picks = make_picks(t, k, e, 7, kind)
+    if t > 3:
+        picks[3, 0] = e + 5  # outside: no slot
+    r = ej.group_by_expert(picks, e)
+    offsets, rows, slots = plain_grouping(picks, e)
+    assert r.offsets.tolist() == offsets
+    assert r.rows.tolist() == rows
+    assert r.slots.tolist() == slots
+    assert bool((r.weights == 1).all())
+
+
+# ---- grouped products ------------------------------------------------------------
+
+def row_groups(offsets, slots):
+    """Group of each slot, -1 for none."""
+    ends = offsets.tolist()
+    owner = torch.full((slots,), -1, dtype=torch.long)
+    for e in range(len(ends) - 1):
+        owner[ends[e]:ends[e + 1]] = e
+    return owner.tolist(), ends
+
+
+def product64(x, rows, offsets, w, slots):
+    out = torch.zeros(slots, w.shape[2], dtype=torch.double, device="cuda")
+    mag = torch.zeros_like(out)
+    _, ends = row_groups(offsets, slots)
+    for e in range(w.shape[0]):
+        a, b = ends[e], ends[e + 1]
+        if a == b:
+            continue
+        xe = x[rows[a:b].long()].double() if rows is not None else x[a:b].double()
+        out[a:b] = xe @ w[e].double()
+        mag[a:b] = xe.abs() @ w[e].double().abs()
+    return out, mag
+
+
+# tokens, experts, picks, k, n, kind of picks
+PRODUCTS = [
+    (1, 1, 1, 64, 64, "even"), (1, 4, 2, 128, 96, "even"), (2, 16, 2, 2048, 512, "even"),
+    (5, 3, 2, 1, 1, "even"), (7, 2, 1, 8, 8, "even"), (40, 6, 3, 72, 200, "padded"),
+    (33, 5, 2, 77, 131, "skew"), (129, 4, 1, 64, 264, "first"), (300, 70, 2, 96, 136, "skew"),
+    (257, 8, 2, 520, 392, "holes"), (600, 3, 2, 320, 640, "skew"), (700, 9, 4, 129, 67, "even"),
+    (64, 4, 2, 256, 128, "none"), (1500, 2, 2, 200, 1030, "skew"), (2048, 2, 1, 1024, 512, "even"),
+]
+
+
+def product_case(t, e, k, n_in, n_out, kind, dtype, order, gather, seed=3):
+    g = rng(seed + t + n_in)
+    r = ej.group_by_expert(make_picks(t, k, e, seed, kind), e)
+    x = randn(g, t if gather else t * k, n_in, dtype=dtype)
+    w = randn(g, e, n_in, n_out, dtype=dtype, scale=n_in ** -0.5)
+    if order == "nk":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    return g, r, x, w
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,n_in,n_out,kind", PRODUCTS)
+def test_grouped_matmul(gpu, t, e, k, n_in, n_out, kind, dtype, order):
+    for gather in (False, True):
+        _, r, x, w = product_case(t, e, k, n_in, n_out, kind, dtype, order, gather)
+        got = ej.grouped_matmul(x, w, r, gather=gather)
+        want, mag = product64(x, r.rows if gather else None, r.offsets, w, t * k)
+        assert got.dtype == dtype
+        assert_within(got, want, sum_bound(want, mag, n_in, dtype))
+        if not gather:
+            again = ej.grouped_matmul(x, w, r.offsets.long(), out_dtype=F32)
+            assert again.dtype == F32
+            assert_within(again, want, sum_bound(want, mag, n_in, F32))
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,n_in,n_out,kind", PRODUCTS)
+def test_grouped_matmul_gradients(gpu, t, e, k, n_in, n_out, kind, dtype, order):
+    for gather in (False, True):
+        g, r, x, w = product_case(t, e, k, n_in, n_out, kind, dtype, order, gather)
+        x.requires_grad_()
+        w = w.detach().requires_grad_()
+        y = ej.grouped_matmul(x, w, r, gather=gather)
+        cot = randn(g, t * k, n_out, dtype=dtype)
+        gx, gw = torch.autograd.grad(y, (x, w), cot)
+        assert gx.dtype == dtype and gw.dtype == dtype and gw.stride() == w.stride()
+        _, ends = row_groups(r.offsets, t * k)
+        x, w = x.detach(), w.detach()
+        wx = torch.zeros(t * k, n_in, dtype=torch.double, device="cuda")
+        mx = torch.zeros_like(wx)
+        for i in range(e):
+            a, b = ends[i], ends[i + 1]
+            at = r.rows[a:b].long() if gather else torch.arange(a, b, device="cuda")
+            xi, gi, wi = x[at].double(), cot[a:b].double(), w[i].double()
+            wx[a:b], mx[a:b] = gi @ wi.T, gi.abs() @ wi.abs().T
+            assert_within(gw[i], xi.T @ gi,
+                          sum_bound(xi.T @ gi, xi.abs().T @ gi.abs(), b - a, dtype))
+        bound = sum_bound(wx, mx, n_out, dtype)
+        if gather:
+            # each slot's row is rounded to the operands' type, then summed
+            total, room, size = (torch.zeros(t, n_in, dtype=torch.double, device="cuda")
+                                 for _ in range(3))
+            at = r.rows[:ends[-1]].long()
+            total.index_add_(0, at, wx[:ends[-1]])
+            room.index_add_(0, at, bound[:ends[-1]])
+            size.index_add_(0, at, wx[:ends[-1]].abs() + bound[:ends[-1]])
+            wx, bound = total, room + UNIT[dtype] * (total.abs() + room) + 2 * (k + 2) * \
+                2.0 ** -24 * size + TINY[dtype]
+        assert_within(gx, wx, bound)
+
+
+def test_grouped_gradients_against_differences(gpu):
+    g, r, x, w = product_case(40, 5, 2, 24, 36, "skew", F32, "kn", True)
+    cot = randn(g, 80, 36)
+    gx, gw = ej.grouped_matmul_vjp(x, w, r, cot, gather=True)
+    dx, dw = randn(g, *x.shape), randn(g, *w.shape)
+    # the product is bilinear: central differences are exact up to rounding
+    for direction, grad, move in ((dx, gx, lambda h: (x + h * dx, w)),
+                                  (dw, gw, lambda h: (x, w + h * dw))):
+        up, down = (ej.grouped_matmul(*move(h), r, gather=True).double() for h in (0.5, -0.5))
+        num = ((up - down) * cot).sum()
+        want = (grad.double() * direction).sum()
+        size = (up.abs() * cot.abs()).sum() + (grad.abs() * direction.abs()).double().sum()
+        assert abs(float(num - want)) <= 2 * 100 * 2.0 ** -24 * float(size)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_grouped_matmul_views(gpu, dtype):
+    """Row strides, bases off 16 bytes and weights of neither order."""
+    g, r, _, _ = product_case(150, 4, 2, 64, 64, "skew", dtype, "kn", False)
+    slots = 300
+    wide = randn(g, slots, 200, dtype=dtype)
+    weights = randn(g, 4, 80, 90, dtype=dtype)
+    for x in (wide[:, :64], wide[:, 1:65], wide[:, 8:72], wide.t()[:64].t(),
+              wide[:1, :64].expand(slots, 64)):
+        for w in (weights[:, :64, :72], weights[:, 1:65, 3:70], weights[:, :, :64].transpose(1, 2)
+                  [:, :, :80], weights[:1, :64].expand(4, 64, 90), weights[:, :64, ::2],
+                  weights.transpose(1, 2)[:, 2:66, 5:75]):
+            got = ej.grouped_matmul(x, w, r)
+            want, mag = product64(x, None, r.offsets, w, slots)
+            assert_within(got, want, sum_bound(want, mag, 64, dtype))
+            cot = randn(g, slots, 2 * w.shape[2], dtype=dtype)[:, ::2]
+            gx, gw = ej.grouped_matmul_vjp(x, w, r, cot)
+            hx, hw = ej.grouped_matmul_vjp(x.contiguous(), w.contiguous(), r, cot.contiguous())
+            assert_within(gx, hx.double(), 4 * UNIT[dtype] * hx.double().abs() + 1e-3)
+            assert_within(gw, hw.double(), 4 * UNIT[dtype] * hw.double().abs() + 1e-3)
+
+
+def test_grouped_matmul_infinities_stay_in_their_rows(gpu):
+    """A NaN or infinity reaches its own results only: not other rows, not
+    other groups, not what pads a tile."""
+    for dtype in (F32, BF16):
+        for n_in, n_out in ((72, 40), (71, 37)):
+            g = rng(1)
+            offsets = torch.tensor([0, 5, 5, 40], dtype=torch.int32, device="cuda")
+            x, w = randn(g, 50, n_in, dtype=dtype), randn(g, 3, n_in, n_out, dtype=dtype)
+            x[3, n_in - 1] = float("inf")
+            x[45:] = float("nan")         # slots of no group
+            w[1] = float("nan")           # an expert without slots
+            w[2, 0, n_out - 1] = float("nan")
+            y = ej.grouped_matmul(x, w, offsets)
+            bad = ~torch.isfinite(y)
+            want = torch.zeros_like(bad)
+            want[3] = True
+            want[5:40, n_out - 1] = True
+            assert torch.equal(bad, want)
+            assert bool((y[40:] == 0).all())
+            cot = randn(g, 50, n_out, dtype=dtype)
+            cot[40:] = float("nan")
+            gx, gw = ej.grouped_matmul_vjp(x, w, offsets, cot)
+            assert bool((gx[40:] == 0).all()) and bool((gw[1] == 0).all())
+            assert torch.isfinite(gx[:5]).all() and torch.isfinite(gw[2]).all()
+
+
+def test_grouped_matmul_offsets_not_covering(gpu):
+    """Slots before the first offset and past the last are zero."""
+    g = rng(2)
+    x, w = randn(g, 500, 64, dtype=BF16), randn(g, 2, 64, 128, dtype=BF16)
+    offsets = torch.tensor([100, 130, 300], dtype=torch.int32, device="cuda")
+    y = ej.grouped_matmul(x, w, offsets)
+    assert bool((y[:100] == 0).all()) and bool((y[300:] == 0).all())
+    want, mag = torch.zeros(500, 128, dtype=torch.double, device="cuda"), None
+    want[100:130] = x[100:130].double() @ w[0].double()
+    want[130:300] = x[130:300].double() @ w[1].double()
+    mag = x.double().abs() @ w.double().abs().amax(0)
+    assert_within(y, want, sum_bound(want, mag, 64, BF16))
+
+
+def test_grouped_matmul_wild_offsets_stay_in_bounds(gpu):
+    """Offsets outside the slots give undefined rows, no access outside."""
+    g = rng(2)
+    x, w = randn(g, 64, 64, dtype=BF16), randn(g, 3, 64, 64, dtype=BF16)
+    for o in ([-5, 10, 7, 1 << 30], [0, 64, 64, 64], [64, 64, 64, 64], [9, 3, 2, 1]):
+        offsets = torch.tensor(o, dtype=torch.int32, device="cuda")
+        assert ej.grouped_matmul(x, w, offsets).shape == (64, 64)
+        gx, gw = ej.grouped_matmul_vjp(x, w, offsets, x)
+        assert gx.shape == x.shape and gw.shape == w.shape
+
+
+def test_grouped_matmul_past_32_bits(gpu):
+    """Operands and results of more than 2^31 elements."""
+    g = rng(4)
+    rows, n_in, n_out = 530_000, 4096, 64
+    x = torch.empty(rows, n_in, dtype=BF16, device="cuda")   # 2.17e9 elements
+    last = randn(g, 40, n_in, dtype=BF16)
+    x[-40:] = last
+    w = randn(g, 2, n_in, n_out, dtype=BF16, scale=n_in ** -0.5)
+    offsets = torch.tensor([rows - 40, rows - 15, rows], dtype=torch.int32, device="cuda")
+    y = ej.grouped_matmul(x, w, offsets)
+    want = torch.cat([last[:25].double() @ w[0].double(), last[25:].double() @ w[1].double()])
+    mag = torch.cat([last[:25].double().abs() @ w[0].double().abs(),
+                     last[25:].double().abs() @ w[1].double().abs()])
+    assert_within(y[-40:], want, sum_bound(want, mag, n_in, BF16))
+    _, gw = ej.grouped_matmul_vjp(x, w, offsets, y, need_x=False)
+    got = y[-40:].double()
+    for i, (a, b) in enumerate(((0, 25), (25, 40))):
+        wg = last[a:b].double().T @ got[a:b]
+        assert_within(gw[i], wg, sum_bound(wg, last[a:b].double().abs().T @ got[a:b].abs(), 25,
+                                           BF16))
+    del x
+    w = randn(g, 1, 8, 131_072, dtype=BF16)
+    x = randn(g, 17_000, 8, dtype=BF16)
+    y = ej.grouped_matmul(x, w, torch.tensor([0, 17_000], device="cuda"))  # 2.2e9 elements
+    want = x[-3:].double() @ w[0].double()
+    assert_within(y[-3:], want, sum_bound(want, x[-3:].double().abs() @ w[0].double().abs(), 8,
+                                          BF16))
+
+
+def test_grouped_matmul_on_another_stream(gpu):
+    _, r, x, w = product_case(300, 4, 2, 256, 256, "skew", BF16, "kn", True)
+    want = ej.grouped_matmul(x, w, r, gather=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ej.grouped_matmul(x, w, r, gather=True)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_expert_layer_in_a_graph(gpu):
+    """Routing, products and the sum captured once and replayed on new data."""
+    g = rng(8)
+    x = randn(g, 64, 128, dtype=BF16)
+    gate = randn(g, 128, 8, dtype=BF16)
+    up, down = randn(g, 8, 128, 256, dtype=BF16), randn(g, 8, 256, 128, dtype=BF16)
+
+    def layer():
+        r = ej.route_experts(x @ gate, 2)
+        h = ej.grouped_matmul(x, up, r, gather=True)
+        return ej.combine_experts(ej.grouped_matmul(h, down, r), r)
+
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer()
+    for i in range(4):
+        x.copy_(randn(g, 64, 128, dtype=BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, layer())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_grouped_results_repeat(gpu, dtype):
+    g, r, x, w = product_case(900, 7, 3, 200, 328, "skew", dtype, "kn", True)
+    cot = randn(g, 2700, 328, dtype=dtype)
+    first = (ej.grouped_matmul(x, w, r, gather=True),
+             *ej.grouped_matmul_vjp(x, w, r, cot, gather=True))
+    for _ in range(3):
+        again = (ej.grouped_matmul(x, w, r, gather=True),
+                 *ej.grouped_matmul_vjp(x, w, r, cot, gather=True))
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+# ---- back to tokens ---------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["even", "padded", "holes", "none"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,n", [(1, 2, 1, 1), (1, 8, 4, 2048), (37, 5, 3, 77), (37, 5, 3, 72),
+                                     (300, 16, 16, 40), (513, 6, 2, 4104)])
+def test_combine(gpu, t, e, k, n, dtype, kind):
+    g = rng(t + n)
+    r = ej.group_by_expert(make_picks(t, k, e, 3, kind), e, torch.rand(t, k, generator=g,
+                                                                       device="cuda"))
+    y = randn(g, t * k, n, dtype=dtype)
+    live = int(r.offsets[-1])
+    y[live:] = float("nan")  # rows of no pair are not read
+    yl, wl = y.clone().requires_grad_(), r.weights.clone().requires_grad_()
+    out = ej.combine_experts(yl, r, wl)
+    assert torch.equal(out, ej.combine_experts(y, r, wl.detach()))
+    slots = r.slots.long()
+    held = slots >= 0
+    if live:
+        at = y[slots.clamp(min=0, max=live - 1)].double() * held[..., None]
+    else:
+        at = torch.zeros(t, k, n, dtype=torch.double, device="cuda")
+    w = r.weights.double()[..., None]
+    want = (w * at).sum(1)
+    assert_within(out, want, sum_bound(want, (w * at).abs().sum(1), k, dtype))
+    cot = randn(g, t, n, dtype=dtype)
+    gy, gw = torch.autograd.grad(out, (yl, wl), cot)
+    wy = torch.zeros(t * k + 1, n, dtype=torch.double, device="cuda")
+    wy[torch.where(held, slots, t * k).reshape(-1)] = \
+        (w * cot.double()[:, None]).reshape(-1, n)
+    wy = wy[:-1]
+    wy[live:] = 0
+    assert_within(gy, wy, (UNIT[dtype] + 2.0 ** -23) * wy.abs() + TINY[dtype])
+    ww = (at * cot.double()[:, None]).sum(2)
+    assert_within(gw, ww, 2 * (n + 2) * 2.0 ** -24 * (at * cot.double()[:, None]).abs().sum(2)
+                  + 1e-37)
+
+
+def test_combine_strided(gpu):
+    g = rng(6)
+    r = ej.group_by_expert(make_picks(50, 2, 4, 3, "holes"), 4)
+    wide = randn(g, 100, 300, dtype=BF16)
+    cots = randn(g, 50, 300, dtype=BF16)
+    for sl in (slice(0, 64), slice(3, 67), slice(0, 128, 2)):
+        y, c = wide[:, sl], cots[:, sl]
+        assert torch.equal(ej.combine_experts(y, r), ej.combine_experts(y.contiguous(), r))
+        a = ej.combine_experts_vjp(y, r, c)
+        b = ej.combine_experts_vjp(y.contiguous(), r, c.contiguous())
+        assert torch.equal(a[0], b[0])
+        bound = 2 * 66 * 2.0 ** -24 * (y.double().abs().amax() * c.double().abs().sum(1))
+        assert ((a[1] - b[1]).double().abs() <= bound[:, None]).all()
+
+
+# ---- 8-bit integers ----------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n", [(0, 5), (1, 1), (3, 64), (5, 77), (130, 2048), (9, 10000)])
+def test_quantize_rows(gpu, m, n, dtype):
+    g = rng(m + n)
+    x = randn(g, m, n, dtype=dtype, scale=3.0)
+    if m >= 3:
+        x[1] = 0
+    q, scale = ej.quantize_rows(x)
+    assert q.dtype == torch.int8 and q.shape == x.shape and scale.shape == (m,)
+    want = x.float().abs().amax(1) * torch.tensor(1 / 127, device="cuda") if m else scale
+    assert torch.equal(scale, want)
+    exact = torch.where(scale[:, None] > 0, x.double() / scale.double()[:, None], 0.0)
+    # a tie may go either way where the quotient's own rounding decides it
+    assert ((q.double() - exact).abs() <= 0.5 + 128 * 2.0 ** -24).all()
+    assert int(q.abs().amax()) <= 127 if m else True
+    if m:
+        assert torch.equal(q.abs().amax(1) == 127, scale > 0)
+
+
+def test_quantize_rows_not_finite_and_tiny(gpu):
+    x = torch.ones(5, 40, device="cuda")
+    x[1, 7] = float("inf")
+    x[2, 39] = float("nan")
+    x[3] = 1e-45
+    x[4] = 3e38
+    q, scale = ej.quantize_rows(x)
+    assert torch.isnan(scale[1:3]).all() and torch.isfinite(scale[[0, 3, 4]]).all()
+    assert bool((q[1:3] == 0).all()) and bool((q[[0, 4]] == 127).all())
+    w, ws = ej.quantize_rows(torch.randn(16, 40, device="cuda"))
+    y = ej.int8_matmul(q, scale, w, ws)
+    assert torch.isnan(y[1:3]).all() and torch.isfinite(y[[0, 3]]).all()
+    # the last row's products reach infinity where bf16 ends, and only there
+    want = (q[4].double() @ w.double().T) * scale[4].double() * ws.double()
+    assert torch.equal(torch.isinf(y[4]), want.abs() >= 2.0 ** 128 - 2.0 ** 119)
+
+
+def test_quantize_rows_views(gpu):
+    g = rng(3)
+    wide = randn(g, 4, 30, 200, dtype=BF16)
+    for x in (wide, wide[:, :, 3:75], wide[:, ::2, :64], wide.transpose(1, 2)):
+        q, s = ej.quantize_rows(x)
+        p, t = ej.quantize_rows(x.contiguous())
+        assert torch.equal(q, p) and torch.equal(s, t)
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,n_in,n_out,kind", PRODUCTS)
+def test_int8_matmul(gpu, t, e, k, n_in, n_out, kind, out_dtype):
+    g = rng(t + n_out)
+    r = ej.group_by_expert(make_picks(t, k, e, 3, kind), e)
+    w = torch.randint(-128, 128, (e, n_out, n_in), generator=g, device="cuda").to(torch.int8)
+    ws = torch.rand(e, n_out, generator=g, device="cuda") * 1e-4
+    for gather in (False, True):
+        m = t if gather else t * k
+        q = torch.randint(-128, 128, (m, n_in), generator=g, device="cuda").to(torch.int8)
+        qs = torch.rand(m, generator=g, device="cuda")
+        got = ej.int8_matmul(q, qs, w, ws, r, gather=gather, out_dtype=out_dtype)
+        assert got.dtype == out_dtype
+        want = torch.zeros(t * k, n_out, dtype=torch.double, device="cuda")
+        _, ends = row_groups(r.offsets, t * k)
+        for i in range(e):
+            a, b = ends[i], ends[i + 1]
+            at = r.rows[a:b].long() if gather else torch.arange(a, b, device="cuda")
+            want[a:b] = (q[at].double() @ w[i].double().T) * qs[at].double()[:, None] \
+                * ws[i].double()
+        # the sum is exact; its conversion and two products round
+        assert_within(got, want, (UNIT[out_dtype] + 4 * 2.0 ** -24) * want.abs()
+                      + TINY[out_dtype])
+
+
+@pytest.mark.parametrize("m,n_in,n_out", [(0, 64, 32), (1, 4096, 256), (4, 100, 33), (200, 256, 300)])
+def test_int8_matmul_dense(gpu, m, n_in, n_out):
+    g = rng(m + 1)
+    x, w = randn(g, m, n_in), randn(g, n_out, n_in)
+    q, qs = ej.quantize_rows(x)
+    p, ps = ej.quantize_rows(w)
+    want = (q.double() @ p.double().T) * qs.double()[:, None] * ps.double()
+    for pw, pss in ((p, ps), (p[None], ps[None])):
+        got = ej.int8_matmul(q, qs, pw, pss, out_dtype=F32)
+        assert_within(got, want, 5 * 2.0 ** -24 * want.abs() + 1e-37)
+    # the largest sums that 32 bits hold
+    k = 131_071
+    a = torch.full((2, k), -128, dtype=torch.int8, device="cuda")
+    one = torch.ones(2, device="cuda")
+    got = ej.int8_matmul(a, one, a, one, out_dtype=F32)
+    assert bool((got.double() == float(torch.tensor(128.0 * 128 * k, dtype=F32))).all())
+
+
+def test_int8_weights_past_32_bits(gpu):
+    g = rng(11)
+    w = torch.empty(1100, 2048, 1024, dtype=torch.int8, device="cuda")  # 2.3e9 bytes
+    w[-1] = torch.randint(-128, 128, (2048, 1024), generator=g, device="cuda").to(torch.int8)
+    q = torch.randint(-128, 128, (5, 1024), generator=g, device="cuda").to(torch.int8)
+    offsets = torch.zeros(1101, dtype=torch.int32, device="cuda")
+    offsets[-1] = 5
+    ws = torch.ones(1100, 2048, device="cuda")
+    got = ej.int8_matmul(q, torch.ones(5, device="cuda"), w, ws, offsets, out_dtype=F32)
+    assert torch.equal(got.double(), q.double() @ w[-1].double().T)
