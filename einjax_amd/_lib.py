@@ -157,7 +157,8 @@ SIGNATURES = {
                                _vp, _sz, _vp]),
     "ej_expert_group": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ej_expert_route_vjp": (_i32, [_vp, _i32, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
-    "ej_expert_combine": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _vp]),
+    "ej_expert_combine": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i32,
+                                 _vp]),
     "ej_expert_combine_vjp": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
                                      _vp, _i64, _vp, _vp, _vp]),
     "ej_quantize_rows": (_i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp]),

@@ -19,18 +19,18 @@ __all__ = ["route_experts", "route_experts_vjp", "grouped_matmul", "grouped_matm
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, k, renormalize):
-        r = K.route(logits.detach(), k, renormalize)
+    def forward(ctx, logits, k, renormalize, made):
+        r = K.route(logits, k, renormalize)
+        made.append(r)
         ctx.renormalize = renormalize
         ctx.save_for_backward(logits, r.experts)
-        ctx.mark_non_differentiable(r.experts, r.offsets, r.rows, r.slots)
-        return r.weights, r.experts, r.offsets, r.rows, r.slots
+        return r.weights
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g, *_):
+    def backward(ctx, g):
         logits, experts = ctx.saved_tensors
-        return K.route_vjp(logits, experts, g, ctx.renormalize), None, None
+        return K.route_vjp(logits, experts, g, ctx.renormalize), None, None, None
 
 
 def route_experts(logits, k: int, *, renormalize: bool = True) -> ExpertRouting:
@@ -46,7 +46,10 @@ def route_experts(logits, k: int, *, renormalize: bool = True) -> ExpertRouting:
     constants."""
     if not (isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled()):
         return K.route(logits, k, renormalize)
-    return ExpertRouting(*_Route.apply(logits, k, renormalize))
+    made = []  # the routing with its integers, which autograd need not see
+    weights = _Route.apply(logits, k, renormalize, made)
+    r = made[0]
+    return ExpertRouting(weights, r.experts, r.offsets, r.rows, r.slots)
 
 
 def route_experts_vjp(logits, experts, grad_weights, *, renormalize: bool = True):
@@ -82,7 +85,7 @@ class _GroupedMatmul(torch.autograd.Function):
     def forward(ctx, x, w, groups, out_dtype):
         ctx.groups = groups
         ctx.save_for_backward(x, w)
-        return K.grouped_product(x.detach(), w.detach(), groups, out_dtype)
+        return K.grouped_product(x, w, groups, out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -95,15 +98,17 @@ class _GroupedMatmul(torch.autograd.Function):
 def _product_vjp(x, w, groups, grad, need_x, need_w):
     # an fp32 cotangent of 16-bit operands is rounded to their type: both
     # gradients are 16-bit products with fp32 sums
-    grad = grad.to(x.dtype)
+    if grad.dtype is not x.dtype:
+        grad = grad.to(x.dtype)
     gx = gw = None
     if need_x:
-        # one row for each slot in the operands' type, as the product's own
-        # results are; a token's slots are then summed in fp32
+        # gathered rows: each slot's gradient stays in fp32 until a token's
+        # slots are summed, so that the sum is rounded once
         slots = K.Groups(groups.offsets, None, None, groups.n_slots)
-        gx = K.grouped_product(grad, w.transpose(1, 2), slots, x.dtype)
-        if groups.rows is not None:
-            gx = K.combine(gx, groups.slots, None)
+        summed = groups.rows is not None
+        gx = K.grouped_product(grad, w.transpose(1, 2), slots, torch.float32 if summed else x.dtype)
+        if summed:
+            gx = K.combine(gx, groups.slots, None, x.dtype)
     if need_w:
         gw = K.grouped_weight_gradient(x, w, groups, grad)
     return gx, gw
@@ -145,7 +150,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, slots, offsets):
         ctx.save_for_backward(y, weights, slots, offsets)
-        return K.combine(y.detach(), slots, weights.detach())
+        return K.combine(y, slots, weights)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -169,7 +174,7 @@ def _check_combine(y, routing, weights):
     if weights.dtype != torch.float32 or weights.shape != routing.slots.shape:
         raise ValueError(f"weights must be float32 {tuple(routing.slots.shape)}, got "
                          f"{weights.dtype} {tuple(weights.shape)}")
-    return (weights.contiguous(), K._index(routing.slots, tuple(routing.slots.shape), "slots"),
+    return (weights if weights.is_contiguous() else weights.contiguous(), K._index(routing.slots, routing.slots.shape, "slots"),
             K._index(routing.offsets, (routing.n_experts + 1,), "offsets"))
 
 

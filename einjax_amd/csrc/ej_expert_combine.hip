@@ -36,14 +36,15 @@ struct Piece {
       v[0] = widen(*p);
     }
   }
-  __device__ inline void store(T *p) const {
+  template <class O>
+  __device__ inline void store(O *p) const {
     if constexpr (VEC) {
-      struct alignas(16) { T e[N]; } w;
+      struct alignas(N * sizeof(O)) { O e[N]; } w;
 #pragma unroll
-      for (int i = 0; i < N; ++i) w.e[i] = static_cast<T>(v[i]);
+      for (int i = 0; i < N; ++i) w.e[i] = static_cast<O>(v[i]);
       *reinterpret_cast<decltype(w) *>(p) = w;
     } else {
-      *p = static_cast<T>(v[0]);
+      *p = static_cast<O>(v[0]);
     }
   }
 };
@@ -62,7 +63,7 @@ struct CombineArgs {
 
 // out[t] = sum_j weights[t, j] y[slots[t, j]]: summed in fp32 in the order of
 // the picks, rounded once.  One workgroup a token and stretch of columns.
-template <class T, bool VEC>
+template <class T, class O, bool VEC>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsigned col_blocks) {
   constexpr int N = Piece<T, VEC>::N;
   const int64_t t = blockIdx.x / col_blocks;
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsign
   Piece<T, VEC> o;
 #pragma unroll
   for (int i = 0; i < N; ++i) o.v[i] = sum[i];
-  o.store(static_cast<T *>(a.out) + t * a.ld_out + col);
+  o.store(static_cast<O *>(a.out) + t * a.ld_out + col);
 }
 
 // grad_y[slots[t, j]] = weights[t, j] grad[t]; grad_w[t, j] = grad[t] . y[slots[t, j]].
@@ -219,30 +220,40 @@ using namespace ej;
 
 extern "C" int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
                                  const float *weights, const int32_t *slots, int64_t n_tokens,
-                                 int32_t k, int32_t n, void *out, ej_stream_t stream) {
+                                 int32_t k, int32_t n, void *out, int32_t out_dtype,
+                                 ej_stream_t stream) {
   EJ_TRY(check_combine(n_slots, n_tokens, k, n));
+  EJ_CHECK_ARG(out_dtype == dtype || dtype == EJ_F32, "a sum of dtype %d from values of dtype %d",
+               out_dtype, dtype);
   return by_type(dtype, [&](auto *tp) {
-    using T = std::remove_pointer_t<decltype(tp)>;
-    if (n_tokens == 0 || n == 0) return EJ_OK;
-    EJ_CHECK_ARG(slots && out && (y || n_slots == 0), "null argument");
-    EJ_CHECK_ARG(ld_y >= n, "row stride %lld below n = %d", (long long)ld_y, n);
-    CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, nullptr, 0, out};
-    const bool vec = aligned16(y, ld_y, sizeof(T)) && aligned16(out, n, sizeof(T));
-    const int64_t cols =
-        ceil_div(n, static_cast<int64_t>(kThreads) * (vec ? 16 / sizeof(T) : 1));
-    if (n_tokens * cols > kMaxBlocks) {
-      set_error("%lld rows of %d: too many for one launch", (long long)n_tokens, n);
-      return EJ_E_UNSUPPORTED;
-    }
-    const dim3 grid(static_cast<unsigned>(n_tokens * cols));
-    if (vec)
-      hipLaunchKernelGGL((combine_kernel<T, true>), grid, dim3(kThreads), 0, as_stream(stream), a,
-                         static_cast<unsigned>(cols));
-    else
-      hipLaunchKernelGGL((combine_kernel<T, false>), grid, dim3(kThreads), 0, as_stream(stream),
-                         a, static_cast<unsigned>(cols));
-    EJ_LAUNCH_CHECK();
-    return EJ_OK;
+    return by_type(out_dtype, [&](auto *op) {
+      using T = std::remove_pointer_t<decltype(tp)>;
+      using O = std::remove_pointer_t<decltype(op)>;
+      if constexpr (std::is_same_v<T, O> || std::is_same_v<T, float>) {
+        if (n_tokens == 0 || n == 0) return EJ_OK;
+        EJ_CHECK_ARG(slots && out && (y || n_slots == 0), "null argument");
+        EJ_CHECK_ARG(ld_y >= n, "row stride %lld below n = %d", (long long)ld_y, n);
+        CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, nullptr, 0, out};
+        // whole 16-byte pieces of y, and the pieces of out aligned to their size
+        constexpr int N = 16 / sizeof(T);
+        const bool vec = aligned16(y, ld_y, sizeof(T)) && n % N == 0 &&
+                         reinterpret_cast<size_t>(out) % (N * sizeof(O)) == 0;
+        const int64_t cols = ceil_div(n, static_cast<int64_t>(kThreads) * (vec ? N : 1));
+        if (n_tokens * cols > kMaxBlocks) {
+          set_error("%lld rows of %d: too many for one launch", (long long)n_tokens, n);
+          return EJ_E_UNSUPPORTED;
+        }
+        const dim3 grid(static_cast<unsigned>(n_tokens * cols));
+        if (vec)
+          hipLaunchKernelGGL((combine_kernel<T, O, true>), grid, dim3(kThreads), 0,
+                             as_stream(stream), a, static_cast<unsigned>(cols));
+        else
+          hipLaunchKernelGGL((combine_kernel<T, O, false>), grid, dim3(kThreads), 0,
+                             as_stream(stream), a, static_cast<unsigned>(cols));
+        EJ_LAUNCH_CHECK();
+      }
+      return EJ_OK;
+    });
   });
 }
 

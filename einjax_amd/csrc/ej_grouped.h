@@ -112,7 +112,7 @@ __device__ inline int swz_k(int row) { return (row >> 1) & 7; }
 // that the lane groups read go to distinct 64-byte groups.
 template <class Op, int CHUNKS>
 __device__ inline int swz_m(int krow) {
-  if constexpr (kElem<Op> == 4) return 4 * ((krow >> 2) & 3);
+  if constexpr (kElem<Op> == 4) return 4 * ((krow >> 2) & (CHUNKS >= 16 ? 3 : 1));
   else if constexpr (CHUNKS >= 16) return (2 * (krow & 3)) ^ (8 * ((krow >> 3) & 1));
   else return 2 * (krow & 3);
 }
@@ -123,7 +123,8 @@ struct Tile {
   static constexpr int kBytes = ROWS * kRowB;
   static constexpr int kLine = KC ? kRowB : ROWS * kElem<Op>;  // bytes of an LDS row
   static constexpr int kChunks = kLine / 16;                   // chunks of an LDS row
-  static_assert(KC || kChunks >= (kElem<Op> == 4 ? 16 : 8), "M tiles: swizzle range");
+  static constexpr int kReads = KC ? 1 : kElem<Op>;            // LDS reads of a fragment
+  static_assert(KC || kChunks >= 8, "M tiles: swizzle range");
 
   // Line (row or k) and unswizzled chunk that the 16 bytes at LDS position
   // `pos` (in chunks) hold.
@@ -131,38 +132,59 @@ struct Tile {
     *line = pos / kChunks;
     *chunk = (pos % kChunks) ^ (KC ? swz_k(*line) : swz_m<Op, kChunks>(*line));
   }
+};
 
-  // This lane's part of the fragment of 16 rows from row0 on, 64-byte slab
-  // `slab` of the stage's k, from the tile at LDS address `base`.
-  __device__ static inline i32v4_t frag(uint32_t base, int row0, int slab, int lane) {
+// This lane's places in the fragments of F x 16 rows from row0 on: K tiles
+// need one address for each 64-byte slab of the stage's k (the swizzle repeats
+// every 16 rows), M tiles one for each fragment; the rest are constant offsets.
+template <class Op, class T, bool KC, int F>
+struct Fragments {
+  static constexpr int kAddr = KC ? 2 : F;
+  uint32_t addr[kAddr];
+
+  __device__ inline void init(uint32_t base, int row0, int lane) {
     if constexpr (KC) {
       const int row = row0 + (lane & 15);
-      const int chunk = (slab * 4 + (lane >> 4)) ^ swz_k(row);
-      return *reinterpret_cast<const __attribute__((address_space(3))) i32v4_t *>(
-          (lds_u8 *)(size_t)(base + row * kRowB + chunk * 16));
-    } else if constexpr (kElem<Op> == 2) {
-      const int t = (lane & 15) >> 2, q = lane & 3;
-      i32v2_t h[2];
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int krow = slab * 32 + (lane >> 4) * 8 + hh * 4 + t;
-        const int chunk = ((row0 >> 3) + (q >> 1)) ^ swz_m<Op, kChunks>(krow);
-        h[hh] = __builtin_bit_cast(
-            i32v2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                         (__attribute__((address_space(3))) i16x4_t *)(size_t)(
-                             base + krow * kLine + chunk * 16 + (q & 1) * 8)));
-      }
-      return i32v4_t{h[0][0], h[0][1], h[1][0], h[1][1]};
+      for (int s = 0; s < 2; ++s)
+        addr[s] = base + row * kRowB + ((s * 4 + (lane >> 4)) ^ swz_k(row)) * 16;
     } else {
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        if constexpr (kElem<Op> == 2) {
+          const int krow = (lane >> 4) * 8 + ((lane & 15) >> 2);
+          const int chunk = ((row0 + i * 16) >> 3) + ((lane & 3) >> 1);
+          addr[i] = base + krow * T::kLine + (chunk ^ swz_m<Op, T::kChunks>(krow)) * 16 +
+                    (lane & 1) * 8;
+        } else {
+          const int krow = (lane >> 4) * 4, col = row0 + i * 16 + (lane & 15);
+          addr[i] = base + krow * T::kLine + ((col >> 2) ^ swz_m<Op, T::kChunks>(krow)) * 16 +
+                    (col & 3) * 4;
+        }
+      }
+    }
+  }
+  // The fragment of rows row0 + 16 i .. + 15, slab `slab`, of the tile `off`
+  // bytes past the base.
+  __device__ inline i32v4_t read(uint32_t off, int i, int slab) const {
+    if constexpr (KC) {
+      return *reinterpret_cast<const __attribute__((address_space(3))) i32v4_t *>(
+          (lds_u8 *)(size_t)(addr[slab] + off) + i * 16 * kRowB);
+    } else if constexpr (kElem<Op> == 2) {
+      lds_u8 *p = (lds_u8 *)(size_t)(addr[i] + off) + slab * 32 * T::kLine;
+      const i32v2_t h0 = __builtin_bit_cast(
+          i32v2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (__attribute__((address_space(3))) i16x4_t *)p));
+      const i32v2_t h1 = __builtin_bit_cast(
+          i32v2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (__attribute__((address_space(3))) i16x4_t *)(p + 4 * T::kLine)));
+      return i32v4_t{h0[0], h0[1], h1[0], h1[1]};
+    } else {
+      lds_u8 *p = (lds_u8 *)(size_t)(addr[i] + off) + slab * 16 * T::kLine;
       i32v4_t v;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int krow = slab * 16 + (lane >> 4) * 4 + c;
-        const int col = row0 + (lane & 15);
-        const int chunk = (col >> 2) ^ swz_m<Op, kChunks>(krow);
-        v[c] = *reinterpret_cast<const __attribute__((address_space(3))) int *>(
-            (lds_u8 *)(size_t)(base + krow * kLine + chunk * 16 + (col & 3) * 4));
-      }
+      for (int c = 0; c < 4; ++c)
+        v[c] = *reinterpret_cast<const __attribute__((address_space(3))) int *>(p + c * T::kLine);
       return v;
     }
   }
@@ -307,7 +329,20 @@ constexpr int kZeroBlocks = 64;  // workgroups appended to a grid for zero_dead_
 
 
 // ---- operand loads ------------------------------------------------------------
-#define EJ_LDS_PTR(p) ((__attribute__((address_space(3))) void *)(p))
+// Loads 16 bytes for each lane straight into LDS, lane l's to `lds` + 16 l
+// (m0 holds the address and needs one wait state before it is used).  As asm,
+// because the compiler holds back every transposing LDS read until all such
+// loads it knows of have landed; the loops wait for them by count (s_waitcnt
+// vmcnt) before the barrier after which a stage is read.  The load has no
+// output register.
+__device__ inline void load_to_lds(const char *src, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds));
+#endif
+}
+__device__ inline uint32_t lds_address(const void *p) {
+  return static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8 *)p));
+}
 
 // 16 bytes at any element alignment, the first `valid` elements of them (the
 // rest zero).
@@ -339,10 +374,26 @@ struct Loader {
   static constexpr int kLoads = T::kBytes / 1024 / NW;  // load instructions per wave and stage
   static_assert(T::kBytes % (1024 * NW) == 0, "whole loads per wave");
 
+  // k-rows between a lane's places in two loads of an M tile.  Its swizzle
+  // repeats after that many, or after twice as many: then a lane has one
+  // column in even loads and one in odd ones.
+  static constexpr int kApart = KC ? 0 : NW * 64 / T::kChunks;
+  static constexpr int kPeriod = T::kChunks >= 16 ? 16 : 8;
+  static constexpr int kCols = KC || kLoads == 1 || kApart % kPeriod == 0 ? 1 : 2;
+  static_assert(kCols == 1 || kApart * 2 % kPeriod == 0, "places repeat");
+
   const char *src[kLoads];  // this lane's source in the next stage
-  int line[kLoads];         // K: first k element of the lane's chunk; M: its k-row
-  int valid[kLoads];        // M, not DIRECT: elements of the lane's chunk inside the extent
+  int line;                 // K: first k element of the lane's chunk; M: its k-row in load 0
+  int col[kCols];           // M: first column of the lane's chunk
+  int valid[kCols];         // M, not DIRECT: elements of the chunk inside the extent
   i32v4_t reg[DIRECT ? 1 : kLoads];
+
+  // k element (K) or k-row (M) of the lane's place in load v; in K tiles the
+  // swizzle repeats every 16 rows, and differs by 4 between its halves.
+  __device__ inline int line_at(int v) const {
+    if constexpr (KC) return NW % 2 == 0 || v % 2 == 0 ? line : line ^ (4 * kChunk<Op>);
+    else return line + v * kApart;
+  }
 
   // K tiles: row_at(i) is the address of output row i's first k element.
   template <class RowAt>
@@ -351,7 +402,7 @@ struct Loader {
     for (int v = 0; v < kLoads; ++v) {
       int row, chunk;
       T::at((v * NW + wave) * 64 + lane, &row, &chunk);
-      line[v] = chunk * kChunk<Op>;
+      if (v == 0) line = chunk * kChunk<Op>;
       src[v] = row_at(row) + chunk * 16;
     }
   }
@@ -360,35 +411,38 @@ struct Loader {
                                 int ext) {
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
-      int chunk;
-      T::at((v * NW + wave) * 64 + lane, &line[v], &chunk);
-      int col = col0 + chunk * kChunk<Op>;
-      if constexpr (DIRECT) {
-        if (col > ext - kChunk<Op>) col = ext - kChunk<Op>;
-      } else {
-        valid[v] = ext - col;
-        if (col >= ext) col = 0;
+      int krow, chunk;
+      T::at((v * NW + wave) * 64 + lane, &krow, &chunk);
+      if (v == 0) line = krow;
+      if (v < kCols) {
+        int c = col0 + chunk * kChunk<Op>;
+        if constexpr (DIRECT) {
+          if (c > ext - kChunk<Op>) c = ext - kChunk<Op>;
+        } else {
+          valid[v] = ext - c;
+          if (c >= ext) c = 0;
+        }
+        col[v] = c;
       }
-      src[v] = base + (line[v] * ld + col) * kElem<Op>;
+      src[v] = base + (line_at(v) * ld + col[v % kCols]) * kElem<Op>;
     }
   }
 
-  // Loads the next stage, of which `left` elements of k exist (>= 1), to the
-  // tile at `tile`, and advances the sources by `step` bytes.
-  __device__ inline void load(unsigned char *tile, int wave, int left, int64_t step) {
-#pragma unroll
-    for (int v = 0; v < kLoads; ++v) {
-      if constexpr (DIRECT) {
-        const char *p = src[v];
-        if (left < kStep<Op>)
-          p = line[v] < left ? p : reinterpret_cast<const char *>(&grouped_zeros);
-        __builtin_amdgcn_global_load_lds(p, EJ_LDS_PTR(tile + (v * NW + wave) * 1024), 16, 0, 0);
-      } else {
-        const int n = KC ? left - line[v] : line[v] < left ? valid[v] : 0;
-        reg[v] = load_chunk<Op>(src[v], n);
-      }
-      src[v] += step;
+  // Starts load v of the next stage, of which `left` elements of k exist
+  // (>= 1), to the tile at `tile`, and advances its source by `step` bytes.
+  // part: the stage may end short of kStep elements.
+  __device__ inline void load(int v, unsigned char *tile, int wave, int left, int64_t step,
+                              bool part) {
+    if constexpr (DIRECT) {
+      const char *p = src[v];
+      if (part && left < kStep<Op>)
+        p = line_at(v) < left ? p : reinterpret_cast<const char *>(&grouped_zeros);
+      load_to_lds(p, lds_address(tile) + (v * NW + wave) * 1024);
+    } else {
+      const int n = KC ? left - line_at(v) : line_at(v) < left ? valid[v % kCols] : 0;
+      reg[v] = load_chunk<Op>(src[v], n);
     }
+    src[v] += step;
   }
   // Not DIRECT: what load() fetched, into the tile at `tile`.
   __device__ inline void store(unsigned char *tile, int wave, int lane) {
@@ -397,16 +451,11 @@ struct Loader {
       *reinterpret_cast<i32v4_t *>(tile + ((v * NW + wave) * 64 + lane) * 16) = reg[v];
   }
 
-  // M tiles whose rows are slots (weight gradient): the sources of the stage
-  // that starts at slot s0, rows through the index array if there is one.
-  __device__ inline void seek_slots(const char *base, int64_t ld, const int32_t *rows,
-                                    int64_t n_rows, int s0, int s_end, const int (&col)[kLoads]) {
-#pragma unroll
-    for (int v = 0; v < kLoads; ++v) {
-      const int s = s0 + line[v];
-      src[v] = base + (slot_row(rows, n_rows, s < s_end ? s : s_end - 1) * ld + col[v]) *
-                          kElem<Op>;
-    }
+  // M tiles of gathered rows (weight gradient): source v of the stage whose
+  // rows' places in the operand lie in the lanes of `row` (lane i: k-row i).
+  __device__ inline void seek(int v, const char *base, int64_t ld, int row) {
+    const int r = __shfl(row, line_at(v));
+    src[v] = base + (r * ld + col[v % kCols]) * kElem<Op>;
   }
 };
 

@@ -1,6 +1,8 @@
 // Choice of tile for one operand type.
 #pragma once
 
+#include <cmath>
+
 #include "ej_grouped_launch.h"
 #include "ej_grouped_tile.h"
 
@@ -20,29 +22,97 @@ int launch_rows(GroupedArgs g, hipStream_t stream) {
   return EJ_OK;
 }
 
-template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS>
-int launch_wgrad(GroupedArgs g, hipStream_t stream) {
+template <class Op, int FM, int BN, int NW, bool BKC, int NS>
+int launch_skinny(GroupedArgs g, hipStream_t stream) {
+  const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
+  g.row_blocks = static_cast<uint32_t>(g.slots / (16 * FM) + groups);
+  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, BN));
+  dim3 grid;
+  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks, NW * 64,
+                      &grid));
+  hipLaunchKernelGGL((grouped_skinny_kernel<Op, FM, BN, NW, BKC, NS>), grid, dim3(NW * 64), 0,
+                     stream, g);
+  EJ_LAUNCH_CHECK();
+  return EJ_OK;
+}
+
+template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
+int launch_wgrad_as(GroupedArgs g, hipStream_t stream) {
   g.row_blocks = static_cast<uint32_t>(ceil_div(g.m, BM));
   g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, BN));
   dim3 grid;
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks * g.n_groups,
                       WR * WC * 64, &grid));
-  hipLaunchKernelGGL((grouped_wgrad_kernel<Op, BM, BN, WR, WC, DIRECT, NS>), grid,
+  hipLaunchKernelGGL((grouped_wgrad_kernel<Op, BM, BN, WR, WC, DIRECT, NS, GATHER>), grid,
                      dim3(WR * WC * 64), 0, stream, g);
   EJ_LAUNCH_CHECK();
   return EJ_OK;
 }
 
-template <class Op, bool BKC>
-int pick_rows(const GroupedRows &r, hipStream_t stream) {
-  if (!r.direct) return launch_rows<Op, 128, 128, 2, 2, BKC, false, 2>(r.g, stream);
-  return launch_rows<Op, 128, 128, 2, 2, BKC, true, 2>(r.g, stream);
+template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS>
+int launch_wgrad(const GroupedArgs &g, hipStream_t stream) {
+  if (g.a_rows) return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 1>(g, stream);
+  if (g.b_rows) return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 2>(g, stream);
+  return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 0>(g, stream);
 }
 
+// Tiles of a rows product: full row blocks and, on average, half of one for
+// each group.
+inline double expected_tiles(const GroupedArgs &g, int bm, int bn, int64_t groups) {
+  return (static_cast<double>(g.slots) / bm + 0.5 * groups) * ceil_div(g.n, bn);
+}
+
+// The choice goes by the mean rows of a group (all that the host knows of the
+// sizes).  Measured on bf16, 16 groups, k = 2048, n = 2048 (us):
+//   rows/group   skinny 16  64 x 64   64 x 128  128 x 128
+//        2 (E=8)   6.5/8.0   9.6       11.4      17.9       k = n = 1024, [n][k]/[k][n]
+//       16 (E=8)  15.2/19.5 16.5       19.5      29
+//       32 (E=8)  25.9      17.2       20.2      34
+//       50        70                   38        39
+//      100                             42        48
+//      200                             62        52
+template <class Op, bool BKC>
+int pick_rows(const GroupedRows &r, hipStream_t stream) {
+  const GroupedArgs &g = r.g;
+  // smaller tiles hide the latency of the unaligned loads behind more waves:
+  // 3022 x 771 x 1283 in 12 groups 47 us, 59 with 128 x 128
+  if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
+  const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
+  const double rows = static_cast<double>(g.slots) / groups;
+  // columns of a skinny block: 32, or what fills 128 bytes of a [k][n] row
+  constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
+  if (rows <= (BKC ? 16 : 8)) return launch_skinny<Op, 1, kSkinny, 4, BKC, 2>(g, stream);
+  if constexpr (kElem<Op> == 4) {
+    // bound by the fp32 matrix instructions at any tile: the finest spreads
+    // best (4096 x 1024 x 2048 in 8 groups 164 us, 212 with 128 x 128; equal
+    // within 2% at 16384 x 2048 x 2048)
+    return launch_rows<Op, 64, 64, 2, 2, BKC, true, 0>(g, stream);
+  } else {
+    if (rows <= 48) return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
+    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, true, 3>(g, stream);
+    // rounds of 256 workgroups at a time, against a fifth less time for a
+    // round of 512 quarter-size ones (two to a CU, which even out)
+    const double big = std::ceil(expected_tiles(g, 256, 256, groups) / 256);
+    const double small = expected_tiles(g, 128, 128, groups) / 512;
+    if (big <= 0.8 * (small > 1 ? small : 1))
+      return launch_rows<Op, 256, 256, 2, 4, BKC, true, 0>(g, stream);
+    return launch_rows<Op, 128, 128, 2, 2, BKC, true, 2>(g, stream);
+  }
+}
+
+// The largest tile that leaves a workgroup for every CU.  Measured (us) on
+// 16384 rows, 16 groups, 2048 x 4096 bf16: 256 x 256 343, 128 x 128 400; fp32
+// 4096 rows, 8 groups, 1024 x 2048: 128 x 128 199, 64 x 64 210; 1200 rows, 5
+// groups, 320 x 520: 30 and 12.
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
-  if (!direct) return launch_wgrad<Op, 128, 128, 2, 2, false, 2>(g, stream);
-  return launch_wgrad<Op, 128, 128, 2, 2, true, 2>(g, stream);
+  if (!direct) return launch_wgrad<Op, 64, 64, 2, 2, false, 2>(g, stream);
+  auto tiles = [&](int b) { return ceil_div(g.m, b) * ceil_div(g.n, b) * g.n_groups; };
+  if constexpr (kElem<Op> == 2) {
+    if (tiles(256) >= 256) return launch_wgrad<Op, 256, 256, 2, 4, true, 0>(g, stream);
+  }
+  if (tiles(128) >= 256) return launch_wgrad<Op, 128, 128, 2, 2, true, 0>(g, stream);
+  return launch_wgrad<Op, 64, 64, 2, 2, true, 0>(g, stream);
 }
 
 }  // namespace ej

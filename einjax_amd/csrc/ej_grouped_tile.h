@@ -4,6 +4,8 @@
 
 #include "ej_grouped.h"
 
+#include <type_traits>
+
 namespace ej {
 
 template <int N>
@@ -15,7 +17,13 @@ __device__ inline void wait_vm() {
 // loads each were issued after it (at most NS - 2).
 template <int NS, int LPS>
 __device__ inline void wait_oldest(int later) {
-  static_assert(NS >= 2 && NS <= 4 && (NS - 2) * LPS < 64, "ring depth");
+  static_assert(NS >= 2 && NS <= 6 && (NS - 2) * LPS < 64, "ring depth");
+  if constexpr (NS >= 6) {
+    if (later >= 4) { wait_vm<4 * LPS>(); return; }
+  }
+  if constexpr (NS >= 5) {
+    if (later >= 3) { wait_vm<3 * LPS>(); return; }
+  }
   if constexpr (NS >= 4) {
     if (later >= 2) { wait_vm<2 * LPS>(); return; }
   }
@@ -44,32 +52,110 @@ struct TileShape {
   static constexpr int FM = WM / 16, FN = WN / 16;
   using TA = Tile<Op, BM, AKC>;
   using TB = Tile<Op, BN, BKC>;
+  using FA = Fragments<Op, TA, AKC, FM>;
+  using FB = Fragments<Op, TB, BKC, FN>;
   using LA = Loader<Op, BM, AKC, kWaves, DIRECT>;
   using LB = Loader<Op, BN, BKC, kWaves, DIRECT>;
   static constexpr int kSlot = TA::kBytes + TB::kBytes;
-  static constexpr int kLds = NS * kSlot;
+  static constexpr int kLds = (NS == 0 ? 2 : NS) * kSlot;
   static constexpr int kLoads = LA::kLoads + LB::kLoads;
 };
 
-// acc[i][j] += A fragment i times B fragment j over the stage at LDS address
-// `slot`.  The B fragment gives the accumulator's register rows, so a lane
+// acc[i][j] += A fragment i times B fragment j over the stage `slot` bytes
+// into the ring.  The B fragment gives the accumulator's register rows, so a lane
 // ends with four consecutive columns of one row of the result.
 template <class Op, class S>
-__device__ inline void stage_mma(typename Op::acc (&acc)[S::FM][S::FN], uint32_t slot, int row0,
-                                 int col0, int lane) {
+__device__ inline void stage_mma(typename Op::acc (&acc)[S::FM][S::FN], const typename S::FA &fa,
+                                 const typename S::FB &fb, uint32_t slot) {
 #pragma unroll
   for (int slab = 0; slab < 2; ++slab) {
     i32v4_t a[S::FM], b[S::FN];
 #pragma unroll
-    for (int i = 0; i < S::FM; ++i) a[i] = S::TA::frag(slot, row0 + i * 16, slab, lane);
+    for (int i = 0; i < S::FM; ++i) a[i] = fa.read(slot, i, slab);
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j)
-      b[j] = S::TB::frag(slot + S::TA::kBytes, col0 + j * 16, slab, lane);
+    for (int j = 0; j < S::FN; ++j) b[j] = fb.read(slot, j, slab);
 #pragma unroll
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
       for (int j = 0; j < S::FN; ++j) mma<Op>(acc[i][j], b[j], a[i]);
   }
+}
+
+// The same with the fragments of one 64-byte slab read while the matrix
+// instructions of the slab before run, so that neither waits for the other:
+//   slab 0 of stage st:  read slab 1's fragments
+//   every wave has read stage st and stage st + 1 has landed: one barrier;
+//   stage st + 2 is loaded into the slot of stage st
+//   slab 1 of stage st:  read slab 0's fragments of stage st + 1
+// Two slots suffice: a stage's loads have a whole stage of matrix
+// instructions to land.
+template <class Op, class S, class Load>
+__device__ inline void run_pipelined(typename Op::acc (&acc)[S::FM][S::FN], unsigned char *ring,
+                                     int stages, const typename S::FA &pa,
+                                     const typename S::FB &pb, Load load_stage) {
+  i32v4_t fa[2][S::FM], fb[2][S::FN];
+  // fragment r of the FN + FM of a slab
+  auto read = [&](int f, uint32_t slot, int slab, int r) {
+    if (r < S::FN) fb[f][r] = pb.read(slot, r, slab);
+    else fa[f][r - S::FN] = pa.read(slot, r - S::FN, slab);
+  };
+  constexpr int kFrags = S::FN + S::FM;
+  auto multiply = [&](int f) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) mma<Op>(acc[i][j], fb[f][j], fa[f][i]);
+  };
+  // matrix instructions between two LDS reads (and loads) of a slab
+  constexpr int kReads = S::FM * S::TA::kReads + S::FN * S::TB::kReads;
+  constexpr int kMma = S::FM * S::FN * (kElem<Op> == 4 ? 4 : 1);
+  auto interleave = [&] {
+    constexpr int kEach = kMma / kReads > 0 ? kMma / kReads : 1;
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+    }
+  };
+  // kLoad: 0 none, 1 a whole stage, 2 perhaps the last one
+  auto step = [&](int st, auto kLoad) {
+    constexpr int load = decltype(kLoad)::value;
+    const uint32_t cur = (st & 1) * S::kSlot, next = (~st & 1) * S::kSlot;
+#pragma unroll
+    for (int r = 0; r < kFrags; ++r) read(1, cur, 1, r);
+    multiply(0);
+    interleave();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < kFrags || r < S::kLoads; ++r) {
+      if (load > 0 && r < S::kLoads)
+        load_stage(r, st + 2, ring + (st & 1) * S::kSlot, load == 2);
+      if (r < kFrags) read(0, next, 0, r);
+    }
+    multiply(1);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (stages == 0) return;
+#pragma unroll
+  for (int v = 0; v < S::kLoads; ++v) load_stage(v, 0, ring, true);
+  if (stages > 1)
+#pragma unroll
+    for (int v = 0; v < S::kLoads; ++v) load_stage(v, 1, ring + S::kSlot, true);
+  if (stages > 1) wait_vm<S::kLoads>();
+  else wait_vm<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < kFrags; ++r) read(0, 0, 0, r);
+  int st = 0;
+  for (; st + 3 < stages; ++st) step(st, std::integral_constant<int, 1>());
+  for (; st + 2 < stages; ++st) step(st, std::integral_constant<int, 2>());
+  // the last read of the last stage takes what the other slot holds, unused
+  for (; st < stages; ++st) step(st, std::integral_constant<int, 0>());
 }
 
 // The ring: load_stage(st, slot pointer) starts the loads of stage st,
@@ -79,10 +165,20 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
                                   int stages, int row0, int col0, int lane, Load load_stage,
                                   Store store_stage) {
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8 *)ring));
-  if constexpr (DIRECT) {
+  typename S::FA fa;
+  typename S::FB fb;
+  fa.init(base, row0, lane);
+  fb.init(base + S::TA::kBytes, col0, lane);
+  auto load_all = [&](int st, unsigned char *slot) {
+#pragma unroll
+    for (int v = 0; v < S::kLoads; ++v) load_stage(v, st, slot, true);
+  };
+  if constexpr (DIRECT && NS == 0) {
+    run_pipelined<Op, S>(acc, ring, stages, fa, fb, load_stage);
+  } else if constexpr (DIRECT) {
     int put = 0, get = 0;
     for (int st = 0; st < NS - 1 && st < stages; ++st) {
-      load_stage(st, ring + put * S::kSlot);
+      load_all(st, ring + put * S::kSlot);
       put = put + 1 == NS ? 0 : put + 1;
     }
     for (int st = 0; st < stages; ++st) {
@@ -91,21 +187,21 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       if (st + NS - 1 < stages) {
-        load_stage(st + NS - 1, ring + put * S::kSlot);
+        load_all(st + NS - 1, ring + put * S::kSlot);
         put = put + 1 == NS ? 0 : put + 1;
       }
-      stage_mma<Op, S>(acc, base + get * S::kSlot, row0, col0, lane);
+      stage_mma<Op, S>(acc, fa, fb, get * S::kSlot);
       get = get + 1 == NS ? 0 : get + 1;
     }
   } else {
     if (stages > 0) {
-      load_stage(0, ring);
+      load_all(0, ring);
       store_stage(ring);
     }
     for (int st = 0; st < stages; ++st) {
       __syncthreads();
-      if (st + 1 < stages) load_stage(st + 1, ring);
-      stage_mma<Op, S>(acc, base + (st & 1) * S::kSlot, row0, col0, lane);
+      if (st + 1 < stages) load_all(st + 1, ring);
+      stage_mma<Op, S>(acc, fa, fb, (st & 1) * S::kSlot);
       if (st + 1 < stages) store_stage(ring + ((st + 1) & 1) * S::kSlot);
     }
   }
@@ -158,10 +254,12 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
     for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
   run_stages<Op, S, DIRECT, NS>(
       acc, ring, (g.k + kStep<Op> - 1) / kStep<Op>, row0, col0, lane,
-      [&](int st, unsigned char *slot) {
+      [&](int v, int st, unsigned char *slot, bool part) {
         const int left = g.k - st * kStep<Op>;
-        la.load(slot, wave, left, kRowB);
-        lb.load(slot + S::TA::kBytes, wave, left, b_step);
+        if (v < S::LA::kLoads)
+          la.load(v, slot, wave, left, kRowB, part);
+        else
+          lb.load(v - S::LA::kLoads, slot + S::TA::kBytes, wave, left, b_step, part);
       },
       [&](unsigned char *slot) {
         la.store(slot, wave, lane);
@@ -195,8 +293,9 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
 
 // D_e block: rows i of P's columns, columns j of Q's, over the slots of group
 // e.  The bound row_blocks x col_blocks covers one group's D; the grid holds
-// n_groups of them, and a group without slots writes zeros.
-template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS>
+// n_groups of them, and a group without slots writes zeros.  GATHER: 1 if P's
+// rows go through an index, 2 if Q's do.
+template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using S = TileShape<Op, BM, BN, WR, WC, false, false, DIRECT, NS>;
@@ -215,15 +314,17 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 
   typename S::LA la;
   typename S::LB lb;
-  la.init_m(wave, lane, g.a, 0, rb * BM, g.m);
-  lb.init_m(wave, lane, g.b, 0, cb * BN, g.n);
-  int acol[S::LA::kLoads], bcol[S::LB::kLoads];
-#pragma unroll
-  for (int v = 0; v < S::LA::kLoads; ++v)
-    acol[v] = static_cast<int>((la.src[v] - g.a) / kElem<Op>);
-#pragma unroll
-  for (int v = 0; v < S::LB::kLoads; ++v)
-    bcol[v] = static_cast<int>((lb.src[v] - g.b) / kElem<Op>);
+  la.init_m(wave, lane, g.a + (GATHER == 1 ? 0 : lo * g.lda * kElem<Op>), g.lda, rb * BM, g.m);
+  lb.init_m(wave, lane, g.b + (GATHER == 2 ? 0 : lo * g.ldb * kElem<Op>), g.ldb, cb * BN, g.n);
+  // the gathered operand's rows of a stage, lane by lane, read a stage ahead
+  const int32_t *rows = GATHER == 1 ? g.a_rows : g.b_rows;
+  const int64_t n_rows = GATHER == 1 ? g.n_a : g.n_b;
+  auto rows_of = [&](int st) {
+    const int64_t s = lo + static_cast<int64_t>(st) * kStep<Op> + lane;
+    return static_cast<int>(slot_row(rows, n_rows, static_cast<int>(s < hi ? s : hi - 1)));
+  };
+  int row_now = 0, row_next = 0;
+  if (GATHER && hi > lo) row_next = rows_of(0);
 
   typename Op::acc acc[S::FM][S::FN];
 #pragma unroll
@@ -232,12 +333,20 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
     for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
   run_stages<Op, S, DIRECT, NS>(
       acc, ring, (hi - lo + kStep<Op> - 1) / kStep<Op>, row0, col0, lane,
-      [&](int st, unsigned char *slot) {
-        const int s0 = lo + st * kStep<Op>;
-        la.seek_slots(g.a, g.lda, g.a_rows, g.n_a, s0, hi, acol);
-        lb.seek_slots(g.b, g.ldb, g.b_rows, g.n_b, s0, hi, bcol);
-        la.load(slot, wave, hi - s0, 0);
-        lb.load(slot + S::TA::kBytes, wave, hi - s0, 0);
+      [&](int v, int st, unsigned char *slot, bool part) {
+        const int left = hi - lo - st * kStep<Op>;
+        if (GATHER && v == 0) {
+          row_now = row_next;
+          row_next = rows_of(st + 1);
+        }
+        if (v < S::LA::kLoads) {
+          if (GATHER == 1) la.seek(v, g.a, g.lda, row_now);
+          la.load(v, slot, wave, left, kStep<Op> * g.lda * kElem<Op>, part);
+        } else {
+          const int u = v - S::LA::kLoads;
+          if (GATHER == 2) lb.seek(u, g.b, g.ldb, row_now);
+          lb.load(u, slot + S::TA::kBytes, wave, left, kStep<Op> * g.ldb * kElem<Op>, part);
+        }
       },
       [&](unsigned char *slot) {
         la.store(slot, wave, lane);
@@ -257,6 +366,135 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
                           static_cast<float>(acc[i][j][2]), static_cast<float>(acc[i][j][3])};
       put4(g.c, g.out, group * g.c_group + static_cast<int64_t>(row) * g.ldc, col, g.n, vec, v);
     }
+  }
+#endif
+}
+
+// Few rows for each group: the time is that of reading the weights once.  A
+// workgroup takes 16 FM rows by BN columns; its waves split k stage by stage
+// (so that together they read long pieces of each weight row), each on a ring
+// of its own without barriers, and add up their parts in LDS at the end, in
+// the order of the waves.
+template <class Op, int FM_, int BN, int NW, bool BKC, int NS>
+struct SkinnyShape {
+  static constexpr int FM = FM_, BM = 16 * FM, FN = BN / 16;
+  using TA = Tile<Op, BM, true>;
+  using TB = Tile<Op, BN, BKC>;
+  using FA = Fragments<Op, TA, true, FM>;
+  using FB = Fragments<Op, TB, BKC, FN>;
+  using LA = Loader<Op, BM, true, 1, true>;
+  using LB = Loader<Op, BN, BKC, 1, true>;
+  static constexpr int kSlot = TA::kBytes + TB::kBytes;
+  static constexpr int kLoads = LA::kLoads + LB::kLoads;
+  static constexpr int kRing = NS * kSlot;
+  static constexpr int kPart = BM * BN * 4;  // bytes of a wave's sums
+  static constexpr int kLds = NW * (kRing > kPart ? kRing : kPart);
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+};
+
+template <class Op, int FM, int BN, int NW, bool BKC, int NS>
+__global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using S = SkinnyShape<Op, FM, BN, NW, BKC, NS>;
+  __shared__ __align__(1024) unsigned char lds[S::kLds];
+  const uint32_t grid = g.row_blocks * g.col_blocks;
+  if (blockIdx.x >= grid) {
+    zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
+    return;
+  }
+  const uint32_t rbs = live_row_blocks(g, S::BM), live = rbs * g.col_blocks;
+  if (blockIdx.x >= live) return;
+  // the row blocks of one group and column block follow each other: they read
+  // the same weights
+  int rb, cb;
+  band_pos(xcd_logical_block(live), rbs, g.col_blocks, 4, &rb, &cb);
+  const RowBlock r = find_row_block(g, S::BM, rb);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = cb * BN;
+  unsigned char *ring = lds + wave * S::kRing;
+
+  typename S::LA la;
+  typename S::LB lb;
+  const int stages = (g.k + kStep<Op> - 1) / kStep<Op>;
+  const int mine = stages > wave ? (stages - wave + NW - 1) / NW : 0;
+  const int64_t k0 = static_cast<int64_t>(wave) * kStep<Op>;
+  la.init_k(0, lane, [&](int i) {
+    const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
+    return g.a + (slot_row(g.a_rows, g.n_a, s) * g.lda + k0) * kElem<Op>;
+  });
+  const char *bg = g.b + r.group * g.b_group * kElem<Op>;
+  int64_t b_step;
+  if constexpr (BKC) {
+    lb.init_k(0, lane, [&](int i) {
+      const int n = n0 + i < g.n ? n0 + i : g.n - 1;
+      return bg + (n * g.ldb + k0) * kElem<Op>;
+    });
+    b_step = kRowB;
+  } else {
+    lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
+    b_step = kStep<Op> * g.ldb * kElem<Op>;
+  }
+  auto load = [&](int i) {
+    unsigned char *slot = ring + i % NS * S::kSlot;
+    const int left = g.k - (wave + i * NW) * kStep<Op>;
+#pragma unroll
+    for (int v = 0; v < S::LA::kLoads; ++v) la.load(v, slot, 0, left, NW * kRowB, true);
+#pragma unroll
+    for (int v = 0; v < S::LB::kLoads; ++v)
+      lb.load(v, slot + S::TA::kBytes, 0, left, NW * b_step, true);
+  };
+  typename S::FA fa;
+  typename S::FB fb;
+  fa.init(lds_address(ring), 0, lane);
+  fb.init(lds_address(ring) + S::TA::kBytes, 0, lane);
+  typename Op::acc acc[FM][S::FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
+  for (int i = 0; i < NS - 1 && i < mine; ++i) load(i);
+  for (int i = 0; i < mine; ++i) {
+    const int later = mine - 1 - i;
+    // the slot that is loaded next was read a stage ago: those reads are done
+    // once their matrix instructions have been issued
+    if (i + NS - 1 < mine) load(i + NS - 1);
+    wait_oldest<NS + 1, S::kLoads>(later < NS - 1 ? later : NS - 1);
+    stage_mma<Op, S>(acc, fa, fb, i % NS * S::kSlot);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+
+  // the waves' sums, added in their order
+  __syncthreads();
+  float *part = reinterpret_cast<float *>(lds);
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j)
+      *reinterpret_cast<typename Op::acc *>(part + wave * (S::BM * BN) +
+                                            (i * 16 + (lane & 15)) * BN + j * 16 +
+                                            (lane >> 4) * 4) = acc[i][j];
+  __syncthreads();
+  const bool vec = vec_rows(g);
+  for (int q = tid; q < S::BM * BN / 4; q += NW * 64) {
+    const int row = q / (BN / 4), col = q % (BN / 4) * 4;
+    const int s = r.lo + row;
+    if (s >= r.hi || n0 + col >= g.n) continue;
+    typename Op::acc sum = *reinterpret_cast<typename Op::acc *>(part + q * 4);
+#pragma unroll
+    for (int w = 1; w < NW; ++w)
+      sum += *reinterpret_cast<typename Op::acc *>(part + w * (S::BM * BN) + q * 4);
+    float v[4];
+    float as = 1.f;
+    if constexpr (Op::kInt) as = g.a_scale[slot_row(g.a_rows, g.n_a, s)];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      v[c] = static_cast<float>(sum[c]);
+      const int n = n0 + col + c;
+      if constexpr (Op::kInt)
+        v[c] *= as * g.b_scale[static_cast<int64_t>(r.group) * g.n + (n < g.n ? n : g.n - 1)];
+    }
+    put4(g.c, g.out, s * g.ldc, n0 + col, g.n, vec, v);
   }
 #endif
 }

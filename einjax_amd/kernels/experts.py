@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from math import prod
 
 import torch
 
@@ -64,29 +65,34 @@ def on_gpu(t, what: str) -> torch.Tensor:
 
 
 def _same_device(ref: torch.Tensor, **tensors) -> None:
+    dev = ref.get_device()
     for name, t in tensors.items():
-        if t is not None and on_gpu(t, name).device != ref.device:
+        if t is not None and on_gpu(t, name).get_device() != dev:
             raise ValueError(f"{name} is on {t.device}, expected {ref.device}")
 
 
 def _value_code(t: torch.Tensor, what: str) -> int:
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
 
 
 def _index(t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
-    return t.to(torch.int32).contiguous()
+    if t.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype is not torch.int32:
+        if t.dtype is not torch.int64:
+            raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t [n, m] with unit stride along its rows and rows that do not overlap
     (itself if it is so already)."""
+    if t.is_contiguous():
+        return t
     n, m = t.shape
     if (m <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= m):
         return t
@@ -97,27 +103,45 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+_entry_points: dict = {}
+
+
 def _call(ref: torch.Tensor, name: str, *args) -> None:
-    # launches go to the operands' device, on that device's current stream
-    if ref.device.index != _device.current_device_index():
-        with torch.cuda.device(ref.device):
-            check(getattr(_lib.load(), name)(*args, _device.stream_ptr()), name)
+    """The library's `name` on the device of ref, on that device's current
+    stream of torch.  Pointers are plain integers: these calls last a few
+    microseconds, of which building ctypes objects would be a good part."""
+    fn = _entry_points.get(name)
+    if fn is None:
+        fn = _entry_points[name] = getattr(_lib.load(), name)
+    dev = ref.get_device()
+    if dev == _device.current_device_index():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        check(getattr(_lib.load(), name)(*args, _device.stream_ptr()), name)
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        check(status, name)
 
 
-def _route_workspace(ref: torch.Tensor, n_tokens: int, n_experts: int) -> torch.Tensor:
+def _route_workspace(ref: torch.Tensor, n_tokens: int, n_experts: int):
+    """(workspace tensor or None, its size)."""
     nbytes = ctypes.c_size_t()
     check(_lib.load().ej_expert_route_workspace_size(n_tokens, n_experts, ctypes.byref(nbytes)),
           "ej_expert_route_workspace_size")
-    return _device.workspace(nbytes.value, ref.device)
+    n = nbytes.value
+    return (_device.workspace(n, ref.device) if n else None), n
 
 
 def _empty_routing(ref: torch.Tensor, n_tokens: int, k: int, n_experts: int):
-    """offsets, rows and slots in one allocation."""
+    """offsets, rows, slots [T, k] and a spare int32 [T, k] in one allocation."""
     n = n_tokens * k
-    buf = torch.empty(2 * n + n_experts + 1, dtype=torch.int32, device=ref.device)
-    return buf[2 * n:], buf[:n], buf[n:2 * n].view(n_tokens, k)
+    buf = torch.empty(3 * n + n_experts + 1, dtype=torch.int32, device=ref.device)
+    rows, slots, spare, offsets = buf.split((n, n, n, n_experts + 1))
+    return offsets, rows, slots.view(n_tokens, k), spare.view(n_tokens, k)
 
 
 def route(logits: torch.Tensor, k: int, renormalize: bool) -> ExpertRouting:
@@ -130,14 +154,13 @@ def route(logits: torch.Tensor, k: int, renormalize: bool) -> ExpertRouting:
     if not 1 <= k <= max(E, 1):
         raise ValueError(f"k = {k}, expected 1 to the number of experts, {E}")
     logits = rows_of(logits)
-    ws = _route_workspace(logits, T, E)
+    ws, ws_bytes = _route_workspace(logits, T, E)
     weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
-    experts = torch.empty((T, k), dtype=torch.int32, device=logits.device)
-    offsets, rows, slots = _empty_routing(logits, T, k, E)
-    p = _device.ptr
+    offsets, rows, slots, experts = _empty_routing(logits, T, k, E)
+    p = _ptr
     _call(logits, "ej_expert_route", p(logits), code, T, E, max(_row_stride(logits), E), k,
-          int(bool(renormalize)), p(weights), p(experts), p(offsets), p(rows), p(slots), p(ws),
-          ws.numel())
+          1 if renormalize else 0, p(weights), p(experts), p(offsets), p(rows), p(slots), p(ws),
+          ws_bytes)
     return ExpertRouting(weights, experts, offsets, rows, slots)
 
 
@@ -160,11 +183,11 @@ def group_by_expert(experts: torch.Tensor, n_experts: int,
     if experts.dtype == torch.int64:  # no wrapping of values past 32 bits into the range
         experts = experts.clamp(-1, E)
     experts = _index(experts, (T, k), "experts")
-    ws = _route_workspace(experts, T, E)
-    offsets, rows, slots = _empty_routing(experts, T, k, E)
-    p = _device.ptr
+    ws, ws_bytes = _route_workspace(experts, T, E)
+    offsets, rows, slots, _ = _empty_routing(experts, T, k, E)
+    p = _ptr
     _call(experts, "ej_expert_group", p(experts), T, k, E, p(offsets), p(rows), p(slots), p(ws),
-          ws.numel())
+          ws_bytes)
     return ExpertRouting(weights, experts, offsets, rows, slots)
 
 
@@ -181,20 +204,23 @@ def route_vjp(logits: torch.Tensor, experts: torch.Tensor, grad_weights: torch.T
     grad_weights = grad_weights.to(torch.float32).contiguous()
     logits = rows_of(logits)
     out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    p = _device.ptr
+    p = _ptr
     _call(logits, "ej_expert_route_vjp", p(logits), code, T, E, max(_row_stride(logits), E), k,
-          int(bool(renormalize)), p(experts), p(grad_weights), p(out))
+          1 if renormalize else 0, p(experts), p(grad_weights), p(out))
     return out
 
 
-def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None) -> torch.Tensor:
-    """Sum over j of weights[t, j] y[slots[t, j]]; no weights: 1."""
+def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor | None,
+            out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Sum over j of weights[t, j] y[slots[t, j]]; no weights: 1.  In y's
+    dtype, or from float32 in out_dtype."""
     y = rows_of(y)
     T, k = slots.shape
-    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
-    p = _device.ptr
+    out_dtype = out_dtype or y.dtype
+    out = torch.empty((T, y.shape[1]), dtype=out_dtype, device=y.device)
+    p = _ptr
     _call(y, "ej_expert_combine", p(y), _value_code(y, "y"), y.shape[0], _row_stride(y),
-          p(weights), p(slots), T, k, y.shape[1], p(out))
+          p(weights), p(slots), T, k, y.shape[1], p(out), _DTYPES[out_dtype])
     return out
 
 
@@ -203,7 +229,7 @@ def combine_vjp(y, slots, offsets, weights, grad, need_y: bool, need_weights: bo
     T, k = slots.shape
     gy = torch.empty((y.shape[0], y.shape[1]), dtype=y.dtype, device=y.device) if need_y else None
     gw = torch.empty((T, k), dtype=torch.float32, device=y.device) if need_weights else None
-    p = _device.ptr
+    p = _ptr
     _call(y, "ej_expert_combine_vjp", p(y), _value_code(y, "y"), y.shape[0], _row_stride(y),
           p(weights), p(slots), p(offsets), offsets.shape[0] - 1, T, k, y.shape[1], p(grad),
           _row_stride(grad), p(gy), p(gw))
@@ -222,16 +248,14 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     code = _value_code(x, "x")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
-    n = x.shape[-1]
-    m = 1
-    for s in x.shape[:-1]:
-        m *= s
-    flat = rows_of(x.reshape(m, n))
-    q = torch.empty((m, n), dtype=torch.int8, device=x.device)
-    scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    p = _device.ptr
+    lead, n = x.shape[:-1], x.shape[-1]
+    m = prod(lead)
+    flat = rows_of(x if x.dim() == 2 else x.reshape(m, n))
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    p = _ptr
     _call(x, "ej_quantize_rows", p(flat), code, m, max(_row_stride(flat), n), n, p(q), p(scale))
-    return q.view(x.shape), scale.view(x.shape[:-1])
+    return q, scale
 
 
 # ---------------------------------------------------------------------------
@@ -269,7 +293,7 @@ def groups_of(x: torch.Tensor, n_groups: int, groups, gather: bool) -> Groups:
         if groups.slots.numel() != n_slots:
             raise ValueError(f"the routing has {groups.slots.numel()} pairs and {n_slots} slots")
         return Groups(offsets, _index(groups.rows, (n_slots,), "rows"),
-                      _index(groups.slots, tuple(groups.slots.shape), "slots"), n_slots)
+                      _index(groups.slots, groups.slots.shape, "slots"), n_slots)
     if gather:
         raise ValueError("gather=True needs an ExpertRouting: offsets alone do not say which "
                          "rows the slots take")
@@ -281,6 +305,8 @@ def weight_order(w: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """(w, order, group stride, row stride) of w [E, k, n] as it lies in
     memory; a copy if neither k nor n is contiguous."""
     E, k, n = w.shape
+    if w.is_contiguous():
+        return w, _lib.EJ_W_KN, k * n, n
     for _ in range(2):
         for order, rows, cols, rs, cs in ((_lib.EJ_W_KN, k, n, w.stride(1), w.stride(2)),
                                           (_lib.EJ_W_NK, n, k, w.stride(2), w.stride(1))):
@@ -306,7 +332,7 @@ def grouped_product(x: torch.Tensor, w: torch.Tensor, g: Groups, out_dtype) -> t
     E, k, n = w.shape
     out = torch.empty((g.n_slots, n), dtype=out_dtype, device=x.device)
     d = _desc(x, _value_code(x, "x"), _DTYPES[out_dtype], order, E, k, n, g.n_slots, gs, rs, n)
-    p = _device.ptr
+    p = _ptr
     _call(x, "ej_grouped_gemm", ctypes.byref(d), p(x), p(g.rows), p(g.offsets), p(w), None, None,
           p(out))
     return out
@@ -326,7 +352,7 @@ def grouped_weight_gradient(x: torch.Tensor, w: torch.Tensor, g: Groups,
         rs = k
     code = _value_code(x, "x")
     d = _desc(x, code, code, order, E, k, n, g.n_slots, k * n, rs, max(_row_stride(grad), n))
-    p = _device.ptr
+    p = _ptr
     _call(x, "ej_grouped_gemm_dw", ctypes.byref(d), p(x), p(g.rows), p(g.offsets), p(grad), p(gw))
     return gw
 
@@ -364,7 +390,7 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
     E, n, k = w.shape
     if q.shape[1] != k:
         raise ValueError(f"q has rows of {q.shape[1]}, w of {k}")
-    if tuple(q_scale.shape) != (q.shape[0],) or tuple(w_scale.shape) != (E, n):
+    if q_scale.shape != (q.shape[0],) or w_scale.shape != (E, n):
         raise ValueError(f"scales have shapes {tuple(q_scale.shape)} and {tuple(w_scale.shape)}, "
                          f"expected {(q.shape[0],)} and {(E, n)}")
     if groups is None:
@@ -374,14 +400,15 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
     else:
         g = groups_of(q, E, groups, gather)
     q = rows_of(q)
-    if (k > 1 and w.stride(2) != 1) or (n > 1 and w.stride(1) < k) or \
-            (E > 1 and w.stride(0) < n * (w.stride(1) if n > 1 else k)):
+    if not w.is_contiguous() and (
+            (k > 1 and w.stride(2) != 1) or (n > 1 and w.stride(1) < k) or
+            (E > 1 and w.stride(0) < n * (w.stride(1) if n > 1 else k))):
         w = w.contiguous()
     rs = w.stride(1) if n > 1 else max(k, 1)
     gs = w.stride(0) if E > 1 else n * rs
     out = torch.empty((g.n_slots, n), dtype=out_dtype, device=q.device)
     d = _desc(q, _lib.EJ_I8, _DTYPES[out_dtype], _lib.EJ_W_NK, E, k, n, g.n_slots, gs, rs, n)
-    p = _device.ptr
+    p = _ptr
     q_scale, w_scale = q_scale.contiguous(), w_scale.contiguous()
     _call(q, "ej_grouped_gemm", ctypes.byref(d), p(q), p(g.rows), p(g.offsets), p(w), p(q_scale),
           p(w_scale), p(out))

@@ -685,10 +685,11 @@ int ej_expert_route_vjp(const void *logits, int32_t dtype, int64_t n_tokens, int
                         const float *grad_weights, void *grad_logits, ej_stream_t stream);
 
 /* out[t] = sum over j of weights[t, j] y[slots[t, j]] (weights NULL: 1), pairs
- * without a slot left out; out [n_tokens, n] contiguous. */
+ * without a slot left out; out [n_tokens, n] contiguous, of out_dtype: y's
+ * dtype, or with EJ_F32 values any. */
 int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
                       const float *weights, const int32_t *slots, int64_t n_tokens, int32_t k,
-                      int32_t n, void *out, ej_stream_t stream);
+                      int32_t n, void *out, int32_t out_dtype, ej_stream_t stream);
 
 /* Its gradients: grad_y [n_slots, n] contiguous, zero in the rows from
  * offsets[n_groups] on, and grad_weights [n_tokens, k]; either may be NULL.

@@ -95,15 +95,19 @@ def test_route_argument_checks():
 
 def test_combine_and_quantize_refusals():
     lib = _lib.load()
-    assert lib.ej_expert_combine(FAKE, _lib.EJ_I32, 4, 8, None, FAKE, 2, 2, 8, FAKE, None) == \
-        _lib.EJ_E_INVAL
-    assert lib.ej_expert_combine(FAKE, _lib.EJ_F32, 4, 7, None, FAKE, 2, 2, 8, FAKE, None) == \
-        _lib.EJ_E_INVAL
-    assert lib.ej_expert_combine(FAKE, _lib.EJ_F32, 4, 8, None, None, 2, 2, 8, FAKE, None) == \
-        _lib.EJ_E_INVAL
-    assert lib.ej_expert_combine(FAKE, _lib.EJ_F32, 4, 8, None, FAKE, 2, 17, 8, FAKE, None) == \
-        _lib.EJ_E_UNSUPPORTED
-    assert lib.ej_expert_combine(FAKE, _lib.EJ_F32, 4, 8, None, FAKE, 0, 2, 8, FAKE, None) == 0
+    f32, bf16 = _lib.EJ_F32, _lib.EJ_BF16
+
+    def combine(dtype=f32, stride=8, slots=FAKE, t=2, k=2, out_dtype=f32):
+        return lib.ej_expert_combine(FAKE, dtype, 4, stride, None, slots, t, k, 8, FAKE, out_dtype,
+                                     None)
+
+    assert combine(dtype=_lib.EJ_I32) == _lib.EJ_E_INVAL
+    assert combine(stride=7) == _lib.EJ_E_INVAL
+    assert combine(slots=None) == _lib.EJ_E_INVAL
+    assert combine(k=17) == _lib.EJ_E_UNSUPPORTED
+    assert combine(dtype=bf16) == _lib.EJ_E_INVAL  # 16-bit values keep their dtype
+    assert combine(out_dtype=_lib.EJ_I8) == _lib.EJ_E_INVAL
+    assert combine(t=0) == 0
     assert lib.ej_expert_combine_vjp(FAKE, _lib.EJ_F32, 4, 8, None, FAKE, None, 2, 2, 2, 8, FAKE,
                                      8, FAKE, FAKE, None) == _lib.EJ_E_INVAL
     assert lib.ej_quantize_rows(FAKE, _lib.EJ_F64, 4, 8, 8, FAKE, FAKE, None) == _lib.EJ_E_INVAL
