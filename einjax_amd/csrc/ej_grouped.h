@@ -344,15 +344,30 @@ __device__ inline uint32_t lds_address(const void *p) {
   return static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8 *)p));
 }
 
-// 16 bytes at any element alignment, the first `valid` elements of them (the
-// rest zero).
+// 16 bytes from p on, at any element alignment, of which `valid` elements
+// exist (any number; the others come out zero).  Where fewer than a chunk do,
+// the last chunk of the row is loaded and shifted down: that needs rows of a
+// chunk at least (`whole`, uniform); shorter ones go element by element.
 template <class Op>
-__device__ inline i32v4_t load_chunk(const char *p, int valid) {
+__device__ inline i32v4_t load_chunk(const char *p, int valid, bool whole) {
   using E = typename Op::elem;
   constexpr int N = kChunk<Op>;
   i32v4_t v = {0, 0, 0, 0};
-  if (valid >= N) {
-    __builtin_memcpy(&v, __builtin_assume_aligned(p, alignof(E)), 16);
+  if (whole) {
+    const int past = valid < N ? N - valid : 0;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p - past * kElem<Op>, alignof(E)), 16);
+    if (__any(past > 0)) {
+      const int bits = past < N ? past * kElem<Op> * 8 : 128;
+      uint64_t w[2];
+      __builtin_memcpy(w, &v, 16);
+      const uint64_t down = bits < 64 ? w[1] >> bits : 0;
+      w[0] = bits == 0    ? w[0]
+             : bits < 64  ? w[0] >> bits | w[1] << (64 - bits)
+             : bits < 128 ? w[1] >> (bits - 64)
+                          : 0;
+      w[1] = down;
+      __builtin_memcpy(&v, w, 16);
+    }
   } else {
     E e[N] = {};
 #pragma unroll
@@ -385,7 +400,8 @@ struct Loader {
   const char *src[kLoads];  // this lane's source in the next stage
   int line;                 // K: first k element of the lane's chunk; M: its k-row in load 0
   int col[kCols];           // M: first column of the lane's chunk
-  int valid[kCols];         // M, not DIRECT: elements of the chunk inside the extent
+  int valid[kCols];         // M, not DIRECT: elements from the column to the extent
+  bool whole;               // not DIRECT: rows hold a chunk
   i32v4_t reg[DIRECT ? 1 : kLoads];
 
   // k element (K) or k-row (M) of the lane's place in load v; in K tiles the
@@ -397,7 +413,8 @@ struct Loader {
 
   // K tiles: row_at(i) is the address of output row i's first k element.
   template <class RowAt>
-  __device__ inline void init_k(int wave, int lane, RowAt row_at) {
+  __device__ inline void init_k(int wave, int lane, int k, RowAt row_at) {
+    whole = k >= kChunk<Op>;
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
       int row, chunk;
@@ -409,6 +426,7 @@ struct Loader {
   // M tiles: column col0 + i of the operand is output row i; extent `ext`.
   __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int col0,
                                 int ext) {
+    whole = ext >= kChunk<Op>;
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
       int krow, chunk;
@@ -420,7 +438,6 @@ struct Loader {
           if (c > ext - kChunk<Op>) c = ext - kChunk<Op>;
         } else {
           valid[v] = ext - c;
-          if (c >= ext) c = 0;
         }
         col[v] = c;
       }
@@ -439,8 +456,13 @@ struct Loader {
         p = line_at(v) < left ? p : reinterpret_cast<const char *>(&grouped_zeros);
       load_to_lds(p, lds_address(tile) + (v * NW + wave) * 1024);
     } else {
-      const int n = KC ? left - line_at(v) : line_at(v) < left ? valid[v % kCols] : 0;
-      reg[v] = load_chunk<Op>(src[v], n);
+      if constexpr (KC) {
+        reg[v] = load_chunk<Op>(src[v], left - line_at(v), whole);
+      } else {
+        const bool there = line_at(v) < left;
+        reg[v] = load_chunk<Op>(there ? src[v] : reinterpret_cast<const char *>(&grouped_zeros),
+                                there ? valid[v % kCols] : whole ? kChunk<Op> : 0, whole);
+      }
     }
     src[v] += step;
   }

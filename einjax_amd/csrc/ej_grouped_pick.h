@@ -74,11 +74,12 @@ inline double expected_tiles(const GroupedArgs &g, int bm, int bn, int64_t group
 template <class Op, bool BKC>
 int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
-  // smaller tiles hide the latency of the unaligned loads behind more waves:
-  // 3022 x 771 x 1283 in 12 groups 47 us, 59 with 128 x 128
-  if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
   const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
   const double rows = static_cast<double>(g.slots) / groups;
+  if (!r.direct) {
+    if (rows > 128) return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
+  }
   // columns of a skinny block: 32, or what fills 128 bytes of a [k][n] row
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
   if (rows <= (BKC ? 16 : 8)) return launch_skinny<Op, 1, kSkinny, 4, BKC, 2>(g, stream);
@@ -111,8 +112,8 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
   if constexpr (kElem<Op> == 2) {
     if (tiles(256) >= 256) return launch_wgrad<Op, 256, 256, 2, 4, true, 0>(g, stream);
   }
-  if (tiles(128) >= 256) return launch_wgrad<Op, 128, 128, 2, 2, true, 0>(g, stream);
-  return launch_wgrad<Op, 64, 64, 2, 2, true, 0>(g, stream);
+  if (tiles(128) >= 256) return launch_wgrad<Op, 128, 128, 2, 2, true, 2>(g, stream);
+  return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
 }
 
 }  // namespace ej

@@ -57,7 +57,7 @@ struct TileShape {
   using LA = Loader<Op, BM, AKC, kWaves, DIRECT>;
   using LB = Loader<Op, BN, BKC, kWaves, DIRECT>;
   static constexpr int kSlot = TA::kBytes + TB::kBytes;
-  static constexpr int kLds = (NS == 0 ? 2 : NS) * kSlot;
+  static constexpr int kLds = NS == 0 ? 3 * TA::kBytes + 2 * TB::kBytes : NS * kSlot;
   static constexpr int kLoads = LA::kLoads + LB::kLoads;
 };
 
@@ -82,80 +82,101 @@ __device__ inline void stage_mma(typename Op::acc (&acc)[S::FM][S::FN], const ty
 }
 
 // The same with the fragments of one 64-byte slab read while the matrix
-// instructions of the slab before run, so that neither waits for the other:
-//   slab 0 of stage st:  read slab 1's fragments
-//   every wave has read stage st and stage st + 1 has landed: one barrier;
-//   stage st + 2 is loaded into the slot of stage st
-//   slab 1 of stage st:  read slab 0's fragments of stage st + 1
-// Two slots suffice: a stage's loads have a whole stage of matrix
-// instructions to land.
+// instructions of the slab before run, on a ring of three stages of A and two
+// of B:
+//   slab 0 of stage st:  read slab 1's fragments; load A of stage st + 2 into
+//                        the slot of stage st - 1
+//   every wave has read stage st and stage st + 1 has landed: one barrier
+//   slab 1 of stage st:  read slab 0's fragments of stage st + 1; load B of
+//                        stage st + 2 into the slot of stage st
+// So loads are under way all the time: the L1 keeps only some hundred requests
+// in flight, and a burst of a whole stage would leave it idle in between.
+// Loads and LDS reads are spread over the matrix instructions.
 template <class Op, class S, class Load>
 __device__ inline void run_pipelined(typename Op::acc (&acc)[S::FM][S::FN], unsigned char *ring,
                                      int stages, const typename S::FA &pa,
                                      const typename S::FB &pb, Load load_stage) {
   i32v4_t fa[2][S::FM], fb[2][S::FN];
-  // fragment r of the FN + FM of a slab
-  auto read = [&](int f, uint32_t slot, int slab, int r) {
-    if (r < S::FN) fb[f][r] = pb.read(slot, r, slab);
-    else fa[f][r - S::FN] = pa.read(slot, r - S::FN, slab);
-  };
+  constexpr int kA = S::TA::kBytes, kB = S::TB::kBytes;
   constexpr int kFrags = S::FN + S::FM;
-  auto multiply = [&](int f) {
-#pragma unroll
-    for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-      for (int j = 0; j < S::FN; ++j) mma<Op>(acc[i][j], fb[f][j], fa[f][i]);
-  };
-  // matrix instructions between two LDS reads (and loads) of a slab
   constexpr int kReads = S::FM * S::TA::kReads + S::FN * S::TB::kReads;
-  constexpr int kMma = S::FM * S::FN * (kElem<Op> == 4 ? 4 : 1);
-  auto interleave = [&] {
-    constexpr int kEach = kMma / kReads > 0 ? kMma / kReads : 1;
+  // fragment r of the FN + FM of a slab
+  auto read = [&](int f, uint32_t a, uint32_t b, int slab, int r) {
+    if (r < S::FN) fb[f][r] = pb.read(b, r, slab);
+    else fa[f][r - S::FN] = pa.read(a, r - S::FN, slab);
+  };
+  // matrix instructions of fragments f, while slab `slab` of the stage at a, b
+  // is read and `n` loads are issued
+  auto slab = [&](int f, uint32_t a, uint32_t b, int slab, auto kN, auto load) {
+    constexpr int n = decltype(kN)::value, cells = S::FM * S::FN;
+    // a part for each load where it has enough matrix instructions
+    constexpr int parts = cells / n >= 8 ? n : 1;
 #pragma unroll
-    for (int r = 0; r < kReads; ++r) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-      __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+    for (int p = 0; p < parts; ++p) {
+      constexpr int kFragsOf = (kFrags + parts - 1) / parts, kLoadsOf = n / parts;
+#pragma unroll
+      for (int q = 0; q < kFragsOf || q < kLoadsOf; ++q) {
+        if (q < kLoadsOf) load(p * kLoadsOf + q);
+        const int r = p * kFrags / parts + q;
+        if (r < (p + 1) * kFrags / parts) read(1 - f, a, b, slab, r);
+      }
+#pragma unroll
+      for (int c = p * cells / parts; c < (p + 1) * cells / parts; ++c)
+        mma<Op>(acc[c / S::FN][c % S::FN], fb[f][c % S::FN], fa[f][c / S::FN]);
+      constexpr int kMma = cells * (kElem<Op> == 4 ? 4 : 1);
+      constexpr int kEach = kMma / kReads > 1 ? 2 : 1;
+#pragma unroll
+      for (int r = 0; r < kReads / parts; ++r) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+        __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // kLoad: 0 none, 1 a whole stage, 2 perhaps the last one
-  auto step = [&](int st, auto kLoad) {
-    constexpr int load = decltype(kLoad)::value;
-    const uint32_t cur = (st & 1) * S::kSlot, next = (~st & 1) * S::kSlot;
-#pragma unroll
-    for (int r = 0; r < kFrags; ++r) read(1, cur, 1, r);
-    multiply(0);
-    interleave();
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int r = 0; r < kFrags || r < S::kLoads; ++r) {
-      if (load > 0 && r < S::kLoads)
-        load_stage(r, st + 2, ring + (st & 1) * S::kSlot, load == 2);
-      if (r < kFrags) read(0, next, 0, r);
-    }
-    multiply(1);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-  };
+  using NA = std::integral_constant<int, S::LA::kLoads>;
+  using NB = std::integral_constant<int, S::LB::kLoads>;
   if (stages == 0) return;
+  // stages past the end are zeros, loaded from one cached line
+  int st = 0;
+  uint32_t a_now = 0, a_next = kA, a_put = 2 * kA, b_now = 3 * kA, b_next = 3 * kA + kB;
 #pragma unroll
-  for (int v = 0; v < S::kLoads; ++v) load_stage(v, 0, ring, true);
-  if (stages > 1)
+  for (int v = 0; v < S::LA::kLoads; ++v) load_stage(v, 0, ring + a_now, true);
 #pragma unroll
-    for (int v = 0; v < S::kLoads; ++v) load_stage(v, 1, ring + S::kSlot, true);
-  if (stages > 1) wait_vm<S::kLoads>();
-  else wait_vm<0>();
+  for (int v = 0; v < S::LB::kLoads; ++v)
+    load_stage(S::LA::kLoads + v, 0, ring + b_now - kA, true);
+#pragma unroll
+  for (int v = 0; v < S::LA::kLoads; ++v) load_stage(v, 1, ring + a_next, true);
+#pragma unroll
+  for (int v = 0; v < S::LB::kLoads; ++v)
+    load_stage(S::LA::kLoads + v, 1, ring + b_next - kA, true);
+  wait_vm<S::kLoads>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int r = 0; r < kFrags; ++r) read(0, 0, 0, r);
-  int st = 0;
-  for (; st + 3 < stages; ++st) step(st, std::integral_constant<int, 1>());
-  for (; st + 2 < stages; ++st) step(st, std::integral_constant<int, 2>());
-  // the last read of the last stage takes what the other slot holds, unused
-  for (; st < stages; ++st) step(st, std::integral_constant<int, 0>());
+  for (int r = 0; r < kFrags; ++r) read(0, a_now, b_now - kA, 0, r);
+  auto step = [&](auto kWhole) {
+    constexpr bool part = !decltype(kWhole)::value;
+    slab(0, a_now, b_now - kA, 1, NA(),
+         [&](int v) { load_stage(v, st + 2, ring + a_put, part); });
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(S::LA::kLoads) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    slab(1, a_next, b_next - kA, 0, NB(), [&](int v) {
+      load_stage(S::LA::kLoads + v, st + 2, ring + b_now - kA, part);
+    });
+    const uint32_t a = a_now, b = b_now;
+    a_now = a_next;
+    a_next = a_put;
+    a_put = a;
+    b_now = b_next;
+    b_next = b;
+    ++st;
+  };
+  while (st + 3 < stages) step(std::true_type());
+  while (st < stages) step(std::false_type());
+  // no load may still be writing LDS when the workgroup ends
+  wait_vm<0>();
 }
 
 // The ring: load_stage(st, slot pointer) starts the loads of stage st,
@@ -230,14 +251,14 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
 
   typename S::LA la;
   typename S::LB lb;
-  la.init_k(wave, lane, [&](int i) {
+  la.init_k(wave, lane, g.k, [&](int i) {
     const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
     return g.a + slot_row(g.a_rows, g.n_a, s) * g.lda * kElem<Op>;
   });
   const char *bg = g.b + r.group * g.b_group * kElem<Op>;
   int64_t b_step;
   if constexpr (BKC) {
-    lb.init_k(wave, lane, [&](int i) {
+    lb.init_k(wave, lane, g.k, [&](int i) {
       const int n = n0 + i < g.n ? n0 + i : g.n - 1;
       return bg + n * g.ldb * kElem<Op>;
     });
@@ -419,14 +440,14 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
   const int stages = (g.k + kStep<Op> - 1) / kStep<Op>;
   const int mine = stages > wave ? (stages - wave + NW - 1) / NW : 0;
   const int64_t k0 = static_cast<int64_t>(wave) * kStep<Op>;
-  la.init_k(0, lane, [&](int i) {
+  la.init_k(0, lane, g.k, [&](int i) {
     const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
     return g.a + (slot_row(g.a_rows, g.n_a, s) * g.lda + k0) * kElem<Op>;
   });
   const char *bg = g.b + r.group * g.b_group * kElem<Op>;
   int64_t b_step;
   if constexpr (BKC) {
-    lb.init_k(0, lane, [&](int i) {
+    lb.init_k(0, lane, g.k, [&](int i) {
       const int n = n0 + i < g.n ? n0 + i : g.n - 1;
       return bg + (n * g.ldb + k0) * kElem<Op>;
     });
