@@ -162,9 +162,12 @@ SIGNATURES = {
     "ej_expert_combine_vjp": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _i32, _i32,
                                      _vp, _i64, _vp, _vp, _vp]),
     "ej_quantize_rows": (_i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "ej_grouped_gemm_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
     "ej_grouped_gemm": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                               _vp]),
-    "ej_grouped_gemm_dw": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
+                               _vp, _sz, _vp]),
+    "ej_grouped_gemm_dw_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
+    "ej_grouped_gemm_dw": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _sz, _vp]),
 }
 
 _lock = threading.Lock()

@@ -145,47 +145,78 @@ __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, co
 // q = round(x / scale), scale = max |x| / 127 (as max |x| times the nearest
 // fp32 to 1/127); ties to even.  A row of zeros has scale 0 and zeros; a row
 // with a NaN or an infinity has scale NaN and zeros, so that whatever is
-// computed with it is NaN.
-template <class T, bool VEC>
-__global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t ld, int32_t n,
-                                                            int8_t *q, float *scale) {
+// computed with it is NaN.  TPR threads a row hold P pieces of it each in
+// registers between the two passes; what a longer row has beyond is read
+// twice (from the cache).
+template <class T, bool VEC, int TPR, int P>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t n_rows, int64_t ld,
+                                                            int32_t n, int8_t *q, float *scale) {
   constexpr int N = Piece<T, VEC>::N, W = kThreads / 64;
-  __shared__ float part[W];
-  const int64_t r = blockIdx.x;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / TPR) + threadIdx.x / TPR;
+  if (TPR == 64 && r >= n_rows) return;  // whole waves; no barrier below then
+  const int64_t first = threadIdx.x % TPR * N;
   const T *row = x + r * ld;
+  Piece<T, VEC> held[P];
   float most = 0.f;
   bool bad = false;
-  for (int64_t col = threadIdx.x * N; col < n; col += kThreads * N) {
-    Piece<T, VEC> v;
-    v.load(row + col);
+  auto look = [&](const Piece<T, VEC> &v) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float m = fabsf(v.v[i]);
       bad |= !(m <= 3.402823466e38f);
       most = fmaxf(most, m);
     }
+  };
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (first + p * TPR * N < n) held[p].load(row + first + p * TPR * N);
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (first + p * TPR * N < n) look(held[p]);
+  for (int64_t col = first + P * TPR * N; col < n; col += TPR * N) {
+    Piece<T, VEC> v;
+    v.load(row + col);
+    look(v);
   }
   if (bad) most = INFINITY;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
-  __syncthreads();
+  if constexpr (TPR > 64) {
+    __shared__ float part[W];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < W; ++w) most = fmaxf(most, part[w]);
-  float s = most * static_cast<float>(1.0 / 127.0);
+    for (int w = 0; w < W; ++w) most = fmaxf(most, part[w]);
+  }
+  const float s = most * static_cast<float>(1.0 / 127.0);
   const bool plain = s > 0.f && most < INFINITY;
-  if (threadIdx.x == 0) scale[r] = most < INFINITY ? s : __uint_as_float(0x7fc00000u);
-  for (int64_t col = threadIdx.x * N; col < n; col += kThreads * N) {
-    Piece<T, VEC> v;
-    v.load(row + col);
+  // The rounded quotient, without dividing where x times 1 / s cannot lie on
+  // the other side of a tie (it is off by less than 2^-14 below 128): the
+  // division takes as long as reading the row, and one in thousands needs it.
+  // (Not for scales so small that 1 / s overflows.)
+  const float inv = s >= 1e-37f ? 1.f / s : 0.f;
+  auto rounded = [&](float x) {
+    const float f = x * inv, q = rintf(f);
+    return inv > 0.f && fabsf(f - q) < 0.4999f ? q : rintf(x / s);
+  };
+  if (first == 0) scale[r] = most < INFINITY ? s : __uint_as_float(0x7fc00000u);
+  auto put = [&](int64_t col, const Piece<T, VEC> &v) {
     struct alignas(N) { int8_t e[N]; } o;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float f = plain ? rintf(v.v[i] / s) : 0.f;
+      const float f = plain ? rounded(v.v[i]) : 0.f;
       // a subnormal scale may round so far down that a quotient passes 127
       o.e[i] = static_cast<int8_t>(fminf(fmaxf(f, -127.f), 127.f));
     }
     *reinterpret_cast<decltype(o) *>(q + r * n + col) = o;
+  };
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+    if (first + p * TPR * N < n) put(first + p * TPR * N, held[p]);
+  for (int64_t col = first + P * TPR * N; col < n; col += TPR * N) {
+    Piece<T, VEC> v;
+    v.load(row + col);
+    put(col, v);
   }
 }
 
@@ -300,13 +331,20 @@ extern "C" int ej_quantize_rows(const void *x, int32_t dtype, int64_t n_rows, in
     constexpr int N = 16 / sizeof(T);
     const bool vec = aligned16(x, ld, sizeof(T)) && n % N == 0 &&
                      reinterpret_cast<size_t>(q) % N == 0;
-    const dim3 grid(static_cast<unsigned>(n_rows));
-    if (vec)
-      hipLaunchKernelGGL((quantize_kernel<T, true>), grid, dim3(kThreads), 0, as_stream(stream),
-                         static_cast<const T *>(x), ld, n, q, scale);
+    const T *xt = static_cast<const T *>(x);
+    auto run = [&](auto kernel, int64_t blocks) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                         as_stream(stream), xt, n_rows, ld, n, q, scale);
+    };
+    // a wave a row where there are rows enough to fill the CUs and a row fits
+    // its registers; otherwise a workgroup a row
+    constexpr int kHeld = 8;
+    if (vec && n_rows >= 1024 && n <= 64 * N * kHeld)
+      run(quantize_kernel<T, true, 64, kHeld>, ceil_div(n_rows, kThreads / 64));
+    else if (vec)
+      run(quantize_kernel<T, true, kThreads, 4>, n_rows);
     else
-      hipLaunchKernelGGL((quantize_kernel<T, false>), grid, dim3(kThreads), 0, as_stream(stream),
-                         static_cast<const T *>(x), ld, n, q, scale);
+      run(quantize_kernel<T, false, kThreads, 8>, n_rows);
     EJ_LAUNCH_CHECK();
     return EJ_OK;
   });

@@ -6,8 +6,9 @@
 // with weights p, or p divided by the sum over the picks.  A logit of -inf
 // excludes its expert; picks beyond the experts left are -1 with weight 0.
 //
-// A token's logits stay in registers: kLanes lanes hold V each, one reduction
-// of (ordered value, expert) words for each pick, no sort.  The grouping is a
+// A token's logits stay in registers: 16 or 64 lanes hold V each, two reductions
+// (the largest ordered value, the lowest expert that has it) for each pick, no
+// sort.  The grouping is a
 // stable counting sort (pairs of one expert in token order, so results do not
 // depend on scheduling): workgroups count their tokens' picks in LDS, then
 // each adds up the counts before its own and places its pairs, ranked among
@@ -59,20 +60,40 @@ __device__ inline float unordered(uint32_t o) {
 }
 constexpr uint32_t kExcluded = 0x007fffffu;  // ordered(-inf)
 
-template <int L>
-__device__ inline uint64_t lanes_max(uint64_t v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) {
-    const uint64_t o = __shfl_xor(v, d, L);
-    v = o > v ? o : v;
+// Reductions over the L lanes of a token, every lane gets the same result:
+// within 16 lanes by DPP (neighbours, pairs, then mirrored halves, whose lanes
+// agree already), across the rows of 16 by shuffles.
+template <int CTRL>
+__device__ inline uint32_t moved(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, false));
+}
+template <int L, class F>
+__device__ inline uint32_t lanes_reduce(uint32_t v, F f) {
+  static_assert(L == 16 || L == 64, "whole DPP rows");
+  v = f(v, moved<0xb1>(v));   // quad_perm [1, 0, 3, 2]
+  v = f(v, moved<0x4e>(v));   // quad_perm [2, 3, 0, 1]
+  v = f(v, moved<0x141>(v));  // row_half_mirror
+  v = f(v, moved<0x140>(v));  // row_mirror
+  if constexpr (L == 64) {
+    v = f(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
+    v = f(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)));
   }
   return v;
 }
 template <int L>
+__device__ inline uint32_t lanes_max(uint32_t v) {
+  return lanes_reduce<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int L>
+__device__ inline uint32_t lanes_min(uint32_t v) {
+  return lanes_reduce<L>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+template <int L>
 __device__ inline float lanes_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d, L);
-  return v;
+  return __uint_as_float(lanes_reduce<L>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 
 // Picks of token t by L lanes holding V logits each (expert v * L + lane);
@@ -100,11 +121,9 @@ __device__ inline void route_token(const RouteArgs &a, int64_t t, int lane, int 
         best = key[v];
         at = v * L + lane;
       }
-    // of equal values the lowest expert wins: its complement is the largest
-    const uint64_t w = lanes_max<L>(
-        static_cast<uint64_t>(best) << 32 | static_cast<uint32_t>(~at));
-    const uint32_t wk = static_cast<uint32_t>(w >> 32);
-    const int we = static_cast<int>(~static_cast<uint32_t>(w));
+    // of equal values the lowest expert wins
+    const uint32_t wk = lanes_max<L>(best);
+    const int we = static_cast<int>(lanes_min<L>(best == wk ? at : 0x7fffffffu));
     if (wk <= kExcluded) break;  // uniform over the L lanes
     if (j == 0) top = wk == 0xffffffffu ? __uint_as_float(0x7fc00000u) : unordered(wk);
     if (lane == j) {
@@ -342,12 +361,10 @@ __global__ __launch_bounds__(kRouteThreads) void route_vjp_kernel(RouteArgs a, c
     nan |= x[v] != x[v];
     top = fmaxf(top, x[v]);
   }
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) {
-    top = fmaxf(top, __shfl_xor(top, d, L));
-    nan |= __shfl_xor(static_cast<int>(nan), d, L) != 0;
-  }
-  if (nan) top = __uint_as_float(0x7fc00000u);
+  top = __uint_as_float(lanes_reduce<L>(__float_as_uint(top), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+  if (lanes_max<L>(nan)) top = __uint_as_float(0x7fc00000u);
   int pick = -1;
   float d = 0.f, w = 0.f;
   if (lane < a.k) {

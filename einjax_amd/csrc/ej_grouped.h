@@ -73,6 +73,10 @@ struct GroupedArgs {
   int32_t n_groups, m, n, k;
   int32_t out;              // EJ_F32, EJ_BF16 or EJ_F16
   uint32_t row_blocks, col_blocks;  // bound on live row blocks; column blocks
+  // The contraction in `splits` parts (grid.y), each into fp32 sums of its own,
+  // [splits][slots][n] or [splits][n_groups][m][n]; 1: none.
+  float *partial;
+  int32_t splits;
 };
 
 // A 16-byte chunk of zeros: what lanes beyond an operand's extent load.
@@ -300,6 +304,12 @@ __device__ inline void put4(void *c, int code, int64_t at, int col, int n, bool 
         if (col + r < n) p[r] = to_16(v[r], code);
     }
   }
+}
+
+// Stages [first, last) of part `part` of `parts`.
+__device__ inline void part_of(int stages, int part, int parts, int *first, int *last) {
+  *first = static_cast<int>(static_cast<int64_t>(stages) * part / parts);
+  *last = static_cast<int>(static_cast<int64_t>(stages) * (part + 1) / parts);
 }
 
 // Whether groups of four columns can be stored as one vector.

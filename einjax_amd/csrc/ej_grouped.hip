@@ -35,14 +35,69 @@ int check_desc(const ej_grouped_desc *d) {
   return EJ_OK;
 }
 
+// Parts of the contraction: 64 x 64 tiles that leave most CUs without work
+// and have a long way to go are split until the CUs are covered, but not below
+// eight stages a part (each part is a pass over its sums).  One group, bf16:
+// weight gradient of 8192 rows x 128 x 128 10 us with the sum of the parts, 49
+// in one; rows product of 512 x 4096 x 64 11 us and 27.
+int split_parts(double tiles, int64_t contraction, int elem) {
+  const int64_t stages = contraction / (128 / elem);
+  if (tiles >= 128 || tiles <= 0 || stages < 16) return 1;
+  const int64_t want = static_cast<int64_t>(256 / tiles), most = stages / 8;
+  const int64_t parts = want < most ? want : most;
+  return static_cast<int>(parts < 2 ? 1 : parts < 32 ? parts : 32);
+}
+
+// Rows of a group on average decide for the rows product, as the choice of
+// kernel does: groups of few rows take the kernel that splits k by itself.
+int rows_parts(const ej_grouped_desc *d) {
+  if (d->dtype == EJ_I8 || d->n_groups == 0 || d->n_slots == 0) return 1;
+  const int64_t groups = d->n_groups < d->n_slots ? d->n_groups : d->n_slots;
+  if (d->n_slots <= 16 * groups) return 1;
+  const double tiles =
+      (static_cast<double>(d->n_slots) / 64 + 0.5 * groups) * ceil_div(d->n, 64);
+  return split_parts(tiles, d->k, elem_size(d->dtype));
+}
+int dw_parts(const ej_grouped_desc *d) {
+  if (d->n_groups == 0) return 1;
+  const double tiles = static_cast<double>(ceil_div(d->k, 64)) * ceil_div(d->n, 64) * d->n_groups;
+  return split_parts(tiles, d->n_slots / d->n_groups, elem_size(d->dtype));
+}
+
+int check_workspace(int parts, int64_t sums, void *workspace, size_t bytes, GroupedArgs *g) {
+  g->splits = parts;
+  if (parts == 1) return EJ_OK;
+  EJ_CHECK_ARG(workspace && bytes >= sizeof(float) * parts * sums,
+               "workspace of %zu bytes, expected %zu", bytes, sizeof(float) * parts * sums);
+  g->partial = static_cast<float *>(workspace);
+  return EJ_OK;
+}
+
 }  // namespace
 }  // namespace ej
 
 using namespace ej;
 
+extern "C" int ej_grouped_gemm_workspace_size(const ej_grouped_desc *d, size_t *bytes) {
+  EJ_TRY(check_desc(d));
+  EJ_CHECK_ARG(bytes, "null bytes");
+  const int parts = rows_parts(d);
+  *bytes = parts > 1 ? sizeof(float) * parts * d->n_slots * d->n : 0;
+  return EJ_OK;
+}
+
+extern "C" int ej_grouped_gemm_dw_workspace_size(const ej_grouped_desc *d, size_t *bytes) {
+  EJ_TRY(check_desc(d));
+  EJ_CHECK_ARG(bytes, "null bytes");
+  const int parts = dw_parts(d);
+  *bytes = parts > 1 ? sizeof(float) * parts * d->n_groups * d->k * d->n : 0;
+  return EJ_OK;
+}
+
 extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const int32_t *rows,
                                const int32_t *offsets, const void *w, const float *x_scale,
-                               const float *w_scale, void *out, ej_stream_t stream) {
+                               const float *w_scale, void *out, void *workspace,
+                               size_t workspace_bytes, ej_stream_t stream) {
   EJ_TRY(check_desc(d));
   const bool i8 = d->dtype == EJ_I8;
   EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype ||
@@ -89,6 +144,7 @@ extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const in
   const bool direct = d->k % chunk == 0 && aligned16(x, d->x_stride, 0, size) &&
                       aligned16(w, d->w_stride, d->w_group, size) &&
                       (d->w_order == EJ_W_NK || d->n % chunk == 0);
+  EJ_TRY(check_workspace(rows_parts(d), d->n_slots * d->n, workspace, workspace_bytes, &g));
   const GroupedRows r{g, d->w_order == EJ_W_NK, direct};
   switch (d->dtype) {
     case EJ_BF16: return grouped_rows_bf16(r, as_stream(stream));
@@ -100,7 +156,7 @@ extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const in
 
 extern "C" int ej_grouped_gemm_dw(const ej_grouped_desc *d, const void *x, const int32_t *rows,
                                   const int32_t *offsets, const void *grad, void *grad_w,
-                                  ej_stream_t stream) {
+                                  void *workspace, size_t workspace_bytes, ej_stream_t stream) {
   EJ_TRY(check_desc(d));
   EJ_CHECK_ARG(d->dtype != EJ_I8, "8-bit products have no gradient");
   EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype,
@@ -133,6 +189,8 @@ extern "C" int ej_grouped_gemm_dw(const ej_grouped_desc *d, const void *x, const
   g.ldb = kn ? d->out_stride : d->x_stride;
   g.n_b = kn ? d->n_slots : d->n_rows;
   g.n = kn ? d->n : d->k;
+  EJ_TRY(check_workspace(dw_parts(d), static_cast<int64_t>(d->n_groups) * d->k * d->n, workspace,
+                         workspace_bytes, &g));
   const bool direct = d->k % chunk == 0 && d->n % chunk == 0 &&
                       aligned16(x, d->x_stride, 0, size) &&
                       aligned16(grad, d->out_stride, 0, size);

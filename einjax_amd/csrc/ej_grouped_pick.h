@@ -8,6 +8,15 @@
 
 namespace ej {
 
+inline int join_parts(const GroupedArgs &g, int64_t rows, int64_t m, bool skip_dead,
+                      hipStream_t stream) {
+  dim3 grid;
+  EJ_TRY(grouped_grid(ceil_div(rows * ceil_div(g.n, 4), 256), 256, &grid));
+  hipLaunchKernelGGL(grouped_join_kernel, grid, dim3(256), 0, stream, g, rows, m, skip_dead);
+  EJ_LAUNCH_CHECK();
+  return EJ_OK;
+}
+
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
 int launch_rows(GroupedArgs g, hipStream_t stream) {
   const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
@@ -16,10 +25,11 @@ int launch_rows(GroupedArgs g, hipStream_t stream) {
   dim3 grid;
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks,
                       WR * WC * 64, &grid));
+  grid.y = g.splits;
   hipLaunchKernelGGL((grouped_rows_kernel<Op, BM, BN, WR, WC, BKC, DIRECT, NS>), grid,
                      dim3(WR * WC * 64), 0, stream, g);
   EJ_LAUNCH_CHECK();
-  return EJ_OK;
+  return g.splits > 1 ? join_parts(g, g.slots, g.slots, true, stream) : EJ_OK;
 }
 
 template <class Op, int FM, int BN, int NW, bool BKC, int NS>
@@ -43,10 +53,12 @@ int launch_wgrad_as(GroupedArgs g, hipStream_t stream) {
   dim3 grid;
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks * g.n_groups,
                       WR * WC * 64, &grid));
+  grid.y = g.splits;
   hipLaunchKernelGGL((grouped_wgrad_kernel<Op, BM, BN, WR, WC, DIRECT, NS, GATHER>), grid,
                      dim3(WR * WC * 64), 0, stream, g);
   EJ_LAUNCH_CHECK();
-  return EJ_OK;
+  return g.splits > 1 ? join_parts(g, static_cast<int64_t>(g.n_groups) * g.m, g.m, false, stream)
+                      : EJ_OK;
 }
 
 template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS>
@@ -74,6 +86,10 @@ inline double expected_tiles(const GroupedArgs &g, int bm, int bn, int64_t group
 template <class Op, bool BKC>
 int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
+  if (g.splits > 1) {
+    if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
+  }
   const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
   const double rows = static_cast<double>(g.slots) / groups;
   if (!r.direct) {
@@ -108,6 +124,7 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
   if (!direct) return launch_wgrad<Op, 64, 64, 2, 2, false, 2>(g, stream);
+  if (g.splits > 1) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
   auto tiles = [&](int b) { return ceil_div(g.m, b) * ceil_div(g.n, b) * g.n_groups; };
   if constexpr (kElem<Op> == 2) {
     if (tiles(256) >= 256) return launch_wgrad<Op, 256, 256, 2, 4, true, 0>(g, stream);

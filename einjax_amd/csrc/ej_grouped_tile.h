@@ -236,7 +236,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
   __shared__ __align__(1024) unsigned char ring[S::kLds];
   const uint32_t grid = g.row_blocks * g.col_blocks;
   if (blockIdx.x >= grid) {
-    zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
+    if (blockIdx.y == 0) zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
     return;
   }
   const uint32_t rbs = live_row_blocks(g, BM), live = rbs * g.col_blocks;
@@ -248,23 +248,27 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row0 = wave / WC * S::WM, col0 = wave % WC * S::WN;
   const int n0 = cb * BN;
+  int st0, st1;
+  part_of((g.k + kStep<Op> - 1) / kStep<Op>, blockIdx.y, g.splits, &st0, &st1);
+  const int64_t k0 = static_cast<int64_t>(st0) * kStep<Op>;
+  const int ks = g.k - static_cast<int>(k0);  // k left from the part's start
 
   typename S::LA la;
   typename S::LB lb;
   la.init_k(wave, lane, g.k, [&](int i) {
     const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
-    return g.a + slot_row(g.a_rows, g.n_a, s) * g.lda * kElem<Op>;
+    return g.a + (slot_row(g.a_rows, g.n_a, s) * g.lda + k0) * kElem<Op>;
   });
   const char *bg = g.b + r.group * g.b_group * kElem<Op>;
   int64_t b_step;
   if constexpr (BKC) {
     lb.init_k(wave, lane, g.k, [&](int i) {
       const int n = n0 + i < g.n ? n0 + i : g.n - 1;
-      return bg + n * g.ldb * kElem<Op>;
+      return bg + (n * g.ldb + k0) * kElem<Op>;
     });
     b_step = kRowB;
   } else {
-    lb.init_m(wave, lane, bg, g.ldb, n0, g.n);
+    lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
 
@@ -274,9 +278,9 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
   run_stages<Op, S, DIRECT, NS>(
-      acc, ring, (g.k + kStep<Op> - 1) / kStep<Op>, row0, col0, lane,
+      acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
-        const int left = g.k - st * kStep<Op>;
+        const int left = ks - st * kStep<Op>;
         if (v < S::LA::kLoads)
           la.load(v, slot, wave, left, kRowB, part);
         else
@@ -287,6 +291,11 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
         lb.store(slot + S::TA::kBytes, wave, lane);
       });
 
+  if (g.splits > 1) {
+    g.c = g.partial + blockIdx.y * g.slots * g.n;
+    g.ldc = g.n;
+    g.out = EJ_F32;
+  }
   const bool vec = vec_rows(g);
 #pragma unroll
   for (int i = 0; i < S::FM; ++i) {
@@ -335,6 +344,15 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 
   typename S::LA la;
   typename S::LB lb;
+  int st0, st1;
+  part_of((hi - lo + kStep<Op> - 1) / kStep<Op>, blockIdx.y, g.splits, &st0, &st1);
+  if (g.splits > 1) {
+    lo += st0 * kStep<Op>;
+    g.c = g.partial + blockIdx.y * (static_cast<int64_t>(g.n_groups) * g.m * g.n);
+    g.c_group = static_cast<int64_t>(g.m) * g.n;
+    g.ldc = g.n;
+    g.out = EJ_F32;
+  }
   la.init_m(wave, lane, g.a + (GATHER == 1 ? 0 : lo * g.lda * kElem<Op>), g.lda, rb * BM, g.m);
   lb.init_m(wave, lane, g.b + (GATHER == 2 ? 0 : lo * g.ldb * kElem<Op>), g.ldb, cb * BN, g.n);
   // the gathered operand's rows of a stage, lane by lane, read a stage ahead
@@ -345,7 +363,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
     return static_cast<int>(slot_row(rows, n_rows, static_cast<int>(s < hi ? s : hi - 1)));
   };
   int row_now = 0, row_next = 0;
-  if (GATHER && hi > lo) row_next = rows_of(0);
+  if (GATHER && st1 > st0) row_next = rows_of(0);
 
   typename Op::acc acc[S::FM][S::FN];
 #pragma unroll
@@ -353,7 +371,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
   run_stages<Op, S, DIRECT, NS>(
-      acc, ring, (hi - lo + kStep<Op> - 1) / kStep<Op>, row0, col0, lane,
+      acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
         const int left = hi - lo - st * kStep<Op>;
         if (GATHER && v == 0) {
@@ -518,6 +536,33 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
     put4(g.c, g.out, s * g.ldc, n0 + col, g.n, vec, v);
   }
 #endif
+}
+
+// Results from the sums of the parts, added in their order: element (row, col)
+// of group-major rows, m to a group, goes to c_group, ldc.  Rows of no group
+// (offsets given) are zero already.
+static __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g, int64_t rows, int64_t m,
+                                                           bool skip_dead) {
+  const int64_t quads = (g.n + 3) / 4, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= rows * quads) return;
+  const int64_t row = i / quads;
+  const int col = static_cast<int>(i % quads) * 4;
+  if (skip_dead && g.offsets && (row < g.offsets[0] || row >= g.offsets[g.n_groups])) return;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+  const float *src = g.partial + row * g.n + col;
+  const int64_t part = rows * g.n;
+  if (g.n % 4 == 0) {
+#pragma unroll 8
+    for (int p = 0; p < g.splits; ++p)
+      sum += *reinterpret_cast<const f32x4_t *>(src + p * part);
+  } else {
+    for (int p = 0; p < g.splits; ++p)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (col + c < g.n) sum[c] += src[p * part + c];
+  }
+  const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+  put4(g.c, g.out, row / m * g.c_group + row % m * g.ldc, col, g.n, vec_rows(g), v);
 }
 
 }  // namespace ej

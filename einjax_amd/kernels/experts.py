@@ -325,6 +325,14 @@ def _desc(x, code, out_code, order, E, k, n, n_slots, w_group, w_stride, out_str
                             max(_row_stride(x), k), w_group, w_stride, out_stride)
 
 
+def _product_workspace(ref: torch.Tensor, query: str, d):
+    """(workspace tensor or None, its size) of a grouped product."""
+    nbytes = ctypes.c_size_t()
+    check(getattr(_lib.load(), query)(ctypes.byref(d), ctypes.byref(nbytes)), query)
+    n = nbytes.value
+    return (_device.workspace(n, ref.device) if n else None), n
+
+
 def grouped_product(x: torch.Tensor, w: torch.Tensor, g: Groups, out_dtype) -> torch.Tensor:
     """out[s] = x[row of s] w[group of s], zero in slots of no group."""
     x = rows_of(x)
@@ -333,8 +341,9 @@ def grouped_product(x: torch.Tensor, w: torch.Tensor, g: Groups, out_dtype) -> t
     out = torch.empty((g.n_slots, n), dtype=out_dtype, device=x.device)
     d = _desc(x, _value_code(x, "x"), _DTYPES[out_dtype], order, E, k, n, g.n_slots, gs, rs, n)
     p = _ptr
+    ws, ws_bytes = _product_workspace(x, "ej_grouped_gemm_workspace_size", d)
     _call(x, "ej_grouped_gemm", ctypes.byref(d), p(x), p(g.rows), p(g.offsets), p(w), None, None,
-          p(out))
+          p(out), p(ws), ws_bytes)
     return out
 
 
@@ -353,7 +362,9 @@ def grouped_weight_gradient(x: torch.Tensor, w: torch.Tensor, g: Groups,
     code = _value_code(x, "x")
     d = _desc(x, code, code, order, E, k, n, g.n_slots, k * n, rs, max(_row_stride(grad), n))
     p = _ptr
-    _call(x, "ej_grouped_gemm_dw", ctypes.byref(d), p(x), p(g.rows), p(g.offsets), p(grad), p(gw))
+    ws, ws_bytes = _product_workspace(x, "ej_grouped_gemm_dw_workspace_size", d)
+    _call(x, "ej_grouped_gemm_dw", ctypes.byref(d), p(x), p(g.rows), p(g.offsets), p(grad), p(gw),
+          p(ws), ws_bytes)
     return gw
 
 
@@ -411,6 +422,6 @@ def int8_matmul(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale
     p = _ptr
     q_scale, w_scale = q_scale.contiguous(), w_scale.contiguous()
     _call(q, "ej_grouped_gemm", ctypes.byref(d), p(q), p(g.rows), p(g.offsets), p(w), p(q_scale),
-          p(w_scale), p(out))
+          p(w_scale), p(out), None, 0)
     return out
 

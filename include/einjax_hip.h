@@ -730,19 +730,24 @@ typedef struct ej_grouped_desc {
  * read as non-decreasing values in [0, n_slots]; others give undefined rows,
  * never an access outside the operands; NULL with n_groups == 1: one group of
  * every slot.  EJ_I8: x_scale [n_rows] and w_scale
- * [n_groups][n], out = x_scale w_scale (exact integer sum); NULL otherwise. */
+ * [n_groups][n], out = x_scale w_scale (exact integer sum); NULL otherwise.
+ * The workspace (NULL where its size is 0) holds the sums of a contraction that
+ * is split to cover the CUs; they are added in a fixed order. */
+int ej_grouped_gemm_workspace_size(const ej_grouped_desc *desc, size_t *bytes);
 int ej_grouped_gemm(const ej_grouped_desc *desc, const void *x, const int32_t *rows,
                     const int32_t *offsets, const void *w, const float *x_scale,
-                    const float *w_scale, void *out, ej_stream_t stream);
+                    const float *w_scale, void *out, void *workspace, size_t workspace_bytes,
+                    ej_stream_t stream);
 
 /* Gradient to the weights: grad_w_e = sum over the slots s of group e of
  * x[rows[s]]^T grad[s], in the order and strides that the descriptor gives
  * w (a group without slots gets zeros).  The gradient to x is ej_grouped_gemm
  * of grad and W with k and n, and EJ_W_KN and EJ_W_NK, exchanged, followed by
  * ej_expert_combine without weights where rows were gathered. */
+int ej_grouped_gemm_dw_workspace_size(const ej_grouped_desc *desc, size_t *bytes);
 int ej_grouped_gemm_dw(const ej_grouped_desc *desc, const void *x, const int32_t *rows,
-                       const int32_t *offsets, const void *grad, void *grad_w,
-                       ej_stream_t stream);
+                       const int32_t *offsets, const void *grad, void *grad_w, void *workspace,
+                       size_t workspace_bytes, ej_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,8 @@ def desc(**kw):
 
 
 def gemm(d, x=FAKE, rows=None, offsets=FAKE, w=FAKE, xs=None, ws=None, out=FAKE):
-    return _lib.load().ej_grouped_gemm(ctypes.byref(d), x, rows, offsets, w, xs, ws, out, None)
+    return _lib.load().ej_grouped_gemm(ctypes.byref(d), x, rows, offsets, w, xs, ws, out, None, 0,
+                                      None)
 
 
 @pytest.mark.parametrize("change,status", [
@@ -53,15 +54,34 @@ def test_product_null_arguments():
     assert gemm(desc(), out=None) == _lib.EJ_E_INVAL
     assert gemm(desc(), offsets=None) == _lib.EJ_E_INVAL  # two groups need offsets
     lib = _lib.load()
-    assert lib.ej_grouped_gemm(None, FAKE, None, FAKE, FAKE, None, None, FAKE, None) == \
+    assert lib.ej_grouped_gemm(None, FAKE, None, FAKE, FAKE, None, None, FAKE, None, 0, None) == \
         _lib.EJ_E_INVAL
     # nothing to write: no launch
     assert gemm(desc(n_slots=0), x=None, w=None, out=None, offsets=None) == 0
     assert gemm(desc(n=0), x=None, w=None, out=None, offsets=None) == 0
     assert lib.ej_grouped_gemm_dw(ctypes.byref(desc(n_groups=0)), None, None, None, None, None,
-                                  None) == 0
+                                  None, 0, None) == 0
     assert lib.ej_grouped_gemm_dw(ctypes.byref(desc(dtype=_lib.EJ_I8)), FAKE, None, FAKE, FAKE,
-                                  FAKE, None) == _lib.EJ_E_INVAL
+                                  FAKE, None, 0, None) == _lib.EJ_E_INVAL
+
+
+def test_split_products_need_their_workspace():
+    lib, n = _lib.load(), ctypes.c_size_t()
+    few = desc(n_groups=1, k=4096, n_slots=512, n_rows=512, x_stride=4096, w_group=4096 * 32)
+    assert lib.ej_grouped_gemm_workspace_size(ctypes.byref(few), ctypes.byref(n)) == 0
+    assert n.value > 0 and n.value % (4 * 512 * 32) == 0
+    assert gemm(few) == _lib.EJ_E_INVAL and b"workspace" in lib.ej_last_error()
+    tall = desc(n_groups=1, n_slots=8192, n_rows=8192)
+    assert lib.ej_grouped_gemm_dw_workspace_size(ctypes.byref(tall), ctypes.byref(n)) == 0
+    assert n.value > 0 and n.value % (4 * 64 * 32) == 0
+    assert lib.ej_grouped_gemm_dw(ctypes.byref(tall), FAKE, None, FAKE, FAKE, FAKE, None, 0,
+                                  None) == _lib.EJ_E_INVAL
+    for d in (desc(), desc(n_groups=0), desc(n_slots=0)):
+        assert lib.ej_grouped_gemm_workspace_size(ctypes.byref(d), ctypes.byref(n)) == 0
+        assert n.value == 0
+        assert lib.ej_grouped_gemm_dw_workspace_size(ctypes.byref(d), ctypes.byref(n)) == 0
+        assert n.value == 0
+    assert lib.ej_grouped_gemm_workspace_size(None, ctypes.byref(n)) == _lib.EJ_E_INVAL
 
 
 @pytest.mark.parametrize("t,e,k,status", [
