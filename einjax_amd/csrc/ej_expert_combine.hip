@@ -145,40 +145,109 @@ __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, co
 // q = round(x / scale), scale = max |x| / 127 (as max |x| times the nearest
 // fp32 to 1/127); ties to even.  A row of zeros has scale 0 and zeros; a row
 // with a NaN or an infinity has scale NaN and zeros, so that whatever is
-// computed with it is NaN.  TPR threads a row hold P pieces of it each in
-// registers between the two passes; what a longer row has beyond is read
-// twice (from the cache).
-template <class T, bool VEC, int TPR, int P>
+// computed with it is NaN.
+//
+// TPR threads a row hold P pieces of it each in registers between the two
+// passes; what a longer row has beyond is read twice (from the cache).  The
+// arithmetic would take longer than the memory if it were written down as
+// above, so
+//   - the maximum is taken of the bits without their signs, two 16-bit values
+//     an instruction (the order of the magnitudes; infinities and NaN are the
+//     largest);
+//   - the rounded quotient comes from x times 1 / scale plus 1.5 2^23, whose
+//     low byte is the result; where that product lies near a tie, which it can
+//     be off by less than 2^-14 of, the piece is divided properly.
+template <class T>
+struct Raw {
+  static constexpr int N = 16 / static_cast<int>(sizeof(T));
+  uint32_t w[4];
+  __device__ inline void load(const T *p) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+  __device__ inline float at(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint32_t u = w[i / 2];
+      if constexpr (std::is_same_v<T, __bf16>)
+        return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+      else
+        return widen(__builtin_bit_cast(_Float16, static_cast<uint16_t>(i & 1 ? u >> 16 : u)));
+    }
+  }
+};
+template <class T>
+struct Scalar {  // one element, for rows that are not aligned
+  static constexpr int N = 1;
+  T v;
+  __device__ inline void load(const T *p) { v = *p; }
+  __device__ inline float at(int) const { return widen(v); }
+};
+
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
+// Largest magnitude seen, as bits.
+template <class T>
+struct Magnitude {
+  uint32_t bits = 0;
+  __device__ inline void look(const Raw<T> &r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t u = r.w[i] & 0x7fffffffu;
+        bits = u > bits ? u : bits;
+      } else {
+        bits = __builtin_bit_cast(
+            uint32_t, __builtin_elementwise_max(
+                          __builtin_bit_cast(u16x2_t, bits),
+                          __builtin_bit_cast(u16x2_t, r.w[i] & 0x7fff7fffu)));
+      }
+    }
+  }
+  __device__ inline void look(const Scalar<T> &r) {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t u = __float_as_uint(r.v) & 0x7fffffffu;
+      bits = u > bits ? u : bits;
+    } else {
+      const uint32_t u = __builtin_bit_cast(uint16_t, r.v) & 0x7fffu;
+      bits = u > bits ? u : bits;
+    }
+  }
+  // As a float; infinity for NaN.
+  __device__ inline float value() const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(bits > 0x7f800000u ? 0x7f800000u : bits);
+    } else {
+      const uint32_t u = (bits & 0xffff) > (bits >> 16) ? bits & 0xffff : bits >> 16;
+      constexpr uint32_t inf = std::is_same_v<T, __bf16> ? 0x7f80u : 0x7c00u;
+      return u >= inf ? INFINITY : widen(__builtin_bit_cast(T, static_cast<uint16_t>(u)));
+    }
+  }
+};
+
+template <class T, class R, int TPR, int P>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t n_rows, int64_t ld,
                                                             int32_t n, int8_t *q, float *scale) {
-  constexpr int N = Piece<T, VEC>::N, W = kThreads / 64;
+  constexpr int N = R::N, W = kThreads / 64;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / TPR) + threadIdx.x / TPR;
   if (TPR == 64 && r >= n_rows) return;  // whole waves; no barrier below then
   const int64_t first = threadIdx.x % TPR * N;
   const T *row = x + r * ld;
-  Piece<T, VEC> held[P];
-  float most = 0.f;
-  bool bad = false;
-  auto look = [&](const Piece<T, VEC> &v) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float m = fabsf(v.v[i]);
-      bad |= !(m <= 3.402823466e38f);
-      most = fmaxf(most, m);
-    }
-  };
+  R held[P];
+  Magnitude<T> seen;
 #pragma unroll
   for (int p = 0; p < P; ++p)
     if (first + p * TPR * N < n) held[p].load(row + first + p * TPR * N);
 #pragma unroll
   for (int p = 0; p < P; ++p)
-    if (first + p * TPR * N < n) look(held[p]);
+    if (first + p * TPR * N < n) seen.look(held[p]);
   for (int64_t col = first + P * TPR * N; col < n; col += TPR * N) {
-    Piece<T, VEC> v;
+    R v;
     v.load(row + col);
-    look(v);
+    seen.look(v);
   }
-  if (bad) most = INFINITY;
+  float most = seen.value();
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
   if constexpr (TPR > 64) {
@@ -190,23 +259,25 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t 
   }
   const float s = most * static_cast<float>(1.0 / 127.0);
   const bool plain = s > 0.f && most < INFINITY;
-  // The rounded quotient, without dividing where x times 1 / s cannot lie on
-  // the other side of a tie (it is off by less than 2^-14 below 128): the
-  // division takes as long as reading the row, and one in thousands needs it.
-  // (Not for scales so small that 1 / s overflows.)
-  const float inv = s >= 1e-37f ? 1.f / s : 0.f;
-  auto rounded = [&](float x) {
-    const float f = x * inv, q = rintf(f);
-    return inv > 0.f && fabsf(f - q) < 0.4999f ? q : rintf(x / s);
-  };
   if (first == 0) scale[r] = most < INFINITY ? s : __uint_as_float(0x7fc00000u);
-  auto put = [&](int64_t col, const Piece<T, VEC> &v) {
+  // 0: divide (a scale so small that its reciprocal overflows)
+  const float inv = s >= 1e-37f ? 1.f / s : 0.f;
+  auto put = [&](int64_t col, const R &v) {
     struct alignas(N) { int8_t e[N]; } o;
+    float off = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float f = plain ? rounded(v.v[i]) : 0.f;
-      // a subnormal scale may round so far down that a quotient passes 127
-      o.e[i] = static_cast<int8_t>(fminf(fmaxf(f, -127.f), 127.f));
+      const float f = v.at(i) * inv, t = f + 12582912.f;
+      off = fmaxf(off, fabsf(f - (t - 12582912.f)));
+      o.e[i] = static_cast<int8_t>(__float_as_uint(t));
+    }
+    if (!(off < 0.4999f) || inv == 0.f || !plain) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float f = plain ? rintf(v.at(i) / s) : 0.f;
+        // a subnormal scale may round so far down that a quotient passes 127
+        o.e[i] = static_cast<int8_t>(fminf(fmaxf(f, -127.f), 127.f));
+      }
     }
     *reinterpret_cast<decltype(o) *>(q + r * n + col) = o;
   };
@@ -214,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t 
   for (int p = 0; p < P; ++p)
     if (first + p * TPR * N < n) put(first + p * TPR * N, held[p]);
   for (int64_t col = first + P * TPR * N; col < n; col += TPR * N) {
-    Piece<T, VEC> v;
+    R v;
     v.load(row + col);
     put(col, v);
   }
@@ -340,11 +411,11 @@ extern "C" int ej_quantize_rows(const void *x, int32_t dtype, int64_t n_rows, in
     // its registers; otherwise a workgroup a row
     constexpr int kHeld = 8;
     if (vec && n_rows >= 1024 && n <= 64 * N * kHeld)
-      run(quantize_kernel<T, true, 64, kHeld>, ceil_div(n_rows, kThreads / 64));
+      run(quantize_kernel<T, Raw<T>, 64, kHeld>, ceil_div(n_rows, kThreads / 64));
     else if (vec)
-      run(quantize_kernel<T, true, kThreads, 4>, n_rows);
+      run(quantize_kernel<T, Raw<T>, kThreads, 4>, n_rows);
     else
-      run(quantize_kernel<T, false, kThreads, 8>, n_rows);
+      run(quantize_kernel<T, Scalar<T>, kThreads, 8>, n_rows);
     EJ_LAUNCH_CHECK();
     return EJ_OK;
   });

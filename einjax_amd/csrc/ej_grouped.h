@@ -483,11 +483,14 @@ struct Loader {
       *reinterpret_cast<i32v4_t *>(tile + ((v * NW + wave) * 64 + lane) * 16) = reg[v];
   }
 
-  // M tiles of gathered rows (weight gradient): source v of the stage whose
+  // M tiles of gathered rows (weight gradient): the sources of the stage whose
   // rows' places in the operand lie in the lanes of `row` (lane i: k-row i).
-  __device__ inline void seek(int v, const char *base, int64_t ld, int row) {
-    const int r = __shfl(row, line_at(v));
-    src[v] = base + (r * ld + col[v % kCols]) * kElem<Op>;
+  __device__ inline void seek(const char *base, int64_t ld, int row) {
+    int r[kLoads];
+#pragma unroll
+    for (int v = 0; v < kLoads; ++v) r[v] = __shfl(row, line_at(v));
+#pragma unroll
+    for (int v = 0; v < kLoads; ++v) src[v] = base + (r[v] * ld + col[v % kCols]) * kElem<Op>;
   }
 };
 

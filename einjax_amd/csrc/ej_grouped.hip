@@ -35,17 +35,18 @@ int check_desc(const ej_grouped_desc *d) {
   return EJ_OK;
 }
 
-// Parts of the contraction: 64 x 64 tiles that leave most CUs without work
-// and have a long way to go are split until the CUs are covered, but not below
-// eight stages a part (each part is a pass over its sums).  One group, bf16:
+// Parts of the contraction: 64 x 64 tiles that leave three CUs of four without
+// work and have a long way to go are split until the CUs are covered, but not
+// below eight stages a part (each part is a pass over its sums, and adding them
+// a launch: in two parts nothing is gained).  One group, bf16:
 // weight gradient of 8192 rows x 128 x 128 10 us with the sum of the parts, 49
 // in one; rows product of 512 x 4096 x 64 11 us and 27.
 int split_parts(double tiles, int64_t contraction, int elem) {
   const int64_t stages = contraction / (128 / elem);
-  if (tiles >= 128 || tiles <= 0 || stages < 16) return 1;
+  if (tiles > 64 || tiles <= 0 || stages < 32) return 1;
   const int64_t want = static_cast<int64_t>(256 / tiles), most = stages / 8;
   const int64_t parts = want < most ? want : most;
-  return static_cast<int>(parts < 2 ? 1 : parts < 32 ? parts : 32);
+  return static_cast<int>(parts < 32 ? parts : 32);
 }
 
 // Rows of a group on average decide for the rows product, as the choice of

@@ -374,16 +374,26 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
       acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
         const int left = hi - lo - st * kStep<Op>;
-        if (GATHER && v == 0) {
-          row_now = row_next;
-          row_next = rows_of(st + 1);
-        }
+        // all sources of the gathered operand at its first load: the lane
+        // moves wait for every LDS read before them
         if (v < S::LA::kLoads) {
-          if (GATHER == 1) la.seek(v, g.a, g.lda, row_now);
+          if constexpr (GATHER == 1) {
+            if (v == 0) {
+              row_now = row_next;
+              row_next = rows_of(st + 1);
+              la.seek(g.a, g.lda, row_now);
+            }
+          }
           la.load(v, slot, wave, left, kStep<Op> * g.lda * kElem<Op>, part);
         } else {
           const int u = v - S::LA::kLoads;
-          if (GATHER == 2) lb.seek(u, g.b, g.ldb, row_now);
+          if constexpr (GATHER == 2) {
+            if (u == 0) {
+              row_now = row_next;
+              row_next = rows_of(st + 1);
+              lb.seek(g.b, g.ldb, row_now);
+            }
+          }
           lb.load(u, slot + S::TA::kBytes, wave, left, kStep<Op> * g.ldb * kElem<Op>, part);
         }
       },
