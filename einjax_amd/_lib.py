@@ -192,6 +192,25 @@ def load() -> ctypes.CDLL:
         return _lib
 
 
+EXPERTS_PATH = Path(__file__).resolve().parent / "_experts.so"
+_experts = None
+
+
+def experts():
+    """The torch binding of the expert operators (einjax_amd/_experts.so)."""
+    global _experts
+    if _experts is None:
+        if not EXPERTS_PATH.exists():
+            raise RuntimeError(f"{EXPERTS_PATH} is not built; run "
+                               "`python -m einjax_amd.csrc.build`")
+        import torch  # noqa: F401  (the binding's libraries are torch's)
+
+        from . import _experts as module
+
+        _experts = module
+    return _experts
+
+
 class CapacityError(RuntimeError):
     """An output buffer was smaller than the size the library counted."""
 

@@ -6,7 +6,9 @@ Usage: python -m einjax_amd.csrc.build   (or einjax_amd.csrc.build.build())
 
 Each ``*.hip`` file under this directory is compiled with hipcc to an
 object in ``_build/`` and linked into ``einjax_amd/libejhip.so``.  Packed
-fp32 VALU forms are disabled for all device code.
+fp32 VALU forms are disabled for all device code.  ``experts_torch.cpp``, the
+host-only torch binding of the expert operators, becomes
+``einjax_amd/_experts.so``, which needs libejhip.so beside it.
 """
 
 from __future__ import annotations
@@ -34,6 +36,10 @@ COMMON_FLAGS = [
 ]
 
 
+TORCH_SOURCE = HERE / "experts_torch.cpp"
+TORCH_PATH = PKG / "_experts.so"
+
+
 def _hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), "/opt/rocm/bin/hipcc", shutil.which("hipcc")):
         if cand and Path(cand).exists():
@@ -58,14 +64,55 @@ def _compile(hipcc: str, src: Path) -> Path:
     return obj
 
 
+def _run(cmd: list, what: str) -> None:
+    res = subprocess.run([str(c) for c in cmd], capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{res.stderr}")
+
+
+def _rocm() -> Path:
+    return Path(_hipcc()).resolve().parent.parent
+
+
+def _compile_torch() -> Path:
+    """Compiles the torch binding (host code only)."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    obj = BUILD_DIR / "experts_torch.o"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          "-DTORCH_EXTENSION_NAME=_experts", "-DTORCH_API_INCLUDE_EXTENSION_H",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
+          f"-I{_rocm()}/include", f"-I{sysconfig.get_paths()['include']}",
+          "-c", TORCH_SOURCE, "-o", obj], f"compiling {TORCH_SOURCE.name}")
+    return obj
+
+
+def _link_torch(obj: Path) -> None:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = TORCH_PATH.with_suffix(".so.tmp")
+    _run(["g++", "-shared", "-o", tmp, obj, f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch",
+          "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", f"-L{PKG}", "-lejhip",
+          "-Wl,-rpath,$ORIGIN"], f"linking {TORCH_PATH.name}")
+    os.replace(tmp, TORCH_PATH)
+
+
 def build(verbose: bool = True) -> Path:
-    """Compiles every HIP source and links libejhip.so; returns its path."""
+    """Compiles every HIP source, links libejhip.so and the torch binding on
+    it; returns the library's path."""
     hipcc = _hipcc()
     BUILD_DIR.mkdir(exist_ok=True)
     srcs = sources()
     workers = min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with ThreadPoolExecutor(max_workers=workers) as ex:
+        binding = ex.submit(_compile_torch)
         objs = list(ex.map(lambda s: _compile(hipcc, s), srcs))
+        binding_obj = binding.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -78,8 +125,9 @@ def build(verbose: bool = True) -> Path:
     except OSError as e:
         raise RuntimeError(f"built library does not load: {e}") from e
     os.replace(tmp, LIB_PATH)
+    _link_torch(binding_obj)
     if verbose:
-        print(f"built {LIB_PATH} from {len(srcs)} sources")
+        print(f"built {LIB_PATH} from {len(srcs)} sources, and {TORCH_PATH.name}")
     return LIB_PATH
 
 

@@ -7,7 +7,6 @@ import torch
 
 import einjax_amd as ej
 from einjax_amd import _lib
-from einjax_amd.kernels import experts as K
 
 FAKE = ctypes.c_void_p(16)  # never dereferenced: checks come first
 
@@ -141,33 +140,36 @@ def test_operands_must_be_on_the_gpu():
     for call in (lambda: ej.route_experts(t, 2), lambda: ej.route_experts(t.numpy(), 2),
                  lambda: ej.group_by_expert(t.int(), 4), lambda: ej.quantize_rows(t),
                  lambda: ej.grouped_matmul(t, t[None], t.int()),
-                 lambda: ej.int8_matmul(t, t, t, t), lambda: ej.combine_experts(t, None),
+                 lambda: ej.int8_matmul(t, t, t, t),
+                 lambda: ej.combine_experts(t, ej.ExpertRouting(t, t, t, t, t)),
                  lambda: ej.route_experts_vjp(t, t, t)):
         with pytest.raises(TypeError, match="on the GPU"):
             call()
+    with pytest.raises(TypeError, match="ExpertRouting"):
+        ej.combine_experts(t, None)
 
 
 def test_weight_order_reads_strides():
     w = torch.zeros(3, 5, 7)
-    same, order, gs, rs = K.weight_order(w)
-    assert same is w and (order, gs, rs) == (_lib.EJ_W_KN, 35, 7)
+    same, order, gs, rs = _lib.experts().weight_order(w)
+    assert same.data_ptr() == w.data_ptr() and (order, gs, rs) == (_lib.EJ_W_KN, 35, 7)
     v = torch.zeros(3, 7, 5).transpose(1, 2)
-    same, order, gs, rs = K.weight_order(v)
-    assert same is v and (order, gs, rs) == (_lib.EJ_W_NK, 35, 5)
+    same, order, gs, rs = _lib.experts().weight_order(v)
+    assert same.data_ptr() == v.data_ptr() and (order, gs, rs) == (_lib.EJ_W_NK, 35, 5)
     part = torch.zeros(3, 9, 20)[:, 2:7, 4:11]
-    same, order, gs, rs = K.weight_order(part)
-    assert same is part and (order, gs, rs) == (_lib.EJ_W_KN, 180, 20)
+    same, order, gs, rs = _lib.experts().weight_order(part)
+    assert same.data_ptr() == part.data_ptr() and (order, gs, rs) == (_lib.EJ_W_KN, 180, 20)
     for odd in (torch.zeros(3, 5, 14)[:, :, ::2], torch.zeros(1, 5, 7).expand(3, 5, 7)):
-        copy, order, gs, rs = K.weight_order(odd)
+        copy, order, gs, rs = _lib.experts().weight_order(odd)
         assert copy.is_contiguous() and (order, gs, rs) == (_lib.EJ_W_KN, 35, 7)
     for shape in ((1, 1, 1), (2, 1, 4), (2, 4, 1), (0, 3, 3)):
-        _, order, gs, rs = K.weight_order(torch.zeros(shape))
+        _, order, gs, rs = _lib.experts().weight_order(torch.zeros(shape))
         assert order in (_lib.EJ_W_KN, _lib.EJ_W_NK)
 
 
 def test_rows_of_copies_only_what_it_must():
     t = torch.zeros(6, 8)
-    assert K.rows_of(t) is t
-    assert K.rows_of(t[:, 2:5]).data_ptr() == t[:, 2:5].data_ptr()
-    assert K.rows_of(t.t()).is_contiguous()
-    assert K.rows_of(t[:1].expand(4, 8)).is_contiguous()
+    assert _lib.experts().rows_of(t).data_ptr() == t.data_ptr()
+    assert _lib.experts().rows_of(t[:, 2:5]).data_ptr() == t[:, 2:5].data_ptr()
+    assert _lib.experts().rows_of(t.t()).is_contiguous()
+    assert _lib.experts().rows_of(t[:1].expand(4, 8)).is_contiguous()

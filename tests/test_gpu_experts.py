@@ -614,3 +614,100 @@ def test_int8_weights_past_32_bits(gpu):
     ws = torch.ones(1100, 2048, device="cuda")
     got = ej.int8_matmul(q, torch.ones(5, device="cuda"), w, ws, offsets, out_dtype=F32)
     assert torch.equal(got.double(), q.double() @ w[-1].double().T)
+
+
+# ---- binding -----------------------------------------------------------------------
+
+def test_lengths_of_zero(gpu):
+    x, offsets = torch.ones(4, 0, device="cuda"), torch.tensor([0, 1, 4], device="cuda")
+    y = ej.grouped_matmul(x, torch.ones(2, 0, 5, device="cuda"), offsets)
+    assert y.shape == (4, 5) and bool((y == 0).all())
+    gx, gw = ej.grouped_matmul_vjp(x, torch.ones(2, 0, 5, device="cuda"), offsets, y)
+    assert gx.shape == (4, 0) and gw.shape == (2, 0, 5)
+    x = torch.ones(4, 6, device="cuda")
+    assert ej.grouped_matmul(x, torch.ones(2, 6, 0, device="cuda"), offsets).shape == (4, 0)
+    gx, gw = ej.grouped_matmul_vjp(x, torch.ones(2, 6, 0, device="cuda"), offsets,
+                                   torch.ones(4, 0, device="cuda"))
+    assert bool((gx == 0).all()) and gw.shape == (2, 6, 0)
+    none = ej.route_experts(torch.ones(0, 5, device="cuda"), 2)
+    w = torch.ones(5, 6, 7, device="cuda")
+    y = ej.grouped_matmul(torch.ones(0, 6, device="cuda"), w, none, gather=True)
+    assert y.shape == (0, 7)
+    gx, gw = ej.grouped_matmul_vjp(torch.ones(0, 6, device="cuda"), w, none, y, gather=True)
+    assert gx.shape == (0, 6) and bool((gw == 0).all()) and gw.shape == w.shape
+    assert ej.combine_experts(y, none).shape == (0, 7)
+    q, s = ej.quantize_rows(torch.ones(3, 0, device="cuda"))
+    assert q.shape == (3, 0) and s.tolist() == [0, 0, 0]
+    assert bool((ej.int8_matmul(q, s, torch.ones(4, 0, device="cuda").to(torch.int8),
+                                torch.ones(4, device="cuda")) == 0).all())
+
+
+def test_gradients_are_first_order(gpu):
+    x = torch.randn(6, 8, device="cuda", requires_grad=True)
+    w = torch.randn(2, 8, 8, device="cuda", requires_grad=True)
+    logits = torch.randn(6, 4, device="cuda", requires_grad=True)
+    offsets = torch.tensor([0, 2, 6], device="cuda")
+    r = ej.route_experts(logits, 1, renormalize=False)
+    for out, leaf in ((ej.grouped_matmul(x, w, offsets), x), (ej.grouped_matmul(x, w, offsets), w),
+                      (r.weights, logits), (ej.combine_experts(x, r), x)):
+        plain = torch.autograd.grad(out.sum(), leaf, retain_graph=True)[0]
+        (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="first order"):
+            g.sum().backward()
+
+
+def test_gradients_of_one_side_and_accumulation(gpu):
+    g = rng(12)
+    offsets = torch.tensor([0, 10, 30], device="cuda")
+    x, w = randn(g, 30, 24), randn(g, 2, 24, 16)
+    both = ej.grouped_matmul_vjp(x, w, offsets, torch.ones(30, 16, device="cuda"))
+    for side in (0, 1):
+        leaf = (x, w)[side].clone().requires_grad_()
+        args = [x, w]
+        args[side] = leaf
+        for _ in range(2):
+            ej.grouped_matmul(*args, offsets).sum().backward()  # an expanded cotangent
+        assert torch.equal(leaf.grad, 2 * both[side])
+    assert ej.grouped_matmul_vjp(x, w, offsets, both[0][:, :16], need_x=False)[0] is None
+    with torch.no_grad():
+        assert not ej.grouped_matmul(x, leaf, offsets).requires_grad
+
+
+def test_refusals_of_gpu_tensors(gpu):
+    f = torch.zeros(4, 8, device="cuda")
+    w = torch.zeros(2, 8, 8, device="cuda")
+    offsets = torch.tensor([0, 2, 4], device="cuda")
+    r = ej.group_by_expert(torch.zeros(4, 1, dtype=torch.long, device="cuda"), 2)
+    value = [lambda: ej.route_experts(f[0], 1), lambda: ej.route_experts(f, 0),
+             lambda: ej.route_experts(f, 9), lambda: ej.grouped_matmul(f, w[0], offsets),
+             lambda: ej.grouped_matmul(f[:, :7], w, offsets),
+             lambda: ej.grouped_matmul(f, w, offsets[:2]),
+             lambda: ej.grouped_matmul(f, w, offsets, gather=True),
+             lambda: ej.grouped_matmul(f[:3], w, r, gather=True),
+             lambda: ej.grouped_matmul(f, w[:1], r),
+             lambda: ej.grouped_matmul_vjp(f, w, offsets, f[:3]),
+             lambda: ej.combine_experts(f[:3], r),
+             lambda: ej.combine_experts(f, r, torch.zeros(4, 2, device="cuda")),
+             lambda: ej.combine_experts(f, r, torch.zeros(4, 1, device="cuda").double()),
+             lambda: ej.combine_experts_vjp(f, r, f[:, :4]),
+             lambda: ej.group_by_expert(offsets, 2),
+             lambda: ej.group_by_expert(offsets[None], 2, f),
+             lambda: ej.quantize_rows(f[0, 0])]
+    kind = [lambda: ej.route_experts(f.int(), 1), lambda: ej.grouped_matmul(f.double(), w, offsets),
+            lambda: ej.grouped_matmul(f, w.bfloat16(), offsets),
+            lambda: ej.grouped_matmul(f, w, offsets.float()),
+            lambda: ej.grouped_matmul(f, w, offsets, out_dtype=torch.float16),
+            lambda: ej.grouped_matmul(f, w, offsets.cpu()),
+            lambda: ej.combine_experts(f.int(), r), lambda: ej.quantize_rows(f.int()),
+            lambda: ej.int8_matmul(f, f[:, 0], f, f[:, 0])]
+    for call in value:
+        with pytest.raises(ValueError):
+            call()
+    for call in kind:
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(NotImplementedError):
+        ej.route_experts(torch.zeros(2, 2000, device="cuda"), 2)
+    with pytest.raises(NotImplementedError):
+        ej.route_experts(torch.zeros(2, 100, device="cuda"), 17)
