@@ -23,7 +23,8 @@ namespace {
 
 constexpr int kMaxPicks = 16;
 constexpr int kMaxExperts = 1024;
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 1024;  // a workgroup a CU: one pass of 64 tokens
+constexpr int kVjpThreads = 256;
 constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / 64;
 constexpr int kRouteBlocks = 256;   // bound on the workgroups whose counts are added up
@@ -345,11 +346,11 @@ __global__ __launch_bounds__(kGroupThreads) void route_small_kernel(RouteArgs a)
 //   renormalized: dl_e = w_e (d_e - dot) at the picks, 0 elsewhere;
 //   otherwise:    dl_e = p_e ([e picked] d_e - dot).
 template <int L, int V>
-__global__ __launch_bounds__(kRouteThreads) void route_vjp_kernel(RouteArgs a, const float *grad,
+__global__ __launch_bounds__(kVjpThreads) void route_vjp_kernel(RouteArgs a, const float *grad,
                                                                   void *grad_logits) {
   const int lane = threadIdx.x % L;
   const int64_t t =
-      static_cast<int64_t>(blockIdx.x) * (kRouteThreads / L) + threadIdx.x / L;
+      static_cast<int64_t>(blockIdx.x) * (kVjpThreads / L) + threadIdx.x / L;
   if (t >= a.n_tokens) return;
   float x[V];
   float top = -INFINITY;
@@ -470,7 +471,7 @@ int run_route(RouteArgs a, void *workspace, size_t workspace_bytes, hipStream_t 
   EJ_CHECK_ARG(workspace && workspace_bytes >= need, "workspace of %zu bytes, expected %zu",
                workspace_bytes, need);
   a.counts = static_cast<int32_t *>(workspace);
-  // whole passes of 16 tokens a workgroup
+  // as many tokens a workgroup as keep the workgroups at one a CU, in sixteens
   a.tokens_per_block =
       static_cast<int32_t>(ceil_div(ceil_div(a.n_tokens, kRouteBlocks), 16) * 16);
   const unsigned blocks = static_cast<unsigned>(ceil_div(a.n_tokens, a.tokens_per_block));
@@ -557,8 +558,8 @@ extern "C" int ej_expert_route_vjp(const void *logits, int32_t dtype, int64_t n_
   return by_experts(n_experts, [&](auto L, auto V) {
     constexpr int l = decltype(L)::value;
     hipLaunchKernelGGL((route_vjp_kernel<l, decltype(V)::value>),
-                       dim3(static_cast<unsigned>(ceil_div(n_tokens, kRouteThreads / l))),
-                       dim3(kRouteThreads), 0, as_stream(stream), a, grad_weights, grad_logits);
+                       dim3(static_cast<unsigned>(ceil_div(n_tokens, kVjpThreads / l))),
+                       dim3(kVjpThreads), 0, as_stream(stream), a, grad_weights, grad_logits);
     EJ_LAUNCH_CHECK();
     return EJ_OK;
   });
