@@ -331,7 +331,10 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
   using S = TileShape<Op, BM, BN, WR, WC, false, false, DIRECT, NS>;
   __shared__ __align__(1024) unsigned char ring[S::kLds];
   const uint32_t per = g.row_blocks * g.col_blocks;
-  const uint32_t lb_ = xcd_logical_block(gridDim.x);
+  // runs of blocks dealt to the XCDs in turn: as one part each, the XCD of the
+  // longest group ends last (16384 rows in 16 groups of unequal length, 2048 x
+  // 4096 bf16: 363 us so, 305 dealt; groups of equal length 285 and 287)
+  const uint32_t lb_ = xcd_logical_block(gridDim.x, kXcdRun);
   const int group = lb_ / per;
   int rb, cb, lo, hi;
   band_pos(lb_ - group * per, g.row_blocks, g.col_blocks, 1024 / BM, &rb, &cb);
