@@ -70,8 +70,7 @@ __device__ inline T ld_uniform(const T *p, int64_t i) {
 // one region, as for skewed sparsity, stays balanced); the last, partial
 // round of runs is split into 8 contiguous parts.  Block ids from `live` on
 // keep their id: they lie beyond the work of a grid sized for a bound.
-__device__ inline uint32_t xcd_logical_block(uint32_t live, uint32_t run = 0) {
-  const uint32_t bid = blockIdx.x;
+__device__ inline uint32_t xcd_logical_of(uint32_t bid, uint32_t live, uint32_t run) {
   if (bid >= live) return bid;
   const uint32_t full = run > 0 ? live / (8 * run) * (8 * run) : 0;
   const uint32_t xcd = bid % 8;
@@ -83,6 +82,9 @@ __device__ inline uint32_t xcd_logical_block(uint32_t live, uint32_t run = 0) {
   const uint32_t per = rest / 8, rem = rest % 8;
   const uint32_t start = xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per;
   return full + start + local;
+}
+__device__ inline uint32_t xcd_logical_block(uint32_t live, uint32_t run = 0) {
+  return xcd_logical_of(blockIdx.x, live, run);
 }
 
 // x / d (and the remainder) of workgroup-uniform values, kept in scalar

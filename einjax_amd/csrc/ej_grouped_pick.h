@@ -32,6 +32,19 @@ int launch_rows(GroupedArgs g, hipStream_t stream) {
   return g.splits > 1 ? join_parts(g, g.slots, g.slots, true, stream) : EJ_OK;
 }
 
+template <class Op, bool BKC>
+int launch_large(GroupedArgs g, hipStream_t stream) {
+  const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
+  g.row_blocks = static_cast<uint32_t>(g.slots / 256 + groups);
+  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, 256));
+  dim3 grid;
+  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kLargeExtra + kZeroBlocks,
+                      512, &grid));
+  hipLaunchKernelGGL((grouped_large_kernel<Op, BKC>), grid, dim3(512), 0, stream, g);
+  EJ_LAUNCH_CHECK();
+  return EJ_OK;
+}
+
 template <class Op, int FM, int BN, int NW, bool BKC, int NS>
 int launch_skinny(GroupedArgs g, hipStream_t stream) {
   const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
@@ -74,15 +87,26 @@ inline double expected_tiles(const GroupedArgs &g, int bm, int bn, int64_t group
   return (static_cast<double>(g.slots) / bm + 0.5 * groups) * ceil_div(g.n, bn);
 }
 
+// Rounds of the large kernel for `tiles` blocks: the last one cut in four or
+// two where that fills it.
+inline double large_rounds(double tiles) {
+  const double whole = std::floor(tiles / kLargeRound), last = tiles / kLargeRound - whole;
+  return whole + (last <= 0 ? 0 : last <= 0.25 ? 0.4 : last <= 0.5 ? 0.6 : 1);
+}
+
 // The choice goes by the mean rows of a group (all that the host knows of the
-// sizes).  Measured on bf16, 16 groups, k = 2048, n = 2048 (us):
-//   rows/group   skinny 16  64 x 64   64 x 128  128 x 128
-//        2 (E=8)   6.5/8.0   9.6       11.4      17.9       k = n = 1024, [n][k]/[k][n]
-//       16 (E=8)  15.2/19.5 16.5       19.5      29
-//       32 (E=8)  25.9      17.2       20.2      34
-//       50        70                   38        39
-//      100                             42        48
-//      200                             62        52
+// sizes) and the number of tiles.  Measured (us) with k = n = 2048, bf16, W
+// [n][k] / [k][n], groups of unequal length; skinny 16 rows at k = n = 1024:
+//   rows/group  groups   skinny 16  64 x 64   64 x 128  128 x 128  large
+//        2         8      6.5/8.0   9.6       11.4      17.9
+//       16         8     15.2/19.5  16.5      19.5      29
+//       50         8                17/18     21/20     28/27      21/21
+//       50        16                33/33     31/32     29/29      29/31
+//      100         8                18/18     21/20     27/27      21/22
+//      100        16                41/41     34/35     33/32      30/33
+//      200        16                57/59     49/50     42/40      50/51
+//      512        16                                    98/98      78/80
+//       64 (k 1024)  64             63/63     59/58     67/69      61/62
 template <class Op, bool BKC>
 int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
@@ -105,14 +129,15 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
     // within 2% at 16384 x 2048 x 2048)
     return launch_rows<Op, 64, 64, 2, 2, BKC, true, 0>(g, stream);
   } else {
-    if (rows <= 48) return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
+    // up to about two small tiles to a CU the finest spread best
+    if (rows <= 48 || expected_tiles(g, 64, 64, groups) <= 576)
+      return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
     if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, true, 3>(g, stream);
-    // rounds of 256 workgroups at a time, against a fifth less time for a
-    // round of 512 quarter-size ones (two to a CU, which even out)
-    const double big = std::ceil(expected_tiles(g, 256, 256, groups) / 256);
+    // rounds of large blocks against a fifth less time for a round of 512
+    // quarter-size ones (two to a CU, which even out)
     const double small = expected_tiles(g, 128, 128, groups) / 512;
-    if (big <= 0.8 * (small > 1 ? small : 1))
-      return launch_rows<Op, 256, 256, 2, 4, BKC, true, 0>(g, stream);
+    if (large_rounds(expected_tiles(g, 256, 256, groups)) <= 0.8 * (small > 1 ? small : 1))
+      return launch_large<Op, BKC>(g, stream);
     return launch_rows<Op, 128, 128, 2, 2, BKC, true, 2>(g, stream);
   }
 }

@@ -228,26 +228,13 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
   }
 }
 
-// C rows of one row block of a group times one block of columns.
+// C rows of one row block of a group times the BN columns from n0.
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
-__global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
-#if defined(__HIP_DEVICE_COMPILE__)
+__device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsigned char *ring) {
   using S = TileShape<Op, BM, BN, WR, WC, true, BKC, DIRECT, NS>;
-  __shared__ __align__(1024) unsigned char ring[S::kLds];
-  const uint32_t grid = g.row_blocks * g.col_blocks;
-  if (blockIdx.x >= grid) {
-    if (blockIdx.y == 0) zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
-    return;
-  }
-  const uint32_t rbs = live_row_blocks(g, BM), live = rbs * g.col_blocks;
-  if (blockIdx.x >= live) return;
-  int rb, cb;
-  band_pos(xcd_logical_block(live), rbs, g.col_blocks, 1024 / BM, &rb, &cb);
-  const RowBlock r = find_row_block(g, BM, rb);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row0 = wave / WC * S::WM, col0 = wave % WC * S::WN;
-  const int n0 = cb * BN;
   int st0, st1;
   part_of((g.k + kStep<Op> - 1) / kStep<Op>, blockIdx.y, g.splits, &st0, &st1);
   const int64_t k0 = static_cast<int64_t>(st0) * kStep<Op>;
@@ -317,6 +304,76 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
       }
       put4(g.c, g.out, s * g.ldc, col, g.n, vec, v);
     }
+  }
+}
+
+// A workgroup for each row block of a group and block of columns.
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
+__global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using S = TileShape<Op, BM, BN, WR, WC, true, BKC, DIRECT, NS>;
+  __shared__ __align__(1024) unsigned char ring[S::kLds];
+  const uint32_t grid = g.row_blocks * g.col_blocks;
+  if (blockIdx.x >= grid) {
+    if (blockIdx.y == 0) zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
+    return;
+  }
+  const uint32_t rbs = live_row_blocks(g, BM), live = rbs * g.col_blocks;
+  if (blockIdx.x >= live) return;
+  int rb, cb;
+  band_pos(xcd_logical_block(live), rbs, g.col_blocks, 1024 / BM, &rb, &cb);
+  rows_block<Op, BM, BN, WR, WC, BKC, DIRECT, NS>(g, find_row_block(g, BM, rb), cb * BN, ring);
+#endif
+}
+
+// The same in blocks of 256 x 256, one workgroup to a CU, which therefore run
+// in rounds of kLargeRound.  Blocks of at most 128 rows (the end of a group)
+// take half the work.  The blocks of a last round that would leave half the
+// CUs idle or more are cut in two or four, a workgroup each.
+constexpr uint32_t kLargeRound = 256;
+constexpr uint32_t kLargeExtra = 192;  // workgroups that cutting adds at most
+
+template <class Op, bool BKC>
+__global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using S = TileShape<Op, 256, 256, 2, 4, true, BKC, true, 0>;
+  __shared__ __align__(1024) unsigned char ring[S::kLds];
+  const uint32_t grid = g.row_blocks * g.col_blocks + kLargeExtra;
+  if (blockIdx.x >= grid) {
+    zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
+    return;
+  }
+  const uint32_t rbs = live_row_blocks(g, 256), live = rbs * g.col_blocks;
+  uint32_t whole = live / kLargeRound * kLargeRound;
+  const uint32_t last = live - whole;
+  const uint32_t parts = last <= kLargeRound / 4 ? 4 : last <= kLargeRound / 2 ? 2 : 1;
+  if (parts == 1) whole = live;
+  uint32_t block, part = 0;
+  if (blockIdx.x < whole) {
+    block = xcd_logical_block(whole);
+  } else {
+    const uint32_t units = (live - whole) * parts;
+    if (blockIdx.x - whole >= units) return;
+    const uint32_t u = xcd_logical_of(blockIdx.x - whole, units, 0);
+    block = whole + u / parts;
+    part = u % parts;
+  }
+  int rb, cb;
+  band_pos(block, rbs, g.col_blocks, 4, &rb, &cb);
+  RowBlock r = find_row_block(g, 256, rb);
+  int n0 = cb * 256;
+  if (blockIdx.x >= whole) {
+    r.lo += (part & 1) * 128;
+    n0 += (part >> 1) * 128;
+    if (r.lo >= r.hi || n0 >= g.n) return;
+    if (parts == 4)
+      rows_block<Op, 128, 128, 2, 4, BKC, true, 0>(g, r, n0, ring);
+    else
+      rows_block<Op, 128, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
+  } else if (r.hi - r.lo <= 128) {
+    rows_block<Op, 128, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
+  } else {
+    rows_block<Op, 256, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
   }
 #endif
 }
