@@ -81,6 +81,25 @@ int launch_wgrad(const GroupedArgs &g, hipStream_t stream) {
   return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 0>(g, stream);
 }
 
+template <class Op, int GATHER>
+int launch_wgrad_large_as(GroupedArgs g, hipStream_t stream) {
+  g.row_blocks = static_cast<uint32_t>(ceil_div(g.m, 256));
+  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, 256));
+  dim3 grid;
+  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks * g.n_groups + kLargeExtra,
+                      512, &grid));
+  hipLaunchKernelGGL((grouped_wgrad_large_kernel<Op, GATHER>), grid, dim3(512), 0, stream, g);
+  EJ_LAUNCH_CHECK();
+  return EJ_OK;
+}
+
+template <class Op>
+int launch_wgrad_large(const GroupedArgs &g, hipStream_t stream) {
+  if (g.a_rows) return launch_wgrad_large_as<Op, 1>(g, stream);
+  if (g.b_rows) return launch_wgrad_large_as<Op, 2>(g, stream);
+  return launch_wgrad_large_as<Op, 0>(g, stream);
+}
+
 // Tiles of a rows product: full row blocks and, on average, half of one for
 // each group.
 inline double expected_tiles(const GroupedArgs &g, int bm, int bn, int64_t groups) {
@@ -142,20 +161,32 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
   }
 }
 
-// The largest tile that leaves a workgroup for every CU.  Measured (us) on
-// 16384 rows, 16 groups, 2048 x 4096 bf16: 256 x 256 343, 128 x 128 400; fp32
-// 4096 rows, 8 groups, 1024 x 2048: 128 x 128 199, 64 x 64 210; 1200 rows, 5
-// groups, 320 x 520: 30 and 12.
+// 64 x 64 where larger tiles leave CUs idle, then 128 x 128 (two to a CU)
+// against rounds of the large blocks.  Measured (us), bf16, rows as they lie /
+// gathered, groups of unequal length:
+//   rows   groups    m x n       64 x 64   128 x 128  large
+//    4096     3   1024 x 1024    20/29      26/36     21/31
+//    8192     5   1024 x 1024    37/44      32/46     34/48
+//    8192    17   1024 x 1024    41/57      33/41     32/37
+//    8192    17   1536 x 1536               62/78     60/67
+//    8192     8   2048 x 2560              107/137    92/107
+//   16384    16   2048 x 4096   547/729    378/474   300/336
+// fp32: 4096 rows, 8 groups, 1024 x 2048: 128 x 128 157, 64 x 64 167; 1200
+// rows, 5 groups, 320 x 520: 32 and 13.
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
   if (!direct) return launch_wgrad<Op, 64, 64, 2, 2, false, 2>(g, stream);
   if (g.splits > 1) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
-  auto tiles = [&](int b) { return ceil_div(g.m, b) * ceil_div(g.n, b) * g.n_groups; };
+  auto tiles = [&](int b) {
+    return static_cast<double>(ceil_div(g.m, b) * ceil_div(g.n, b) * g.n_groups);
+  };
+  if (tiles(128) < 256) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
   if constexpr (kElem<Op> == 2) {
-    if (tiles(256) >= 256) return launch_wgrad<Op, 256, 256, 2, 4, true, 0>(g, stream);
+    const double small = tiles(128) / 512;
+    if (large_rounds(tiles(256)) <= 0.55 * (small > 1 ? small : 1))
+      return launch_wgrad_large<Op>(g, stream);
   }
-  if (tiles(128) >= 256) return launch_wgrad<Op, 128, 128, 2, 2, true, 2>(g, stream);
-  return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
+  return launch_wgrad<Op, 128, 128, 2, 2, true, 2>(g, stream);
 }
 
 }  // namespace ej

@@ -326,13 +326,40 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
 #endif
 }
 
-// The same in blocks of 256 x 256, one workgroup to a CU, which therefore run
-// in rounds of kLargeRound.  Blocks of at most 128 rows (the end of a group)
-// take half the work.  The blocks of a last round that would leave half the
-// CUs idle or more are cut in two or four, a workgroup each.
+// Large blocks of 256 x 256 results, one workgroup to a CU, run in rounds of
+// kLargeRound.  The blocks of a last round that would leave half the CUs idle
+// or more are cut in two (128 x 256) or four (128 x 128), a workgroup each.
 constexpr uint32_t kLargeRound = 256;
 constexpr uint32_t kLargeExtra = 192;  // workgroups that cutting adds at most
 
+// The work of a workgroup: a block, or from row, col of it one of `parts`.
+struct LargeUnit {
+  uint32_t block, parts;
+  int row, col;
+  __device__ inline bool find(uint32_t live, uint32_t run) {
+    uint32_t whole = live / kLargeRound * kLargeRound;
+    const uint32_t last = live - whole;
+    const uint32_t cut = last <= kLargeRound / 4 ? 4 : last <= kLargeRound / 2 ? 2 : 1;
+    if (cut == 1) whole = live;
+    parts = 1;
+    row = col = 0;
+    if (blockIdx.x < whole) {
+      block = xcd_logical_block(whole, run);
+      return true;
+    }
+    const uint32_t units = (live - whole) * cut;
+    if (blockIdx.x - whole >= units) return false;
+    const uint32_t u = xcd_logical_of(blockIdx.x - whole, units, 0), part = u % cut;
+    parts = cut;
+    block = whole + u / cut;
+    row = (part & 1) * 128;
+    col = (part >> 1) * 128;
+    return true;
+  }
+};
+
+// Rows in large blocks.  One of at most 128 rows (the end of a group) takes
+// half the work.
 template <class Op, bool BKC>
 __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -343,58 +370,31 @@ __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
     zero_dead_rows(g, blockIdx.x - grid, gridDim.x - grid);
     return;
   }
-  const uint32_t rbs = live_row_blocks(g, 256), live = rbs * g.col_blocks;
-  uint32_t whole = live / kLargeRound * kLargeRound;
-  const uint32_t last = live - whole;
-  const uint32_t parts = last <= kLargeRound / 4 ? 4 : last <= kLargeRound / 2 ? 2 : 1;
-  if (parts == 1) whole = live;
-  uint32_t block, part = 0;
-  if (blockIdx.x < whole) {
-    block = xcd_logical_block(whole);
-  } else {
-    const uint32_t units = (live - whole) * parts;
-    if (blockIdx.x - whole >= units) return;
-    const uint32_t u = xcd_logical_of(blockIdx.x - whole, units, 0);
-    block = whole + u / parts;
-    part = u % parts;
-  }
+  const uint32_t rbs = live_row_blocks(g, 256);
+  LargeUnit u;
+  if (!u.find(rbs * g.col_blocks, 0)) return;
   int rb, cb;
-  band_pos(block, rbs, g.col_blocks, 4, &rb, &cb);
+  band_pos(u.block, rbs, g.col_blocks, 4, &rb, &cb);
   RowBlock r = find_row_block(g, 256, rb);
-  int n0 = cb * 256;
-  if (blockIdx.x >= whole) {
-    r.lo += (part & 1) * 128;
-    n0 += (part >> 1) * 128;
-    if (r.lo >= r.hi || n0 >= g.n) return;
-    if (parts == 4)
-      rows_block<Op, 128, 128, 2, 4, BKC, true, 0>(g, r, n0, ring);
-    else
-      rows_block<Op, 128, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
-  } else if (r.hi - r.lo <= 128) {
+  r.lo += u.row;
+  const int n0 = cb * 256 + u.col;
+  if (r.lo >= r.hi || n0 >= g.n) return;
+  if (u.parts == 4)
+    rows_block<Op, 128, 128, 2, 4, BKC, true, 0>(g, r, n0, ring);
+  else if (u.parts == 2 || r.hi - r.lo <= 128)
     rows_block<Op, 128, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
-  } else {
+  else
     rows_block<Op, 256, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
-  }
 #endif
 }
 
-// D_e block: rows i of P's columns, columns j of Q's, over the slots of group
-// e.  The bound row_blocks x col_blocks covers one group's D; the grid holds
-// n_groups of them, and a group without slots writes zeros.  GATHER: 1 if P's
-// rows go through an index, 2 if Q's do.
+// D_e block: the BM columns of P from m0 (rows of the result) by the BN
+// columns of Q from n0, over the slots of a group; one without slots writes
+// zeros.  GATHER: 1 if P's rows go through an index, 2 if Q's do.
 template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
-__global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs g) {
-#if defined(__HIP_DEVICE_COMPILE__)
+__device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, unsigned char *ring) {
   using S = TileShape<Op, BM, BN, WR, WC, false, false, DIRECT, NS>;
-  __shared__ __align__(1024) unsigned char ring[S::kLds];
-  const uint32_t per = g.row_blocks * g.col_blocks;
-  // runs of blocks dealt to the XCDs in turn: as one part each, the XCD of the
-  // longest group ends last (16384 rows in 16 groups of unequal length, 2048 x
-  // 4096 bf16: 363 us so, 305 dealt; groups of equal length 285 and 287)
-  const uint32_t lb_ = xcd_logical_block(gridDim.x, kXcdRun);
-  const int group = lb_ / per;
-  int rb, cb, lo, hi;
-  band_pos(lb_ - group * per, g.row_blocks, g.col_blocks, 1024 / BM, &rb, &cb);
+  int lo, hi;
   group_range(g, group, &lo, &hi);
   lo = __builtin_amdgcn_readfirstlane(lo);
   hi = __builtin_amdgcn_readfirstlane(hi);
@@ -413,8 +413,8 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
     g.ldc = g.n;
     g.out = EJ_F32;
   }
-  la.init_m(wave, lane, g.a + (GATHER == 1 ? 0 : lo * g.lda * kElem<Op>), g.lda, rb * BM, g.m);
-  lb.init_m(wave, lane, g.b + (GATHER == 2 ? 0 : lo * g.ldb * kElem<Op>), g.ldb, cb * BN, g.n);
+  la.init_m(wave, lane, g.a + (GATHER == 1 ? 0 : lo * g.lda * kElem<Op>), g.lda, m0, g.m);
+  lb.init_m(wave, lane, g.b + (GATHER == 2 ? 0 : lo * g.ldb * kElem<Op>), g.ldb, n0, g.n);
   // the gathered operand's rows of a stage, lane by lane, read a stage ahead
   const int32_t *rows = GATHER == 1 ? g.a_rows : g.b_rows;
   const int64_t n_rows = GATHER == 1 ? g.n_a : g.n_b;
@@ -465,17 +465,58 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
   const bool vec = vec_rows(g);
 #pragma unroll
   for (int i = 0; i < S::FM; ++i) {
-    const int row = rb * BM + row0 + i * 16 + (lane & 15);
+    const int row = m0 + row0 + i * 16 + (lane & 15);
     if (row >= g.m) continue;
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
-      const int col = cb * BN + col0 + j * 16 + (lane >> 4) * 4;
+      const int col = n0 + col0 + j * 16 + (lane >> 4) * 4;
       if (col >= g.n) continue;
       const float v[4] = {static_cast<float>(acc[i][j][0]), static_cast<float>(acc[i][j][1]),
                           static_cast<float>(acc[i][j][2]), static_cast<float>(acc[i][j][3])};
       put4(g.c, g.out, group * g.c_group + static_cast<int64_t>(row) * g.ldc, col, g.n, vec, v);
     }
   }
+}
+
+// row_blocks x col_blocks covers one group's D; the grid holds n_groups of
+// them.
+template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
+__global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using S = TileShape<Op, BM, BN, WR, WC, false, false, DIRECT, NS>;
+  __shared__ __align__(1024) unsigned char ring[S::kLds];
+  const uint32_t per = g.row_blocks * g.col_blocks;
+  // runs of blocks dealt to the XCDs in turn: as one part each, the XCD of the
+  // longest group ends last (16384 rows in 16 groups of unequal length, 2048 x
+  // 4096 bf16, 256 x 256: 363 us so, 305 dealt; groups of equal length 285 and
+  // 287)
+  const uint32_t block = xcd_logical_block(gridDim.x, kXcdRun), group = block / per;
+  int rb, cb;
+  band_pos(block - group * per, g.row_blocks, g.col_blocks, 1024 / BM, &rb, &cb);
+  wgrad_block<Op, BM, BN, WR, WC, DIRECT, NS, GATHER>(g, group, rb * BM, cb * BN, ring);
+#endif
+}
+
+// The same in blocks of 256 x 256, cut as grouped_large_kernel's.
+template <class Op, int GATHER>
+__global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using S = TileShape<Op, 256, 256, 2, 4, false, false, true, 0>;
+  __shared__ __align__(1024) unsigned char ring[S::kLds];
+  const uint32_t per = g.row_blocks * g.col_blocks;
+  LargeUnit u;
+  if (!u.find(per * g.n_groups, kXcdRun)) return;
+  const uint32_t group = u.block / per;
+  int rb, cb;
+  band_pos(u.block - group * per, g.row_blocks, g.col_blocks, 4, &rb, &cb);
+  const int m0 = rb * 256 + u.row, n0 = cb * 256 + u.col;
+  if (m0 >= g.m || n0 >= g.n) return;
+  if (u.parts == 4)
+    wgrad_block<Op, 128, 128, 2, 4, true, 0, GATHER>(g, group, m0, n0, ring);
+  else if (u.parts == 2 || g.m - m0 <= 128)
+    wgrad_block<Op, 128, 256, 2, 4, true, 0, GATHER>(g, group, m0, n0, ring);
+  else
+    wgrad_block<Op, 256, 256, 2, 4, true, 0, GATHER>(g, group, m0, n0, ring);
 #endif
 }
 

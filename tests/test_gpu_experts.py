@@ -297,6 +297,73 @@ def test_grouped_matmul_gradients(gpu, t, e, k, n_in, n_out, kind, dtype, order)
         assert_within(gx, wx, bound)
 
 
+# Groups of 256-row blocks that are cut in different ways: rows of each group,
+# slots of no group behind them, k, n.
+LARGE = [
+    ([1000], 24, 64, 4096), ([1024, 0, 512], 0, 64, 4104), ([300, 0, 724], 0, 128, 6144),
+    ([900, 1100, 1000, 1096], 5, 72, 4096), ([900, 1100, 1000, 1096], 0, 16, 6400),
+    ([129, 128, 1, 1790], 3, 192, 4112),
+]
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("sizes,dead,k,n", LARGE)
+def test_grouped_matmul_large_blocks(gpu, sizes, dead, k, n, dtype, order):
+    g, e, live = rng(k + n), len(sizes), sum(sizes)
+    offsets = torch.tensor([sum(sizes[:i]) for i in range(e + 1)], dtype=torch.int32,
+                           device="cuda")
+    x = randn(g, live + dead, k, dtype=dtype)
+    w = randn(g, e, k, n, dtype=dtype, scale=k ** -0.5)
+    if order == "nk":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    x[live:] = float("nan")
+    got = ej.grouped_matmul(x, w, offsets)
+    x[live:] = 0
+    want, mag = product64(x, None, offsets, w, live + dead)
+    assert_within(got, want, sum_bound(want, mag, k, dtype))
+    if dtype == F16:
+        return
+    # the gradient to x with the same blocks, k and n exchanged, and in 8 bits
+    wt = w.transpose(1, 2)
+    cot = randn(g, live + dead, k, dtype=dtype)
+    gx, _ = ej.grouped_matmul_vjp(randn(g, live + dead, n, dtype=dtype), wt, offsets, cot,
+                                  need_w=False)
+    cot[live:] = 0
+    want, mag = product64(cot, None, offsets, w, live + dead)
+    assert_within(gx, want, sum_bound(want, mag, k, dtype))
+    q = torch.randint(-128, 128, (live + dead, k), generator=g, device="cuda").to(torch.int8)
+    p = torch.randint(-128, 128, (e, n, k), generator=g, device="cuda").to(torch.int8)
+    qs, ps = (torch.rand(s, generator=g, device="cuda") for s in (live + dead, (e, n)))
+    got = ej.int8_matmul(q, qs, p, ps, offsets, out_dtype=F32)
+    q[live:] = 0
+    want, _ = product64(q, None, offsets, p.transpose(1, 2), live + dead)
+    owner = torch.tensor([max(o, 0) for o in row_groups(offsets, live + dead)[0]], device="cuda")
+    want = want * qs.double()[:, None] * ps[owner].double()
+    assert_within(got, want, 5 * 2.0 ** -24 * want.abs() + TINY[F32])
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("sizes,m,n", [
+    ([70, 0, 131, 64], 1024, 1024), ([40, 0, 200, 1, 65, 31, 90, 33, 64], 2048, 2048),
+    ([3, 70, 64, 90, 1, 0, 128, 40, 10], 2048, 2312), ([129, 30, 0, 77], 2048, 4000)])
+def test_grouped_weight_gradient_large_blocks(gpu, sizes, m, n, dtype, gather):
+    g, e, live = rng(m + n), len(sizes), sum(sizes)
+    r = ej.group_by_expert(torch.repeat_interleave(torch.arange(e), torch.tensor(sizes))
+                           [torch.randperm(live, generator=torch.Generator().manual_seed(n))]
+                           .cuda()[:, None], e)
+    x, w = randn(g, live, m, dtype=dtype), randn(g, e, m, n, dtype=dtype)
+    cot = randn(g, live, n, dtype=dtype)
+    _, gw = ej.grouped_matmul_vjp(x, w, r, cot, gather=gather, need_x=False)
+    _, ends = row_groups(r.offsets, live)
+    for i in range(e):
+        a, b = ends[i], ends[i + 1]
+        xi = (x[r.rows[a:b].long()] if gather else x[a:b]).double()
+        gi = cot[a:b].double()
+        assert_within(gw[i], xi.T @ gi, sum_bound(xi.T @ gi, xi.abs().T @ gi.abs(), b - a, dtype))
+
+
 def test_grouped_gradients_against_differences(gpu):
     g, r, x, w = product_case(40, 5, 2, 24, 36, "skew", F32, "kn", True)
     cot = randn(g, 80, 36)
