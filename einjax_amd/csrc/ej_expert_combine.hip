@@ -62,7 +62,10 @@ struct CombineArgs {
 };
 
 // out[t] = sum_j weights[t, j] y[slots[t, j]]: summed in fp32 in the order of
-// the picks, rounded once.  One workgroup a token and stretch of columns.
+// the picks, rounded once.  One workgroup a token and stretch of columns, so a
+// token's indices and weights are read once for 256 lanes.  16384 tokens of 4
+// picks, 4096 columns of bf16, 1 pair in 20 left out: 139 us (0.65 GB, 4.6
+// TB/s; a large copy reaches 5.2).
 template <class T, class O, bool VEC>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsigned col_blocks) {
   constexpr int N = Piece<T, VEC>::N;
@@ -87,7 +90,8 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsign
 
 // grad_y[slots[t, j]] = weights[t, j] grad[t]; grad_w[t, j] = grad[t] . y[slots[t, j]].
 // One workgroup a token, so every dot product is summed in a fixed order;
-// workgroups past the tokens zero grad_y's rows that no pair holds.
+// workgroups past the tokens zero grad_y's rows that no pair holds.  At the
+// sizes above 230 us (1.18 GB, 5.1 TB/s).
 template <class T, bool VEC>
 __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, const void *grad,
                                                                int64_t ld_grad, void *grad_y,
@@ -157,6 +161,7 @@ __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, co
 //   - the rounded quotient comes from x times 1 / scale plus 1.5 2^23, whose
 //     low byte is the result; where that product lies near a tie, which it can
 //     be off by less than 2^-14 of, the piece is divided properly.
+// 8192 x 4096 bf16: 31 us (0.1 GB, 3.2 TB/s).
 template <class T>
 struct Raw {
   static constexpr int N = 16 / static_cast<int>(sizeof(T));

@@ -17,17 +17,8 @@ __device__ inline void wait_vm() {
 // loads each were issued after it (at most NS - 2).
 template <int NS, int LPS>
 __device__ inline void wait_oldest(int later) {
-  static_assert(NS >= 2 && NS <= 6 && (NS - 2) * LPS < 64, "ring depth");
-  if constexpr (NS >= 6) {
-    if (later >= 4) { wait_vm<4 * LPS>(); return; }
-  }
-  if constexpr (NS >= 5) {
-    if (later >= 3) { wait_vm<3 * LPS>(); return; }
-  }
-  if constexpr (NS >= 4) {
-    if (later >= 2) { wait_vm<2 * LPS>(); return; }
-  }
-  if constexpr (NS >= 3) {
+  static_assert((NS == 2 || NS == 3) && (NS - 2) * LPS < 64, "ring depth");
+  if constexpr (NS == 3) {
     if (later >= 1) { wait_vm<LPS>(); return; }
   }
   wait_vm<0>();
@@ -90,8 +81,13 @@ __device__ inline void stage_mma(typename Op::acc (&acc)[S::FM][S::FN], const ty
 //   slab 1 of stage st:  read slab 0's fragments of stage st + 1; load B of
 //                        stage st + 2 into the slot of stage st
 // So loads are under way all the time: the L1 keeps only some hundred requests
-// in flight, and a burst of a whole stage would leave it idle in between.
-// Loads and LDS reads are spread over the matrix instructions.
+// of 128 bytes in flight, for 500 cycles or more each, which is what bounds
+// the large blocks, and a burst of a whole stage would leave it idle in
+// between.  Loads and LDS reads are spread over the matrix instructions.  One
+// group of 16384 x 4096 x 2048 in bf16, 256 x 256: 205 us (1340 TFLOP/s);
+// 8192 cubed, W [n][k]: 769 us (1430 TFLOP/s; the library's product 728).
+// Measured no better: loads at higher wave priority, padded rows instead of
+// the swizzle, stages of half the depth in a longer ring.
 template <class Op, class S, class Load>
 __device__ inline void run_pipelined(typename Op::acc (&acc)[S::FM][S::FN], unsigned char *ring,
                                      int stages, const typename S::FA &pa,
@@ -307,7 +303,14 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
   }
 }
 
-// A workgroup for each row block of a group and block of columns.
+// A workgroup for each row block of a group and block of columns.  Bound by the
+// loads into LDS (operands of two bytes, see run_pipelined) or by the matrix
+// instructions (fp32).  4096 rows in 8 groups, k = 1024, n = 2048 in fp32, 64 x
+// 64: 154 us (111 TFLOP/s, of 128 that a large fp32 product reaches).  Rows off
+// 16 bytes (3022 rows in 12 groups, k = 771, n = 1283, f16), 128 x 128 through
+// registers: 36 us, 23 us of it at aligned extents; the rest are the unaligned
+// loads, two lines for most of them.  Aligned loads with the bytes shifted into
+// place afterwards took as long.
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -359,7 +362,10 @@ struct LargeUnit {
 };
 
 // Rows in large blocks.  One of at most 128 rows (the end of a group) takes
-// half the work.
+// half the work.  16384 rows in 16 groups, k = 4096, n = 2048 in bf16: 268 us
+// (1026 TFLOP/s), 315 with whole blocks alone; 32768 rows, k = n = 4096: 923 us
+// (1190 TFLOP/s) and 970; 16384 rows in 8 groups in 8 bits, k = n = 4096: 301 us
+// (1825 TOP/s) and 349.
 template <class Op, bool BKC>
 __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -497,7 +503,9 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 #endif
 }
 
-// The same in blocks of 256 x 256, cut as grouped_large_kernel's.
+// The same in blocks of 256 x 256, cut as grouped_large_kernel's.  16384 rows
+// in 16 groups, 2048 x 4096 bf16: 300 us (916 TFLOP/s), 336 with P gathered:
+// the sources of every stage's loads are then moved between the lanes.
 template <class Op, int GATHER>
 __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -524,7 +532,9 @@ __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g)
 // workgroup takes 16 FM rows by BN columns; its waves split k stage by stage
 // (so that together they read long pieces of each weight row), each on a ring
 // of its own without barriers, and add up their parts in LDS at the end, in
-// the order of the waves.
+// the order of the waves.  32 slots of 16 groups, W [n][k] of 2048 x 4096 in
+// bf16: 41 us for the 218 MB of the groups that have slots (5.4 TB/s); 4 rows x
+// 4096 x 8192 in 8 bits 8.1 us (4.1 TB/s).
 template <class Op, int FM_, int BN, int NW, bool BKC, int NS>
 struct SkinnyShape {
   static constexpr int FM = FM_, BM = 16 * FM, FN = BN / 16;
@@ -651,7 +661,8 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
 
 // Results from the sums of the parts, added in their order: element (row, col)
 // of group-major rows, m to a group, goes to c_group, ldc.  Rows of no group
-// (offsets given) are zero already.
+// (offsets given) are zero already.  Bound by its launch: 3.5 us for 16 parts
+// of 128 x 128.
 static __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g, int64_t rows, int64_t m,
                                                            bool skip_dead) {
   const int64_t quads = (g.n + 3) / 4, i = blockIdx.x * 256ll + threadIdx.x;
