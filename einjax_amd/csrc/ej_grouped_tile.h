@@ -224,6 +224,44 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
   }
 }
 
+// The results of a wave: row(i, &at) gives the element offset of fragment row
+// i's results and whether there is such a row, value(i, j, c) its result c of
+// four in fragment column j.
+template <class S, class Row, class Value>
+__device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row row,
+                                   Value value) {
+  if (S::FN % 2 == 0 && vec8_rows(g)) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) {
+      int64_t at;
+      const bool there = row(i, &at);
+#pragma unroll
+      for (int j = 0; j + 1 < S::FN; j += 2) {
+        float v[2][4];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c / 4][c % 4] = value(i, j + c / 4, c % 4);
+        put8(g.c, g.out, at, col0 + j * 16, g.n, lane, there, v);
+      }
+    }
+    return;
+  }
+  const bool vec = vec_rows(g);
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i) {
+    int64_t at;
+    if (!row(i, &at)) continue;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      const int col = col0 + j * 16 + (lane >> 4) * 4;
+      if (col >= g.n) continue;
+      float v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = value(i, j, c);
+      put4(g.c, g.out, at, col, g.n, vec, v);
+    }
+  }
+}
+
 // C rows of one row block of a group times the BN columns from n0.
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
 __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsigned char *ring) {
@@ -279,28 +317,33 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
     g.ldc = g.n;
     g.out = EJ_F32;
   }
-  const bool vec = vec_rows(g);
+  float as[S::FM], bs[S::FN][4];  // 8 bits: scales of the rows and columns
+  if constexpr (Op::kInt) {
 #pragma unroll
-  for (int i = 0; i < S::FM; ++i) {
-    const int s = r.lo + row0 + i * 16 + (lane & 15);
-    if (s >= r.hi) continue;
-    float as = 1.f;
-    if constexpr (Op::kInt) as = g.a_scale[slot_row(g.a_rows, g.n_a, s)];
+    for (int i = 0; i < S::FM; ++i) {
+      const int s = r.lo + row0 + i * 16 + (lane & 15);
+      as[i] = g.a_scale[slot_row(g.a_rows, g.n_a, s < r.hi ? s : r.hi - 1)];
+    }
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-      const int col = n0 + col0 + j * 16 + (lane >> 4) * 4;
-      if (col >= g.n) continue;
-      float v[4];
+    for (int j = 0; j < S::FN; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        v[c] = static_cast<float>(acc[i][j][c]);
-        if constexpr (Op::kInt)
-          v[c] *= as * g.b_scale[static_cast<int64_t>(r.group) * g.n +
-                                 (col + c < g.n ? col + c : g.n - 1)];
+        const int col = n0 + col0 + j * 16 + (lane >> 4) * 4 + c;
+        bs[j][c] = g.b_scale[static_cast<int64_t>(r.group) * g.n + (col < g.n ? col : g.n - 1)];
       }
-      put4(g.c, g.out, s * g.ldc, col, g.n, vec, v);
-    }
   }
+  put_results<S>(
+      g, n0 + col0, lane,
+      [&](int i, int64_t *at) {
+        const int s = r.lo + row0 + i * 16 + (lane & 15);
+        *at = s * g.ldc;
+        return s < r.hi;
+      },
+      [&](int i, int j, int c) {
+        const float v = static_cast<float>(acc[i][j][c]);
+        if constexpr (Op::kInt) return v * (as[i] * bs[j][c]);
+        else return v;
+      });
 }
 
 // A workgroup for each row block of a group and block of columns.  Bound by the
@@ -468,20 +511,14 @@ __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, uns
         lb.store(slot + S::TA::kBytes, wave, lane);
       });
 
-  const bool vec = vec_rows(g);
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i) {
-    const int row = m0 + row0 + i * 16 + (lane & 15);
-    if (row >= g.m) continue;
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-      const int col = n0 + col0 + j * 16 + (lane >> 4) * 4;
-      if (col >= g.n) continue;
-      const float v[4] = {static_cast<float>(acc[i][j][0]), static_cast<float>(acc[i][j][1]),
-                          static_cast<float>(acc[i][j][2]), static_cast<float>(acc[i][j][3])};
-      put4(g.c, g.out, group * g.c_group + static_cast<int64_t>(row) * g.ldc, col, g.n, vec, v);
-    }
-  }
+  put_results<S>(
+      g, n0 + col0, lane,
+      [&](int i, int64_t *at) {
+        const int row = m0 + row0 + i * 16 + (lane & 15);
+        *at = group * g.c_group + static_cast<int64_t>(row) * g.ldc;
+        return row < g.m;
+      },
+      [&](int i, int j, int c) { return static_cast<float>(acc[i][j][c]); });
 }
 
 // row_blocks x col_blocks covers one group's D; the grid holds n_groups of
