@@ -26,6 +26,10 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef int i32v2_t __attribute__((ext_vector_type(2)));
 typedef int i32v4_t __attribute__((ext_vector_type(4)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
+// vectors at any element's alignment
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // Storage types of the operands.  kStep = elements of k in a 128-byte row.
 struct OpBf16 {
@@ -277,13 +281,12 @@ __device__ inline uint16_t to_16(float v, int code) {
 }
 
 // Stores v[0..3] as columns col .. col + 3 of a row at element offset `at`
-// (of column 0); vec: the row's groups of four columns are aligned and whole.
-__device__ inline void put4(void *c, int code, int64_t at, int col, int n, bool vec,
-                            const float (&v)[4]) {
+// (of column 0), as one vector at any element's alignment.
+__device__ inline void put4(void *c, int code, int64_t at, int col, int n, const float (&v)[4]) {
   if (code == EJ_F32) {
     float *p = static_cast<float *>(c) + at + col;
-    if (vec && col + 4 <= n) {
-      *reinterpret_cast<f32x4_t *>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
+    if (col + 4 <= n) {
+      *reinterpret_cast<f32x4_any_t *>(p) = f32x4_any_t{v[0], v[1], v[2], v[3]};
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -291,29 +294,27 @@ __device__ inline void put4(void *c, int code, int64_t at, int col, int n, bool 
     }
   } else {
     uint16_t *p = static_cast<uint16_t *>(c) + at + col;
-    if (vec && col + 4 <= n) {
-      ushort4 o;
-      o.x = to_16(v[0], code);
-      o.y = to_16(v[1], code);
-      o.z = to_16(v[2], code);
-      o.w = to_16(v[3], code);
-      *reinterpret_cast<ushort4 *>(p) = o;
+    const u16x4_any_t o = {to_16(v[0], code), to_16(v[1], code), to_16(v[2], code),
+                           to_16(v[3], code)};
+    if (col + 4 <= n) {
+      *reinterpret_cast<u16x4_any_t *>(p) = o;
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (col + r < n) p[r] = to_16(v[r], code);
+        if (col + r < n) p[r] = o[r];
     }
   }
 }
 
-// Two fragments' results of a row, at columns col and col + 16 on, as whole
-// 16-byte pieces: lanes 16 apart exchange four columns, so that each holds
+// 16-bit results of two fragments of a row, at columns col and col + 16 on, in
+// pieces of 16 bytes: lanes 16 apart exchange four columns, so that each holds
 // eight of one fragment.  Stores of 8 bytes a lane take the large blocks of
-// 16384 x 512 x 4096 bf16 96 us, these 80.
+// 16384 x 512 x 4096 bf16 96 us, these 80; in rows off 16 bytes (3022 x 771 x
+// 1283) single elements 37 us, these 33.
 __device__ inline void put8(void *c, int code, int64_t at, int col, int n, int lane, bool there,
                             const float (&v)[2][4]) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  uint32_t w[4];
+  u32x4_any_t w;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint32_t p[2];
@@ -325,9 +326,14 @@ __device__ inline void put8(void *c, int code, int64_t at, int col, int n, int l
     w[2 + h] = both[1];
   }
   const int first = col + (lane >> 4 & 1) * 16 + (lane >> 5) * 8;
-  if (there && first + 8 <= n)
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(c) + at + first) =
-        make_uint4(w[0], w[1], w[2], w[3]);
+  uint16_t *p = static_cast<uint16_t *>(c) + at + first;
+  if (there && first + 8 <= n) {
+    *reinterpret_cast<u32x4_any_t *>(p) = w;
+  } else if (there) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (first + r < n) p[r] = static_cast<uint16_t>(w[r / 2] >> 16 * (r & 1));
+  }
 #endif
 }
 
@@ -335,18 +341,6 @@ __device__ inline void put8(void *c, int code, int64_t at, int col, int n, int l
 __device__ inline void part_of(int stages, int part, int parts, int *first, int *last) {
   *first = static_cast<int>(static_cast<int64_t>(stages) * part / parts);
   *last = static_cast<int>(static_cast<int64_t>(stages) * (part + 1) / parts);
-}
-
-// Whether groups of four columns can be stored as one vector.
-__device__ inline bool vec_rows(const GroupedArgs &g) {
-  const int b = g.out == EJ_F32 ? 4 : 2;
-  return g.ldc % 4 == 0 && g.c_group % 4 == 0 && reinterpret_cast<size_t>(g.c) % (4 * b) == 0;
-}
-
-// Whether groups of eight can be, and columns end with one.
-__device__ inline bool vec8_rows(const GroupedArgs &g) {
-  return g.out != EJ_F32 && g.ldc % 8 == 0 && g.c_group % 8 == 0 && g.n % 8 == 0 &&
-         reinterpret_cast<size_t>(g.c) % 16 == 0;
 }
 
 // Zeroes the rows of C that no group covers (slots before the first offset

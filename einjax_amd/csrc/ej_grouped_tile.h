@@ -230,7 +230,7 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
 template <class S, class Row, class Value>
 __device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row row,
                                    Value value) {
-  if (S::FN % 2 == 0 && vec8_rows(g)) {
+  if (S::FN % 2 == 0 && g.out != EJ_F32) {
 #pragma unroll
     for (int i = 0; i < S::FM; ++i) {
       int64_t at;
@@ -245,7 +245,6 @@ __device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row
     }
     return;
   }
-  const bool vec = vec_rows(g);
 #pragma unroll
   for (int i = 0; i < S::FM; ++i) {
     int64_t at;
@@ -257,7 +256,7 @@ __device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row
       float v[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) v[c] = value(i, j, c);
-      put4(g.c, g.out, at, col, g.n, vec, v);
+      put4(g.c, g.out, at, col, g.n, v);
     }
   }
 }
@@ -351,9 +350,9 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
 // instructions (fp32).  4096 rows in 8 groups, k = 1024, n = 2048 in fp32, 64 x
 // 64: 154 us (111 TFLOP/s, of 128 that a large fp32 product reaches).  Rows off
 // 16 bytes (3022 rows in 12 groups, k = 771, n = 1283, f16), 128 x 128 through
-// registers: 36 us, 23 us of it at aligned extents; the rest are the unaligned
-// loads, two lines for most of them.  Aligned loads with the bytes shifted into
-// place afterwards took as long.
+// registers: 33 us, 21 us at aligned extents; the rest are another column of
+// tiles and stage of k, and the unaligned loads, two lines for most of them.
+// Aligned loads with the bytes shifted into place afterwards took as long.
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -672,7 +671,6 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
                                             (i * 16 + (lane & 15)) * BN + j * 16 +
                                             (lane >> 4) * 4) = acc[i][j];
   __syncthreads();
-  const bool vec = vec_rows(g);
   for (int q = tid; q < S::BM * BN / 4; q += NW * 64) {
     const int row = q / (BN / 4), col = q % (BN / 4) * 4;
     const int s = r.lo + row;
@@ -691,7 +689,7 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
       if constexpr (Op::kInt)
         v[c] *= as * g.b_scale[static_cast<int64_t>(r.group) * g.n + (n < g.n ? n : g.n - 1)];
     }
-    put4(g.c, g.out, s * g.ldc, n0 + col, g.n, vec, v);
+    put4(g.c, g.out, s * g.ldc, n0 + col, g.n, v);
   }
 #endif
 }
@@ -721,7 +719,7 @@ static __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g,
         if (col + c < g.n) sum[c] += src[p * part + c];
   }
   const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-  put4(g.c, g.out, row / m * g.c_group + row % m * g.ldc, col, g.n, vec_rows(g), v);
+  put4(g.c, g.out, row / m * g.c_group + row % m * g.ldc, col, g.n, v);
 }
 
 }  // namespace ej
