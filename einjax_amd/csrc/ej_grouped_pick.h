@@ -114,18 +114,24 @@ inline double large_rounds(double tiles) {
 }
 
 // The choice goes by the mean rows of a group (all that the host knows of the
-// sizes) and the number of tiles.  Measured (us) with k = n = 2048, bf16, W
-// [n][k] / [k][n], groups of unequal length; skinny 16 rows at k = n = 1024:
-//   rows/group  groups   skinny 16  64 x 64   64 x 128  128 x 128  large
-//        2         8      6.5/8.0   9.6       11.4      17.9
-//       16         8     15.2/19.5  16.5      19.5      29
-//       50         8                17/18     21/20     28/27      21/21
-//       50        16                33/33     31/32     29/29      29/31
-//      100         8                18/18     21/20     27/27      21/22
-//      100        16                41/41     34/35     33/32      30/33
-//      200        16                57/59     49/50     42/40      50/51
-//      512        16                                    98/98      78/80
-//       64 (k 1024)  64             63/63     59/58     67/69      61/62
+// sizes) and the number of tiles.  Measured (us), bf16, W [n][k] / [k][n]:
+//   rows/group  groups     k x n      skinny  64 x 64  64 x 128  128 x 128  large
+//      4..16       8   1024 x 1024     7/7     9/10     11/11      15/15    10/11
+//        48        8   1024 x 1024     9/9     9/10
+//      4..16       1   4096 x 8192    13/16   25/26
+//        48        1   4096 x 8192    17/20   25/29
+//         4       16   2048 x 4096    40/41   44/43
+//        16       16   2048 x 4096    42/45   45/44
+//        32       16   2048 x 4096    61/55   51/50
+//        50        8   2048 x 2048            16/17    20/19      26/25    20/21
+//        50       16   2048 x 2048            32/32    30/31      28/27    28/30
+//       100        8   2048 x 2048            20/18    20/20      26/26    20/21
+//       100       16   2048 x 2048            40/41    33/36      31/30    29/31
+//       200       16   2048 x 2048            56/55    47/51      41/39    48/49
+//       512       16   2048 x 2048           115/119  111/112     90/92    74/75
+//        64       64   1024 x 2048            64/63    58/58      65/66    58/59
+// fp32, 16 groups, 2048 x 4096: 24 rows 134/142 skinny, 159/160 in 64 x 64; 32
+// rows 156/155 and 156/158.
 template <class Op, bool BKC>
 int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
@@ -136,12 +142,16 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
   const double rows = static_cast<double>(g.slots) / groups;
   if (!r.direct) {
+    // k = 771, n = 1283 in f16, 128 x 128 and 64 x 64: 100 rows/group, 8 groups
+    // 22 and 19 us; 200, 8: 22 and 22; 250, 12: 33 and 38; 500, 12: 50 and 55
     if (rows > 128) return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2>(g, stream);
     return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
   }
   // columns of a skinny block: 32, or what fills 128 bytes of a [k][n] row
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
-  if (rows <= (BKC ? 16 : 8)) return launch_skinny<Op, 1, kSkinny, 4, BKC, 2>(g, stream);
+  const double tiles = expected_tiles(g, 64, 64, groups);
+  if (rows <= (kElem<Op> == 4 ? 24 : 16) || (rows <= 48 && tiles <= 192))
+    return launch_skinny<Op, 1, kSkinny, 4, BKC, 2>(g, stream);
   if constexpr (kElem<Op> == 4) {
     // bound by the fp32 matrix instructions at any tile: the finest spreads
     // best (4096 x 1024 x 2048 in 8 groups 164 us, 212 with 128 x 128; equal
@@ -149,7 +159,7 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
     return launch_rows<Op, 64, 64, 2, 2, BKC, true, 0>(g, stream);
   } else {
     // up to about two small tiles to a CU the finest spread best
-    if (rows <= 48 || expected_tiles(g, 64, 64, groups) <= 576)
+    if (rows <= 48 || tiles <= 576)
       return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
     if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, true, 3>(g, stream);
     // rounds of large blocks against a fifth less time for a round of 512
@@ -165,13 +175,13 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
 // against rounds of the large blocks.  Measured (us), bf16, rows as they lie /
 // gathered, groups of unequal length:
 //   rows   groups    m x n       64 x 64   128 x 128  large
-//    4096     3   1024 x 1024    20/29      26/36     21/31
-//    8192     5   1024 x 1024    37/44      32/46     34/48
-//    8192    17   1024 x 1024    41/57      33/41     32/37
-//    8192    17   1536 x 1536               62/78     60/67
-//    8192     8   2048 x 2560              107/137    92/107
-//   16384    16   2048 x 4096   547/729    378/474   300/336
-// fp32: 4096 rows, 8 groups, 1024 x 2048: 128 x 128 157, 64 x 64 167; 1200
+//    4096     3   1024 x 1024    21/29      26/36     21/31
+//    8192     5   1024 x 1024    37/46      33/46     34/47
+//    8192    17   1024 x 1024    40/58      35/38     28/34
+//    8192    17   1536 x 1536    82/123     61/74     54/62
+//    8192     8   2048 x 2560   153/219    101/129    86/102
+//   16384    16   2048 x 4096   522/721    350/442   273/308
+// fp32: 4096 rows, 8 groups, 1024 x 2048: 128 x 128 153, 64 x 64 173; 1200
 // rows, 5 groups, 320 x 520: 32 and 13.
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {

@@ -84,8 +84,8 @@ __device__ inline void stage_mma(typename Op::acc (&acc)[S::FM][S::FN], const ty
 // of 128 bytes in flight, for 500 cycles or more each, which is what bounds
 // the large blocks, and a burst of a whole stage would leave it idle in
 // between.  Loads and LDS reads are spread over the matrix instructions.  One
-// group of 16384 x 4096 x 2048 in bf16, 256 x 256: 205 us (1340 TFLOP/s);
-// 8192 cubed, W [n][k]: 769 us (1430 TFLOP/s; the library's product 728).
+// group of 16384 x 4096 x 2048 in bf16, 256 x 256: 198 us (1386 TFLOP/s);
+// 8192 cubed, W [n][k]: 755 us (1456 TFLOP/s; the library's product 728).
 // Measured no better: loads at higher wave priority, padded rows instead of
 // the swizzle, stages of half the depth in a longer ring.
 template <class Op, class S, class Load>
@@ -404,10 +404,13 @@ struct LargeUnit {
 };
 
 // Rows in large blocks.  One of at most 128 rows (the end of a group) takes
-// half the work.  16384 rows in 16 groups, k = 4096, n = 2048 in bf16: 268 us
-// (1026 TFLOP/s), 315 with whole blocks alone; 32768 rows, k = n = 4096: 923 us
-// (1190 TFLOP/s) and 970; 16384 rows in 8 groups in 8 bits, k = n = 4096: 301 us
-// (1825 TOP/s) and 349.
+// half the work.  16384 rows in 16 groups, k = 4096, n = 2048 in bf16: 265 us
+// (1040 TFLOP/s), uncut and with whole blocks alone 40 us more; 32768 rows, k =
+// n = 4096: 945 us (1164 TFLOP/s), 50 more; 16384 rows in 8 groups in 8 bits, k
+// = n = 4096: 260 us (2115 TOP/s), 45 more.  256 workgroups that walk the blocks
+// and load the next while they store the last were 5% faster in one group and
+// in 8 bits, 3 to 10% slower in 16 groups (dealt out beforehand, the short
+// blocks leave CUs waiting, and the registers spill).
 template <class Op, bool BKC>
 __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -540,7 +543,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 }
 
 // The same in blocks of 256 x 256, cut as grouped_large_kernel's.  16384 rows
-// in 16 groups, 2048 x 4096 bf16: 300 us (916 TFLOP/s), 336 with P gathered:
+// in 16 groups, 2048 x 4096 bf16: 272 us (1010 TFLOP/s), 306 with P gathered:
 // the sources of every stage's loads are then moved between the lanes.
 template <class Op, int GATHER>
 __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g) {
