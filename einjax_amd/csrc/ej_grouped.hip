@@ -35,34 +35,61 @@ int check_desc(const ej_grouped_desc *d) {
   return EJ_OK;
 }
 
-// Parts of the contraction: 64 x 64 tiles that leave three CUs of four without
-// work and have a long way to go are split until the CUs are covered, but not
-// below eight stages a part (each part is a pass over its sums, and adding them
-// a launch: in two parts nothing is gained).  One group, bf16:
-// weight gradient of 8192 rows x 128 x 128 10 us with the sum of the parts, 49
-// in one; rows product of 512 x 4096 x 64 11 us and 27.
-int split_parts(double tiles, int64_t contraction, int elem) {
-  const int64_t stages = contraction / (128 / elem);
-  if (tiles > 64 || tiles <= 0 || stages < 32) return 1;
-  const int64_t want = static_cast<int64_t>(256 / tiles), most = stages / 8;
-  const int64_t parts = want < most ? want : most;
-  return static_cast<int>(parts < 32 ? parts : 32);
+// Whether rows and weights can be loaded as whole, aligned chunks, going by the
+// descriptor (the workspace is sized without the operands' addresses).
+bool whole_chunks(const ej_grouped_desc *d) {
+  const int size = elem_size(d->dtype), chunk = 16 / size;
+  return d->k % chunk == 0 && aligned16(nullptr, d->x_stride, 0, size) &&
+         aligned16(nullptr, d->w_stride, d->w_group, size) &&
+         (d->w_order == EJ_W_NK || d->n % chunk == 0);
 }
 
-// Rows of a group on average decide for the rows product, as the choice of
-// kernel does: groups of few rows take the kernel that splits k by itself.
+// Parts of the contraction, for 64 x 64 tiles that leave CUs without work and
+// have a long way to go.  A part is a pass over its sums (`sums` elements,
+// written and read at 4 TB/s), and adding the parts is a launch (5 us); a stage
+// takes a workgroup 0.4 us in 16 bits and 0.7 in fp32, and twice that through
+// registers, where more workgroups to a CU are of use.  Measured (us) in one
+// part and in the parts taken:
+//   rows product     256 x 4096 x 4096 bf16              27   23 (2)
+//                    512 x 4096 x 64 bf16                27   11 (8)
+//                    1515 x 3392 x 135 fp32, 25 groups   77   50 (5)
+//                    45 x 1539 x 294 fp32, 30 groups     72   31 (8)
+//   weight gradient  8192 rows, 128 x 128 bf16           49   10 (16)
+//                    4096 rows, 1024 x 1024 bf16         28   25 (2)
+//                    26556 rows, 6 groups, 311 x 215 f16 272  68 (8)
+// and with 512 tiles 29 and 39 in two parts.
+int split_parts(double tiles, int64_t contraction, int elem, bool whole, double sums) {
+  const int64_t stages = contraction / (128 / elem);
+  // fp32 tiles on every CU are bound by their matrix instructions (258 x 3608 x
+  // 2497 in 6 groups, 281 tiles: 66 us, 78 in two parts)
+  if (tiles <= 0 || stages < 8 || (whole && elem == 4 && tiles > 192)) return 1;
+  const int64_t want = static_cast<int64_t>((whole ? 576 : 1152) / tiles);
+  const int64_t most = whole ? (stages / 8 < 32 ? stages / 8 : 32) : stages / 4 < 8 ? stages / 4 : 8;
+  const int64_t parts = want < most ? want : most;
+  if (parts < 2) return 1;
+  const double saved = stages * (1 - 1. / parts) * (elem == 4 ? 0.7 : 0.4) * (whole ? 1 : 2);
+  return saved > 5 + parts * sums * 8 / 4e6 ? static_cast<int>(parts) : 1;
+}
+
 int rows_parts(const ej_grouped_desc *d) {
   if (d->dtype == EJ_I8 || d->n_groups == 0 || d->n_slots == 0) return 1;
   const int64_t groups = d->n_groups < d->n_slots ? d->n_groups : d->n_slots;
-  if (d->n_slots <= 16 * groups) return 1;
-  const double tiles =
-      (static_cast<double>(d->n_slots) / 64 + 0.5 * groups) * ceil_div(d->n, 64);
-  return split_parts(tiles, d->k, elem_size(d->dtype));
+  const double rows = static_cast<double>(d->n_slots) / groups;
+  const double tiles = (rows / 64 + 0.5) * groups * ceil_div(d->n, 64);
+  const int elem = elem_size(d->dtype);
+  const bool whole = whole_chunks(d);
+  // the kernel for few rows splits k by itself
+  if (whole && few_rows(rows, tiles, elem) && (rows <= 16 || tiles > 64)) return 1;
+  return split_parts(tiles, d->k, elem, whole, static_cast<double>(d->n_slots) * d->n);
 }
 int dw_parts(const ej_grouped_desc *d) {
   if (d->n_groups == 0) return 1;
+  const int size = elem_size(d->dtype), chunk = 16 / size;
+  const bool whole = d->k % chunk == 0 && d->n % chunk == 0 &&
+                     aligned16(nullptr, d->x_stride, d->out_stride, size);
   const double tiles = static_cast<double>(ceil_div(d->k, 64)) * ceil_div(d->n, 64) * d->n_groups;
-  return split_parts(tiles, d->n_slots / d->n_groups, elem_size(d->dtype));
+  return split_parts(tiles, d->n_slots / d->n_groups, size, whole,
+                     static_cast<double>(d->n_groups) * d->k * d->n);
 }
 
 int check_workspace(int parts, int64_t sums, void *workspace, size_t bytes, GroupedArgs *g) {

@@ -20,6 +20,12 @@ int grouped_wgrad_bf16(const GroupedArgs &g, bool direct, hipStream_t stream);
 int grouped_wgrad_f16(const GroupedArgs &g, bool direct, hipStream_t stream);
 int grouped_wgrad_f32(const GroupedArgs &g, bool direct, hipStream_t stream);
 
+// Whether a rows product takes the kernel for few rows a group; tiles: 64 x 64
+// ones (measured beside the choice of kernel).
+inline bool few_rows(double rows, double tiles, int elem) {
+  return rows <= (elem == 4 ? 24 : 16) || (rows <= 48 && tiles <= 192);
+}
+
 // A grid of `blocks` workgroups of `threads`, or EJ_E_UNSUPPORTED: launches
 // hold fewer than 2^32 threads.
 inline int grouped_grid(int64_t blocks, int threads, dim3 *grid) {

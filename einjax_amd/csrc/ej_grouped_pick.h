@@ -137,20 +137,27 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
   if (g.splits > 1) {
     if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
-    return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, true, kElem<Op> == 4 ? 0 : 3>(g, stream);
   }
   const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
   const double rows = static_cast<double>(g.slots) / groups;
+  const double tiles = expected_tiles(g, 64, 64, groups);
   if (!r.direct) {
-    // k = 771, n = 1283 in f16, 128 x 128 and 64 x 64: 100 rows/group, 8 groups
-    // 22 and 19 us; 200, 8: 22 and 22; 250, 12: 33 and 38; 500, 12: 50 and 55
-    if (rows > 128) return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2>(g, stream);
-    return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
+    // (us) 64 x 64, 64 x 128 and 128 x 128; in 12 groups 3022 x 771 x 1283
+    // f16 38, 31, 33, fp32 120, 103, 130; in 4 groups 6000 x 1001 x 1001 fp32
+    // 157, 126, 157; in 6 3000 x 517 x 2051 f16 31, 32, 25; few tiles: in 8
+    // groups 800 x 771 x 1283 f16 19, 18, 22; in 4 2000 x 255 x 333 fp32 13, 16,
+    // 24, 8 bits 7 and 9 in 128 x 128
+    if (tiles <= 512 || rows <= 128)
+      return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
+    if constexpr (kElem<Op> == 4)
+      return launch_rows<Op, 64, 128, 2, 4, BKC, false, 2>(g, stream);
+    else
+      return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2>(g, stream);
   }
   // columns of a skinny block: 32, or what fills 128 bytes of a [k][n] row
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
-  const double tiles = expected_tiles(g, 64, 64, groups);
-  if (rows <= (kElem<Op> == 4 ? 24 : 16) || (rows <= 48 && tiles <= 192))
+  if (few_rows(rows, tiles, kElem<Op>))
     return launch_skinny<Op, 1, kSkinny, 4, BKC, 2>(g, stream);
   if constexpr (kElem<Op> == 4) {
     // bound by the fp32 matrix instructions at any tile: the finest spreads
