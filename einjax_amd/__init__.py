@@ -5,7 +5,9 @@ The public names mirror the reference package's sparse-path exports
 relations, dense and sparse tensor metadata and tile-shape selection, the
 three-phase execute_sparse, the execution engine over chains of sparse
 steps, the kernel registry, the block-sparse matmul
-and the coordinate joins.  All computation runs in
+and the coordinate joins; beside them the operators of a
+mixture-of-experts layer (routing, products grouped by expert, their
+combination, 8-bit rows and products).  All computation runs in
 libejhip.so (HIP kernels behind a C ABI, include/einjax_hip.h).
 """
 

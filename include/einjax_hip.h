@@ -38,6 +38,12 @@
  *                 (the accumulation half of segment_sum, execution/sparse_dispatch.py:164-171)
  *   backward      ej_index_plan / ej_pair_einsum_vjp
  *                 (replace sparse_einsum_raw's backward, autodiff/custom_vjp.py:254-275)
+ *   experts       ej_expert_route / ej_expert_group / ej_expert_route_vjp (the
+ *                 relation of tokens and experts), ej_grouped_gemm /
+ *                 ej_grouped_gemm_dw (products grouped by expert),
+ *                 ej_expert_combine / ej_expert_combine_vjp (back to tokens),
+ *                 ej_quantize_rows (8-bit rows for ej_grouped_gemm)
+ *                 (no counterpart in the reference)
  *
  * Conventions
  *   - Every pointer argument named *coords, *values, *_idx, *keys, perm,
@@ -47,6 +53,8 @@
  *     the scalar outputs n_pairs, n_segments, n_tiles, nnz and the
  *     statistics num_tuples / value_count are HOST pointers; `counts` of the
  *     *_async functions is PINNED host memory (hipHostMalloc).
+ *     The expert functions take DEVICE pointers throughout but for desc and
+ *     bytes.
  *   - Work is enqueued on `stream` (a hipStream_t; NULL = the null stream).
  *     Functions whose name ends in _count, and the ej_scheme_stats_*
  *     functions, synchronize `stream` because they return data-dependent
