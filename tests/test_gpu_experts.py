@@ -364,6 +364,46 @@ def test_grouped_weight_gradient_large_blocks(gpu, sizes, m, n, dtype, gather):
         assert_within(gw[i], xi.T @ gi, sum_bound(xi.T @ gi, xi.abs().T @ gi.abs(), b - a, dtype))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("sizes,k,n,shift", [
+    ([4, 0, 9, 1], 1539, 294, 0), ([16, 30, 2], 2047, 129, 0), ([130], 2500, 70, 0),
+    ([60, 12], 2048, 72, 0), ([60, 12], 2048, 72, 1), ([100, 0, 300], 4096, 64, 0)])
+def test_grouped_matmul_split_contractions(gpu, sizes, k, n, shift, dtype):
+    """Few tiles over a long contraction, whose parts are summed apart: rows on
+    and off 16 bytes, operands that start off 16 bytes (shift elements)."""
+    g, e, slots = rng(k + n + shift), len(sizes), sum(sizes) + 3
+    offsets = torch.tensor([sum(sizes[:i]) for i in range(e + 1)], dtype=torch.int32,
+                           device="cuda")
+    x = randn(g, slots * k + 8, dtype=dtype)[shift:shift + slots * k].view(slots, k)
+    for order in ("kn", "nk"):
+        w = randn(g, e, k, n, dtype=dtype, scale=k ** -0.5)
+        if order == "nk":
+            w = w.transpose(1, 2).contiguous().transpose(1, 2)
+        got = ej.grouped_matmul(x, w, offsets)
+        want, mag = product64(x, None, offsets, w, slots)
+        assert_within(got, want, sum_bound(want, mag, k, dtype))
+        assert bool((got[sum(sizes):] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("sizes,m,n,shift", [
+    ([3000, 0, 700], 75, 151, 0), ([9, 5000], 64, 40, 0), ([2500], 128, 128, 1),
+    ([1200, 800, 1], 77, 64, 0)])
+def test_grouped_weight_gradient_split_contractions(gpu, sizes, m, n, shift, dtype):
+    g, e, slots = rng(m + n + shift), len(sizes), sum(sizes)
+    offsets = torch.tensor([sum(sizes[:i]) for i in range(e + 1)], dtype=torch.int32,
+                           device="cuda")
+    x = randn(g, slots * m + 8, dtype=dtype)[shift:shift + slots * m].view(slots, m)
+    cot, w = randn(g, slots, n, dtype=dtype), randn(g, e, m, n, dtype=dtype)
+    for wt in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
+        _, gw = ej.grouped_matmul_vjp(x, wt, offsets, cot, need_x=False)
+        ends = offsets.tolist()
+        for i in range(e):
+            xi, gi = (v[ends[i]:ends[i + 1]].double() for v in (x, cot))
+            assert_within(gw[i], xi.T @ gi,
+                          sum_bound(xi.T @ gi, xi.abs().T @ gi.abs(), len(xi), dtype))
+
+
 def test_grouped_gradients_against_differences(gpu):
     g, r, x, w = product_case(40, 5, 2, 24, 36, "skew", F32, "kn", True)
     cot = randn(g, 80, 36)
