@@ -3,7 +3,9 @@
 //
 // All three are bound by memory: every row is read once (the second pass of
 // the quantization over a row comes from the cache) and written once, sixteen
-// bytes a lane where the rows are aligned.
+// bytes a lane at any element's alignment.  The last piece of a row that holds
+// no whole number of them is moved back over the one before: its elements are
+// computed twice, with one result.
 #include "ej_internal.h"
 
 #include <type_traits>
@@ -22,6 +24,15 @@ __device__ inline float widen(T v) {
   return static_cast<float>(v);
 }
 
+// Four words at any element's alignment.
+typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// First column of the piece of N that begins at col, moved back into the row.
+template <int N>
+__device__ inline int64_t piece_at(int64_t col, int32_t n) {
+  return N == 1 || col + N <= n ? col : n - N;
+}
+
 // N consecutive elements (16 bytes when VEC), widened.
 template <class T, bool VEC>
 struct Piece {
@@ -29,7 +40,8 @@ struct Piece {
   float v[N];
   __device__ inline void load(const T *p) {
     if constexpr (VEC) {
-      struct alignas(16) { T e[N]; } w = *reinterpret_cast<const decltype(w) *>(p);
+      struct Chunk { T e[N]; };
+      const Chunk w = __builtin_bit_cast(Chunk, *reinterpret_cast<const words_t *>(p));
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = widen(w.e[i]);
     } else {
@@ -39,10 +51,10 @@ struct Piece {
   template <class O>
   __device__ inline void store(O *p) const {
     if constexpr (VEC) {
-      struct alignas(N * sizeof(O)) { O e[N]; } w;
+      struct { O e[N]; } w;
 #pragma unroll
       for (int i = 0; i < N; ++i) w.e[i] = static_cast<O>(v[i]);
-      *reinterpret_cast<decltype(w) *>(p) = w;
+      __builtin_memcpy(p, &w, sizeof(w));
     } else {
       *p = static_cast<O>(v[0]);
     }
@@ -65,13 +77,16 @@ struct CombineArgs {
 // the picks, rounded once.  One workgroup a token and stretch of columns, so a
 // token's indices and weights are read once for 256 lanes.  16384 tokens of 4
 // picks, 4096 columns of bf16, 1 pair in 20 left out: 139 us (0.65 GB, 4.6
-// TB/s; a large copy reaches 5.2).
+// TB/s; a large copy reaches 5.2).  4095 columns take as long (element by
+// element 3 times that).
 template <class T, class O, bool VEC>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsigned col_blocks) {
   constexpr int N = Piece<T, VEC>::N;
   const int64_t t = blockIdx.x / col_blocks;
-  const int64_t col = (static_cast<int64_t>(blockIdx.x % col_blocks) * kThreads + threadIdx.x) * N;
-  if (col >= a.n) return;
+  const int64_t begin =
+      (static_cast<int64_t>(blockIdx.x % col_blocks) * kThreads + threadIdx.x) * N;
+  if (begin >= a.n) return;
+  const int64_t col = piece_at<N>(begin, a.n);
   float sum[N] = {};
   for (int j = 0; j < a.k; ++j) {
     const int64_t s = a.slots[t * a.k + j];
@@ -92,7 +107,8 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsign
 // One workgroup a token, so every dot product is summed in a fixed order;
 // workgroups past the tokens zero grad_y's rows that no pair holds.  At the
 // sizes above 230 us (1.18 GB, 5.1 TB/s).
-template <class T, bool VEC>
+// WHOLE: rows of whole pieces; otherwise the last one is moved back.
+template <class T, bool VEC, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, const void *grad,
                                                                int64_t ld_grad, void *grad_y,
                                                                float *grad_w) {
@@ -117,14 +133,23 @@ __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, co
       const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
       const T *y = static_cast<const T *>(a.y) + s * a.ld_y;
       T *d = static_cast<T *>(grad_y) + s * a.n;
-      for (int64_t col = threadIdx.x * N; col < a.n; col += kThreads * N) {
+      for (int64_t begin = threadIdx.x * N; begin < a.n; begin += kThreads * N) {
+        const int64_t col = WHOLE ? begin : piece_at<N>(begin, a.n);
+        // elements of the piece before
+        const int twice = WHOLE ? 0 : static_cast<int>(begin - col);
         Piece<T, VEC> gv;
         gv.load(g + col);
         if (grad_w) {
           Piece<T, VEC> yv;
           yv.load(y + col);
+          if (twice > 0) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) dot += gv.v[i] * yv.v[i];
+            for (int i = 0; i < N; ++i)
+              if (i >= twice) dot += gv.v[i] * yv.v[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot += gv.v[i] * yv.v[i];
+          }
         }
         if (grad_y) {
 #pragma unroll
@@ -161,14 +186,16 @@ __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, co
 //   - the rounded quotient comes from x times 1 / scale plus 1.5 2^23, whose
 //     low byte is the result; where that product lies near a tie, which it can
 //     be off by less than 2^-14 of, the piece is divided properly.
-// 8192 x 4096 bf16: 31 us (0.1 GB, 3.2 TB/s).
+// 8192 x 4096 bf16: 31 us (0.1 GB, 3.2 TB/s; 26 with the rows in the cache, as
+// 8192 x 4095, which takes 34 element by element).
 template <class T>
 struct Raw {
   static constexpr int N = 16 / static_cast<int>(sizeof(T));
   uint32_t w[4];
   __device__ inline void load(const T *p) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    const words_t v = *reinterpret_cast<const words_t *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = v[i];
   }
   __device__ inline float at(int i) const {
     if constexpr (sizeof(T) == 4) {
@@ -183,7 +210,7 @@ struct Raw {
   }
 };
 template <class T>
-struct Scalar {  // one element, for rows that are not aligned
+struct Scalar {  // one element, for rows below 16 bytes
   static constexpr int N = 1;
   T v;
   __device__ inline void load(const T *p) { v = *p; }
@@ -243,13 +270,13 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t 
   Magnitude<T> seen;
 #pragma unroll
   for (int p = 0; p < P; ++p)
-    if (first + p * TPR * N < n) held[p].load(row + first + p * TPR * N);
+    if (first + p * TPR * N < n) held[p].load(row + piece_at<N>(first + p * TPR * N, n));
 #pragma unroll
   for (int p = 0; p < P; ++p)
     if (first + p * TPR * N < n) seen.look(held[p]);
   for (int64_t col = first + P * TPR * N; col < n; col += TPR * N) {
     R v;
-    v.load(row + col);
+    v.load(row + piece_at<N>(col, n));
     seen.look(v);
   }
   float most = seen.value();
@@ -267,8 +294,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t 
   if (first == 0) scale[r] = most < INFINITY ? s : __uint_as_float(0x7fc00000u);
   // 0: divide (a scale so small that its reciprocal overflows)
   const float inv = s >= 1e-37f ? 1.f / s : 0.f;
-  auto put = [&](int64_t col, const R &v) {
-    struct alignas(N) { int8_t e[N]; } o;
+  auto put = [&](int64_t begin, const R &v) {
+    struct { int8_t e[N]; } o;
     float off = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -284,14 +311,14 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T *x, int64_t 
         o.e[i] = static_cast<int8_t>(fminf(fmaxf(f, -127.f), 127.f));
       }
     }
-    *reinterpret_cast<decltype(o) *>(q + r * n + col) = o;
+    __builtin_memcpy(q + r * n + piece_at<N>(begin, n), &o, N);
   };
 #pragma unroll
   for (int p = 0; p < P; ++p)
     if (first + p * TPR * N < n) put(first + p * TPR * N, held[p]);
   for (int64_t col = first + P * TPR * N; col < n; col += TPR * N) {
     R v;
-    v.load(row + col);
+    v.load(row + piece_at<N>(col, n));
     put(col, v);
   }
 }
@@ -303,10 +330,6 @@ int by_type(int32_t dtype, F f) {
   if (dtype == EJ_F16) return f(static_cast<_Float16 *>(nullptr));
   set_error("values of dtype %d: expected EJ_F32, EJ_BF16 or EJ_F16", dtype);
   return EJ_E_INVAL;
-}
-
-bool aligned16(const void *p, int64_t ld, int size) {
-  return reinterpret_cast<size_t>(p) % 16 == 0 && ld * size % 16 == 0;
 }
 
 int check_combine(int64_t n_slots, int64_t n_tokens, int32_t k, int32_t n) {
@@ -341,10 +364,8 @@ extern "C" int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, 
         EJ_CHECK_ARG(slots && out && (y || n_slots == 0), "null argument");
         EJ_CHECK_ARG(ld_y >= n, "row stride %lld below n = %d", (long long)ld_y, n);
         CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, nullptr, 0, out};
-        // whole 16-byte pieces of y, and the pieces of out aligned to their size
         constexpr int N = 16 / sizeof(T);
-        const bool vec = aligned16(y, ld_y, sizeof(T)) && n % N == 0 &&
-                         reinterpret_cast<size_t>(out) % (N * sizeof(O)) == 0;
+        const bool vec = n >= N;
         const int64_t cols = ceil_div(n, static_cast<int64_t>(kThreads) * (vec ? N : 1));
         if (n_tokens * cols > kMaxBlocks) {
           set_error("%lld rows of %d: too many for one launch", (long long)n_tokens, n);
@@ -378,15 +399,21 @@ extern "C" int ej_expert_combine_vjp(const void *y, int32_t dtype, int64_t n_slo
     EJ_CHECK_ARG(offsets && (n_tokens == 0 || (slots && (grad || n == 0))), "null argument");
     EJ_CHECK_ARG(ld_y >= n && ld_grad >= n, "row stride below n = %d", n);
     CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, offsets, n_groups, nullptr};
-    const bool vec = aligned16(y, ld_y, sizeof(T)) && aligned16(grad, ld_grad, sizeof(T)) &&
-                     aligned16(grad_y, n, sizeof(T));
     const dim3 grid(static_cast<unsigned>(n_tokens + kZeroBlocks));
-    if (vec)
-      hipLaunchKernelGGL((combine_vjp_kernel<T, true>), grid, dim3(kThreads), 0,
-                         as_stream(stream), a, grad, ld_grad, grad_y, grad_weights);
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, as_stream(stream), a, grad, ld_grad,
+                         grad_y, grad_weights);
+    };
+    // Rows of no whole pieces, 16384 tokens of 4 picks, with the last piece moved
+    // back and element by element: bf16 4095 columns 311 and 609 us, f16 1001
+    // 109 and 155, 501 57 and 61, 150 53 and 39; fp32 2047 276 and 280, 501 110
+    // and 81.
+    if (n % (16 / static_cast<int>(sizeof(T))) == 0)
+      run(combine_vjp_kernel<T, true, true>);
+    else if (sizeof(T) == 2 && n >= 512)
+      run(combine_vjp_kernel<T, sizeof(T) == 2, false>);
     else
-      hipLaunchKernelGGL((combine_vjp_kernel<T, false>), grid, dim3(kThreads), 0,
-                         as_stream(stream), a, grad, ld_grad, grad_y, grad_weights);
+      run(combine_vjp_kernel<T, false, true>);
     EJ_LAUNCH_CHECK();
     return EJ_OK;
   });
@@ -405,8 +432,7 @@ extern "C" int ej_quantize_rows(const void *x, int32_t dtype, int64_t n_rows, in
       return EJ_E_UNSUPPORTED;
     }
     constexpr int N = 16 / sizeof(T);
-    const bool vec = aligned16(x, ld, sizeof(T)) && n % N == 0 &&
-                     reinterpret_cast<size_t>(q) % N == 0;
+    const bool vec = n >= N;
     const T *xt = static_cast<const T *>(x);
     auto run = [&](auto kernel, int64_t blocks) {
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,

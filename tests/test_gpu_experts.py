@@ -642,6 +642,18 @@ def test_quantize_rows(gpu, m, n, dtype):
         assert torch.equal(q.abs().amax(1) == 127, scale > 0)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [7, 9, 513, 1001, 2055, 4095])
+def test_combine_rows_of_no_whole_pieces(gpu, n, dtype):
+    test_combine(gpu, 33, 5, 3, n, dtype, "holes")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n", [(2000, 77), (2000, 1001), (1100, 4095), (3, 4097), (2, 30001)])
+def test_quantize_rows_of_no_whole_pieces(gpu, m, n, dtype):
+    test_quantize_rows(gpu, m, n, dtype)
+
+
 def test_quantize_rows_not_finite_and_tiny(gpu):
     x = torch.ones(5, 40, device="cuda")
     x[1, 7] = float("inf")
