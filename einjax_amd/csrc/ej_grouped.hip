@@ -64,8 +64,8 @@ int split_parts(double tiles, int64_t contraction, int elem, bool whole, double 
   // 2497 in 6 groups, 281 tiles: 66 us, 78 in two parts)
   if (tiles <= 0 || stages < 8 || (whole && elem == 4 && tiles > 192)) return 1;
   const int64_t want = static_cast<int64_t>((whole ? 576 : 1152) / tiles);
-  const int64_t most = whole ? (stages / 8 < 32 ? stages / 8 : 32) : stages / 4 < 8 ? stages / 4 : 8;
-  const int64_t parts = want < most ? want : most;
+  const int64_t most = whole ? stages / 8 : stages / 4, cap = whole ? 32 : 8;
+  const int64_t parts = want < most && want < cap ? want : most < cap ? most : cap;
   if (parts < 2) return 1;
   const double saved = stages * (1 - 1. / parts) * (elem == 4 ? 0.7 : 0.4) * (whole ? 1 : 2);
   return saved > 5 + parts * sums * 8 / 4e6 ? static_cast<int>(parts) : 1;

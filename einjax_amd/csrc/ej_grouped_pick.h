@@ -189,14 +189,24 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
 //    8192     8   2048 x 2560   153/219    101/129    86/102
 //   16384    16   2048 x 4096   522/721    350/442   273/308
 // fp32: 4096 rows, 8 groups, 1024 x 2048: 128 x 128 153, 64 x 64 173; 1200
-// rows, 5 groups, 320 x 520: 32 and 13.
+// rows, 5 groups, 320 x 520: 32 and 13.  Through registers, f16, 64 x 64 and 128
+// x 128: 16384 rows, 8 groups, 1023 x 2047 267/294 and 182/200; 4096, 4, 771 x
+// 1283 52/56 and 43/49; 5820, 7, 512 x 1477 43/51 and 43/47, in very
+// unequal groups 16 more (few tiles of the longest one); fp32 4096, 4, 771 x
+// 1283 153 and 200.
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
-  if (!direct) return launch_wgrad<Op, 64, 64, 2, 2, false, 2>(g, stream);
-  if (g.splits > 1) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
   auto tiles = [&](int b) {
     return static_cast<double>(ceil_div(g.m, b) * ceil_div(g.n, b) * g.n_groups);
   };
+  if (!direct) {
+    if constexpr (kElem<Op> == 2) {
+      if (g.splits == 1 && tiles(128) >= 512)
+        return launch_wgrad<Op, 128, 128, 2, 4, false, 2>(g, stream);
+    }
+    return launch_wgrad<Op, 64, 64, 2, 2, false, 2>(g, stream);
+  }
+  if (g.splits > 1) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
   if (tiles(128) < 256) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
   if constexpr (kElem<Op> == 2) {
     const double small = tiles(128) / 512;

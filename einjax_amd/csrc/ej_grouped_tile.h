@@ -701,8 +701,8 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
 // of group-major rows, m to a group, goes to c_group, ldc.  Rows of no group
 // (offsets given) are zero already.  Bound by its launch: 3.5 us for 16 parts
 // of 128 x 128.
-static __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g, int64_t rows, int64_t m,
-                                                           bool skip_dead) {
+static __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g, int64_t rows,
+                                                                  int64_t m, bool skip_dead) {
   const int64_t quads = (g.n + 3) / 4, i = blockIdx.x * 256ll + threadIdx.x;
   if (i >= rows * quads) return;
   const int64_t row = i / quads;

@@ -347,7 +347,8 @@ def test_grouped_matmul_large_blocks(gpu, sizes, dead, k, n, dtype, order):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("sizes,m,n", [
     ([70, 0, 131, 64], 1024, 1024), ([40, 0, 200, 1, 65, 31, 90, 33, 64], 2048, 2048),
-    ([3, 70, 64, 90, 1, 0, 128, 40, 10], 2048, 2312), ([129, 30, 0, 77], 2048, 4000)])
+    ([3, 70, 64, 90, 1, 0, 128, 40, 10], 2048, 2312), ([129, 30, 0, 77], 2048, 4000),
+    ([70, 0, 131, 64, 3, 9, 20, 1], 1023, 1029), ([5, 200, 0, 77, 1], 1031, 1800)])
 def test_grouped_weight_gradient_large_blocks(gpu, sizes, m, n, dtype, gather):
     g, e, live = rng(m + n), len(sizes), sum(sizes)
     r = ej.group_by_expert(torch.repeat_interleave(torch.arange(e), torch.tensor(sizes))
