@@ -7,6 +7,7 @@
 // the C entry points of include/einjax_hip.h and computes nothing itself.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/util/Exception.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -28,15 +29,19 @@ using torch::autograd::variable_list;
 
 // ---- checks ------------------------------------------------------------------
 
+// Raised as NotImplementedError.  A C++ exception that holds no Python state:
+// gradients are computed on autograd's thread, which does not hold Python's lock.
+[[noreturn]] void not_implemented(const std::string &msg) {
+  C10_THROW_ERROR(NotImplementedError, msg);
+}
+
 void check(int status, const char *what) {
   if (status == EJ_OK) return;
   const std::string msg = std::string(what) + ": " + ej_last_error();
   switch (status) {
     case EJ_E_INVAL:
     case EJ_E_RANGE: throw py::value_error(msg);
-    case EJ_E_UNSUPPORTED:
-      PyErr_SetString(PyExc_NotImplementedError, msg.c_str());
-      throw py::error_already_set();
+    case EJ_E_UNSUPPORTED: not_implemented(msg);
     default: throw std::runtime_error("HIP error in " + msg);
   }
 }
@@ -680,6 +685,13 @@ Tensor int8_matmul(py::handle q_, py::handle q_scale_, py::handle w_, py::handle
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "Expert operators for torch tensors over libejhip.so.";
+  py::register_local_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const c10::NotImplementedError &e) {
+      PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
+    }
+  });
   m.def("route", &route);
   m.def("route_vjp", &route_vjp);
   m.def("group", &group);

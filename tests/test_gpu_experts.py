@@ -831,3 +831,16 @@ def test_refusals_of_gpu_tensors(gpu):
         ej.route_experts(torch.zeros(2, 2000, device="cuda"), 2)
     with pytest.raises(NotImplementedError):
         ej.route_experts(torch.zeros(2, 100, device="cuda"), 17)
+
+
+def test_a_refused_gradient_raises(gpu):
+    """Refusals of a backward, which runs on autograd's thread without Python's lock."""
+    e = 1 << 24
+    x = torch.zeros(0, 1, device="cuda")
+    w = torch.zeros(e, 1, 1, device="cuda", requires_grad=True)
+    offsets = torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    y = ej.grouped_matmul(x, w, offsets)
+    with pytest.raises(NotImplementedError, match="too many"):
+        y.sum().backward()
+    with pytest.raises(NotImplementedError, match="too many"):
+        ej.grouped_matmul_vjp(x, w.detach(), offsets, y.detach(), need_x=False)
