@@ -45,8 +45,8 @@ def grouped_matmul(x, w, groups, *, gather: bool = False, out_dtype=None):
     are already grouped.  x [slots, k]; with ``gather=True`` x [tokens, k] and
     slot s takes its token's row, without a copy.  Rows of no group are zero.
     float32, bfloat16 or float16, summed in fp32; the result has x's dtype
-    unless ``out_dtype=torch.float32``.  Differentiable in x and w; the
-    gradient to w lies as w does."""
+    unless ``out_dtype=torch.float32``.  Differentiable in x and w (in gathered
+    x for routings of 1 to 16 picks); the gradient to w lies as w does."""
     offsets, rows, slots = group_args(groups)
     return _lib.experts().grouped_matmul(x, w, offsets, rows, slots, gather, out_dtype)
 

@@ -14,7 +14,6 @@ namespace ej {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxPicks = 16;
 constexpr int kZeroBlocks = 256;  // workgroups that zero the rows no pair holds
 // HIP launches hold fewer than 2^32 threads.
 constexpr int64_t kMaxBlocks = ((int64_t{1} << 32) - 1) / kThreads;
@@ -123,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, co
         static_cast<T *>(grad_y)[s * a.n + col] = static_cast<T>(0.f);
     return;
   }
-  __shared__ float part[W][kMaxPicks];
+  __shared__ float part[W][EJ_MAX_PICKS];
   const int64_t t = blockIdx.x;
   const T *g = static_cast<const T *>(grad) + t * ld_grad;
   for (int j = 0; j < a.k; ++j) {
@@ -335,9 +334,9 @@ int by_type(int32_t dtype, F f) {
 int check_combine(int64_t n_slots, int64_t n_tokens, int32_t k, int32_t n) {
   EJ_CHECK_ARG(n_slots >= 0 && n_tokens >= 0 && n >= 0, "negative size");
   EJ_CHECK_ARG(k >= 1, "k = %d, expected at least 1", k);
-  if (k > kMaxPicks || n_tokens > kMaxBlocks - kZeroBlocks || n_slots >= (int64_t{1} << 31)) {
+  if (k > EJ_MAX_PICKS || n_tokens > kMaxBlocks - kZeroBlocks || n_slots >= (int64_t{1} << 31)) {
     set_error("%lld tokens of %d picks: at most %lld of %d are supported", (long long)n_tokens, k,
-              (long long)(kMaxBlocks - kZeroBlocks), kMaxPicks);
+              (long long)(kMaxBlocks - kZeroBlocks), EJ_MAX_PICKS);
     return EJ_E_UNSUPPORTED;
   }
   return EJ_OK;

@@ -21,7 +21,6 @@
 namespace ej {
 namespace {
 
-constexpr int kMaxPicks = 16;
 constexpr int kMaxExperts = 1024;
 constexpr int kRouteThreads = 1024;  // a workgroup a CU: one pass of 64 tokens
 constexpr int kVjpThreads = 256;
@@ -439,9 +438,9 @@ int check_route(int64_t n_tokens, int32_t n_experts, int32_t k) {
   EJ_CHECK_ARG(n_tokens >= 0, "n_tokens = %lld is negative", (long long)n_tokens);
   EJ_CHECK_ARG(n_experts >= 1, "n_experts = %d, expected at least 1", n_experts);
   EJ_CHECK_ARG(k >= 1 && k <= n_experts, "k = %d, expected 1 to n_experts = %d", k, n_experts);
-  if (n_experts > kMaxExperts || k > kMaxPicks) {
+  if (n_experts > kMaxExperts || k > EJ_MAX_PICKS) {
     set_error("%d experts and %d picks: at most %d and %d are supported", n_experts, k,
-              kMaxExperts, kMaxPicks);
+              kMaxExperts, EJ_MAX_PICKS);
     return EJ_E_UNSUPPORTED;
   }
   if (n_tokens >= (int64_t{1} << 26) || n_tokens * k >= (int64_t{1} << 31)) {

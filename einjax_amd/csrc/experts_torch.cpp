@@ -585,12 +585,21 @@ at::ScalarType check_product(const Tensor &x, const Tensor &w, py::handle out_dt
   return t;
 }
 
+// The gradient to gathered rows is the sum of each token's slots.
+void check_picks(const Tensor &slots) {
+  if (slots.size(1) < 1 || slots.size(1) > EJ_MAX_PICKS)
+    not_implemented("the gradient to gathered rows adds 1 to " + std::to_string(EJ_MAX_PICKS) +
+                    " slots of a token, the routing has " + std::to_string(slots.size(1)));
+}
+
 Tensor grouped_matmul(py::handle x_, py::handle w_, py::handle offsets, py::handle rows,
                       py::handle slots, bool gather, py::handle out_dtype) {
   const Tensor x = on_gpu(x_, "x"), w = on_gpu_of(x, w_, "w");
   const at::ScalarType t = check_product(x, w, out_dtype);
   const Groups g = groups_of(x, w.size(0), offsets, rows, slots, gather);
   if (!wants_grad(x) && !wants_grad(w)) return product(x, w, g, t);
+  // refused now, not when the gradient is asked for
+  if (wants_grad(x) && g.slots.defined()) check_picks(g.slots);
   return ProductFunction::apply(x, w, &g, static_cast<int64_t>(t));
 }
 
@@ -600,6 +609,7 @@ py::tuple grouped_matmul_vjp(py::handle x_, py::handle w_, py::handle offsets, p
   const Tensor x = on_gpu(x_, "x"), w = on_gpu_of(x, w_, "w");
   check_product(x, w, py::none());
   const Groups g = groups_of(x, w.size(0), offsets, rows, slots, gather);
+  if (need_x && g.slots.defined()) check_picks(g.slots);
   const Tensor grad = on_gpu_of(x, grad_, "grad_out");
   if (grad.dim() != 2 || grad.size(0) != g.n_slots || grad.size(1) != w.size(2))
     throw py::value_error("grad_out has shape " + str(grad.sizes()) + ", expected " +

@@ -673,9 +673,10 @@ int ej_relation_to_dense(const int32_t *coords, const void *values, int64_t n_ti
  * [n_tokens, k]: the softmax over all logits at the picks, or with
  * renormalize != 0 the softmax over the picks.  A token with fewer than k
  * experts left has experts -1, weights 0 and slots -1 for the rest.
- * At most 1024 experts and 16 picks.  The workspace may be NULL where its size
+ * At most 1024 experts and EJ_MAX_PICKS picks.  The workspace may be NULL where its size
  * is 0.  ej_expert_group groups picks that the caller made (int32
  * [n_tokens, k]; a value outside [0, n_experts) has no slot). */
+#define EJ_MAX_PICKS 16
 int ej_expert_route_workspace_size(int64_t n_tokens, int32_t n_experts, size_t *bytes);
 int ej_expert_route(const void *logits, int32_t dtype, int64_t n_tokens, int32_t n_experts,
                     int64_t ld, int32_t k, int32_t renormalize, float *weights, int32_t *experts,

@@ -844,3 +844,26 @@ def test_a_refused_gradient_raises(gpu):
         y.sum().backward()
     with pytest.raises(NotImplementedError, match="too many"):
         ej.grouped_matmul_vjp(x, w.detach(), offsets, y.detach(), need_x=False)
+
+
+@pytest.mark.parametrize("k", [0, 17])
+def test_gathered_products_refuse_a_gradient_they_do_not_have(gpu, k):
+    """More picks than the sum back to the tokens takes: said before the product."""
+    g = rng(17)
+    x, w = randn(g, 3, 8), randn(g, 2, 8, 5)
+    slots = torch.arange(3 * k, dtype=torch.int32, device="cuda").reshape(3, k)
+    r = ej.ExpertRouting(torch.ones(3, k, device="cuda"), torch.zeros_like(slots),
+                         torch.tensor([0, 3 * k, 3 * k], dtype=torch.int32, device="cuda"),
+                         (torch.arange(3 * k, device="cuda") // max(k, 1)).int(), slots)
+    y = ej.grouped_matmul(x, w, r, gather=True)
+    want, mag = product64(x, r.rows, r.offsets, w, 3 * k)
+    assert_within(y, want, sum_bound(want, mag, 8, F32))
+    with pytest.raises(NotImplementedError, match="slots of a token"):
+        ej.grouped_matmul(x.clone().requires_grad_(), w, r, gather=True)
+    with pytest.raises(NotImplementedError, match="slots of a token"):
+        ej.grouped_matmul_vjp(x, w, r, y, gather=True)
+    leaf = w.clone().requires_grad_()
+    (gw,) = torch.autograd.grad(ej.grouped_matmul(x, leaf, r, gather=True), leaf, y)
+    xi = x[r.rows.long()].double()
+    assert_within(gw[0], xi.T @ y.double(),
+                  sum_bound(xi.T @ y.double(), xi.abs().T @ y.double().abs(), 3 * k, F32))
