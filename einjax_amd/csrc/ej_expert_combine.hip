@@ -334,11 +334,25 @@ int by_type(int32_t dtype, F f) {
 int check_combine(int64_t n_slots, int64_t n_tokens, int32_t k, int32_t n) {
   EJ_CHECK_ARG(n_slots >= 0 && n_tokens >= 0 && n >= 0, "negative size");
   EJ_CHECK_ARG(k >= 1, "k = %d, expected at least 1", k);
-  if (k > EJ_MAX_PICKS || n_tokens > kMaxBlocks - kZeroBlocks || n_slots >= (int64_t{1} << 31)) {
-    set_error("%lld tokens of %d picks: at most %lld of %d are supported", (long long)n_tokens, k,
-              (long long)(kMaxBlocks - kZeroBlocks), EJ_MAX_PICKS);
+  if (k > EJ_MAX_PICKS || n_tokens >= (int64_t{1} << 31) || n_slots >= (int64_t{1} << 31)) {
+    set_error("%lld tokens of %d picks, %lld slots: at most %d picks and fewer than 2^31 tokens "
+              "and slots are supported", (long long)n_tokens, k, (long long)n_slots, EJ_MAX_PICKS);
     return EJ_E_UNSUPPORTED;
   }
+  return EJ_OK;
+}
+
+// launch(first, count) for ranges of tokens, of which a launch holds `most`
+// (a first range also where there are none).
+template <class F>
+int by_tokens(int64_t n_tokens, int64_t most, F launch) {
+  int64_t first = 0;
+  do {
+    const int64_t count = n_tokens - first < most ? n_tokens - first : most;
+    launch(first, count);
+    EJ_LAUNCH_CHECK();
+    first += count;
+  } while (first < n_tokens);
   return EJ_OK;
 }
 
@@ -366,18 +380,16 @@ extern "C" int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, 
         constexpr int N = 16 / sizeof(T);
         const bool vec = n >= N;
         const int64_t cols = ceil_div(n, static_cast<int64_t>(kThreads) * (vec ? N : 1));
-        if (n_tokens * cols > kMaxBlocks) {
-          set_error("%lld rows of %d: too many for one launch", (long long)n_tokens, n);
-          return EJ_E_UNSUPPORTED;
-        }
-        const dim3 grid(static_cast<unsigned>(n_tokens * cols));
-        if (vec)
-          hipLaunchKernelGGL((combine_kernel<T, O, true>), grid, dim3(kThreads), 0,
-                             as_stream(stream), a, static_cast<unsigned>(cols));
-        else
-          hipLaunchKernelGGL((combine_kernel<T, O, false>), grid, dim3(kThreads), 0,
-                             as_stream(stream), a, static_cast<unsigned>(cols));
-        EJ_LAUNCH_CHECK();
+        return by_tokens(n_tokens, kMaxBlocks / cols, [&](int64_t first, int64_t count) {
+          CombineArgs b = a;
+          b.n_tokens = count;
+          b.slots += first * k;
+          if (b.weights) b.weights += first * k;
+          b.out = static_cast<O *>(out) + first * n;
+          hipLaunchKernelGGL((vec ? combine_kernel<T, O, true> : combine_kernel<T, O, false>),
+                             dim3(static_cast<unsigned>(count * cols)), dim3(kThreads), 0,
+                             as_stream(stream), b, static_cast<unsigned>(cols));
+        });
       }
       return EJ_OK;
     });
@@ -398,23 +410,28 @@ extern "C" int ej_expert_combine_vjp(const void *y, int32_t dtype, int64_t n_slo
     EJ_CHECK_ARG(offsets && (n_tokens == 0 || (slots && (grad || n == 0))), "null argument");
     EJ_CHECK_ARG(ld_y >= n && ld_grad >= n, "row stride below n = %d", n);
     CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, offsets, n_groups, nullptr};
-    const dim3 grid(static_cast<unsigned>(n_tokens + kZeroBlocks));
     auto run = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, as_stream(stream), a, grad, ld_grad,
-                         grad_y, grad_weights);
+      return by_tokens(n_tokens, kMaxBlocks - kZeroBlocks, [&](int64_t first, int64_t count) {
+        CombineArgs b = a;
+        b.n_tokens = count;
+        b.slots += first * k;
+        if (b.weights) b.weights += first * k;
+        hipLaunchKernelGGL(kernel,
+                           dim3(static_cast<unsigned>(count + (first == 0 ? kZeroBlocks : 0))),
+                           dim3(kThreads), 0, as_stream(stream), b,
+                           static_cast<const T *>(grad) + first * ld_grad, ld_grad, grad_y,
+                           grad_weights ? grad_weights + first * k : nullptr);
+      });
     };
     // Rows of no whole pieces, 16384 tokens of 4 picks, with the last piece moved
     // back and element by element: bf16 4095 columns 311 and 609 us, f16 1001
     // 109 and 155, 501 57 and 61, 150 53 and 39; fp32 2047 276 and 280, 501 110
     // and 81.
     if (n % (16 / static_cast<int>(sizeof(T))) == 0)
-      run(combine_vjp_kernel<T, true, true>);
-    else if (sizeof(T) == 2 && n >= 512)
-      run(combine_vjp_kernel<T, sizeof(T) == 2, false>);
-    else
-      run(combine_vjp_kernel<T, false, true>);
-    EJ_LAUNCH_CHECK();
-    return EJ_OK;
+      return run(combine_vjp_kernel<T, true, true>);
+    if (sizeof(T) == 2 && n >= 512)
+      return run(combine_vjp_kernel<T, sizeof(T) == 2, false>);
+    return run(combine_vjp_kernel<T, false, true>);
   });
 }
 

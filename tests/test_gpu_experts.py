@@ -867,3 +867,25 @@ def test_gathered_products_refuse_a_gradient_they_do_not_have(gpu, k):
     xi = x[r.rows.long()].double()
     assert_within(gw[0], xi.T @ y.double(),
                   sum_bound(xi.T @ y.double(), xi.abs().T @ y.double().abs(), 3 * k, F32))
+
+
+@pytest.mark.parametrize("n", [1, 8])
+def test_combine_of_more_tokens_than_a_launch_holds(gpu, n):
+    """2^24 workgroups and more, of which a launch holds fewer."""
+    g, t = rng(n), (1 << 24) + 777
+    slots = torch.arange(t, device="cuda").flip(0).int()[:, None]
+    slots[-3:] = -1
+    offsets = torch.tensor([0, t], dtype=torch.int32, device="cuda")
+    weights = randn(g, t, 1)
+    y, cot = randn(g, t, n, dtype=BF16), randn(g, t, n, dtype=BF16)
+    r = ej.ExpertRouting(weights, torch.zeros_like(slots), offsets, slots.flatten(), slots)
+    at = y.flip(0)
+    at[-3:] = 0
+    # one product and one rounding: the same in torch
+    assert torch.equal(ej.combine_experts(y, r), (weights * at.float()).to(BF16))
+    gy, gw = ej.combine_experts_vjp(y, r, cot)
+    want = (weights * cot.float()).to(BF16).flip(0)
+    assert torch.equal(gy[3:], want[3:])
+    ww = (at.double() * cot.double()).sum(1, keepdim=True)
+    mag = (at.double() * cot.double()).abs().sum(1, keepdim=True)
+    assert_within(gw, ww, 2 * (n + 2) * 2.0 ** -24 * mag + 1e-37)
