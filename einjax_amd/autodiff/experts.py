@@ -43,7 +43,9 @@ def grouped_matmul(x, w, groups, *, gather: bool = False, out_dtype=None):
     weights [E, n, k] is taken as it lies).  groups: an ``ExpertRouting``, or
     offsets [E + 1] (non-decreasing, int32 or int64, on the GPU) of rows that
     are already grouped.  x [slots, k]; with ``gather=True`` x [tokens, k] and
-    slot s takes its token's row, without a copy.  Rows of no group are zero.
+    slot s takes its token's row, without a copy (the gradient to x is the sum
+    over routing.slots, see ``ExpertRouting`` on pairs taken out).  Rows of no
+    group are zero.
     float32, bfloat16 or float16, summed in fp32; the result has x's dtype
     unless ``out_dtype=torch.float32``.  Differentiable in x and w (in gathered
     x for routings of 1 to 16 picks); the gradient to w lies as w does."""
@@ -72,7 +74,8 @@ def combine_experts(y, routing: ExpertRouting, weights=None):
     y [slots, n] (float32, bfloat16 or float16), a row for each slot; weights
     float32 [T, k], by default the routing's own.  Summed in fp32 in the order
     of the picks and rounded once to y's dtype; pairs without a slot are left
-    out (a token without any gets zeros).  Differentiable in y and weights."""
+    out (a token without any gets zeros).  Differentiable in y (rows that no
+    pair holds have a gradient of zero) and weights."""
     return _lib.experts().combine(*_combine_args(y, routing, weights))
 
 

@@ -14,7 +14,8 @@ namespace ej {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kZeroBlocks = 256;  // workgroups that zero the rows no pair holds
+constexpr int kZeroBlocks = 128;   // workgroups that zero the rows no pair holds
+constexpr int kHeldWords = 2048;   // bits of rows that one of them keeps at a time, / 32
 // HIP launches hold fewer than 2^32 threads.
 constexpr int64_t kMaxBlocks = ((int64_t{1} << 32) - 1) / kThreads;
 
@@ -63,12 +64,10 @@ struct Piece {
 struct CombineArgs {
   const void *y;
   int64_t ld_y, ld_out;
-  int64_t n_slots, n_tokens;
+  int64_t n_slots;
   int32_t k, n;
-  const float *weights;    // null: every weight is 1
+  const float *weights;  // null: every weight is 1
   const int32_t *slots;
-  const int32_t *offsets;  // gradient: offsets[n_groups] = live slots
-  int32_t n_groups;
   void *out;
 };
 
@@ -102,28 +101,78 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a, unsign
   o.store(static_cast<O *>(a.out) + t * a.ld_out + col);
 }
 
+// Zeroes the rows of grad_y that no pair holds.  Which those are goes by the
+// slots alone (a caller may take pairs out by a slot of -1).  Workgroup `block`
+// of kZeroBlocks looks after every kZeroBlocks-th row: it notes in LDS which of
+// its rows the n_pairs pairs hold, then zeroes the others, a wave a row.  So all
+// pairs' slots are read by each of them, from the L2 and beside the gradients:
+// 16384 tokens of 4 picks, bf16, gradients alone and with the rows (none, all
+// unheld): 4096 columns 250, 250 and 128 us, 512 columns 75, 77 and 36, 64
+// columns 43, 45 and 29.  64 workgroups are 1 us faster with no such row and up
+// to 17 slower with half of them, 256 the other way round.  Numbers left in the
+// rows by a launch before and looked at by another took 5 to 13 us more.
+template <class T>
+__device__ inline void zero_unheld_rows(const CombineArgs &a, int64_t n_pairs, T *grad_y,
+                                        int block) {
+  constexpr int N = 16 / static_cast<int>(sizeof(T)), W = kThreads / 64;
+  __shared__ uint32_t held[kHeldWords];
+  const int lane = threadIdx.x & 63;
+  const int64_t mine = (a.n_slots - block + kZeroBlocks - 1) / kZeroBlocks;
+  for (int64_t i0 = 0; i0 < mine; i0 += 32 * kHeldWords) {
+    const int count = static_cast<int>(mine - i0 < 32 * kHeldWords ? mine - i0 : 32 * kHeldWords);
+    const int words = (count + 31) / 32;
+    for (int w = threadIdx.x; w < words; w += kThreads) held[w] = 0;
+    __syncthreads();
+    auto look = [&](int64_t s) {
+      if ((s & (kZeroBlocks - 1)) != block || s < 0) return;
+      const int64_t i = s / kZeroBlocks - i0;
+      if (i >= 0 && i < count) atomicOr(&held[i >> 5], 1u << (i & 31));
+    };
+    const int64_t quads = n_pairs / 4;
+#pragma unroll 4
+    for (int64_t q = threadIdx.x; q < quads; q += kThreads) {
+      const words_t v = *reinterpret_cast<const words_t *>(a.slots + 4 * q);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) look(static_cast<int32_t>(v[c]));
+    }
+    if (threadIdx.x < n_pairs - 4 * quads) look(a.slots[4 * quads + threadIdx.x]);
+    __syncthreads();
+    for (int w = threadIdx.x >> 6; w < words; w += W) {
+      const int last = count - 32 * w;
+      uint32_t left = __builtin_amdgcn_readfirstlane(~held[w] &
+                                                     (last < 32 ? (1u << last) - 1 : ~0u));
+      for (; left; left &= left - 1) {
+        T *row = grad_y + ((i0 + 32 * w + __builtin_ctz(left)) * kZeroBlocks + block) * a.n;
+        if (a.n >= N) {
+          const words_t zero = {0, 0, 0, 0};
+          for (int64_t col = lane * N; col < a.n; col += 64 * N)
+            *reinterpret_cast<words_t *>(row + piece_at<N>(col, a.n)) = zero;
+        } else if (lane < a.n) {
+          row[lane] = static_cast<T>(0.f);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
 // grad_y[slots[t, j]] = weights[t, j] grad[t]; grad_w[t, j] = grad[t] . y[slots[t, j]].
-// One workgroup a token, so every dot product is summed in a fixed order;
-// workgroups past the tokens zero grad_y's rows that no pair holds.  At the
-// sizes above 230 us (1.18 GB, 5.1 TB/s).
+// One workgroup a token, so every dot product is summed in a fixed order; the
+// first `zeroing` workgroups zero grad_y's rows that no pair of the n_pairs holds.
+// At the sizes above 230 us (1.18 GB, 5.1 TB/s).
 // WHOLE: rows of whole pieces; otherwise the last one is moved back.
 template <class T, bool VEC, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void combine_vjp_kernel(CombineArgs a, const void *grad,
                                                                int64_t ld_grad, void *grad_y,
-                                                               float *grad_w) {
+                                                               float *grad_w, int zeroing,
+                                                               int64_t n_pairs) {
   constexpr int N = Piece<T, VEC>::N, W = kThreads / 64;
-  if (blockIdx.x >= a.n_tokens) {
-    if (!grad_y) return;
-    int64_t live = a.offsets[a.n_groups];
-    live = live < 0 ? 0 : live;
-    for (int64_t s = live + (blockIdx.x - a.n_tokens); s < a.n_slots;
-         s += gridDim.x - a.n_tokens)
-      for (int64_t col = threadIdx.x; col < a.n; col += kThreads)
-        static_cast<T *>(grad_y)[s * a.n + col] = static_cast<T>(0.f);
+  if (blockIdx.x < zeroing) {
+    zero_unheld_rows(a, n_pairs, static_cast<T *>(grad_y), blockIdx.x);
     return;
   }
   __shared__ float part[W][EJ_MAX_PICKS];
-  const int64_t t = blockIdx.x;
+  const int64_t t = blockIdx.x - zeroing;
   const T *g = static_cast<const T *>(grad) + t * ld_grad;
   for (int j = 0; j < a.k; ++j) {
     const int64_t s = a.slots[t * a.k + j];
@@ -334,8 +383,9 @@ int by_type(int32_t dtype, F f) {
 int check_combine(int64_t n_slots, int64_t n_tokens, int32_t k, int32_t n) {
   EJ_CHECK_ARG(n_slots >= 0 && n_tokens >= 0 && n >= 0, "negative size");
   EJ_CHECK_ARG(k >= 1, "k = %d, expected at least 1", k);
-  if (k > EJ_MAX_PICKS || n_tokens >= (int64_t{1} << 31) || n_slots >= (int64_t{1} << 31)) {
-    set_error("%lld tokens of %d picks, %lld slots: at most %d picks and fewer than 2^31 tokens "
+  if (k > EJ_MAX_PICKS || n_tokens >= ((int64_t{1} << 31) + k - 1) / k ||
+      n_slots >= (int64_t{1} << 31)) {
+    set_error("%lld tokens of %d picks, %lld slots: at most %d picks and fewer than 2^31 pairs "
               "and slots are supported", (long long)n_tokens, k, (long long)n_slots, EJ_MAX_PICKS);
     return EJ_E_UNSUPPORTED;
   }
@@ -376,13 +426,12 @@ extern "C" int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, 
         if (n_tokens == 0 || n == 0) return EJ_OK;
         EJ_CHECK_ARG(slots && out && (y || n_slots == 0), "null argument");
         EJ_CHECK_ARG(ld_y >= n, "row stride %lld below n = %d", (long long)ld_y, n);
-        CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, nullptr, 0, out};
+        CombineArgs a{y, ld_y, n, n_slots, k, n, weights, slots, out};
         constexpr int N = 16 / sizeof(T);
         const bool vec = n >= N;
         const int64_t cols = ceil_div(n, static_cast<int64_t>(kThreads) * (vec ? N : 1));
         return by_tokens(n_tokens, kMaxBlocks / cols, [&](int64_t first, int64_t count) {
           CombineArgs b = a;
-          b.n_tokens = count;
           b.slots += first * k;
           if (b.weights) b.weights += first * k;
           b.out = static_cast<O *>(out) + first * n;
@@ -409,18 +458,19 @@ extern "C" int ej_expert_combine_vjp(const void *y, int32_t dtype, int64_t n_slo
     if (n_slots == 0 && n_tokens == 0) return EJ_OK;
     EJ_CHECK_ARG(offsets && (n_tokens == 0 || (slots && (grad || n == 0))), "null argument");
     EJ_CHECK_ARG(ld_y >= n && ld_grad >= n, "row stride below n = %d", n);
-    CombineArgs a{y, ld_y, n, n_slots, n_tokens, k, n, weights, slots, offsets, n_groups, nullptr};
+    CombineArgs a{y, ld_y, n, n_slots, k, n, weights, slots, nullptr};
     auto run = [&](auto kernel) {
       return by_tokens(n_tokens, kMaxBlocks - kZeroBlocks, [&](int64_t first, int64_t count) {
         CombineArgs b = a;
-        b.n_tokens = count;
         b.slots += first * k;
         if (b.weights) b.weights += first * k;
-        hipLaunchKernelGGL(kernel,
-                           dim3(static_cast<unsigned>(count + (first == 0 ? kZeroBlocks : 0))),
-                           dim3(kThreads), 0, as_stream(stream), b,
+        const int zeroing = first == 0 && grad_y ? kZeroBlocks : 0;
+        if (count + zeroing == 0) return;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(count + zeroing)), dim3(kThreads), 0,
+                           as_stream(stream), b,
                            static_cast<const T *>(grad) + first * ld_grad, ld_grad, grad_y,
-                           grad_weights ? grad_weights + first * k : nullptr);
+                           grad_weights ? grad_weights + first * k : nullptr, zeroing,
+                           n_tokens * k);
       });
     };
     // Rows of no whole pieces, 16384 tokens of 4 picks, with the last piece moved

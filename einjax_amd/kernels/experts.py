@@ -33,7 +33,15 @@ class ExpertRouting:
     experts: int32 [T, k], -1 where a token has fewer than k experts;
     offsets: int32 [E + 1], slots [offsets[e], offsets[e + 1]) are expert e's;
     rows: int32 [T * k], the token of each slot (0 past the last slot in use);
-    slots: int32 [T, k], the slot of each pair (-1 where there is none).
+    slots: int32 [T, k], the slot of each pair (-1 where there is none); no two
+    pairs have the same slot, and rows[slots[t, j]] = t.
+
+    A caller may take single pairs out by setting their slot to -1 (an expert's
+    capacity, say).  ``combine_experts`` then leaves them out, and the gradient
+    to their rows is zero.  The products, which go by offsets and rows, still
+    compute those rows and take them into the gradient to the weights; the
+    gradient to gathered rows, which adds up a token's slots, does not.  The two
+    agree where the rows are used through ``combine_experts`` alone.
     """
 
     weights: torch.Tensor

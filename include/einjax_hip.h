@@ -700,10 +700,10 @@ int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_
                       const float *weights, const int32_t *slots, int64_t n_tokens, int32_t k,
                       int32_t n, void *out, int32_t out_dtype, ej_stream_t stream);
 
-/* Its gradients: grad_y [n_slots, n] contiguous, zero in the rows from
- * offsets[n_groups] on, and grad_weights [n_tokens, k]; either may be NULL.
- * Every slot below offsets[n_groups] must be held by exactly one pair, as
- * ej_expert_route makes them. */
+/* Its gradients: grad_y [n_slots, n] contiguous, zero in the rows that no pair
+ * holds, and grad_weights [n_tokens, k]; either may be NULL.  No slot may be
+ * held by two pairs.  Which slots are held goes by `slots` alone; offsets, of
+ * n_groups groups, must be given and is not read. */
 int ej_expert_combine_vjp(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
                           const float *weights, const int32_t *slots, const int32_t *offsets,
                           int32_t n_groups, int64_t n_tokens, int32_t k, int32_t n,

@@ -889,3 +889,51 @@ def test_combine_of_more_tokens_than_a_launch_holds(gpu, n):
     ww = (at.double() * cot.double()).sum(1, keepdim=True)
     mag = (at.double() * cot.double()).abs().sum(1, keepdim=True)
     assert_within(gw, ww, 2 * (n + 2) * 2.0 ** -24 * mag + 1e-37)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,k,n", [(40, 3, 1), (40, 3, 2), (40, 3, 77), (900, 4, 1024),
+                                   (901, 3, 2047), (300_000, 4, 2), (300_001, 4, 3)])
+def test_combine_gradient_of_pairs_taken_out(gpu, t, k, n, dtype):
+    """Pairs whose slot a caller set to -1, as beyond an expert's capacity: their
+    rows of y get a gradient of zero, whatever the memory held before."""
+    g = rng(t + n)
+    r = ej.group_by_expert(make_picks(t, k, 6, 3, "holes"), 6,
+                           torch.rand(t, k, generator=g, device="cuda"))
+    r.slots[torch.rand(t, k, generator=g, device="cuda") < 0.2] = -1
+    y, cot = randn(g, t * k, n, dtype=dtype), randn(g, t, n, dtype=dtype)
+    held = r.slots >= 0
+    at = y[r.slots.clamp(min=0).long()].double() * held[..., None]
+    want = torch.zeros(t * k, n, dtype=torch.double, device="cuda")
+    want[r.slots[held].long()] = (r.weights.double()[..., None] * cot.double()[:, None])[held]
+    ww = (at * cot.double()[:, None]).sum(2)
+    for before in (float("nan"), 0, -1):
+        fill = torch.full((t * k, n), before, dtype=dtype, device="cuda")
+        del fill  # the allocator hands out the same block again
+        gy, gw = ej.combine_experts_vjp(y, r, cot)
+        assert_within(gy, want, (UNIT[dtype] + 2.0 ** -23) * want.abs() + TINY[dtype])
+        assert bool((gy[~torch.isin(torch.arange(t * k, device="cuda"), r.slots)] == 0).all())
+        assert_within(gw, ww, 2 * (n + 2) * 2.0 ** -24 * (at * cot.double()[:, None]).abs().sum(2)
+                      + 1e-37)
+        del gy
+
+
+def test_combine_gradient_below_the_first_offset(gpu):
+    """Slots of no pair in front of the groups, and offsets short of the last pair."""
+    g = rng(3)
+    slots = torch.tensor([[7, 3], [4, -1], [6, 9]], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([3, 5, 8], dtype=torch.int32, device="cuda")
+    w = torch.rand(3, 2, generator=g, device="cuda")
+    r = ej.ExpertRouting(w, torch.zeros_like(slots), offsets, torch.zeros_like(slots).flatten(),
+                         slots)
+    y = randn(g, 6, 40)
+    with pytest.raises(ValueError):
+        ej.combine_experts_vjp(randn(g, 10, 40), r, randn(g, 3, 40))
+    r.slots = torch.where(slots >= 4, slots - 4, -1)  # 3, -1; 0, -1; 2, 5
+    cot = randn(g, 3, 40)
+    gy, gw = ej.combine_experts_vjp(y, r, cot)
+    want = torch.zeros(6, 40, device="cuda")
+    for i, j in ((0, 0), (1, 0), (2, 0), (2, 1)):
+        want[int(r.slots[i, j])] = w[i, j] * cot[i]
+    assert torch.equal(gy, want)
+    assert bool((gw[r.slots < 0] == 0).all())
