@@ -2,8 +2,9 @@
 
 ``route_experts``, ``grouped_matmul`` and ``combine_experts`` carry gradients
 through torch.autograd; their backward kernels are also callable directly
-(``*_vjp``).  Gradients are first order, as ``sparse_einsum_raw``'s.  The
-reference has no such operators.
+(``*_vjp``).  Gradients are first order, as ``sparse_einsum_raw``'s, and
+reverse mode only: dual tensors are refused.  The reference has no such
+operators.
 """
 
 from __future__ import annotations

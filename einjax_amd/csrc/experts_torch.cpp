@@ -6,6 +6,7 @@
 // part: that is why this part of the library's binding is compiled.  It calls
 // the C entry points of include/einjax_hip.h and computes nothing itself.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/util/Exception.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -169,6 +170,15 @@ variable_list first_order(variable_list grads) {
 
 bool wants_grad(const Tensor &t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
+// A dual tensor's tangent would be dropped, which is a derivative of zero.
+template <class... Operands>
+void no_tangents(const Operands &...t) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  if ((... || (t.defined() && t._fw_grad(0).defined())))
+    not_implemented("the expert operators have no forward-mode derivatives: an operand is a dual "
+                    "tensor");
+}
+
 // ---- routing -------------------------------------------------------------------
 
 struct Routing {
@@ -193,6 +203,7 @@ Tensor route_workspace(const Tensor &ref, int64_t T, int64_t E, size_t *bytes) {
 
 Routing run_route(const Tensor &given, int64_t k, bool renorm) {
   const int code = value_code(given, "logits");
+  no_tangents(given);
   const Tensor logits = rows_of(given);
   const int64_t T = logits.size(0), E = logits.size(1);
   Launch on(logits);
@@ -211,6 +222,7 @@ Routing run_route(const Tensor &given, int64_t k, bool renorm) {
 
 Tensor run_route_vjp(const Tensor &given, const Tensor &experts, const Tensor &grad, bool renorm) {
   const int code = value_code(given, "logits");
+  no_tangents(given, grad);
   const Tensor logits = rows_of(given);
   const int64_t T = logits.size(0), E = logits.size(1), k = experts.size(1);
   const Tensor g = grad.to(at::kFloat).contiguous();
@@ -301,6 +313,7 @@ py::tuple group(py::handle experts_, int64_t E, py::handle weights_) {
 
 Tensor run_combine(const Tensor &given, const Tensor &slots, const Tensor &weights,
                    at::ScalarType out_type) {
+  no_tangents(given, weights);
   const Tensor y = rows_of(given);
   const int64_t T = slots.size(0), n = y.size(1);
   Launch on(y);
@@ -315,6 +328,7 @@ Tensor run_combine(const Tensor &given, const Tensor &slots, const Tensor &weigh
 variable_list run_combine_vjp(const Tensor &y_, const Tensor &slots, const Tensor &offsets,
                               const Tensor &weights, const Tensor &grad_, bool need_y,
                               bool need_w) {
+  no_tangents(y_, weights, grad_);
   const Tensor y = rows_of(y_), grad = rows_of(grad_);
   const int64_t T = slots.size(0), n = y.size(1);
   Launch on(y);
@@ -480,6 +494,7 @@ ej_grouped_desc describe(const Tensor &x, int code, int out_code, const Order &o
 Tensor run_product(const Tensor &x_, const Order &o, int64_t k, int64_t n, const Groups &g,
                    at::ScalarType out_type, const Tensor &x_scale = Tensor(),
                    const Tensor &w_scale = Tensor()) {
+  no_tangents(x_, o.w, x_scale, w_scale);
   const Tensor x = rows_of(x_);
   const int code = x_scale.defined() ? EJ_I8 : code_of(x.scalar_type());
   Launch on(x);
@@ -501,6 +516,7 @@ Tensor product(const Tensor &x, const Tensor &w, const Groups &g, at::ScalarType
 
 // Gradient to w [E, k, n], in the order w lies in.
 Tensor weight_gradient(const Tensor &x_, const Tensor &w, const Groups &g, const Tensor &grad_) {
+  no_tangents(x_, grad_);
   const Tensor x = rows_of(x_), grad = rows_of(grad_);
   const int64_t E = w.size(0), k = w.size(1), n = w.size(2);
   Order o = weight_order(w);
@@ -622,7 +638,8 @@ py::tuple grouped_matmul_vjp(py::handle x_, py::handle w_, py::handle offsets, p
 // ---- 8-bit integers -----------------------------------------------------------------------
 
 py::tuple quantize_rows(py::handle x_) {
-  const Tensor x = on_gpu(x_, "x").detach();
+  const Tensor given = on_gpu(x_, "x"), x = given.detach();
+  no_tangents(given);
   const int code = value_code(x, "x");
   if (x.dim() < 1) throw py::value_error("x must have at least one dimension");
   const int64_t n = x.size(-1);

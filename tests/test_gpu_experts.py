@@ -937,3 +937,40 @@ def test_combine_gradient_below_the_first_offset(gpu):
         want[int(r.slots[i, j])] = w[i, j] * cot[i]
     assert torch.equal(gy, want)
     assert bool((gw[r.slots < 0] == 0).all())
+
+
+def test_forward_mode_is_refused(gpu):
+    """No operator drops the tangent of a dual tensor, with or without reverse mode."""
+    import torch.autograd.forward_ad as forward
+
+    g = rng(31)
+    offsets = torch.tensor([0, 2, 6], device="cuda")
+    r = ej.route_experts(randn(g, 6, 4), 1)
+    q, s = ej.quantize_rows(randn(g, 6, 8))
+    p, ps = ej.quantize_rows(randn(g, 4, 8))
+    x, w, cot = randn(g, 6, 8), randn(g, 2, 8, 4), randn(g, 6, 4)
+    calls = {
+        "logits": (randn(g, 6, 4), lambda d: ej.route_experts(d, 2)),
+        "x": (x, lambda d: ej.grouped_matmul(d, w, offsets)),
+        "w": (w, lambda d: ej.grouped_matmul(x, d, offsets)),
+        "w transposed": (w, lambda d: ej.grouped_matmul(cot, d.transpose(1, 2), offsets)),
+        "y": (x, lambda d: ej.combine_experts(d, r)),
+        "weights": (r.weights, lambda d: ej.combine_experts(x, r, d)),
+        "rows": (x, lambda d: ej.quantize_rows(d)),
+        "row scales": (s, lambda d: ej.int8_matmul(q, d, p, ps)),
+        "column scales": (ps, lambda d: ej.int8_matmul(q, s, p, d)),
+        "cotangent of weights": (r.weights, lambda d: ej.route_experts_vjp(cot, r.experts, d)),
+        "cotangent of product": (cot, lambda d: ej.grouped_matmul_vjp(x, w, offsets, d)),
+        "cotangent of sum": (x, lambda d: ej.combine_experts_vjp(x, r, d)),
+    }
+    for leaf in (False, True):
+        for primal, call in calls.values():
+            with forward.dual_level():
+                primal = primal.detach().clone().requires_grad_(leaf)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(forward.make_dual(primal, torch.ones_like(primal)))
+    # a backward on a dual cotangent
+    leaf = x.clone().requires_grad_()
+    y = ej.grouped_matmul(leaf, w, offsets)
+    with forward.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.autograd.grad(y, leaf, forward.make_dual(cot, cot))
