@@ -49,7 +49,10 @@ def grouped_matmul(x, w, groups, *, gather: bool = False, out_dtype=None):
     group are zero.
     float32, bfloat16 or float16, summed in fp32; the result has x's dtype
     unless ``out_dtype=torch.float32``.  Differentiable in x and w (in gathered
-    x for routings of 1 to 16 picks); the gradient to w lies as w does."""
+    x for routings of 1 to 16 picks); the gradient to w lies as w does.  Both
+    gradients are products in x's dtype, summed in fp32: the float32 cotangent of
+    an ``out_dtype=torch.float32`` product is rounded to x's dtype before them
+    (in float16 beyond 65504 to infinity)."""
     offsets, rows, slots = group_args(groups)
     return _lib.experts().grouped_matmul(x, w, offsets, rows, slots, gather, out_dtype)
 
@@ -57,7 +60,7 @@ def grouped_matmul(x, w, groups, *, gather: bool = False, out_dtype=None):
 def grouped_matmul_vjp(x, w, groups, grad_out, *, gather: bool = False, need_x: bool = True,
                        need_w: bool = True):
     """(grad_x, grad_w) of ``grouped_matmul`` for the cotangent grad_out
-    [slots, n]; None where not needed."""
+    [slots, n], which is rounded to x's dtype; None where not needed."""
     offsets, rows, slots = group_args(groups)
     return _lib.experts().grouped_matmul_vjp(x, w, offsets, rows, slots, gather, grad_out, need_x,
                                              need_w)
@@ -83,6 +86,6 @@ def combine_experts(y, routing: ExpertRouting, weights=None):
 def combine_experts_vjp(y, routing: ExpertRouting, grad_out, weights=None, *, need_y: bool = True,
                         need_weights: bool = True):
     """(grad_y, grad_weights) of ``combine_experts`` for the cotangent
-    grad_out [T, n]; None where not needed."""
+    grad_out [T, n], which is rounded to y's dtype; None where not needed."""
     return _lib.experts().combine_vjp(*_combine_args(y, routing, weights), grad_out, need_y,
                                       need_weights)

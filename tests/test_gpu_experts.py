@@ -974,3 +974,48 @@ def test_forward_mode_is_refused(gpu):
     y = ej.grouped_matmul(leaf, w, offsets)
     with forward.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         torch.autograd.grad(y, leaf, forward.make_dual(cot, cot))
+
+
+@pytest.mark.parametrize("out_dtype", [None, F32])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("t,e,k,n_in,n_out", [(40, 6, 3, 72, 200), (33, 5, 2, 77, 131),
+                                              (300, 9, 4, 520, 392), (1500, 4, 4, 256, 128)])
+def test_gathered_gradients_are_rounded_once(gpu, t, e, k, n_in, n_out, dtype, out_dtype):
+    """A token's slots are added in fp32 and their sum is rounded once; a float32
+    cotangent is rounded to the operands' dtype, element by element, before."""
+    g, r, x, w = product_case(t, e, k, n_in, n_out, "holes", dtype, "kn", True)
+    x.requires_grad_()
+    w.requires_grad_()
+    y = ej.grouped_matmul(x, w, r, gather=True, out_dtype=out_dtype)
+    assert y.dtype == (out_dtype or dtype)
+    cot = randn(g, t * k, n_out, dtype=y.dtype)
+    gx, gw = torch.autograd.grad(y, (x, w), cot)
+    assert gx.dtype == dtype and gw.dtype == dtype
+    off = UNIT[dtype] if out_dtype == F32 else 0.0   # of the cotangent, and below its normals:
+    low = TINY[dtype] if out_dtype == F32 else 0.0
+    x, w = x.detach().double(), w.detach().double()
+    _, ends = row_groups(r.offsets, t * k)
+    total, room, size = (torch.zeros(t, n_in, dtype=torch.double, device="cuda") for _ in range(3))
+    for i in range(e):
+        a, b = ends[i], ends[i + 1]
+        at, gi = r.rows[a:b].long(), cot[a:b].double()
+        s, mag = gi @ w[i].T, gi.abs() @ w[i].abs().T
+        slack = (off + 2 * (n_out + 2) * 2.0 ** -24) * mag + low * w[i].abs().sum(1)
+        total.index_add_(0, at, s)
+        room.index_add_(0, at, slack)
+        size.index_add_(0, at, s.abs() + slack)
+        wg, mg = x[at].T @ gi, x[at].abs().T @ gi.abs()
+        assert_within(gw[i], wg, sum_bound(wg, mg, b - a, dtype) + off * mg * (1 + UNIT[dtype])
+                      + low * x[at].abs().sum(0)[:, None])
+    room = room + 2 * (k + 2) * 2.0 ** -24 * size
+    assert_within(gx, total, room + UNIT[dtype] * (total.abs() + room) + TINY[dtype])
+
+
+def test_cotangents_beyond_float16(gpu):
+    """The float32 cotangent of a float16 product is a float16 one to its gradients."""
+    x, w = (torch.ones(2, 8, dtype=F16, device="cuda") for _ in range(2))
+    w, offsets = w[None, :, :].transpose(1, 2).contiguous(), torch.tensor([0, 2], device="cuda")
+    cot = torch.tensor([[65504.0, -65504.0], [65520.0, 1.0]], device="cuda")
+    gx, gw = ej.grouped_matmul_vjp(x, w, offsets, cot)
+    assert bool((gx[0] == 0).all()) and bool((gx[1] == float("inf")).all())
+    assert bool((gw[0, :, 0] == float("inf")).all()) and bool((gw[0, :, 1] == -65504).all())
