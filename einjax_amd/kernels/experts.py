@@ -84,7 +84,8 @@ def quantize_rows(x) -> tuple:
     scale = max |row| / 127, q rounded to nearest (ties to even).  A row of
     zeros has scale 0; a row that holds a NaN or an infinity has scale NaN, so
     that every product with it is NaN.  Rows of activations give a scale for
-    each token, rows of [experts, n_out, n_in] weights one for each channel."""
+    each token, rows of [experts, n_out, n_in] weights one for each channel.
+    Not differentiable: q and scale are constants to torch.autograd."""
     return _lib.experts().quantize_rows(x)
 
 
@@ -101,7 +102,10 @@ def int8_matmul(q, q_scale, w, w_scale, groups=None, *, gather: bool = False,
     Without groups: w [n, k] or [1, n, k], w_scale [n] or [1, n], the dense
     product [m, n].  With groups (an ``ExpertRouting`` or offsets [E + 1]):
     w [E, n, k], w_scale [E, n]; slot s of group e is q's row s, or with
-    ``gather`` the row of its token, times w[e]; zero in slots of no group."""
+    ``gather`` the row of its token, times w[e]; zero in slots of no group.
+
+    Not differentiable, in the scales either: the result is a constant to
+    torch.autograd."""
     offsets, rows, slots = group_args(groups)
     return _lib.experts().int8_matmul(q, q_scale, w, w_scale, offsets, rows, slots, gather,
                                       out_dtype)

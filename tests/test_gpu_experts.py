@@ -1019,3 +1019,11 @@ def test_cotangents_beyond_float16(gpu):
     gx, gw = ej.grouped_matmul_vjp(x, w, offsets, cot)
     assert bool((gx[0] == 0).all()) and bool((gx[1] == float("inf")).all())
     assert bool((gw[0, :, 0] == float("inf")).all()) and bool((gw[0, :, 1] == -65504).all())
+
+
+def test_8_bit_results_are_constants(gpu):
+    x = torch.randn(4, 8, device="cuda", requires_grad=True)
+    q, s = ej.quantize_rows(x)
+    assert not q.requires_grad and not s.requires_grad
+    scale = s.clone().requires_grad_()
+    assert not ej.int8_matmul(q, scale, q, scale).requires_grad
