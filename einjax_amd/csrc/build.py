@@ -8,15 +8,19 @@ Each ``*.hip`` file under this directory is compiled with hipcc to an
 object in ``_build/`` and linked into ``einjax_amd/libejhip.so``.  Packed
 fp32 VALU forms are disabled for all device code.  ``experts_torch.cpp``, the
 host-only torch binding of the expert operators, becomes
-``einjax_amd/_experts.so``, which needs libejhip.so beside it.
+``einjax_amd/_experts.so``, which needs libejhip.so beside it.  Where g++, torch
+or the headers of torch or Python are missing, the library is built without it
+(and the expert operators raise).
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -74,13 +78,26 @@ def _rocm() -> Path:
     return Path(_hipcc()).resolve().parent.parent
 
 
+def _torch_root() -> Path | None:
+    spec = importlib.util.find_spec("torch")
+    return Path(spec.origin).resolve().parent if spec and spec.origin else None
+
+
+def torch_binding_lacks() -> list[str]:
+    """What the torch binding's build needs and this machine does not have."""
+    root = _torch_root()
+    return [what for what, there in (
+        ("g++", shutil.which("g++")),
+        ("Python's headers", (Path(sysconfig.get_paths()["include"]) / "Python.h").exists()),
+        ("torch and its headers", root and (root / "include/torch/extension.h").exists()),
+    ) if not there]
+
+
 def _compile_torch() -> Path:
     """Compiles the torch binding (host code only)."""
-    import sysconfig
-
     import torch
 
-    root = Path(torch.__file__).resolve().parent
+    root = _torch_root()
     obj = BUILD_DIR / "experts_torch.o"
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
           "-DTORCH_EXTENSION_NAME=_experts", "-DTORCH_API_INCLUDE_EXTENSION_H",
@@ -92,9 +109,7 @@ def _compile_torch() -> Path:
 
 
 def _link_torch(obj: Path) -> None:
-    import torch
-
-    root = Path(torch.__file__).resolve().parent
+    root = _torch_root()
     tmp = TORCH_PATH.with_suffix(".so.tmp")
     _run(["g++", "-shared", "-o", tmp, obj, f"-L{root}/lib", "-lc10", "-lc10_hip", "-ltorch",
           "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", f"-L{PKG}", "-lejhip",
@@ -103,16 +118,16 @@ def _link_torch(obj: Path) -> None:
 
 
 def build(verbose: bool = True) -> Path:
-    """Compiles every HIP source, links libejhip.so and the torch binding on
-    it; returns the library's path."""
+    """Compiles every HIP source, links libejhip.so and (where it can be built)
+    the torch binding on it; returns the library's path."""
     hipcc = _hipcc()
+    lacks = torch_binding_lacks()
     BUILD_DIR.mkdir(exist_ok=True)
     srcs = sources()
     workers = min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with ThreadPoolExecutor(max_workers=workers) as ex:
-        binding = ex.submit(_compile_torch)
+        binding = None if lacks else ex.submit(_compile_torch)
         objs = list(ex.map(lambda s: _compile(hipcc, s), srcs))
-        binding_obj = binding.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -125,9 +140,15 @@ def build(verbose: bool = True) -> Path:
     except OSError as e:
         raise RuntimeError(f"built library does not load: {e}") from e
     os.replace(tmp, LIB_PATH)
-    _link_torch(binding_obj)
+    if binding is None:
+        TORCH_PATH.unlink(missing_ok=True)  # one of an earlier library would not fit this one
+        print(f"{TORCH_PATH.name} (the expert operators for torch) is not built: it needs "
+              f"{' and '.join(lacks)}", file=sys.stderr)
+    else:
+        _link_torch(binding.result())
     if verbose:
-        print(f"built {LIB_PATH} from {len(srcs)} sources, and {TORCH_PATH.name}")
+        print(f"built {LIB_PATH} from {len(srcs)} sources" +
+              (f", and {TORCH_PATH.name}" if binding else ""))
     return LIB_PATH
 
 
