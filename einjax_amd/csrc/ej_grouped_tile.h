@@ -340,7 +340,7 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
       },
       [&](int i, int j, int c) {
         const float v = static_cast<float>(acc[i][j][c]);
-        if constexpr (Op::kInt) return v * (as[i] * bs[j][c]);
+        if constexpr (Op::kInt) return scaled(v, as[i], bs[j][c]);
         else return v;
       });
 }
@@ -690,7 +690,8 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
       v[c] = static_cast<float>(sum[c]);
       const int n = n0 + col + c;
       if constexpr (Op::kInt)
-        v[c] *= as * g.b_scale[static_cast<int64_t>(r.group) * g.n + (n < g.n ? n : g.n - 1)];
+        v[c] = scaled(v[c], as,
+                      g.b_scale[static_cast<int64_t>(r.group) * g.n + (n < g.n ? n : g.n - 1)]);
     }
     put4(g.c, g.out, s * g.ldc, n0 + col, g.n, v);
   }

@@ -1027,3 +1027,22 @@ def test_8_bit_results_are_constants(gpu):
     assert not q.requires_grad and not s.requires_grad
     scale = s.clone().requires_grad_()
     assert not ej.int8_matmul(q, scale, q, scale).requires_grad
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(3, 64, 70), (3, 77, 70), (200, 256, 300), (200, 1000, 301),
+                                   (700, 500, 900), (4096, 128, 4096)])
+def test_int8_scales_far_apart(gpu, m, k, n, out_dtype):
+    """Scales whose product leaves float32's range, under sums that bring it back.
+    They are powers of two and the sums below 2^24, so the results are exact."""
+    g = rng(m + k)
+    q, w = (torch.randint(-128, 128, s, generator=g, device="cuda").to(torch.int8)
+            for s in ((m, k), (n, k)))
+    q[0] = 0
+    qs, ws = (2.0 ** torch.randint(-140, 100, (s,), generator=g, device="cuda").double()
+              for s in (m, n))
+    qs[0], qs[1], ws[0], ws[1] = 2.0 ** 90, 2.0 ** -75, 2.0 ** 90, 2.0 ** -75
+    qs, ws = qs.float().double(), ws.float().double()  # the power function's last bit
+    want = (q.double() @ w.double().T) * qs[:, None] * ws
+    got = ej.int8_matmul(q, qs.float(), w, ws.float(), out_dtype=out_dtype)
+    assert torch.equal(got, want.float().to(out_dtype))
