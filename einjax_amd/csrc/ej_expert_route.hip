@@ -27,6 +27,9 @@ constexpr int kVjpThreads = 256;
 constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / 64;
 constexpr int kRouteBlocks = 256;   // bound on the workgroups whose counts are added up
+// The gradient gives a token a wave at most, and HIP launches hold fewer than
+// 2^32 threads.
+constexpr int64_t kMaxTokens = (int64_t{1} << 26) - 4;
 constexpr int kSmallTokens = 256;   // batches routed and grouped by one workgroup
 
 struct RouteArgs {
@@ -443,9 +446,9 @@ int check_route(int64_t n_tokens, int32_t n_experts, int32_t k) {
               kMaxExperts, EJ_MAX_PICKS);
     return EJ_E_UNSUPPORTED;
   }
-  if (n_tokens >= (int64_t{1} << 26) || n_tokens * k >= (int64_t{1} << 31)) {
-    set_error("%lld tokens of %d picks: fewer than 2^26 tokens and 2^31 pairs are supported",
-              (long long)n_tokens, k);
+  if (n_tokens > kMaxTokens || n_tokens * k >= (int64_t{1} << 31)) {
+    set_error("%lld tokens of %d picks: at most %lld tokens and fewer than 2^31 pairs are supported",
+              (long long)n_tokens, k, (long long)kMaxTokens);
     return EJ_E_UNSUPPORTED;
   }
   return EJ_OK;

@@ -173,3 +173,15 @@ def test_rows_of_copies_only_what_it_must():
     assert _lib.experts().rows_of(t[:, 2:5]).data_ptr() == t[:, 2:5].data_ptr()
     assert _lib.experts().rows_of(t.t()).is_contiguous()
     assert _lib.experts().rows_of(t[:1].expand(4, 8)).is_contiguous()
+
+
+def test_routing_takes_no_more_tokens_than_its_gradient():
+    """A token of more than 256 experts is a wave of the gradient; a launch holds
+    fewer than 2^32 threads."""
+    lib, n = _lib.load(), ctypes.c_size_t()
+    for t, status in (((1 << 26) - 3, _lib.EJ_E_UNSUPPORTED), ((1 << 26) - 4, 0)):
+        assert lib.ej_expert_route_workspace_size(t, 300, ctypes.byref(n)) == status
+        # null operands are noticed after the sizes
+        refused = status or _lib.EJ_E_INVAL
+        assert lib.ej_expert_route_vjp(None, _lib.EJ_F32, t, 300, 300, 1, 1, None, None, None,
+                                       None) == refused
