@@ -10,6 +10,9 @@ bool aligned16(const void *p, int64_t a, int64_t b, int size) {
   return reinterpret_cast<size_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0;
 }
 
+// The kernels count slots in 32 bits, up to two blocks or stages past the last.
+constexpr int64_t kMaxSlots = (int64_t{1} << 31) - 512;
+
 int elem_size(int32_t dtype) { return dtype == EJ_F32 ? 4 : dtype == EJ_I8 ? 1 : 2; }
 
 int check_desc(const ej_grouped_desc *d) {
@@ -27,9 +30,9 @@ int check_desc(const ej_grouped_desc *d) {
   EJ_CHECK_ARG(d->n_groups <= 1 || d->w_group >= w_rows * d->w_stride || w_rows * w_row == 0,
                "groups of w overlap: stride %lld for %lld rows of %lld", (long long)d->w_group,
                (long long)w_rows, (long long)d->w_stride);
-  if (d->n_slots >= (int64_t{1} << 31) || d->n_rows >= (int64_t{1} << 31)) {
-    set_error("%lld slots of %lld rows: fewer than 2^31 are supported", (long long)d->n_slots,
-              (long long)d->n_rows);
+  if (d->n_slots > kMaxSlots || d->n_rows >= (int64_t{1} << 31)) {
+    set_error("%lld slots of %lld rows: at most %lld slots and fewer than 2^31 rows are supported",
+              (long long)d->n_slots, (long long)d->n_rows, (long long)kMaxSlots);
     return EJ_E_UNSUPPORTED;
   }
   return EJ_OK;

@@ -726,7 +726,7 @@ typedef struct ej_grouped_desc {
   int32_t w_order;
   int32_t n_groups;
   int32_t k, n;
-  int64_t n_slots;    /* rows of the result; below 2^31 */
+  int64_t n_slots;    /* rows of the result; at most 2^31 - 512 */
   int64_t n_rows;     /* rows of x */
   int64_t x_stride;   /* between rows of x */
   int64_t w_group;    /* between groups of w */

@@ -185,3 +185,13 @@ def test_routing_takes_no_more_tokens_than_its_gradient():
         refused = status or _lib.EJ_E_INVAL
         assert lib.ej_expert_route_vjp(None, _lib.EJ_F32, t, 300, 300, 1, 1, None, None, None,
                                        None) == refused
+
+
+def test_slots_that_32_bits_do_not_count():
+    """Blocks and stages end past the last slot, by less than 512."""
+    lib, n = _lib.load(), ctypes.c_size_t()
+    for slots, status in (((1 << 31) - 1, _lib.EJ_E_UNSUPPORTED),
+                          ((1 << 31) - 511, _lib.EJ_E_UNSUPPORTED), ((1 << 31) - 512, 0)):
+        d = desc(n_slots=slots, n_rows=slots)
+        assert lib.ej_grouped_gemm_workspace_size(ctypes.byref(d), ctypes.byref(n)) == status
+        assert lib.ej_grouped_gemm_dw_workspace_size(ctypes.byref(d), ctypes.byref(n)) == status
