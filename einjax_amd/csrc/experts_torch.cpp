@@ -296,16 +296,21 @@ py::tuple group(py::handle experts_, int64_t E, py::handle weights_) {
   // no wrapping of values past 32 bits into the range
   if (experts.scalar_type() == at::kLong) experts = experts.clamp(-1, E);
   experts = index(experts, {T, k}, "experts");
+  // The library groups no more picks than experts.  There may be more, of
+  // experts elsewhere: then for groups that stay empty behind those that are here.
+  const int64_t groups = E >= 1 ? std::max(E, k) : E;
+  if (groups > E) experts = experts.masked_fill(experts.ge(E), -1);
   Launch on(experts);
   size_t bytes;
-  const Tensor ws = route_workspace(experts, T, E, &bytes);
-  Routing r = empty_routing(experts, T, k, E);
+  const Tensor ws = route_workspace(experts, T, groups, &bytes);
+  Routing r = empty_routing(experts, T, k, groups);
   r.weights = weights;
   r.experts = experts;
-  check(ej_expert_group(ints(experts), T, int32_of(k, "k"), static_cast<int32_t>(E),
+  check(ej_expert_group(ints(experts), T, int32_of(k, "k"), static_cast<int32_t>(groups),
                         mut_ints(r.offsets), mut_ints(r.rows), mut_ints(r.slots), mut(ws), bytes,
                         on.stream),
         "ej_expert_group");
+  if (groups > E) r.offsets = r.offsets.narrow(0, 0, E + 1);
   return r.tuple();
 }
 

@@ -72,8 +72,10 @@ def group_args(groups) -> tuple:
 
 def group_by_expert(experts, n_experts: int, weights=None) -> ExpertRouting:
     """The routing of picks that the caller made: experts [T, k], int32 or
-    int64, distinct for each token, -1 (or anything outside [0, n_experts))
-    for none; weights float32 [T, k], 1 for every pair if not given."""
+    int64, distinct for each token, -1 (or anything outside [0, n_experts), such
+    as experts held elsewhere) for none; weights float32 [T, k], 1 for every pair
+    if not given.  At most 1024 experts and 16 picks; there may be more picks
+    than experts."""
     return ExpertRouting(*_lib.experts().group(experts, n_experts, weights))
 
 

@@ -1046,3 +1046,21 @@ def test_int8_scales_far_apart(gpu, m, k, n, out_dtype):
     want = (q.double() @ w.double().T) * qs[:, None] * ws
     got = ej.int8_matmul(q, qs.float(), w, ws.float(), out_dtype=out_dtype)
     assert torch.equal(got, want.float().to(out_dtype))
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("t,e,k", [(5, 1, 2), (300, 3, 8), (2000, 7, 16)])
+def test_group_by_expert_of_fewer_experts_than_picks(gpu, t, e, k, index):
+    """Some of the experts that the tokens picked, as one device of several holds them."""
+    picks = make_picks(t, k, 32, t, "holes").to(index)
+    r = ej.group_by_expert(picks, e)
+    offsets, rows, slots = plain_grouping(picks, e)
+    assert r.n_experts == e and r.offsets.tolist() == offsets
+    assert r.rows.tolist() == rows and r.slots.tolist() == slots
+    g = rng(e)
+    x, w = randn(g, t, 24), randn(g, e, 24, 40)
+    got = ej.grouped_matmul(x, w, r, gather=True)
+    want, mag = product64(x, r.rows, r.offsets, w, t * k)
+    assert_within(got, want, sum_bound(want, mag, 24, F32))
+    with pytest.raises(ValueError):
+        ej.group_by_expert(picks, 0)
