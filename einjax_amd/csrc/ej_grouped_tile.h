@@ -208,6 +208,8 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
         put = put + 1 == NS ? 0 : put + 1;
       }
       stage_mma<Op, S>(acc, fa, fb, get * S::kSlot);
+      // read before the barrier after which other waves load into this slot
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       get = get + 1 == NS ? 0 : get + 1;
     }
   } else {
