@@ -45,15 +45,15 @@ int launch_large(GroupedArgs g, hipStream_t stream) {
   return EJ_OK;
 }
 
-template <class Op, int FM, int BN, int NW, bool BKC, int NS>
+template <class Op, int BN, int NW, bool BKC, int NS>
 int launch_skinny(GroupedArgs g, hipStream_t stream) {
   const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
-  g.row_blocks = static_cast<uint32_t>(g.slots / (16 * FM) + groups);
+  g.row_blocks = static_cast<uint32_t>(g.slots / 16 + groups);
   g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, BN));
   dim3 grid;
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks, NW * 64,
                       &grid));
-  hipLaunchKernelGGL((grouped_skinny_kernel<Op, FM, BN, NW, BKC, NS>), grid, dim3(NW * 64), 0,
+  hipLaunchKernelGGL((grouped_skinny_kernel<Op, BN, NW, BKC, NS>), grid, dim3(NW * 64), 0,
                      stream, g);
   EJ_LAUNCH_CHECK();
   return EJ_OK;
@@ -158,7 +158,7 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
   // columns of a skinny block: 32, or what fills 128 bytes of a [k][n] row
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
   if (few_rows(rows, tiles, kElem<Op>))
-    return launch_skinny<Op, 1, kSkinny, 4, BKC, 2>(g, stream);
+    return launch_skinny<Op, kSkinny, 4, BKC, 2>(g, stream);
   if constexpr (kElem<Op> == 4) {
     // bound by the fp32 matrix instructions at any tile: the finest spreads
     // best (4096 x 1024 x 2048 in 8 groups 164 us, 212 with 128 x 128; equal

@@ -570,15 +570,15 @@ __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g)
 }
 
 // Few rows for each group: the time is that of reading the weights once.  A
-// workgroup takes 16 FM rows by BN columns; its waves split k stage by stage
+// workgroup takes 16 rows by BN columns; its waves split k stage by stage
 // (so that together they read long pieces of each weight row), each on a ring
 // of its own without barriers, and add up their parts in LDS at the end, in
 // the order of the waves.  32 slots of 16 groups, W [n][k] of 2048 x 4096 in
 // bf16: 41 us for the 218 MB of the groups that have slots (5.4 TB/s); 4 rows x
 // 4096 x 8192 in 8 bits 8.1 us (4.1 TB/s).
-template <class Op, int FM_, int BN, int NW, bool BKC, int NS>
+template <class Op, int BN, int NW, bool BKC, int NS>
 struct SkinnyShape {
-  static constexpr int FM = FM_, BM = 16 * FM, FN = BN / 16;
+  static constexpr int BM = 16, FM = 1, FN = BN / 16;
   using TA = Tile<Op, BM, true>;
   using TB = Tile<Op, BN, BKC>;
   using FA = Fragments<Op, TA, true, FM>;
@@ -593,10 +593,10 @@ struct SkinnyShape {
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
-template <class Op, int FM, int BN, int NW, bool BKC, int NS>
+template <class Op, int BN, int NW, bool BKC, int NS>
 __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using S = SkinnyShape<Op, FM, BN, NW, BKC, NS>;
+  using S = SkinnyShape<Op, BN, NW, BKC, NS>;
   __shared__ __align__(1024) unsigned char lds[S::kLds];
   const uint32_t grid = g.row_blocks * g.col_blocks;
   if (blockIdx.x >= grid) {
@@ -649,11 +649,9 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
   typename S::FB fb;
   fa.init(lds_address(ring), 0, lane);
   fb.init(lds_address(ring) + S::TA::kBytes, 0, lane);
-  typename Op::acc acc[FM][S::FN];
+  typename Op::acc acc[1][S::FN];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
+  for (int j = 0; j < S::FN; ++j) acc[0][j] = typename Op::acc{0, 0, 0, 0};
   for (int i = 0; i < NS - 1 && i < mine; ++i) load(i);
   for (int i = 0; i < mine; ++i) {
     const int later = mine - 1 - i;
@@ -669,12 +667,9 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
   __syncthreads();
   float *part = reinterpret_cast<float *>(lds);
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j)
-      *reinterpret_cast<typename Op::acc *>(part + wave * (S::BM * BN) +
-                                            (i * 16 + (lane & 15)) * BN + j * 16 +
-                                            (lane >> 4) * 4) = acc[i][j];
+  for (int j = 0; j < S::FN; ++j)
+    *reinterpret_cast<typename Op::acc *>(part + wave * (S::BM * BN) + (lane & 15) * BN + j * 16 +
+                                          (lane >> 4) * 4) = acc[0][j];
   __syncthreads();
   for (int q = tid; q < S::BM * BN / 4; q += NW * 64) {
     const int row = q / (BN / 4), col = q % (BN / 4) * 4;
