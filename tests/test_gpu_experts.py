@@ -1064,3 +1064,132 @@ def test_group_by_expert_of_fewer_experts_than_picks(gpu, t, e, k, index):
     assert_within(got, want, sum_bound(want, mag, 24, F32))
     with pytest.raises(ValueError):
         ej.group_by_expert(picks, 0)
+
+
+# name -> (shapes of the inputs, call)
+STREAM_CALLS = {
+    "route": (((500, 20),), lambda l: ej.route_experts(l, 3)),
+    "route small": (((9, 20),), lambda l: ej.route_experts(l, 3)),
+    "route gradient": (((500, 20), (500, 3)),
+                       lambda l, d: ej.route_experts_vjp(l, ej.route_experts(l, 3).experts, d)),
+    "group": (((500, 20),), lambda l: ej.group_by_expert(l.argmax(1, keepdim=True), 20)),
+    "product": (((300, 64), (3, 64, 96)), lambda x, w: ej.grouped_matmul(x, w, _thirds(x))),
+    "product in parts": (((300, 4096), (3, 4096, 64)),
+                         lambda x, w: ej.grouped_matmul(x, w, _thirds(x))),
+    "product gradients": (((300, 64), (3, 64, 96), (300, 96)),
+                          lambda x, w, d: ej.grouped_matmul_vjp(x, w, _thirds(x), d)),
+    "product gradients in parts": (((9000, 64), (3, 64, 40), (9000, 40)),
+                                   lambda x, w, d: ej.grouped_matmul_vjp(x, w, _thirds(x), d)),
+    "gathered gradients": (((300, 20), (300, 64), (20, 64, 96), (600, 96)),
+                           lambda l, x, w, d: ej.grouped_matmul_vjp(
+                               x, w, ej.route_experts(l, 2), d, gather=True)),
+    "sum": (((300, 20), (600, 70)), lambda l, y: ej.combine_experts(y, ej.route_experts(l, 2))),
+    "sum gradients": (((300, 20), (600, 70), (300, 70)),
+                      lambda l, y, d: ej.combine_experts_vjp(y, ej.route_experts(l, 2), d)),
+    "8 bits": (((300, 128), (90, 128)),
+               lambda x, w: ej.int8_matmul(*ej.quantize_rows(x), *ej.quantize_rows(w))),
+    "layer": (((300, 20), (300, 64), (20, 64, 96), (300, 96)), lambda *v: _layer_gradients(*v)),
+}
+
+
+def _thirds(x):
+    n = x.shape[0] // 3
+    return torch.arange(4, device="cuda") * n
+
+
+def _layer_gradients(logits, x, w, cot):
+    leaves = [v.detach().requires_grad_() for v in (logits, x, w)]
+    r = ej.route_experts(leaves[0], 2)
+    out = ej.combine_experts(ej.grouped_matmul(leaves[1], leaves[2], r, gather=True), r)
+    return [out.detach(), *torch.autograd.grad(out, leaves, cot)]
+
+
+def _tensors(out):
+    if isinstance(out, ej.ExpertRouting):
+        return [out.weights, out.experts, out.offsets, out.rows, out.slots]
+    return list(out) if isinstance(out, (tuple, list)) else [out]
+
+
+@pytest.mark.parametrize("name", list(STREAM_CALLS))
+def test_operators_run_on_the_current_stream(gpu, name):
+    """On a side stream: the inputs are filled there behind work that takes a while,
+    and the results are read there.  Work on any other stream would see zeros."""
+    shapes, call = STREAM_CALLS[name]
+    g = rng(len(name))
+    values = [randn(g, *s) for s in shapes]
+    want = [t.clone() for t in _tensors(call(*values))]
+    inputs = [torch.zeros_like(v) for v in values]
+    busy = randn(g, 4096, 4096)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(8):
+            busy = busy @ busy * 0.01
+        for i, v in zip(inputs, values):
+            i.copy_(v)
+        got = [t.clone() for t in _tensors(call(*inputs))]
+        for i in inputs:
+            i.zero_()
+    torch.cuda.current_stream().wait_stream(side)
+    assert len(got) == len(want)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,k,n_in,n_out,shift", [(60, 2, 2048, 72, 0), (60, 2, 2047, 72, 0),
+                                                  (60, 2, 2048, 72, 1), (200, 1, 4096, 64, 0)])
+def test_gathered_products_in_parts(gpu, t, k, n_in, n_out, shift, dtype):
+    """Few tiles over a long contraction, summed in parts, of gathered rows."""
+    g, e = rng(t + n_in), 3
+    r = ej.group_by_expert(make_picks(t, k, e, 5, "holes"), e)
+    x = randn(g, t * n_in + 8, dtype=dtype)[shift:shift + t * n_in].view(t, n_in)
+    for order in ("kn", "nk"):
+        w = randn(g, e, n_in, n_out, dtype=dtype, scale=n_in ** -0.5)
+        if order == "nk":
+            w = w.transpose(1, 2).contiguous().transpose(1, 2)
+        got = ej.grouped_matmul(x, w, r, gather=True)
+        want, mag = product64(x, r.rows, r.offsets, w, t * k)
+        assert_within(got, want, sum_bound(want, mag, n_in, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,k,n_in,n_out,shift", [(3000, 2, 72, 152, 0), (3000, 2, 75, 151, 0),
+                                                  (2500, 1, 128, 128, 1)])
+def test_gathered_weight_gradients_in_parts(gpu, t, k, n_in, n_out, shift, dtype):
+    g, e = rng(t + n_in), 3
+    r = ej.group_by_expert(make_picks(t, k, e, 5, "holes"), e)
+    x = randn(g, t * n_in + 8, dtype=dtype)[shift:shift + t * n_in].view(t, n_in)
+    cot, w = randn(g, t * k, n_out, dtype=dtype), randn(g, e, n_in, n_out, dtype=dtype)
+    ends = r.offsets.tolist()
+    for wt in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
+        _, gw = ej.grouped_matmul_vjp(x, wt, r, cot, gather=True, need_x=False)
+        for i in range(e):
+            a, b = ends[i], ends[i + 1]
+            xi, gi = x[r.rows[a:b].long()].double(), cot[a:b].double()
+            assert_within(gw[i], xi.T @ gi,
+                          sum_bound(xi.T @ gi, xi.abs().T @ gi.abs(), b - a, dtype))
+
+
+def test_int8_matmul_views(gpu):
+    """Rows and weights with strides, off 16 bytes, expanded, and not in rows of k."""
+    g, e = rng(40), 4
+    r = ej.group_by_expert(make_picks(150, 2, e, 3, "skew"), e)
+    wide = torch.randint(-128, 128, (300, 400), generator=g, device="cuda").to(torch.int8)
+    base = torch.randint(-128, 128, (e, 90, 200), generator=g, device="cuda").to(torch.int8)
+    scales = torch.rand(300, 2, generator=g, device="cuda")
+    for q in (wide[:, :128], wide[:, 1:129], wide[:, 16:144], wide[:, ::2][:, :128],
+              wide[:, :128].t().contiguous().t(), wide[:1, :128].expand(300, 128)):
+        for w in (base[:, :, :128], base[:, 3:80, 1:129], base[:1, :, :128].expand(e, 90, 128),
+                  base[:, :, ::2][:, :, :100], base.transpose(1, 2)[:, 5:133]):
+            k = min(q.shape[1], w.shape[2])
+            a, b = q[:, :k], w[:, :, :k]
+            qs = scales[:, 0]
+            ws = torch.rand(2, e, b.shape[1], generator=g, device="cuda").transpose(0, 1)[:, 0]
+            got = ej.int8_matmul(a, qs, b, ws, r, out_dtype=F32)
+            same = ej.int8_matmul(a.contiguous(), qs.contiguous(), b.contiguous(),
+                                  ws.contiguous(), r, out_dtype=F32)
+            want, _ = product64(a, None, r.offsets, b.transpose(1, 2), 300)
+            owner = torch.tensor([max(o, 0) for o in row_groups(r.offsets, 300)[0]], device="cuda")
+            want = want * qs.double()[:, None] * ws.double()[owner]
+            assert_within(got, want, 5 * 2.0 ** -24 * want.abs() + TINY[F32])
+            assert torch.equal(got, same)
