@@ -30,7 +30,22 @@ constexpr int kRouteBlocks = 256;   // bound on the workgroups whose counts are 
 // The gradient gives a token a wave at most, and HIP launches hold fewer than
 // 2^32 threads.
 constexpr int64_t kMaxTokens = (int64_t{1} << 26) - 4;
-constexpr int kSmallTokens = 256;   // batches routed and grouped by one workgroup
+
+// Whether one workgroup routes and groups (`routes`), or only groups, a batch.
+// Routing takes it a pass for every 32 tokens (8 of more than 256 experts).
+// Measured (us) so and in two launches over all CUs, tokens x experts, picks:
+//   32 x 128, 8   6.4  8.8      64 x 64, 4   6.0   7.8    128 x 32, 4   7.3  8.0
+//   64 x 128, 8   9.6  8.8      96 x 64, 4   7.4   7.9    256 x 32, 4  12.2  7.9
+//   256 x 128, 8 29.8 10.0     128 x 64, 4   9.0   7.9    128 x 16, 8   8.5  7.7
+//   32 x 256, 8   8.9 10.9     8 x 1024, 16 14.9  17.7    128 x 8, 2    5.6  8.0
+//   48 x 256, 8  13.1 10.8    32 x 1024, 16 44.2  24.1    256 x 8, 2    8.4  7.9
+// and grouping alone 256 x 128, 8 6.1 and 7.7, 256 x 1024, 2 4.8 and 9.5, 256 x
+// 1024, 16 11.9 and 9.7.
+bool one_workgroup(int64_t n_tokens, int32_t n_experts, bool routes) {
+  if (!routes) return n_tokens <= 256;
+  return n_tokens <= kGroupThreads / (n_experts <= 256 ? 16 : 64) ||
+         (n_tokens <= 128 && n_tokens * n_experts <= 4096);
+}
 
 struct RouteArgs {
   const void *logits;
@@ -466,7 +481,7 @@ int check_logits(const void *logits, int32_t dtype, int64_t ld, int32_t n_expert
 // Routes (logits given) or only groups.
 int run_route(RouteArgs a, void *workspace, size_t workspace_bytes, hipStream_t stream) {
   const size_t group_lds = (2 + kGroupWaves) * a.n_experts * sizeof(int);
-  if (a.n_tokens <= kSmallTokens) {
+  if (one_workgroup(a.n_tokens, a.n_experts, a.logits != nullptr)) {
     const size_t lds =
         ((1 + kGroupWaves) * a.n_experts + a.n_tokens * a.k) * sizeof(int);
     auto run = [&](auto L, auto V) {
@@ -515,7 +530,9 @@ using namespace ej;
 extern "C" int ej_expert_route_workspace_size(int64_t n_tokens, int32_t n_experts, size_t *bytes) {
   EJ_CHECK_ARG(bytes, "null bytes");
   EJ_TRY(check_route(n_tokens, n_experts, 1));
-  *bytes = n_tokens <= kSmallTokens ? 0 : sizeof(int32_t) * kRouteBlocks * n_experts;
+  // what routing needs, grouping alone needs at most
+  *bytes = one_workgroup(n_tokens, n_experts, true) ? 0
+                                                    : sizeof(int32_t) * kRouteBlocks * n_experts;
   return EJ_OK;
 }
 

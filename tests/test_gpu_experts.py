@@ -1193,3 +1193,24 @@ def test_int8_matmul_views(gpu):
             want = want * qs.double()[:, None] * ws.double()[owner]
             assert_within(got, want, 5 * 2.0 ** -24 * want.abs() + TINY[F32])
             assert torch.equal(got, same)
+
+
+@pytest.mark.parametrize("e,k", [(4, 2), (32, 4), (33, 4), (64, 8), (128, 8), (256, 3), (257, 3),
+                                 (1024, 16)])
+def test_route_of_every_small_batch(gpu, e, k):
+    """One workgroup or all: the same picks, weights and groups on both sides of
+    every number of tokens at which that changes."""
+    g = rng(e)
+    logits = randn(g, 260, e)
+    whole = ej.route_experts(logits, k)
+    for t in (1, 7, 8, 9, 12, 15, 16, 17, 31, 32, 33, 63, 64, 65, 124, 125, 127, 128, 129, 255,
+              256, 257):
+        r = ej.route_experts(logits[:t], k)
+        assert torch.equal(r.experts, whole.experts[:t])
+        assert torch.equal(r.weights, whole.weights[:t])
+        offsets, rows, slots = plain_grouping(r.experts, e)
+        assert r.offsets.tolist() == offsets
+        assert r.rows.tolist() == rows and r.slots.tolist() == slots
+        again = ej.group_by_expert(r.experts, e)
+        assert all(torch.equal(getattr(again, f), getattr(r, f))
+                   for f in ("offsets", "rows", "slots"))
