@@ -280,14 +280,14 @@ __device__ inline uint16_t to_16(float v, int code) {
                          : __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
 }
 
-// An 8-bit product's sum times both scales, the smaller first: so it leaves the
-// range of fp32 only where the result does (the scales' own product may be below
-// it or past it by far).  A NaN stays one in either place.
+// An 8-bit product's sum times (a b), without the range of fp32 for the scales'
+// product: the result leaves it only where sum a b does; elsewhere its bits are
+// those of sum * (a * b).  16384 rows in 8 groups, k = n = 4096: 269 us, 267 with
+// sum * (a * b), 273 with the smaller scale picked as the first factor.
 __device__ inline float scaled(float sum, float a, float b) {
-  const bool less = fabsf(a) < fabsf(b);
-  return sum * (less ? a : b) * (less ? b : a);
+  return ldexpf(sum * (__builtin_amdgcn_frexp_mantf(a) * __builtin_amdgcn_frexp_mantf(b)),
+                __builtin_amdgcn_frexp_expf(a) + __builtin_amdgcn_frexp_expf(b));
 }
-
 // Stores v[0..3] as columns col .. col + 3 of a row at element offset `at`
 // (of column 0), as one vector at any element's alignment.
 __device__ inline void put4(void *c, int code, int64_t at, int col, int n, const float (&v)[4]) {

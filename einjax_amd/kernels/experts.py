@@ -98,8 +98,8 @@ def int8_matmul(q, q_scale, w, w_scale, groups=None, *, gather: bool = False,
     q int8 [m, k] and q_scale float32 [m] are rows and their scales
     (``quantize_rows``); w int8 holds one row of k for each output channel,
     w_scale float32 their scales.  The integer sum is exact (k < 131072), times
-    both scales in float32 (the smaller one first), rounded once to out_dtype
-    (float32, bfloat16 or float16).
+    both scales in float32 (whose own product may pass its range), rounded once to
+    out_dtype (float32, bfloat16 or float16).
 
     Without groups: w [n, k] or [1, n, k], w_scale [n] or [1, n], the dense
     product [m, n].  With groups (an ``ExpertRouting`` or offsets [E + 1]):
