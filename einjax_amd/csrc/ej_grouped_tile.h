@@ -545,8 +545,10 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 }
 
 // The same in blocks of 256 x 256, cut as grouped_large_kernel's.  16384 rows
-// in 16 groups, 2048 x 4096 bf16: 272 us (1010 TFLOP/s), 306 with P gathered:
-// the sources of every stage's loads are then moved between the lanes.
+// in 16 groups, 2048 x 4096 bf16: 272 us (1010 TFLOP/s), 306 with P gathered
+// (128 x 128: 350 and 442, 64 x 64: 522 and 721).  The bounds check of a row's
+// index, in rows_of, follows its load, and waiting for that is waiting for every
+// load in flight: each stage empties the ring that the others keep full.
 template <class Op, int GATHER>
 __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
