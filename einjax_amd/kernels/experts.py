@@ -37,7 +37,7 @@ class ExpertRouting:
     pairs have the same slot, and rows[slots[t, j]] = t.
 
     A caller may take single pairs out by setting their slot to -1 (an expert's
-    capacity, say).  ``combine_experts`` then leaves them out, and the gradient
+    capacity, say) before the relation is used.  ``combine_experts`` then leaves them out, and the gradient
     to their rows is zero.  The products, which go by offsets and rows, still
     compute those rows and take them into the gradient to the weights; the
     gradient to gathered rows, which adds up a token's slots, does not.  The two
