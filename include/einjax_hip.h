@@ -673,9 +673,10 @@ int ej_relation_to_dense(const int32_t *coords, const void *values, int64_t n_ti
  * [n_tokens, k]: the softmax over all logits at the picks, or with
  * renormalize != 0 the softmax over the picks.  A token with fewer than k
  * experts left has experts -1, weights 0 and slots -1 for the rest.
- * At most 1024 experts and EJ_MAX_PICKS picks.  The workspace may be NULL where its size
- * is 0.  ej_expert_group groups picks that the caller made (int32
- * [n_tokens, k]; a value outside [0, n_experts) has no slot). */
+ * At most 1024 experts, EJ_MAX_PICKS picks (and no more than experts) and
+ * 2^26 - 4 tokens.  The workspace may be NULL where its size is 0.
+ * ej_expert_group groups picks that the caller made (int32 [n_tokens, k]; a
+ * value outside [0, n_experts) has no slot). */
 #define EJ_MAX_PICKS 16
 int ej_expert_route_workspace_size(int64_t n_tokens, int32_t n_experts, size_t *bytes);
 int ej_expert_route(const void *logits, int32_t dtype, int64_t n_tokens, int32_t n_experts,
@@ -695,7 +696,8 @@ int ej_expert_route_vjp(const void *logits, int32_t dtype, int64_t n_tokens, int
 
 /* out[t] = sum over j of weights[t, j] y[slots[t, j]] (weights NULL: 1), pairs
  * without a slot left out; out [n_tokens, n] contiguous, of out_dtype: y's
- * dtype, or with EJ_F32 values any. */
+ * dtype, or with EJ_F32 values any.  At most EJ_MAX_PICKS picks, fewer than
+ * 2^31 pairs and slots. */
 int ej_expert_combine(const void *y, int32_t dtype, int64_t n_slots, int64_t ld_y,
                       const float *weights, const int32_t *slots, int64_t n_tokens, int32_t k,
                       int32_t n, void *out, int32_t out_dtype, ej_stream_t stream);
@@ -739,7 +741,8 @@ typedef struct ej_grouped_desc {
  * read as non-decreasing values in [0, n_slots]; others give undefined rows,
  * never an access outside the operands; NULL with n_groups == 1: one group of
  * every slot.  EJ_I8: x_scale [n_rows] and w_scale
- * [n_groups][n], out = x_scale w_scale (exact integer sum); NULL otherwise.
+ * [n_groups][n], out = x_scale w_scale (exact integer sum), also where the
+ * scales' own product passes fp32's range; NULL otherwise.
  * The workspace (NULL where its size is 0) holds the sums of a contraction that
  * is split to cover the CUs; they are added in a fixed order. */
 int ej_grouped_gemm_workspace_size(const ej_grouped_desc *desc, size_t *bytes);
