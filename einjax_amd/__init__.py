@@ -14,6 +14,8 @@ libejhip.so (HIP kernels behind a C ABI, include/einjax_hip.h).
 from .autodiff import (
     combine_experts,
     combine_experts_vjp,
+    gated_matmul,
+    gated_matmul_vjp,
     grouped_matmul,
     grouped_matmul_vjp,
     route_experts,
@@ -85,6 +87,7 @@ __all__ = [
     "coordinate_join_sorted", "sparse_einsum", "sparse_einsum_raw", "sparse_einsum_raw_vjp",
     "ExecutionEngine", "build_dependency_graph", "topological_sort",
     "ExpertRouting", "route_experts", "route_experts_vjp", "group_by_expert", "grouped_matmul",
-    "grouped_matmul_vjp", "combine_experts", "combine_experts_vjp", "quantize_rows",
+    "grouped_matmul_vjp", "gated_matmul", "gated_matmul_vjp", "combine_experts",
+    "combine_experts_vjp", "quantize_rows",
     "int8_matmul",
 ]

@@ -36,6 +36,10 @@ EJ_I8 = 6
 EJ_W_KN = 0
 EJ_W_NK = 1
 
+EJ_SILU = 0
+EJ_GELU = 1
+EJ_GELU_TANH = 2
+
 EJ_ORDER_PROBE = 0
 EJ_ORDER_SORTED = 1
 
@@ -168,6 +172,10 @@ SIGNATURES = {
     "ej_grouped_gemm_dw_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
     "ej_grouped_gemm_dw": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp,
                                   _sz, _vp]),
+    "ej_gated_gemm_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
+    "ej_gated_gemm": (_i32, [ctypes.POINTER(GroupedDesc), _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                             _sz, _vp]),
+    "ej_gated_vjp": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _i32, _vp, _vp]),
 }
 
 _lock = threading.Lock()

@@ -10,6 +10,8 @@ from .custom_vjp import sparse_einsum, sparse_einsum_raw, sparse_einsum_raw_vjp
 from .experts import (
     combine_experts,
     combine_experts_vjp,
+    gated_matmul,
+    gated_matmul_vjp,
     grouped_matmul,
     grouped_matmul_vjp,
     route_experts,
@@ -17,5 +19,5 @@ from .experts import (
 )
 
 __all__ = ["sparse_einsum", "sparse_einsum_raw", "sparse_einsum_raw_vjp", "route_experts",
-           "route_experts_vjp", "grouped_matmul", "grouped_matmul_vjp", "combine_experts",
-           "combine_experts_vjp"]
+           "route_experts_vjp", "grouped_matmul", "grouped_matmul_vjp", "gated_matmul",
+           "gated_matmul_vjp", "combine_experts", "combine_experts_vjp"]

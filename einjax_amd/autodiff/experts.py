@@ -1,7 +1,7 @@
 """Differentiable expert operators.
 
-``route_experts``, ``grouped_matmul`` and ``combine_experts`` carry gradients
-through torch.autograd; their backward kernels are also callable directly
+``route_experts``, ``grouped_matmul``, ``gated_matmul`` and ``combine_experts``
+carry gradients through torch.autograd; their backward kernels are also callable directly
 (``*_vjp``).  Gradients are first order, as ``sparse_einsum_raw``'s, and
 reverse mode only: dual tensors are refused.  The reference has no such
 operators.
@@ -13,7 +13,7 @@ from .. import _lib
 from ..kernels.experts import ExpertRouting, group_args
 
 __all__ = ["route_experts", "route_experts_vjp", "grouped_matmul", "grouped_matmul_vjp",
-           "combine_experts", "combine_experts_vjp"]
+           "gated_matmul", "gated_matmul_vjp", "combine_experts", "combine_experts_vjp"]
 
 
 def route_experts(logits, k: int, *, renormalize: bool = True) -> ExpertRouting:
@@ -64,6 +64,40 @@ def grouped_matmul_vjp(x, w, groups, grad_out, *, gather: bool = False, need_x: 
     offsets, rows, slots = group_args(groups)
     return _lib.experts().grouped_matmul_vjp(x, w, offsets, rows, slots, gather, grad_out, need_x,
                                              need_w)
+
+
+def gated_matmul(x, w, groups=None, *, activation: str = "silu", gather: bool = False):
+    """Gated products: out[s] = act(x[s] @ gate[e]) * (x[s] @ up[e]) for the
+    slots s of group e, both products, the activation and their product in one
+    kernel.
+
+    w [E, k, 2 n] holds gate[e] in its first n columns and up[e] in the others,
+    n- or k-contiguous (``weight.transpose(1, 2)`` of linear weights [E, 2 n, k]
+    is taken as it lies).  groups, x, gather and rows of no group as
+    ``grouped_matmul``'s; without groups w is [k, 2 n] or [1, k, 2 n] and every
+    row of x takes it.
+
+    activation: "silu", g / (1 + exp(-g)); "gelu", g times the normal
+    distribution function of g; "gelu_tanh", its form by a hyperbolic tangent,
+    g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2.
+
+    float32, bfloat16 or float16; sums, activation and product in fp32, the
+    result rounded once to x's dtype.  Differentiable in x and w as
+    ``grouped_matmul`` is.  Where a gradient is wanted, both projections are
+    kept in fp32 ([slots, 2 n]) for the backward pass, whose products take their
+    gradients rounded once to x's dtype."""
+    offsets, rows, slots = group_args(groups)
+    return _lib.experts().gated_matmul(x, w, offsets, rows, slots, gather, activation)
+
+
+def gated_matmul_vjp(x, w, groups, grad_out, *, activation: str = "silu", gather: bool = False,
+                     need_x: bool = True, need_w: bool = True):
+    """(grad_x, grad_w) of ``gated_matmul`` for the cotangent grad_out
+    [slots, n], which is rounded to x's dtype; None where not needed.  Both
+    projections are formed anew."""
+    offsets, rows, slots = group_args(groups)
+    return _lib.experts().gated_matmul_vjp(x, w, offsets, rows, slots, gather, activation,
+                                           grad_out, need_x, need_w)
 
 
 def _combine_args(y, routing, weights) -> tuple:

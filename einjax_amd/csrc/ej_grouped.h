@@ -81,6 +81,9 @@ struct GroupedArgs {
   // [splits][slots][n] or [splits][n_groups][m][n]; 1: none.
   float *partial;
   int32_t splits;
+  // Gated products: n columns of results from the 2 n of B, the gate's first.
+  float *gate_up;           // [slots][2 n] (null: not kept)
+  int32_t activation;       // EJ_SILU, EJ_GELU or EJ_GELU_TANH
 };
 
 // A 16-byte chunk of zeros: what lanes beyond an operand's extent load.
@@ -355,7 +358,7 @@ __device__ inline void part_of(int stages, int part, int parts, int *first, int 
 // and past the last), by the `nb` workgroups of which this is number `b`.
 __device__ inline void zero_dead_rows(const GroupedArgs &g, int b, int nb) {
   const int s = static_cast<int>(g.slots);
-  if (!g.offsets) return;
+  if (!g.offsets || !g.c) return;
   int first = g.offsets[0], last = g.offsets[g.n_groups];
   first = first < 0 ? 0 : first > s ? s : first;
   last = last < first ? first : last > s ? s : last;
@@ -469,6 +472,16 @@ struct Loader {
   // M tiles: column col0 + i of the operand is output row i; extent `ext`.
   __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int col0,
                                 int ext) {
+    init_m(wave, lane, base, ld, ext, [&](int i, int *shift) {
+      *shift = 0;
+      return col0 + i;
+    });
+  }
+  // M tiles: output row i is column col_at(i, &shift) of an extent `ext` that
+  // begins at column shift; a chunk's columns follow each other.
+  template <class ColAt>
+  __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int ext,
+                                ColAt col_at) {
     whole = ext >= kChunk<Op>;
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
@@ -476,13 +489,13 @@ struct Loader {
       T::at((v * NW + wave) * 64 + lane, &krow, &chunk);
       if (v == 0) line = krow;
       if (v < kCols) {
-        int c = col0 + chunk * kChunk<Op>;
+        int shift, c = col_at(chunk * kChunk<Op>, &shift);
         if constexpr (DIRECT) {
           if (c > ext - kChunk<Op>) c = ext - kChunk<Op>;
         } else {
           valid[v] = ext - c;
         }
-        col[v] = c;
+        col[v] = c + shift;
       }
       src[v] = base + (line_at(v) * ld + col[v % kCols]) * kElem<Op>;
     }

@@ -15,7 +15,8 @@ constexpr int64_t kMaxSlots = (int64_t{1} << 31) - 512;
 
 int elem_size(int32_t dtype) { return dtype == EJ_F32 ? 4 : dtype == EJ_I8 ? 1 : 2; }
 
-int check_desc(const ej_grouped_desc *d) {
+// n_w: columns of W (the result's, twice as many of a gated product).
+int check_desc(const ej_grouped_desc *d, int64_t n_w) {
   EJ_CHECK_ARG(d, "null descriptor");
   EJ_CHECK_ARG(d->dtype == EJ_F32 || d->dtype == EJ_BF16 || d->dtype == EJ_F16 ||
                    d->dtype == EJ_I8,
@@ -23,8 +24,8 @@ int check_desc(const ej_grouped_desc *d) {
   EJ_CHECK_ARG(d->w_order == EJ_W_KN || d->w_order == EJ_W_NK, "w_order = %d", d->w_order);
   EJ_CHECK_ARG(d->n_groups >= 0 && d->k >= 0 && d->n >= 0 && d->n_slots >= 0 && d->n_rows >= 0,
                "negative size");
-  const int64_t w_row = d->w_order == EJ_W_KN ? d->n : d->k;
-  const int64_t w_rows = d->w_order == EJ_W_KN ? d->k : d->n;
+  const int64_t w_row = d->w_order == EJ_W_KN ? n_w : d->k;
+  const int64_t w_rows = d->w_order == EJ_W_KN ? d->k : n_w;
   EJ_CHECK_ARG(d->x_stride >= d->k && d->out_stride >= d->n && d->w_stride >= w_row,
                "a row stride is below its row's length");
   EJ_CHECK_ARG(d->n_groups <= 1 || d->w_group >= w_rows * d->w_stride || w_rows * w_row == 0,
@@ -33,6 +34,18 @@ int check_desc(const ej_grouped_desc *d) {
   if (d->n_slots > kMaxSlots || d->n_rows >= (int64_t{1} << 31)) {
     set_error("%lld slots of %lld rows: at most %lld slots and fewer than 2^31 rows are supported",
               (long long)d->n_slots, (long long)d->n_rows, (long long)kMaxSlots);
+    return EJ_E_UNSUPPORTED;
+  }
+  return EJ_OK;
+}
+
+int check_desc(const ej_grouped_desc *d) { return check_desc(d, d ? d->n : 0); }
+
+int check_gated(const ej_grouped_desc *d) {
+  EJ_TRY(check_desc(d, d ? 2 * static_cast<int64_t>(d->n) : 0));
+  EJ_CHECK_ARG(d->dtype != EJ_I8, "gated products take fp32 and 16-bit operands");
+  if (d->n >= (1 << 30)) {
+    set_error("n = %d: gated products of fewer than 2^30 columns are supported", d->n);
     return EJ_E_UNSUPPORTED;
   }
   return EJ_OK;
@@ -74,16 +87,17 @@ int split_parts(double tiles, int64_t contraction, int elem, bool whole, double 
   return saved > 5 + parts * sums * 8 / 4e6 ? static_cast<int>(parts) : 1;
 }
 
-int rows_parts(const ej_grouped_desc *d) {
+// n: columns of W
+int rows_parts(const ej_grouped_desc *d, int64_t n) {
   if (d->dtype == EJ_I8 || d->n_groups == 0 || d->n_slots == 0) return 1;
   const int64_t groups = d->n_groups < d->n_slots ? d->n_groups : d->n_slots;
   const double rows = static_cast<double>(d->n_slots) / groups;
-  const double tiles = (rows / 64 + 0.5) * groups * ceil_div(d->n, 64);
+  const double tiles = (rows / 64 + 0.5) * groups * ceil_div(n, 64);
   const int elem = elem_size(d->dtype);
   const bool whole = whole_chunks(d);
   // the kernel for few rows splits k by itself
   if (whole && few_rows(rows, tiles, elem) && (rows <= 16 || tiles > 64)) return 1;
-  return split_parts(tiles, d->k, elem, whole, static_cast<double>(d->n_slots) * d->n);
+  return split_parts(tiles, d->k, elem, whole, static_cast<double>(d->n_slots) * n);
 }
 int dw_parts(const ej_grouped_desc *d) {
   if (d->n_groups == 0) return 1;
@@ -93,6 +107,42 @@ int dw_parts(const ej_grouped_desc *d) {
   const double tiles = static_cast<double>(ceil_div(d->k, 64)) * ceil_div(d->n, 64) * d->n_groups;
   return split_parts(tiles, d->n_slots / d->n_groups, size, whole,
                      static_cast<double>(d->n_groups) * d->k * d->n);
+}
+
+int check_operands(const ej_grouped_desc *d, const void *x, const int32_t *rows,
+                   const int32_t *offsets, const void *w) {
+  EJ_CHECK_ARG(offsets || d->n_groups == 1, "null offsets of %d groups", d->n_groups);
+  EJ_CHECK_ARG(rows || d->n_rows >= d->n_slots, "%lld rows for %lld slots without a row index",
+               (long long)d->n_rows, (long long)d->n_slots);
+  EJ_CHECK_ARG(d->n_groups == 0 || d->n_rows > 0, "%lld slots of no rows",
+               (long long)d->n_slots);
+  EJ_CHECK_ARG(d->k == 0 || d->n_groups == 0 || (x && w), "null operand");
+  return EJ_OK;
+}
+
+// The operands of a rows product.
+GroupedRows rows_args(const ej_grouped_desc *d, const void *x, const int32_t *rows,
+                      const int32_t *offsets, const void *w, void *out) {
+  GroupedArgs g = {};
+  g.a = static_cast<const char *>(x);
+  g.b = static_cast<const char *>(w);
+  g.c = out;
+  g.a_rows = rows;
+  g.offsets = offsets;
+  g.lda = d->x_stride;
+  g.ldb = d->w_stride;
+  g.ldc = d->out_stride;
+  g.b_group = d->w_group;
+  g.n_a = d->n_rows;
+  g.slots = d->n_slots;
+  g.n_groups = d->n_groups;
+  g.n = d->n;
+  g.k = d->k;
+  g.out = d->out_dtype;
+  // 16-byte loads need whole, aligned chunks in every row
+  const int size = elem_size(d->dtype);
+  const bool direct = whole_chunks(d) && aligned16(x, 0, 0, size) && aligned16(w, 0, 0, size);
+  return GroupedRows{g, d->w_order == EJ_W_NK, direct};
 }
 
 int check_workspace(int parts, int64_t sums, void *workspace, size_t bytes, GroupedArgs *g) {
@@ -112,7 +162,7 @@ using namespace ej;
 extern "C" int ej_grouped_gemm_workspace_size(const ej_grouped_desc *d, size_t *bytes) {
   EJ_TRY(check_desc(d));
   EJ_CHECK_ARG(bytes, "null bytes");
-  const int parts = rows_parts(d);
+  const int parts = rows_parts(d, d->n);
   *bytes = parts > 1 ? sizeof(float) * parts * d->n_slots * d->n : 0;
   return EJ_OK;
 }
@@ -143,40 +193,14 @@ extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const in
   }
   if (d->n_slots == 0 || d->n == 0) return EJ_OK;
   EJ_CHECK_ARG(out, "null result");
-  EJ_CHECK_ARG(offsets || d->n_groups == 1, "null offsets of %d groups", d->n_groups);
-  EJ_CHECK_ARG(rows || d->n_rows >= d->n_slots, "%lld rows for %lld slots without a row index",
-               (long long)d->n_rows, (long long)d->n_slots);
-  EJ_CHECK_ARG(d->n_groups == 0 || d->n_rows > 0, "%lld slots of no rows",
-               (long long)d->n_slots);
-  EJ_CHECK_ARG(d->k == 0 || d->n_groups == 0 || (x && w), "null operand");
+  EJ_TRY(check_operands(d, x, rows, offsets, w));
   EJ_CHECK_ARG(!i8 || d->n_groups == 0 || (x_scale && w_scale), "null scale");
 
-  const int size = elem_size(d->dtype);
-  GroupedArgs g = {};
-  g.a = static_cast<const char *>(x);
-  g.b = static_cast<const char *>(w);
-  g.c = out;
-  g.a_rows = rows;
-  g.offsets = offsets;
-  g.a_scale = x_scale;
-  g.b_scale = w_scale;
-  g.lda = d->x_stride;
-  g.ldb = d->w_stride;
-  g.ldc = d->out_stride;
-  g.b_group = d->w_group;
-  g.n_a = d->n_rows;
-  g.slots = d->n_slots;
-  g.n_groups = d->n_groups;
-  g.n = d->n;
-  g.k = d->k;
-  g.out = d->out_dtype;
-  // 16-byte loads need whole, aligned chunks in every row
-  const int chunk = 16 / size;
-  const bool direct = d->k % chunk == 0 && aligned16(x, d->x_stride, 0, size) &&
-                      aligned16(w, d->w_stride, d->w_group, size) &&
-                      (d->w_order == EJ_W_NK || d->n % chunk == 0);
-  EJ_TRY(check_workspace(rows_parts(d), d->n_slots * d->n, workspace, workspace_bytes, &g));
-  const GroupedRows r{g, d->w_order == EJ_W_NK, direct};
+  GroupedRows r = rows_args(d, x, rows, offsets, w, out);
+  r.g.a_scale = x_scale;
+  r.g.b_scale = w_scale;
+  EJ_TRY(check_workspace(rows_parts(d, d->n), d->n_slots * d->n, workspace, workspace_bytes,
+                         &r.g));
   switch (d->dtype) {
     case EJ_BF16: return grouped_rows_bf16(r, as_stream(stream));
     case EJ_F16: return grouped_rows_f16(r, as_stream(stream));
@@ -229,5 +253,38 @@ extern "C" int ej_grouped_gemm_dw(const ej_grouped_desc *d, const void *x, const
     case EJ_BF16: return grouped_wgrad_bf16(g, direct, as_stream(stream));
     case EJ_F16: return grouped_wgrad_f16(g, direct, as_stream(stream));
     default: return grouped_wgrad_f32(g, direct, as_stream(stream));
+  }
+}
+
+extern "C" int ej_gated_gemm_workspace_size(const ej_grouped_desc *d, size_t *bytes) {
+  EJ_TRY(check_gated(d));
+  EJ_CHECK_ARG(bytes, "null bytes");
+  const int64_t n2 = 2 * static_cast<int64_t>(d->n);
+  const int parts = rows_parts(d, n2);
+  *bytes = parts > 1 ? sizeof(float) * parts * d->n_slots * n2 : 0;
+  return EJ_OK;
+}
+
+extern "C" int ej_gated_gemm(const ej_grouped_desc *d, int32_t activation, const void *x,
+                             const int32_t *rows, const int32_t *offsets, const void *w, void *out,
+                             float *gate_up, void *workspace, size_t workspace_bytes,
+                             ej_stream_t stream) {
+  EJ_TRY(check_gated(d));
+  EJ_CHECK_ARG(activation == EJ_SILU || activation == EJ_GELU || activation == EJ_GELU_TANH,
+               "activation %d", activation);
+  EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype,
+               "result of dtype %d from operands of dtype %d", d->out_dtype, d->dtype);
+  if (d->n_slots == 0 || d->n == 0) return EJ_OK;
+  EJ_CHECK_ARG(out || gate_up, "null result");
+  EJ_TRY(check_operands(d, x, rows, offsets, w));
+  const int64_t n2 = 2 * static_cast<int64_t>(d->n);
+  GroupedRows r = rows_args(d, x, rows, offsets, w, out);
+  r.g.gate_up = gate_up;
+  r.g.activation = activation;
+  EJ_TRY(check_workspace(rows_parts(d, n2), d->n_slots * n2, workspace, workspace_bytes, &r.g));
+  switch (d->dtype) {
+    case EJ_BF16: return gated_rows_bf16(r, as_stream(stream));
+    case EJ_F16: return gated_rows_f16(r, as_stream(stream));
+    default: return gated_rows_f32(r, as_stream(stream));
   }
 }

@@ -17,43 +17,61 @@ inline int join_parts(const GroupedArgs &g, int64_t rows, int64_t m, bool skip_d
   return EJ_OK;
 }
 
-template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
-int launch_rows(GroupedArgs g, hipStream_t stream) {
-  const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
-  g.row_blocks = static_cast<uint32_t>(g.slots / BM + groups);
-  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, BN));
+template <bool FINE>
+int join_gated(const GroupedArgs &g, hipStream_t stream) {
   dim3 grid;
-  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks,
-                      WR * WC * 64, &grid));
-  grid.y = g.splits;
-  hipLaunchKernelGGL((grouped_rows_kernel<Op, BM, BN, WR, WC, BKC, DIRECT, NS>), grid,
-                     dim3(WR * WC * 64), 0, stream, g);
-  EJ_LAUNCH_CHECK();
-  return g.splits > 1 ? join_parts(g, g.slots, g.slots, true, stream) : EJ_OK;
-}
-
-template <class Op, bool BKC>
-int launch_large(GroupedArgs g, hipStream_t stream) {
-  const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
-  g.row_blocks = static_cast<uint32_t>(g.slots / 256 + groups);
-  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, 256));
-  dim3 grid;
-  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kLargeExtra + kZeroBlocks,
-                      512, &grid));
-  hipLaunchKernelGGL((grouped_large_kernel<Op, BKC>), grid, dim3(512), 0, stream, g);
+  EJ_TRY(grouped_grid(ceil_div(g.slots * ceil_div(g.n, 4), 256), 256, &grid));
+  hipLaunchKernelGGL(gated_join_kernel<FINE>, grid, dim3(256), 0, stream, g);
   EJ_LAUNCH_CHECK();
   return EJ_OK;
 }
 
-template <class Op, int BN, int NW, bool BKC, int NS>
+// Columns of the results that a tile of `bn` columns of B gives.
+template <bool GATED>
+constexpr int result_cols(int bn) {
+  return GATED ? bn / 2 : bn;
+}
+
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS,
+          bool GATED = false>
+int launch_rows(GroupedArgs g, hipStream_t stream) {
+  const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
+  g.row_blocks = static_cast<uint32_t>(g.slots / BM + groups);
+  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, result_cols<GATED>(BN)));
+  dim3 grid;
+  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks,
+                      WR * WC * 64, &grid));
+  grid.y = g.splits;
+  hipLaunchKernelGGL((grouped_rows_kernel<Op, BM, BN, WR, WC, BKC, DIRECT, NS, GATED>), grid,
+                     dim3(WR * WC * 64), 0, stream, g);
+  EJ_LAUNCH_CHECK();
+  if (g.splits == 1) return EJ_OK;
+  if constexpr (GATED) return join_gated<kElem<Op> == 4>(g, stream);
+  else return join_parts(g, g.slots, g.slots, true, stream);
+}
+
+template <class Op, bool BKC, bool GATED = false>
+int launch_large(GroupedArgs g, hipStream_t stream) {
+  const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
+  g.row_blocks = static_cast<uint32_t>(g.slots / 256 + groups);
+  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, result_cols<GATED>(256)));
+  dim3 grid;
+  EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kLargeExtra + kZeroBlocks,
+                      512, &grid));
+  hipLaunchKernelGGL((grouped_large_kernel<Op, BKC, GATED>), grid, dim3(512), 0, stream, g);
+  EJ_LAUNCH_CHECK();
+  return EJ_OK;
+}
+
+template <class Op, int BN, int NW, bool BKC, int NS, bool GATED = false>
 int launch_skinny(GroupedArgs g, hipStream_t stream) {
   const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
   g.row_blocks = static_cast<uint32_t>(g.slots / 16 + groups);
-  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, BN));
+  g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, result_cols<GATED>(BN)));
   dim3 grid;
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks, NW * 64,
                       &grid));
-  hipLaunchKernelGGL((grouped_skinny_kernel<Op, BN, NW, BKC, NS>), grid, dim3(NW * 64), 0,
+  hipLaunchKernelGGL((grouped_skinny_kernel<Op, BN, NW, BKC, NS, GATED>), grid, dim3(NW * 64), 0,
                      stream, g);
   EJ_LAUNCH_CHECK();
   return EJ_OK;
@@ -214,6 +232,45 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
       return launch_wgrad_large<Op>(g, stream);
   }
   return launch_wgrad<Op, 128, 128, 2, 2, true, 2>(g, stream);
+}
+
+// Gated rows: the same rules, with the columns of both projections for the
+// tiles' (each tile's epilogue gives half as many results).
+template <class Op, bool BKC>
+int pick_gated(const GroupedRows &r, hipStream_t stream) {
+  const GroupedArgs &g = r.g;
+  if (g.splits > 1) {
+    if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2, true>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, true, kElem<Op> == 4 ? 0 : 3, true>(g, stream);
+  }
+  const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
+  const double rows = static_cast<double>(g.slots) / groups;
+  auto tiles_of = [&](int bm, int bn) {
+    return (static_cast<double>(g.slots) / bm + 0.5 * groups) * ceil_div(g.n, bn / 2);
+  };
+  const double tiles = tiles_of(64, 64);
+  if (!r.direct) {
+    if (tiles <= 512 || rows <= 128)
+      return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2, true>(g, stream);
+    if constexpr (kElem<Op> == 4)
+      return launch_rows<Op, 64, 128, 2, 4, BKC, false, 2, true>(g, stream);
+    else
+      return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2, true>(g, stream);
+  }
+  constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
+  if (few_rows(rows, tiles, kElem<Op>))
+    return launch_skinny<Op, kSkinny, 4, BKC, 2, true>(g, stream);
+  if constexpr (kElem<Op> == 4) {
+    return launch_rows<Op, 64, 64, 2, 2, BKC, true, 0, true>(g, stream);
+  } else {
+    if (rows <= 48 || tiles <= 576)
+      return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3, true>(g, stream);
+    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, true, 3, true>(g, stream);
+    const double small = tiles_of(128, 128) / 512;
+    if (large_rounds(tiles_of(256, 256)) <= 0.8 * (small > 1 ? small : 1))
+      return launch_large<Op, BKC, true>(g, stream);
+    return launch_rows<Op, 128, 128, 2, 2, BKC, true, 2, true>(g, stream);
+  }
 }
 
 }  // namespace ej

@@ -2,6 +2,7 @@
 // workgroup, WR x WC waves, a ring of NS stages in LDS.
 #pragma once
 
+#include "ej_gated.h"
 #include "ej_grouped.h"
 
 #include <type_traits>
@@ -37,6 +38,7 @@ __device__ inline void band_pos(uint32_t lb, uint32_t rbs, uint32_t cbs, uint32_
 
 template <class Op, int BM, int BN, int WR, int WC, bool AKC, bool BKC, bool DIRECT, int NS>
 struct TileShape {
+  using elem = typename Op::elem;
   static constexpr int kWaves = WR * WC;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int WM = BM / WR, WN = BN / WC;
@@ -229,16 +231,16 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
 // The results of a wave: row(i, &at) gives the element offset of fragment row
 // i's results and whether there is such a row, value(i, j, c) its result c of
 // four in fragment column j.
-template <class S, class Row, class Value>
+template <class S, int FN = S::FN, class Row, class Value>
 __device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row row,
                                    Value value) {
-  if (S::FN % 2 == 0 && g.out != EJ_F32) {
+  if (FN % 2 == 0 && g.out != EJ_F32) {
 #pragma unroll
     for (int i = 0; i < S::FM; ++i) {
       int64_t at;
       const bool there = row(i, &at);
 #pragma unroll
-      for (int j = 0; j + 1 < S::FN; j += 2) {
+      for (int j = 0; j + 1 < FN; j += 2) {
         float v[2][4];
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[c / 4][c % 4] = value(i, j + c / 4, c % 4);
@@ -252,7 +254,7 @@ __device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row
     int64_t at;
     if (!row(i, &at)) continue;
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
+    for (int j = 0; j < FN; ++j) {
       const int col = col0 + j * 16 + (lane >> 4) * 4;
       if (col >= g.n) continue;
       float v[4];
@@ -263,8 +265,59 @@ __device__ inline void put_results(const GroupedArgs &g, int col0, int lane, Row
   }
 }
 
-// C rows of one row block of a group times the BN columns from n0.
-template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
+// The gated results of a wave: fragment columns j of the gate and j + FN / 2 of
+// the other projection give columns col0 + 16 j on; row0 is the slot of the
+// wave's first row.  With the contraction in parts, their sums instead.
+template <class S, class Acc>
+__device__ inline void put_gated(const GroupedArgs &g, int col0, int lane, int row0, int hi,
+                                 const Acc &acc) {
+  constexpr int H = S::FN / 2;
+  float *both = g.splits > 1 ? g.partial + blockIdx.y * g.slots * (2 * static_cast<int64_t>(g.n))
+                             : g.gate_up;
+  if (both) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i) {
+      const int s = row0 + i * 16 + (lane & 15);
+      if (s >= hi) continue;
+      const int64_t at = s * (2 * static_cast<int64_t>(g.n));
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) {
+        const int col = col0 + j % H * 16 + (lane >> 4) * 4;
+        if (col >= g.n) continue;
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        put4(both, EJ_F32, at + j / H * static_cast<int64_t>(g.n), col, g.n, v);
+      }
+    }
+  }
+  if (g.splits > 1 || !g.c) return;
+  auto put = [&](auto act) {
+    put_results<S, H>(
+        g, col0, lane,
+        [&](int i, int64_t *at) {
+          const int s = row0 + i * 16 + (lane & 15);
+          *at = s * g.ldc;
+          return s < hi;
+        },
+        [&](int i, int j, int c) { return act(acc[i][j][c]) * acc[i][j + H][c]; });
+  };
+  by_activation<sizeof(typename S::elem) == 4>(g.activation, put);
+}
+
+// Gated products: the columns of B that a tile of BN holds are, for each WN of
+// them that a wave takes, WN / 2 of the gate and the same ones of the other
+// projection, so that both of a result's factors end in one lane.  Column of
+// the tile's results from n0 on, and where its half of B begins.
+template <int WN>
+__device__ inline int gated_col(int i, int n0, int n, int *shift) {
+  const int in = i % WN;
+  *shift = in < WN / 2 ? 0 : n;
+  return n0 + i / WN * (WN / 2) + in % (WN / 2);
+}
+
+// C rows of one row block of a group times the BN columns from n0; GATED: the
+// BN / 2 gated columns from n0.
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS,
+          bool GATED = false>
 __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsigned char *ring) {
   using S = TileShape<Op, BM, BN, WR, WC, true, BKC, DIRECT, NS>;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -285,12 +338,18 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
   int64_t b_step;
   if constexpr (BKC) {
     lb.init_k(wave, lane, g.k, [&](int i) {
-      const int n = n0 + i < g.n ? n0 + i : g.n - 1;
-      return bg + (n * g.ldb + k0) * kElem<Op>;
+      int shift = 0, n = n0 + i;
+      if constexpr (GATED) n = gated_col<S::WN>(i, n0, g.n, &shift);
+      n = n < g.n ? n : g.n - 1;
+      return bg + (static_cast<int64_t>(n + shift) * g.ldb + k0) * kElem<Op>;
     });
     b_step = kRowB;
   } else {
-    lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
+    if constexpr (GATED)
+      lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, g.n,
+                [&](int i, int *shift) { return gated_col<S::WN>(i, n0, g.n, shift); });
+    else
+      lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
 
@@ -313,6 +372,10 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
         lb.store(slot + S::TA::kBytes, wave, lane);
       });
 
+  if constexpr (GATED) {
+    put_gated<S>(g, n0 + wave % WC * (S::WN / 2), lane, r.lo + row0, r.hi, acc);
+    return;
+  }
   if (g.splits > 1) {
     g.c = g.partial + blockIdx.y * g.slots * g.n;
     g.ldc = g.n;
@@ -355,7 +418,7 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
 // registers: 33 us, 21 us at aligned extents; the rest are another column of
 // tiles and stage of k, and the unaligned loads, two lines for most of them.
 // Aligned loads with the bytes shifted into place afterwards took as long.
-template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS>
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS, bool GATED>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using S = TileShape<Op, BM, BN, WR, WC, true, BKC, DIRECT, NS>;
@@ -369,7 +432,8 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
   if (blockIdx.x >= live) return;
   int rb, cb;
   band_pos(xcd_logical_block(live), rbs, g.col_blocks, 1024 / BM, &rb, &cb);
-  rows_block<Op, BM, BN, WR, WC, BKC, DIRECT, NS>(g, find_row_block(g, BM, rb), cb * BN, ring);
+  rows_block<Op, BM, BN, WR, WC, BKC, DIRECT, NS, GATED>(g, find_row_block(g, BM, rb),
+                                                         cb * (GATED ? BN / 2 : BN), ring);
 #endif
 }
 
@@ -413,7 +477,7 @@ struct LargeUnit {
 // and load the next while they store the last were 5% faster in one group and
 // in 8 bits, 3 to 10% slower in 16 groups (dealt out beforehand, the short
 // blocks leave CUs waiting, and the registers spill).
-template <class Op, bool BKC>
+template <class Op, bool BKC, bool GATED>
 __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using S = TileShape<Op, 256, 256, 2, 4, true, BKC, true, 0>;
@@ -430,14 +494,14 @@ __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
   band_pos(u.block, rbs, g.col_blocks, 4, &rb, &cb);
   RowBlock r = find_row_block(g, 256, rb);
   r.lo += u.row;
-  const int n0 = cb * 256 + u.col;
+  const int n0 = (cb * 256 + u.col) / (GATED ? 2 : 1);
   if (r.lo >= r.hi || n0 >= g.n) return;
   if (u.parts == 4)
-    rows_block<Op, 128, 128, 2, 4, BKC, true, 0>(g, r, n0, ring);
+    rows_block<Op, 128, 128, 2, 4, BKC, true, 0, GATED>(g, r, n0, ring);
   else if (u.parts == 2 || r.hi - r.lo <= 128)
-    rows_block<Op, 128, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
+    rows_block<Op, 128, 256, 2, 4, BKC, true, 0, GATED>(g, r, n0, ring);
   else
-    rows_block<Op, 256, 256, 2, 4, BKC, true, 0>(g, r, n0, ring);
+    rows_block<Op, 256, 256, 2, 4, BKC, true, 0, GATED>(g, r, n0, ring);
 #endif
 }
 
@@ -571,6 +635,24 @@ __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g)
 #endif
 }
 
+// Columns col .. col + 3 of slot s from the sums of both projections.
+template <bool FINE>
+__device__ inline void put_gated_quad(const GroupedArgs &g, int64_t s, int col, const f32x4_t &gate,
+                                      const f32x4_t &up) {
+  const int64_t at = s * (2 * static_cast<int64_t>(g.n));
+  if (g.gate_up) {
+    const float a[4] = {gate[0], gate[1], gate[2], gate[3]}, b[4] = {up[0], up[1], up[2], up[3]};
+    put4(g.gate_up, EJ_F32, at, col, g.n, a);
+    put4(g.gate_up, EJ_F32, at + g.n, col, g.n, b);
+  }
+  if (!g.c) return;
+  by_activation<FINE>(g.activation, [&](auto act) {
+    const float v[4] = {act(gate[0]) * up[0], act(gate[1]) * up[1], act(gate[2]) * up[2],
+                        act(gate[3]) * up[3]};
+    put4(g.c, g.out, s * g.ldc, col, g.n, v);
+  });
+}
+
 // Few rows for each group: the time is that of reading the weights once.  A
 // workgroup takes 16 rows by BN columns; its waves split k stage by stage
 // (so that together they read long pieces of each weight row), each on a ring
@@ -595,7 +677,7 @@ struct SkinnyShape {
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 
-template <class Op, int BN, int NW, bool BKC, int NS>
+template <class Op, int BN, int NW, bool BKC, int NS, bool GATED>
 __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using S = SkinnyShape<Op, BN, NW, BKC, NS>;
@@ -614,7 +696,7 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
   const RowBlock r = find_row_block(g, S::BM, rb);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = cb * BN;
+  const int n0 = cb * (GATED ? BN / 2 : BN);
   unsigned char *ring = lds + wave * S::kRing;
 
   typename S::LA la;
@@ -630,12 +712,18 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
   int64_t b_step;
   if constexpr (BKC) {
     lb.init_k(0, lane, g.k, [&](int i) {
-      const int n = n0 + i < g.n ? n0 + i : g.n - 1;
-      return bg + (n * g.ldb + k0) * kElem<Op>;
+      int shift = 0, n = n0 + i;
+      if constexpr (GATED) n = gated_col<BN>(i, n0, g.n, &shift);
+      n = n < g.n ? n : g.n - 1;
+      return bg + (static_cast<int64_t>(n + shift) * g.ldb + k0) * kElem<Op>;
     });
     b_step = kRowB;
   } else {
-    lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
+    if constexpr (GATED)
+      lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, g.n,
+                [&](int i, int *shift) { return gated_col<BN>(i, n0, g.n, shift); });
+    else
+      lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
   auto load = [&](int i) {
@@ -673,6 +761,22 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
     *reinterpret_cast<typename Op::acc *>(part + wave * (S::BM * BN) + (lane & 15) * BN + j * 16 +
                                           (lane >> 4) * 4) = acc[0][j];
   __syncthreads();
+  if constexpr (GATED) {
+    for (int q = tid; q < S::BM * BN / 8; q += NW * 64) {
+      const int row = q / (BN / 8), col = q % (BN / 8) * 4;
+      const int s = r.lo + row;
+      if (s >= r.hi || n0 + col >= g.n) continue;
+      f32x4_t sum[2] = {};
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sum[h] += *reinterpret_cast<f32x4_t *>(part + w * (S::BM * BN) + row * BN +
+                                                 h * (BN / 2) + col);
+      put_gated_quad<kElem<Op> == 4>(g, s, n0 + col, sum[0], sum[1]);
+    }
+    return;
+  }
   for (int q = tid; q < S::BM * BN / 4; q += NW * 64) {
     const int row = q / (BN / 4), col = q % (BN / 4) * 4;
     const int s = r.lo + row;
@@ -723,6 +827,33 @@ static __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g,
   }
   const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
   put4(g.c, g.out, row / m * g.c_group + row % m * g.ldc, col, g.n, v);
+}
+
+// Gated results from the sums of the parts, added in their order.  Rows of no
+// group (offsets given) are zero already.
+template <bool FINE>
+__global__ __launch_bounds__(256) void gated_join_kernel(GroupedArgs g) {
+  const int64_t quads = (g.n + 3) / 4, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= g.slots * quads) return;
+  const int64_t row = i / quads;
+  const int col = static_cast<int>(i % quads) * 4;
+  if (g.offsets && (row < g.offsets[0] || row >= g.offsets[g.n_groups])) return;
+  f32x4_t sum[2] = {};
+  const float *src = g.partial + row * (2 * static_cast<int64_t>(g.n)) + col;
+  const int64_t part = g.slots * (2 * static_cast<int64_t>(g.n));
+  for (int p = 0; p < g.splits; ++p)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float *v = src + p * part + h * static_cast<int64_t>(g.n);
+      if (g.n % 4 == 0) {
+        sum[h] += *reinterpret_cast<const f32x4_t *>(v);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (col + c < g.n) sum[h][c] += v[c];
+      }
+    }
+  put_gated_quad<FINE>(g, row, col, sum[0], sum[1]);
 }
 
 }  // namespace ej

@@ -640,6 +640,137 @@ py::tuple grouped_matmul_vjp(py::handle x_, py::handle w_, py::handle offsets, p
                         need_w ? py::cast(v[1]) : py::none());
 }
 
+// ---- gated products ----------------------------------------------------------------------
+
+int32_t activation_code(const std::string &name) {
+  if (name == "silu") return EJ_SILU;
+  if (name == "gelu") return EJ_GELU;
+  if (name == "gelu_tanh") return EJ_GELU_TANH;
+  throw py::value_error("activation must be 'silu', 'gelu' or 'gelu_tanh', got '" + name + "'");
+}
+
+// act(gate) up for the halves of x w; gate_up: the halves in fp32, where asked
+// for (the result then may be left out).
+Tensor run_gated(const Tensor &x_, const Tensor &w, const Groups &g, int32_t act, bool result,
+                 Tensor *gate_up) {
+  no_tangents(x_, w);
+  const Tensor x = rows_of(x_);
+  const Order o = weight_order(w);
+  const int64_t k = w.size(1), n = w.size(2) / 2;
+  const int code = code_of(x.scalar_type());
+  Launch on(x);
+  const Tensor out = result ? at::empty({g.n_slots, n}, x.options()) : Tensor();
+  if (gate_up) *gate_up = at::empty({g.n_slots, 2 * n}, x.options().dtype(at::kFloat));
+  const ej_grouped_desc d = describe(x, code, code, o, w.size(0), k, n, g.n_slots, n);
+  size_t bytes;
+  check(ej_gated_gemm_workspace_size(&d, &bytes), "ej_gated_gemm_workspace_size");
+  const Tensor ws = workspace(x, bytes);
+  check(ej_gated_gemm(&d, act, ptr(x), ints(g.rows), ints(g.offsets), ptr(o.w), mut(out),
+                      gate_up ? mut_floats(*gate_up) : nullptr, mut(ws), bytes, on.stream),
+        "ej_gated_gemm");
+  return out;
+}
+
+variable_list gated_vjp(const Tensor &x, const Tensor &w, const Groups &g, int32_t act,
+                        const Tensor &gate_up, const Tensor &grad_, bool need_x, bool need_w) {
+  at::NoGradGuard no_grad;
+  no_tangents(grad_);
+  const Tensor grad = rows_of(grad_.to(x.scalar_type()));
+  Tensor both = at::empty(gate_up.sizes(), x.options());
+  {
+    Launch on(x);
+    const int64_t n = grad.size(1);
+    check(ej_gated_vjp(floats(gate_up), ptr(grad), code_of(x.scalar_type()), grad.size(0),
+                       int32_of(n, "n"), std::max(row_stride(grad), n), act, mut(both), on.stream),
+          "ej_gated_vjp");
+  }
+  return product_vjp(x, w, g, both, need_x, need_w);
+}
+
+struct GatedFunction : public Function<GatedFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Groups *g,
+                        int64_t act) {
+    Tensor gate_up;
+    const Tensor out = run_gated(x, w, *g, static_cast<int32_t>(act), true, &gate_up);
+    variable_list saved = {x, w, gate_up};
+    for (const Tensor *t : {&g->offsets, &g->rows, &g->slots})
+      if (t->defined()) saved.push_back(*t);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["n_slots"] = g->n_slots;
+    ctx->saved_data["act"] = act;
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    Groups g;
+    if (s.size() > 3) g.offsets = s[3];
+    if (s.size() > 4) {
+      g.rows = s[4];
+      g.slots = s[5];
+    }
+    g.n_slots = ctx->saved_data["n_slots"].toInt();
+    variable_list v = gated_vjp(s[0], s[1], g, static_cast<int32_t>(ctx->saved_data["act"].toInt()),
+                                s[2], grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    return first_order({v[0], v[1], Tensor(), Tensor()});
+  }
+};
+
+struct GatedArgs {
+  Tensor x, w;
+  Groups g;
+};
+
+// groups None: w [k, 2 n] or [1, k, 2 n], one group of every row of x.
+GatedArgs gated_args(py::handle x_, py::handle w_, py::handle offsets, py::handle rows,
+                     py::handle slots, bool gather) {
+  GatedArgs a;
+  a.x = on_gpu(x_, "x");
+  a.w = on_gpu_of(a.x, w_, "w");
+  const bool dense = offsets.is_none();
+  if (dense && a.w.dim() == 2) a.w = a.w.unsqueeze(0);
+  check_product(a.x, a.w, py::none());
+  if (a.w.size(2) % 2)
+    throw py::value_error("w has " + std::to_string(a.w.size(2)) +
+                          " columns, expected the gate's and as many of the other projection");
+  if (dense) {
+    if (gather || a.w.size(0) != 1)
+      throw py::value_error("more than one weight matrix, or gather=True, needs groups");
+    a.g.n_slots = a.x.size(0);
+  } else {
+    a.g = groups_of(a.x, a.w.size(0), offsets, rows, slots, gather);
+  }
+  return a;
+}
+
+Tensor gated_matmul(py::handle x, py::handle w, py::handle offsets, py::handle rows,
+                    py::handle slots, bool gather, const std::string &activation) {
+  const int32_t act = activation_code(activation);
+  const GatedArgs a = gated_args(x, w, offsets, rows, slots, gather);
+  if (!wants_grad(a.x) && !wants_grad(a.w)) return run_gated(a.x, a.w, a.g, act, true, nullptr);
+  // refused now, not when the gradient is asked for
+  if (wants_grad(a.x) && a.g.slots.defined()) check_picks(a.g.slots);
+  return GatedFunction::apply(a.x, a.w, &a.g, static_cast<int64_t>(act));
+}
+
+py::tuple gated_matmul_vjp(py::handle x, py::handle w, py::handle offsets, py::handle rows,
+                           py::handle slots, bool gather, const std::string &activation,
+                           py::handle grad_, bool need_x, bool need_w) {
+  const int32_t act = activation_code(activation);
+  const GatedArgs a = gated_args(x, w, offsets, rows, slots, gather);
+  if (need_x && a.g.slots.defined()) check_picks(a.g.slots);
+  const Tensor grad = on_gpu_of(a.x, grad_, "grad_out");
+  if (grad.dim() != 2 || grad.size(0) != a.g.n_slots || grad.size(1) != a.w.size(2) / 2)
+    throw py::value_error("grad_out has shape " + str(grad.sizes()) + ", expected " +
+                          str({a.g.n_slots, a.w.size(2) / 2}));
+  at::NoGradGuard no_grad;
+  Tensor gate_up;
+  run_gated(a.x, a.w, a.g, act, false, &gate_up);
+  variable_list v = gated_vjp(a.x, a.w, a.g, act, gate_up, grad, need_x, need_w);
+  if (need_w && py::cast<Tensor>(w).dim() == 2) v[1] = v[1].squeeze(0);
+  return py::make_tuple(need_x ? py::cast(v[0]) : py::none(),
+                        need_w ? py::cast(v[1]) : py::none());
+}
+
 // ---- 8-bit integers -----------------------------------------------------------------------
 
 py::tuple quantize_rows(py::handle x_) {
@@ -731,6 +862,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("combine_vjp", &combine_vjp);
   m.def("grouped_matmul", &grouped_matmul);
   m.def("grouped_matmul_vjp", &grouped_matmul_vjp);
+  m.def("gated_matmul", &gated_matmul);
+  m.def("gated_matmul_vjp", &gated_matmul_vjp);
   m.def("quantize_rows", &quantize_rows);
   m.def("int8_matmul", &int8_matmul);
   m.def("rows_of", &rows_of);

@@ -64,7 +64,8 @@ class ExpertRouting:
 
 
 def group_args(groups) -> tuple:
-    """(offsets, rows, slots) of an ``ExpertRouting``, or of offsets alone."""
+    """(offsets, rows, slots) of an ``ExpertRouting``, or of offsets alone
+    (None: no groups)."""
     if isinstance(groups, ExpertRouting):
         return groups.offsets, groups.rows, groups.slots
     return groups, None, None

@@ -761,6 +761,30 @@ int ej_grouped_gemm_dw(const ej_grouped_desc *desc, const void *x, const int32_t
                        const int32_t *offsets, const void *grad, void *grad_w, void *workspace,
                        size_t workspace_bytes, ej_stream_t stream);
 
+/* Gated products: with G | U = x[rows[s]] W_e, out[s] = act(G) U.  W holds 2 n
+ * columns, the gate's n first (EJ_W_KN: rows of 2 n; EJ_W_NK: 2 n rows); the
+ * descriptor's n, out_dtype and out_stride are the result's.  fp32 and 16-bit
+ * operands (n < 2^30); groups, rows and the workspace as ej_grouped_gemm's.
+ * gate_up (NULL: not wanted) gets G | U in fp32, [n_slots][2 n], rows that no
+ * group covers left as they were; out may be NULL if gate_up is not.
+ *   EJ_SILU       g / (1 + exp(-g))
+ *   EJ_GELU       g erfc(-g / sqrt 2) / 2
+ *   EJ_GELU_TANH  g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+#define EJ_SILU 0
+#define EJ_GELU 1
+#define EJ_GELU_TANH 2
+int ej_gated_gemm_workspace_size(const ej_grouped_desc *desc, size_t *bytes);
+int ej_gated_gemm(const ej_grouped_desc *desc, int32_t activation, const void *x,
+                  const int32_t *rows, const int32_t *offsets, const void *w, void *out,
+                  float *gate_up, void *workspace, size_t workspace_bytes, ej_stream_t stream);
+
+/* Gradient to G | U: out [n_rows][2 n] = (grad U act'(G)) | (grad act(G)) for
+ * gate_up [n_rows][2 n] in fp32 and grad [n_rows][n], rows grad_stride apart;
+ * grad and out of `dtype`, rounded once.  The gradients to x and W are
+ * ej_grouped_gemm's of a product with 2 n columns whose gradient this is. */
+int ej_gated_vjp(const float *gate_up, const void *grad, int32_t dtype, int64_t n_rows, int32_t n,
+                 int64_t grad_stride, int32_t activation, void *out, ej_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,84 @@
+"""Gated products, block-scaled 8-bit products and token rows: what they refuse,
+and what is decided without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+import einjax_amd as ej
+from einjax_amd import _lib
+from test_experts_host import FAKE, desc
+
+INVAL, UNSUPPORTED = _lib.EJ_E_INVAL, _lib.EJ_E_UNSUPPORTED
+
+
+def gated_desc(**kw):
+    """k = 64, n = 32 results of 64 columns of w."""
+    return desc(**{**dict(w_group=64 * 64, w_stride=64), **kw})
+
+
+def gated(d, act=_lib.EJ_SILU, x=FAKE, rows=None, offsets=FAKE, w=FAKE, out=FAKE, gate_up=None):
+    return _lib.load().ej_gated_gemm(ctypes.byref(d), act, x, rows, offsets, w, out, gate_up, None,
+                                     0, None)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dtype=_lib.EJ_F64), INVAL), (dict(dtype=_lib.EJ_I8), INVAL),
+    (dict(out_dtype=_lib.EJ_F16), INVAL), (dict(w_order=2), INVAL), (dict(k=-1), INVAL),
+    (dict(x_stride=63), INVAL), (dict(w_stride=63), INVAL), (dict(out_stride=31), INVAL),
+    (dict(w_group=64 * 64 - 1), INVAL), (dict(n_rows=9), INVAL),
+    (dict(w_order=_lib.EJ_W_NK, w_group=64 * 64 - 1), INVAL),
+    (dict(n_slots=(1 << 31) - 511), UNSUPPORTED),
+    (dict(n=1 << 30, w_stride=1 << 31, out_stride=1 << 30, w_group=1 << 40), UNSUPPORTED),
+])
+def test_gated_refusals(change, status):
+    assert gated(gated_desc(**change)) == status
+    assert _lib.load().ej_last_error()
+
+
+def test_gated_arguments():
+    lib, n = _lib.load(), ctypes.c_size_t()
+    assert gated(gated_desc(), act=3) == INVAL
+    assert gated(gated_desc(), x=None) == INVAL
+    assert gated(gated_desc(), w=None) == INVAL
+    assert gated(gated_desc(), out=None) == INVAL
+    assert gated(gated_desc(), offsets=None) == INVAL
+    assert lib.ej_gated_gemm(None, 0, FAKE, None, FAKE, FAKE, FAKE, None, None, 0, None) == INVAL
+    # nothing to write: no launch
+    assert gated(gated_desc(n_slots=0), x=None, w=None, out=None, offsets=None) == 0
+    assert gated(gated_desc(n=0), x=None, w=None, out=None, offsets=None) == 0
+    # a contraction in parts needs room for the sums of both projections
+    few = gated_desc(n_groups=1, k=4096, n_slots=512, n_rows=512, x_stride=4096,
+                     w_group=4096 * 64)
+    assert lib.ej_gated_gemm_workspace_size(ctypes.byref(few), ctypes.byref(n)) == 0
+    assert n.value > 0 and n.value % (4 * 512 * 64) == 0
+    assert gated(few) == INVAL and b"workspace" in lib.ej_last_error()
+    for d in (gated_desc(), gated_desc(n_groups=0), gated_desc(n_slots=0)):
+        assert lib.ej_gated_gemm_workspace_size(ctypes.byref(d), ctypes.byref(n)) == 0
+        assert n.value == 0
+    assert lib.ej_gated_gemm_workspace_size(None, ctypes.byref(n)) == INVAL
+
+
+def test_gated_vjp_arguments():
+    def vjp(both=FAKE, grad=FAKE, dtype=_lib.EJ_BF16, rows=4, n=8, stride=8, act=0, out=FAKE):
+        return _lib.load().ej_gated_vjp(both, grad, dtype, rows, n, stride, act, out, None)
+
+    assert vjp(dtype=_lib.EJ_I8) == INVAL
+    assert vjp(stride=7) == INVAL
+    assert vjp(rows=-1) == INVAL
+    assert vjp(act=-1) == INVAL
+    assert vjp(both=None) == INVAL and vjp(grad=None) == INVAL and vjp(out=None) == INVAL
+    assert vjp(rows=0, both=None, grad=None, out=None) == 0
+    assert vjp(n=0, stride=0, both=None, grad=None, out=None) == 0
+    assert vjp(rows=1 << 40) == UNSUPPORTED
+    assert vjp(rows=1 << 62) == UNSUPPORTED
+    assert vjp(n=1 << 30, stride=1 << 30) == UNSUPPORTED
+
+
+def test_operands_must_be_on_the_gpu():
+    t = torch.zeros(4, 4)
+    for call in (lambda: ej.gated_matmul(t, t), lambda: ej.gated_matmul(t, t[None], t.int()),
+                 lambda: ej.gated_matmul_vjp(t, t, None, t)):
+        with pytest.raises(TypeError, match="on the GPU"):
+            call()
