@@ -40,8 +40,10 @@ from .kernels import (
     block_sparse_matmul_generic,
     coordinate_join_hash,
     coordinate_join_sorted,
+    fp8_matmul,
     group_by_expert,
     int8_matmul,
+    quantize_blocks,
     quantize_rows,
 )
 from .tensor import (
@@ -89,5 +91,5 @@ __all__ = [
     "ExpertRouting", "route_experts", "route_experts_vjp", "group_by_expert", "grouped_matmul",
     "grouped_matmul_vjp", "gated_matmul", "gated_matmul_vjp", "combine_experts",
     "combine_experts_vjp", "quantize_rows",
-    "int8_matmul",
+    "int8_matmul", "quantize_blocks", "fp8_matmul",
 ]

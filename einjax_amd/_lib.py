@@ -32,6 +32,7 @@ EJ_I32 = 3
 EJ_I64 = 4
 EJ_F16 = 5
 EJ_I8 = 6
+EJ_E4M3 = 7
 
 EJ_W_KN = 0
 EJ_W_NK = 1
@@ -172,6 +173,7 @@ SIGNATURES = {
     "ej_grouped_gemm_dw_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
     "ej_grouped_gemm_dw": (_i32, [ctypes.POINTER(GroupedDesc), _vp, _vp, _vp, _vp, _vp, _vp,
                                   _sz, _vp]),
+    "ej_quantize_blocks": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
     "ej_gated_gemm_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
     "ej_gated_gemm": (_i32, [ctypes.POINTER(GroupedDesc), _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                              _sz, _vp]),

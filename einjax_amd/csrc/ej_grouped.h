@@ -25,6 +25,7 @@ namespace ej {
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef int i32v2_t __attribute__((ext_vector_type(2)));
 typedef int i32v4_t __attribute__((ext_vector_type(4)));
+typedef int i32v8_t __attribute__((ext_vector_type(8)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 // vectors at any element's alignment
 typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -53,6 +54,19 @@ struct OpI8 {
   static constexpr bool kInt = true;
 };
 
+// 8-bit floating point (e4m3) with a scale for each 128 of k: kBlocks.  FINE:
+// by the 16-bit matrix instructions, see mma_block.
+template <bool FINE>
+struct OpBlocks {
+  using elem = uint8_t;
+  using acc = f32x4_t;
+  static constexpr bool kInt = false;
+};
+using OpF8 = OpBlocks<false>;
+using OpF8Fine = OpBlocks<true>;
+template <class Op>
+constexpr bool kBlocks = __is_same(Op, OpF8) || __is_same(Op, OpF8Fine);
+
 template <class Op>
 constexpr int kElem = static_cast<int>(sizeof(typename Op::elem));
 constexpr int kRowB = 128;                       // bytes of a K tile's row
@@ -68,8 +82,8 @@ struct GroupedArgs {
   const int32_t *a_rows;    // row of each slot in A (null: the slot itself)
   const int32_t *b_rows;    // weight gradient: row of each slot in Q
   const int32_t *offsets;   // [n_groups + 1] (null: one group of every slot)
-  const float *a_scale;     // 8-bit: scale of each row of A
-  const float *b_scale;     // 8-bit: scales [e][n]
+  const float *a_scale;     // 8-bit: scale of each row of A; blocks: [n_a][k blocks]
+  const float *b_scale;     // 8-bit: scales [e][n]; blocks: [e][n blocks][k blocks]
   int64_t lda, ldb, ldc;    // row strides, elements
   int64_t b_group, c_group; // elements between the groups of B and of D
   int64_t n_a, n_b;         // rows of A; rows of Q
@@ -108,6 +122,56 @@ __device__ inline void mma(typename Op::acc &acc, const i32v4_t &x, const i32v4_
     for (int c = 0; c < 4; ++c)
       acc = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[c], yf[c], acc, 0, 0, 0);
   }
+}
+
+// A fragment's 128 of k in 8-bit floats, 32 a lane (16 of each 64-byte slab),
+// and X Y^T over it.  Which of k lies in which lane is the same for X and Y, so
+// the sum does not depend on it.  The form without scales: those of the blocks
+// are fp32, not powers of two, and are applied to the sum.
+//
+// The 8-bit matrix instruction aligns the products of 8 consecutive k to the
+// largest of them and drops what lies below 2^-13 of it (measured: 65536 + v
+// keeps the multiples of 8 of v, toward zero); the eights are added in fp32.
+// Values of one size lose about 2^-14 of the sum, a sixteenth of what rounding to
+// bf16 does and a fourth of fp16's.  Results in fp32 take FINE: e4m3 values
+// are bf16 values, and the sum of those is formed in fp32, at half the rate.
+template <class Op>
+struct BlockFragment {
+  i32v8_t v;
+  __device__ inline void set(const i32v4_t &lo, const i32v4_t &hi) {
+    v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+template <>
+struct BlockFragment<OpF8Fine> {
+  bf16x8_t v[4];
+  __device__ inline void set(const i32v4_t &lo, const i32v4_t &hi) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint32_t word = w < 4 ? lo[w] : hi[w - 4];
+      const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, false);
+      const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.f, true);
+      v[w / 2][w % 2 * 4] = a[0];
+      v[w / 2][w % 2 * 4 + 1] = a[1];
+      v[w / 2][w % 2 * 4 + 2] = b[0];
+      v[w / 2][w % 2 * 4 + 3] = b[1];
+    }
+#endif
+  }
+};
+__device__ inline f32x4_t mma_block(const BlockFragment<OpF8> &x, const BlockFragment<OpF8> &y) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x.v, y.v, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0,
+                                                          0, 0, 0, 0, 0);
+}
+__device__ inline f32x4_t mma_block(const BlockFragment<OpF8Fine> &x,
+                                    const BlockFragment<OpF8Fine> &y) {
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v[c], y.v[c], sum, 0, 0, 0);
+  return sum;
 }
 
 // ---- LDS tiles --------------------------------------------------------------
@@ -384,6 +448,12 @@ constexpr int kZeroBlocks = 64;  // workgroups appended to a grid for zero_dead_
 __device__ inline void load_to_lds(const char *src, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds));
+#endif
+}
+// The same for 4 bytes, lane l's to `lds` + 4 l.
+__device__ inline void load_word_to_lds(const float *src, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(src), "{m0}"(lds));
 #endif
 }
 __device__ inline uint32_t lds_address(const void *p) {

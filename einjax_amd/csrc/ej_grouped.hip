@@ -13,14 +13,17 @@ bool aligned16(const void *p, int64_t a, int64_t b, int size) {
 // The kernels count slots in 32 bits, up to two blocks or stages past the last.
 constexpr int64_t kMaxSlots = (int64_t{1} << 31) - 512;
 
-int elem_size(int32_t dtype) { return dtype == EJ_F32 ? 4 : dtype == EJ_I8 ? 1 : 2; }
+// 8-bit operands, with scales beside them.
+bool scaled_8(int32_t dtype) { return dtype == EJ_I8 || dtype == EJ_E4M3; }
+int elem_size(int32_t dtype) { return dtype == EJ_F32 ? 4 : scaled_8(dtype) ? 1 : 2; }
 
 // n_w: columns of W (the result's, twice as many of a gated product).
 int check_desc(const ej_grouped_desc *d, int64_t n_w) {
   EJ_CHECK_ARG(d, "null descriptor");
   EJ_CHECK_ARG(d->dtype == EJ_F32 || d->dtype == EJ_BF16 || d->dtype == EJ_F16 ||
-                   d->dtype == EJ_I8,
-               "operands of dtype %d: expected EJ_F32, EJ_BF16, EJ_F16 or EJ_I8", d->dtype);
+                   scaled_8(d->dtype),
+               "operands of dtype %d: expected EJ_F32, EJ_BF16, EJ_F16, EJ_I8 or EJ_E4M3",
+               d->dtype);
   EJ_CHECK_ARG(d->w_order == EJ_W_KN || d->w_order == EJ_W_NK, "w_order = %d", d->w_order);
   EJ_CHECK_ARG(d->n_groups >= 0 && d->k >= 0 && d->n >= 0 && d->n_slots >= 0 && d->n_rows >= 0,
                "negative size");
@@ -43,7 +46,7 @@ int check_desc(const ej_grouped_desc *d) { return check_desc(d, d ? d->n : 0); }
 
 int check_gated(const ej_grouped_desc *d) {
   EJ_TRY(check_desc(d, d ? 2 * static_cast<int64_t>(d->n) : 0));
-  EJ_CHECK_ARG(d->dtype != EJ_I8, "gated products take fp32 and 16-bit operands");
+  EJ_CHECK_ARG(!scaled_8(d->dtype), "gated products take fp32 and 16-bit operands");
   if (d->n >= (1 << 30)) {
     set_error("n = %d: gated products of fewer than 2^30 columns are supported", d->n);
     return EJ_E_UNSUPPORTED;
@@ -89,7 +92,7 @@ int split_parts(double tiles, int64_t contraction, int elem, bool whole, double 
 
 // n: columns of W
 int rows_parts(const ej_grouped_desc *d, int64_t n) {
-  if (d->dtype == EJ_I8 || d->n_groups == 0 || d->n_slots == 0) return 1;
+  if (scaled_8(d->dtype) || d->n_groups == 0 || d->n_slots == 0) return 1;
   const int64_t groups = d->n_groups < d->n_slots ? d->n_groups : d->n_slots;
   const double rows = static_cast<double>(d->n_slots) / groups;
   const double tiles = (rows / 64 + 0.5) * groups * ceil_div(n, 64);
@@ -180,13 +183,13 @@ extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const in
                                const float *w_scale, void *out, void *workspace,
                                size_t workspace_bytes, ej_stream_t stream) {
   EJ_TRY(check_desc(d));
-  const bool i8 = d->dtype == EJ_I8;
+  const bool scaled = scaled_8(d->dtype);
   EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype ||
-                   (i8 && (d->out_dtype == EJ_BF16 || d->out_dtype == EJ_F16)),
+                   (scaled && (d->out_dtype == EJ_BF16 || d->out_dtype == EJ_F16)),
                "result of dtype %d from operands of dtype %d", d->out_dtype, d->dtype);
-  EJ_CHECK_ARG(d->out_dtype != EJ_I8, "8-bit results are not products");
-  if (i8) {
-    EJ_CHECK_ARG(d->w_order == EJ_W_NK, "8-bit weights are k-contiguous (EJ_W_NK)");
+  EJ_CHECK_ARG(!scaled_8(d->out_dtype), "8-bit results are not products");
+  EJ_CHECK_ARG(!scaled || d->w_order == EJ_W_NK, "8-bit weights are k-contiguous (EJ_W_NK)");
+  if (d->dtype == EJ_I8) {
     // |sum| <= 128 * 128 * k
     EJ_CHECK_ARG(d->k < (1 << 17), "k = %d: the 32-bit sum of 8-bit products holds k < 131072",
                  d->k);
@@ -194,7 +197,9 @@ extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const in
   if (d->n_slots == 0 || d->n == 0) return EJ_OK;
   EJ_CHECK_ARG(out, "null result");
   EJ_TRY(check_operands(d, x, rows, offsets, w));
-  EJ_CHECK_ARG(!i8 || d->n_groups == 0 || (x_scale && w_scale), "null scale");
+  EJ_CHECK_ARG(!scaled || d->n_groups == 0 || (d->dtype == EJ_E4M3 && d->k == 0) ||
+                   (x_scale && w_scale),
+               "null scale");
 
   GroupedRows r = rows_args(d, x, rows, offsets, w, out);
   r.g.a_scale = x_scale;
@@ -205,6 +210,7 @@ extern "C" int ej_grouped_gemm(const ej_grouped_desc *d, const void *x, const in
     case EJ_BF16: return grouped_rows_bf16(r, as_stream(stream));
     case EJ_F16: return grouped_rows_f16(r, as_stream(stream));
     case EJ_I8: return grouped_rows_i8(r, as_stream(stream));
+    case EJ_E4M3: return grouped_rows_f8(r, as_stream(stream));
     default: return grouped_rows_f32(r, as_stream(stream));
   }
 }
@@ -213,7 +219,7 @@ extern "C" int ej_grouped_gemm_dw(const ej_grouped_desc *d, const void *x, const
                                   const int32_t *offsets, const void *grad, void *grad_w,
                                   void *workspace, size_t workspace_bytes, ej_stream_t stream) {
   EJ_TRY(check_desc(d));
-  EJ_CHECK_ARG(d->dtype != EJ_I8, "8-bit products have no gradient");
+  EJ_CHECK_ARG(!scaled_8(d->dtype), "8-bit products have no gradient");
   EJ_CHECK_ARG(d->out_dtype == EJ_F32 || d->out_dtype == d->dtype,
                "gradient of dtype %d from operands of dtype %d", d->out_dtype, d->dtype);
   if (d->n_groups == 0 || d->k == 0 || d->n == 0) return EJ_OK;

@@ -16,6 +16,7 @@ int grouped_rows_bf16(const GroupedRows &r, hipStream_t stream);
 int grouped_rows_f16(const GroupedRows &r, hipStream_t stream);
 int grouped_rows_f32(const GroupedRows &r, hipStream_t stream);
 int grouped_rows_i8(const GroupedRows &r, hipStream_t stream);
+int grouped_rows_f8(const GroupedRows &r, hipStream_t stream);
 int gated_rows_bf16(const GroupedRows &r, hipStream_t stream);
 int gated_rows_f16(const GroupedRows &r, hipStream_t stream);
 int gated_rows_f32(const GroupedRows &r, hipStream_t stream);

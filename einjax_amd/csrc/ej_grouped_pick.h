@@ -273,4 +273,22 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
   }
 }
 
+// Products of 8-bit floats with block scales.
+template <class Op>
+int pick_f8(const GroupedRows &r, hipStream_t stream) {
+  const GroupedArgs &g = r.g;
+  const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
+  const double rows = static_cast<double>(g.slots) / groups;
+  const double tiles = expected_tiles(g, 64, 64, groups);
+  if (!r.direct) {
+    if (tiles <= 512 || rows <= 128)
+      return launch_rows<Op, 64, 64, 2, 2, true, false, 2>(g, stream);
+    return launch_rows<Op, 128, 128, 2, 4, true, false, 2>(g, stream);
+  }
+  if (few_rows(rows, tiles, 1)) return launch_skinny<Op, 32, 4, true, 2>(g, stream);
+  if (rows <= 48 || tiles <= 576)
+    return launch_rows<Op, 64, 64, 2, 2, true, true, 3>(g, stream);
+  return launch_rows<Op, 128, 128, 2, 2, true, true, 2>(g, stream);
+}
+
 }  // namespace ej

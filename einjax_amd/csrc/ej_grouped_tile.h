@@ -41,6 +41,7 @@ struct TileShape {
   using elem = typename Op::elem;
   static constexpr int kWaves = WR * WC;
   static constexpr int kThreads = kWaves * 64;
+  static constexpr int kRows = BM;
   static constexpr int WM = BM / WR, WN = BN / WC;
   static constexpr int FM = WM / 16, FN = WN / 16;
   using TA = Tile<Op, BM, AKC>;
@@ -49,9 +50,13 @@ struct TileShape {
   using FB = Fragments<Op, TB, BKC, FN>;
   using LA = Loader<Op, BM, AKC, kWaves, DIRECT>;
   using LB = Loader<Op, BN, BKC, kWaves, DIRECT>;
-  static constexpr int kSlot = TA::kBytes + TB::kBytes;
+  // scales of a stage, one a thread: the tile's rows', then its columns'
+  static constexpr int kScaleAt = TA::kBytes + TB::kBytes;
+  static constexpr int kScales = kBlocks<Op> ? kThreads * 4 : 0;
+  static_assert(!kBlocks<Op> || BM + BN <= kThreads, "a thread for each scale");
+  static constexpr int kSlot = TA::kBytes + TB::kBytes + kScales;
   static constexpr int kLds = NS == 0 ? 3 * TA::kBytes + 2 * TB::kBytes : NS * kSlot;
-  static constexpr int kLoads = LA::kLoads + LB::kLoads;
+  static constexpr int kLoads = LA::kLoads + LB::kLoads + (kBlocks<Op> ? 1 : 0);
 };
 
 // acc[i][j] += A fragment i times B fragment j over the stage `slot` bytes
@@ -71,6 +76,45 @@ __device__ inline void stage_mma(typename Op::acc (&acc)[S::FM][S::FN], const ty
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
       for (int j = 0; j < S::FN; ++j) mma<Op>(acc[i][j], b[j], a[i]);
+  }
+}
+
+// This lane's places among a stage's scales: its row in the first fragment, and
+// the wave's columns, which lie in one block of 128.
+struct ScalePlace {
+  uint32_t row, col;
+  __device__ inline void init(uint32_t base, int rows, int row0, int col0, int lane) {
+    row = base + (row0 + (lane & 15)) * 4;
+    col = base + (rows + col0) * 4;
+  }
+  __device__ static inline float at(uint32_t lds) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) float *>(
+        (lds_u8 *)(size_t)lds);
+  }
+};
+
+// acc[i][j] += (A fragment i times B fragment j over one block of 128) times
+// the product of their scales.
+template <class Op, class S>
+__device__ inline void stage_blocks(f32x4_t (&acc)[S::FM][S::FN], const typename S::FA &fa,
+                                    const typename S::FB &fb, const ScalePlace &scales,
+                                    uint32_t slot) {
+  static_assert(128 % (S::FN * 16) == 0, "a wave's columns lie in one block");
+  BlockFragment<Op> b[S::FN];
+#pragma unroll
+  for (int j = 0; j < S::FN; ++j) b[j].set(fb.read(slot, j, 0), fb.read(slot, j, 1));
+  const float bs = ScalePlace::at(scales.col + slot);
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i) {
+    BlockFragment<Op> a;
+    a.set(fa.read(slot, i, 0), fa.read(slot, i, 1));
+    const float s = ScalePlace::at(scales.row + slot + i * 64) * bs;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      const f32x4_t t = mma_block(b[j], a);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = fmaf(t[c], s, acc[i][j][c]);
+    }
   }
 }
 
@@ -188,6 +232,12 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
   typename S::FB fb;
   fa.init(base, row0, lane);
   fb.init(base + S::TA::kBytes, col0, lane);
+  ScalePlace scales;
+  if constexpr (kBlocks<Op>) scales.init(base + S::kScaleAt, S::kRows, row0, col0, lane);
+  auto stage = [&](uint32_t slot) {
+    if constexpr (kBlocks<Op>) stage_blocks<Op, S>(acc, fa, fb, scales, slot);
+    else stage_mma<Op, S>(acc, fa, fb, slot);
+  };
   auto load_all = [&](int st, unsigned char *slot) {
 #pragma unroll
     for (int v = 0; v < S::kLoads; ++v) load_stage(v, st, slot, true);
@@ -209,7 +259,7 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
         load_all(st + NS - 1, ring + put * S::kSlot);
         put = put + 1 == NS ? 0 : put + 1;
       }
-      stage_mma<Op, S>(acc, fa, fb, get * S::kSlot);
+      stage(get * S::kSlot);
       // read before the barrier after which other waves load into this slot
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       get = get + 1 == NS ? 0 : get + 1;
@@ -222,7 +272,7 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
     for (int st = 0; st < stages; ++st) {
       __syncthreads();
       if (st + 1 < stages) load_all(st + 1, ring);
-      stage_mma<Op, S>(acc, fa, fb, (st & 1) * S::kSlot);
+      stage((st & 1) * S::kSlot);
       if (st + 1 < stages) store_stage(ring + ((st + 1) & 1) * S::kSlot);
     }
   }
@@ -314,6 +364,36 @@ __device__ inline int gated_col(int i, int n0, int n, int *shift) {
   return n0 + i / WN * (WN / 2) + in % (WN / 2);
 }
 
+// The scales of a stage: thread t's is that of row t of the tile, or of column
+// t - rows.
+struct ScaleLoader {
+  const float *src;
+  float held;
+  __device__ inline void init(const GroupedArgs &g, const RowBlock &r, int rows, int cols, int n0,
+                              int t, int st) {
+    const int64_t k_blocks = (g.k + 127) / 128;
+    if (t < rows) {
+      const int s = r.lo + t < r.hi ? r.lo + t : r.hi - 1;
+      src = g.a_scale + slot_row(g.a_rows, g.n_a, s) * k_blocks + st;
+    } else {
+      int n = n0 + (t - rows < cols ? t - rows : cols - 1);
+      n = n < g.n ? n : g.n - 1;
+      const int64_t n_blocks = (g.n + 127) / 128;
+      src = g.b_scale + (r.group * n_blocks + n / 128) * k_blocks + st;
+    }
+  }
+  // The next stage's, `step` stages on from the one before.
+  template <bool DIRECT>
+  __device__ inline void load(unsigned char *to, int wave, int step) {
+    if constexpr (DIRECT) load_word_to_lds(src, lds_address(to) + wave * 256);
+    else held = *src;
+    src += step;
+  }
+  __device__ inline void store(unsigned char *to, int t) const {
+    *reinterpret_cast<float *>(to + t * 4) = held;
+  }
+};
+
 // C rows of one row block of a group times the BN columns from n0; GATED: the
 // BN / 2 gated columns from n0.
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS,
@@ -353,6 +433,9 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
 
+  ScaleLoader scales;
+  if constexpr (kBlocks<Op>) scales.init(g, r, BM, BN, n0, tid, st0);
+
   typename Op::acc acc[S::FM][S::FN];
 #pragma unroll
   for (int i = 0; i < S::FM; ++i)
@@ -364,12 +447,15 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
         const int left = ks - st * kStep<Op>;
         if (v < S::LA::kLoads)
           la.load(v, slot, wave, left, kRowB, part);
-        else
+        else if (v < S::LA::kLoads + S::LB::kLoads)
           lb.load(v - S::LA::kLoads, slot + S::TA::kBytes, wave, left, b_step, part);
+        else
+          scales.load<DIRECT>(slot + S::kScaleAt, wave, 1);
       },
       [&](unsigned char *slot) {
         la.store(slot, wave, lane);
         lb.store(slot + S::TA::kBytes, wave, lane);
+        if constexpr (kBlocks<Op>) scales.store(slot + S::kScaleAt, tid);
       });
 
   if constexpr (GATED) {
@@ -669,8 +755,11 @@ struct SkinnyShape {
   using FB = Fragments<Op, TB, BKC, FN>;
   using LA = Loader<Op, BM, true, 1, true>;
   using LB = Loader<Op, BN, BKC, 1, true>;
-  static constexpr int kSlot = TA::kBytes + TB::kBytes;
-  static constexpr int kLoads = LA::kLoads + LB::kLoads;
+  static constexpr int kRows = BM;
+  static constexpr int kScaleAt = TA::kBytes + TB::kBytes;
+  static_assert(!kBlocks<Op> || BM + BN <= 64, "a lane for each scale");
+  static constexpr int kSlot = TA::kBytes + TB::kBytes + (kBlocks<Op> ? 256 : 0);
+  static constexpr int kLoads = LA::kLoads + LB::kLoads + (kBlocks<Op> ? 1 : 0);
   static constexpr int kRing = NS * kSlot;
   static constexpr int kPart = BM * BN * 4;  // bytes of a wave's sums
   static constexpr int kLds = NW * (kRing > kPart ? kRing : kPart);
@@ -726,6 +815,8 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
       lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
+  ScaleLoader scales;
+  if constexpr (kBlocks<Op>) scales.init(g, r, S::BM, BN, n0, lane, wave);
   auto load = [&](int i) {
     unsigned char *slot = ring + i % NS * S::kSlot;
     const int left = g.k - (wave + i * NW) * kStep<Op>;
@@ -734,11 +825,14 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
 #pragma unroll
     for (int v = 0; v < S::LB::kLoads; ++v)
       lb.load(v, slot + S::TA::kBytes, 0, left, NW * b_step, true);
+    if constexpr (kBlocks<Op>) scales.load<true>(slot + S::kScaleAt, 0, NW);
   };
   typename S::FA fa;
   typename S::FB fb;
   fa.init(lds_address(ring), 0, lane);
   fb.init(lds_address(ring) + S::TA::kBytes, 0, lane);
+  ScalePlace place;
+  if constexpr (kBlocks<Op>) place.init(lds_address(ring) + S::kScaleAt, S::BM, 0, 0, lane);
   typename Op::acc acc[1][S::FN];
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) acc[0][j] = typename Op::acc{0, 0, 0, 0};
@@ -749,7 +843,8 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
     // once their matrix instructions have been issued
     if (i + NS - 1 < mine) load(i + NS - 1);
     wait_oldest<NS + 1, S::kLoads>(later < NS - 1 ? later : NS - 1);
-    stage_mma<Op, S>(acc, fa, fb, i % NS * S::kSlot);
+    if constexpr (kBlocks<Op>) stage_blocks<Op, S>(acc, fa, fb, place, i % NS * S::kSlot);
+    else stage_mma<Op, S>(acc, fa, fb, i % NS * S::kSlot);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 

@@ -501,7 +501,9 @@ Tensor run_product(const Tensor &x_, const Order &o, int64_t k, int64_t n, const
                    const Tensor &w_scale = Tensor()) {
   no_tangents(x_, o.w, x_scale, w_scale);
   const Tensor x = rows_of(x_);
-  const int code = x_scale.defined() ? EJ_I8 : code_of(x.scalar_type());
+  const int code = x.scalar_type() == at::kChar            ? EJ_I8
+                   : x.scalar_type() == at::kFloat8_e4m3fn ? EJ_E4M3
+                                                           : code_of(x.scalar_type());
   Launch on(x);
   Tensor out = at::empty({g.n_slots, n}, x.options().dtype(out_type));
   const ej_grouped_desc d =
@@ -792,56 +794,138 @@ py::tuple quantize_rows(py::handle x_) {
   return py::make_tuple(q, scale);
 }
 
-Tensor int8_matmul(py::handle q_, py::handle q_scale_, py::handle w_, py::handle w_scale_,
-                   py::handle offsets, py::handle rows, py::handle slots, bool gather,
-                   at::ScalarType out_type) {
-  const Tensor q = on_gpu(q_, "q");
-  Tensor q_scale = on_gpu_of(q, q_scale_, "q_scale"), w = on_gpu_of(q, w_, "w");
-  Tensor w_scale = on_gpu_of(q, w_scale_, "w_scale");
-  if (q.scalar_type() != at::kChar || w.scalar_type() != at::kChar)
-    throw py::type_error("q and w must be int8, got " + name_of(q.scalar_type()) + " and " +
-                         name_of(w.scalar_type()));
-  if (q_scale.scalar_type() != at::kFloat || w_scale.scalar_type() != at::kFloat)
-    throw py::type_error("scales must be float32, got " + name_of(q_scale.scalar_type()) +
-                         " and " + name_of(w_scale.scalar_type()));
+// What the products of 8-bit operands with scales check alike: q [m, k] and w
+// [groups, n, k] (or [n, k] without groups).
+struct Scaled {
+  Tensor q, q_scale, w, w_scale;
+  Groups g;
+  int64_t E, n, k;
+};
+
+Scaled scaled_args(py::handle q_, py::handle q_scale_, py::handle w_, py::handle w_scale_,
+                   bool dense, at::ScalarType out_type, at::ScalarType type,
+                   const char *type_name) {
+  Scaled a;
+  a.q = on_gpu(q_, "q");
+  a.q_scale = on_gpu_of(a.q, q_scale_, "q_scale");
+  a.w = on_gpu_of(a.q, w_, "w");
+  a.w_scale = on_gpu_of(a.q, w_scale_, "w_scale");
+  if (a.q.scalar_type() != type || a.w.scalar_type() != type)
+    throw py::type_error("q and w must be " + std::string(type_name) + ", got " +
+                         name_of(a.q.scalar_type()) + " and " + name_of(a.w.scalar_type()));
+  if (a.q_scale.scalar_type() != at::kFloat || a.w_scale.scalar_type() != at::kFloat)
+    throw py::type_error("scales must be float32, got " + name_of(a.q_scale.scalar_type()) +
+                         " and " + name_of(a.w_scale.scalar_type()));
   if (code_of(out_type) < 0)
     throw py::type_error("out_dtype must be float32, bfloat16 or float16, got " +
                          name_of(out_type));
-  if (q.dim() != 2) throw py::value_error("q must be [rows, k], got shape " + str(q.sizes()));
-  const bool dense = offsets.is_none();
-  if (dense && w.dim() == 2) {
-    w = w.unsqueeze(0);
-    w_scale = w_scale.unsqueeze(0);
+  if (a.q.dim() != 2) throw py::value_error("q must be [rows, k], got shape " + str(a.q.sizes()));
+  if (dense && a.w.dim() == 2) {
+    a.w = a.w.unsqueeze(0);
+    a.w_scale = a.w_scale.unsqueeze(0);
   }
-  if (w.dim() != 3)
+  if (a.w.dim() != 3)
     throw py::value_error("w must be [groups, n, k] (or [n, k] without groups), got shape " +
-                          str(w.sizes()));
-  const int64_t E = w.size(0), n = w.size(1), k = w.size(2);
-  if (q.size(1) != k)
-    throw py::value_error("q has rows of " + std::to_string(q.size(1)) + ", w of " +
-                          std::to_string(k));
-  if (q_scale.dim() != 1 || q_scale.size(0) != q.size(0) || w_scale.dim() != 2 ||
-      w_scale.size(0) != E || w_scale.size(1) != n)
-    throw py::value_error("scales have shapes " + str(q_scale.sizes()) + " and " +
-                          str(w_scale.sizes()) + ", expected " + str({q.size(0)}) + " and " +
-                          str({E, n}));
-  Groups g;
-  if (dense) {
-    if (gather || E != 1)
-      throw py::value_error("more than one weight matrix, or gather=True, needs groups");
-    g.n_slots = q.size(0);
-  } else {
-    g = groups_of(q, E, offsets, rows, slots, gather);
+                          str(a.w.sizes()));
+  a.E = a.w.size(0);
+  a.n = a.w.size(1);
+  a.k = a.w.size(2);
+  if (a.q.size(1) != a.k)
+    throw py::value_error("q has rows of " + std::to_string(a.q.size(1)) + ", w of " +
+                          std::to_string(a.k));
+  return a;
+}
+
+// groups None: one matrix for every row.
+void set_groups(Scaled *a, py::handle offsets, py::handle rows, py::handle slots, bool gather) {
+  if (!offsets.is_none()) {
+    a->g = groups_of(a->q, a->E, offsets, rows, slots, gather);
+    return;
   }
+  if (gather || a->E != 1)
+    throw py::value_error("more than one weight matrix, or gather=True, needs groups");
+  a->g.n_slots = a->q.size(0);
+}
+
+void check_scales(const Scaled &a, c10::IntArrayRef q_scale, c10::IntArrayRef w_scale) {
+  if (a.q_scale.sizes() != q_scale || a.w_scale.sizes() != w_scale)
+    throw py::value_error("scales have shapes " + str(a.q_scale.sizes()) + " and " +
+                          str(a.w_scale.sizes()) + ", expected " + str(q_scale) + " and " +
+                          str(w_scale));
+}
+
+Tensor run_scaled(const Scaled &a, at::ScalarType out_type) {
   // rows of k, as they lie where they can be read so
-  Order o{w, EJ_W_NK, E > 1 ? w.stride(0) : 0, n > 1 ? w.stride(1) : std::max<int64_t>(k, 1)};
-  if (E <= 1) o.group = n * o.row;
-  if (!((k <= 1 || w.stride(2) == 1) && o.row >= k && o.group >= n * o.row)) {
-    o.w = w.contiguous();
-    o.row = std::max<int64_t>(k, 1);
-    o.group = n * o.row;
+  Order o{a.w, EJ_W_NK, a.E > 1 ? a.w.stride(0) : 0,
+          a.n > 1 ? a.w.stride(1) : std::max<int64_t>(a.k, 1)};
+  if (a.E <= 1) o.group = a.n * o.row;
+  if (!((a.k <= 1 || a.w.stride(2) == 1) && o.row >= a.k && o.group >= a.n * o.row)) {
+    o.w = a.w.contiguous();
+    o.row = std::max<int64_t>(a.k, 1);
+    o.group = a.n * o.row;
   }
-  return run_product(q, o, k, n, g, out_type, q_scale.contiguous(), w_scale.contiguous());
+  return run_product(a.q, o, a.k, a.n, a.g, out_type, a.q_scale.contiguous(),
+                     a.w_scale.contiguous());
+}
+
+Tensor int8_matmul(py::handle q, py::handle q_scale, py::handle w, py::handle w_scale,
+                   py::handle offsets, py::handle rows, py::handle slots, bool gather,
+                   at::ScalarType out_type) {
+  Scaled a = scaled_args(q, q_scale, w, w_scale, offsets.is_none(), out_type, at::kChar, "int8");
+  check_scales(a, {a.q.size(0)}, {a.E, a.n});
+  set_groups(&a, offsets, rows, slots, gather);
+  return run_scaled(a, out_type);
+}
+
+// ---- 8-bit floats with block scales ---------------------------------------------------------
+
+constexpr at::ScalarType kE4m3 = at::kFloat8_e4m3fn;
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+py::tuple quantize_blocks(py::handle x_, int64_t block_rows) {
+  const Tensor given = on_gpu(x_, "x"), x = given.detach();
+  no_tangents(given);
+  const int code = value_code(x, "x");
+  if (block_rows != 1 && block_rows != 128)
+    throw py::value_error("block_rows must be 1 or 128, got " + std::to_string(block_rows));
+  const int64_t least = block_rows == 1 ? 1 : 2;
+  if (x.dim() < least)
+    throw py::value_error("x must have at least " + std::to_string(least) + " dimension" +
+                          (least > 1 ? "s" : "") + " for blocks of " +
+                          std::to_string(block_rows) + " rows, got shape " + str(x.sizes()));
+  const int64_t n = x.size(-1), rows = x.dim() > 1 ? x.size(-2) : 1;
+  int64_t mats = 1;
+  for (int64_t d = 0; d + 2 < x.dim(); ++d) mats *= x.size(d);
+  Tensor flat = x.dim() == 3 ? x : x.reshape({mats, rows, n});
+  // rows and matrices as they lie where they can be read so
+  auto lies = [&] {
+    return (n <= 1 || flat.stride(2) == 1) && (rows <= 1 || flat.stride(1) >= n) &&
+           (mats <= 1 || flat.stride(0) >= 0);
+  };
+  if (!lies()) flat = flat.contiguous();
+  const int64_t ld = rows > 1 ? flat.stride(1) : n, mat_ld = mats > 1 ? flat.stride(0) : 0;
+  Launch on(x);
+  Tensor q = at::empty(x.sizes(), x.options().dtype(kE4m3));
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = blocks_of(n);
+  if (block_rows == 128) shape[shape.size() - 2] = blocks_of(rows);
+  Tensor scale = at::empty(shape, x.options().dtype(at::kFloat));
+  check(ej_quantize_blocks(ptr(flat), code, mats, mat_ld, rows, ld, int32_of(n, "n"),
+                           static_cast<int32_t>(block_rows), static_cast<uint8_t *>(mut(q)),
+                           mut_floats(scale), on.stream),
+        "ej_quantize_blocks");
+  return py::make_tuple(q, scale);
+}
+
+Tensor fp8_matmul(py::handle q, py::handle q_scale, py::handle w, py::handle w_scale,
+                  py::handle offsets, py::handle rows, py::handle slots, bool gather,
+                  at::ScalarType out_type) {
+  Scaled a = scaled_args(q, q_scale, w, w_scale, offsets.is_none(), out_type, kE4m3,
+                         "float8_e4m3fn");
+  check_scales(a, {a.q.size(0), blocks_of(a.k)}, {a.E, blocks_of(a.n), blocks_of(a.k)});
+  set_groups(&a, offsets, rows, slots, gather);
+  return run_scaled(a, out_type);
 }
 
 }  // namespace
@@ -866,6 +950,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_matmul_vjp", &gated_matmul_vjp);
   m.def("quantize_rows", &quantize_rows);
   m.def("int8_matmul", &int8_matmul);
+  m.def("quantize_blocks", &quantize_blocks);
+  m.def("fp8_matmul", &fp8_matmul);
   m.def("rows_of", &rows_of);
   m.def("weight_order", [](const Tensor &w) {
     const Order o = weight_order(w);

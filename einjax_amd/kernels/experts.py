@@ -1,5 +1,5 @@
 """Expert operators on the GPU: the routing relation, and rows and products in
-8-bit integers.
+8-bit integers and 8-bit floating point.
 
 A mixture of experts is a relation between tokens and experts that every call
 makes anew: ``route_experts`` (or ``group_by_expert``, for picks that the caller
@@ -112,3 +112,47 @@ def int8_matmul(q, q_scale, w, w_scale, groups=None, *, gather: bool = False,
     offsets, rows, slots = group_args(groups)
     return _lib.experts().int8_matmul(q, q_scale, w, w_scale, offsets, rows, slots, gather,
                                       out_dtype)
+
+
+def quantize_blocks(x, *, block_rows: int = 1) -> tuple:
+    """x in 8-bit floating point (e4m3) with a scale for each block of 128:
+    (q float8_e4m3fn of x's shape, scale float32), x ~ q scale.
+
+    block_rows=1, for activations: x [..., n] has a scale for every 128 values
+    of a row, scale [..., ceil(n / 128)].  block_rows=128, for weights: x
+    [..., m, n] has one for every 128 x 128 block of a matrix, scale
+    [..., ceil(m / 128), ceil(n / 128)].  Blocks at the ends may be smaller.
+
+    scale = max |block| / 448, q = x / scale rounded to nearest (ties to even).
+    A block of zeros has scale 0; a block that holds a NaN or an infinity has
+    scale NaN, so that every product with it is NaN.
+    Not differentiable: q and scale are constants to torch.autograd."""
+    return _lib.experts().quantize_blocks(x, block_rows)
+
+
+def fp8_matmul(q, q_scale, w, w_scale, groups=None, *, gather: bool = False,
+               out_dtype: torch.dtype = torch.bfloat16):
+    """Product of rows and weights in 8-bit floating point with block scales.
+
+    q float8_e4m3fn [m, k] and q_scale float32 [m, ceil(k / 128)] are rows and
+    their scales (``quantize_blocks``); w float8_e4m3fn holds one row of k for
+    each output channel, w_scale float32 its scales
+    (``quantize_blocks(w, block_rows=128)``).  The sum of each block of 128 of k,
+    times the product of its two scales (formed in float32, whose range it must
+    not pass), is added up in float32 and rounded once to out_dtype (float32,
+    bfloat16 or float16).  For 16-bit results the 8-bit matrix instructions form
+    the blocks' sums: of 8 consecutive k they drop what lies below 2^-13 of the
+    largest product.  For float32 ones the sums are formed in float32, at half
+    the rate.
+
+    Without groups: w [n, k] or [1, n, k], w_scale [ceil(n / 128),
+    ceil(k / 128)] or with a leading 1, the dense product [m, n].  With groups
+    (an ``ExpertRouting`` or offsets [E + 1]): w [E, n, k], w_scale [E,
+    ceil(n / 128), ceil(k / 128)]; slot s of group e is q's row s, or with
+    ``gather`` the row of its token, times w[e]; zero in slots of no group.
+
+    Not differentiable, in the scales either: the result is a constant to
+    torch.autograd."""
+    offsets, rows, slots = group_args(groups)
+    return _lib.experts().fp8_matmul(q, q_scale, w, w_scale, offsets, rows, slots, gather,
+                                     out_dtype)

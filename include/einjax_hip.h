@@ -100,6 +100,7 @@ extern "C" {
 #define EJ_I64 4 /* ej_segment_sum */
 #define EJ_F16 5 /* ej_segment_sum and the expert operators */
 #define EJ_I8 6  /* ej_grouped_gemm with scales */
+#define EJ_E4M3 7  /* 8-bit floats (4 bits of exponent, 3 of mantissa, no infinities), the same */
 
 /* Pair orders of the join.  With n_keys == 0 both give the cross product in
  * lhs-major order (sparse_dispatch.py:53-59, pallas_gather.py:50-54). */
@@ -723,8 +724,9 @@ int ej_quantize_rows(const void *x, int32_t dtype, int64_t n_rows, int64_t ld, i
 #define EJ_W_KN 0
 #define EJ_W_NK 1
 typedef struct ej_grouped_desc {
-  int32_t dtype;      /* of x and w: EJ_F32, EJ_BF16, EJ_F16, or EJ_I8 (EJ_W_NK, k < 2^17) */
-  int32_t out_dtype;  /* of the result: EJ_F32, or the 16-bit dtype (EJ_I8: any) */
+  int32_t dtype;      /* of x and w: EJ_F32, EJ_BF16, EJ_F16, EJ_I8 (EJ_W_NK, k < 2^17) or
+                         EJ_E4M3 (EJ_W_NK) */
+  int32_t out_dtype;  /* of the result: EJ_F32, or the 16-bit dtype (EJ_I8, EJ_E4M3: any) */
   int32_t w_order;
   int32_t n_groups;
   int32_t k, n;
@@ -742,7 +744,13 @@ typedef struct ej_grouped_desc {
  * never an access outside the operands; NULL with n_groups == 1: one group of
  * every slot.  EJ_I8: x_scale [n_rows] and w_scale
  * [n_groups][n], out = x_scale w_scale (exact integer sum), also where the
- * scales' own product passes fp32's range; NULL otherwise.
+ * scales' own product passes fp32's range.  EJ_E4M3: x_scale [n_rows][kb] and
+ * w_scale [n_groups][nb][kb], kb = ceil(k / 128) and nb = ceil(n / 128), are the
+ * scales of 1 x 128 blocks of x and 128 x 128 blocks of w; each block's sum times
+ * the fp32 product of its two scales is added up in fp32.  The blocks' sums are
+ * in fp32 for an EJ_F32 result; for 16-bit ones the 8-bit matrix instructions
+ * drop, of 8 consecutive k, what lies below 2^-13 of the largest product.  Scales
+ * are NULL otherwise.
  * The workspace (NULL where its size is 0) holds the sums of a contraction that
  * is split to cover the CUs; they are added in a fixed order. */
 int ej_grouped_gemm_workspace_size(const ej_grouped_desc *desc, size_t *bytes);
@@ -760,6 +768,17 @@ int ej_grouped_gemm_dw_workspace_size(const ej_grouped_desc *desc, size_t *bytes
 int ej_grouped_gemm_dw(const ej_grouped_desc *desc, const void *x, const int32_t *rows,
                        const int32_t *offsets, const void *grad, void *grad_w, void *workspace,
                        size_t workspace_bytes, ej_stream_t stream);
+
+/* x [n_mats][n_rows][n] in EJ_F32, EJ_BF16 or EJ_F16 as e4m3 values q of the
+ * same shape (contiguous) with a scale for each block of block_rows (1 or 128)
+ * rows and 128 columns: scale [n_mats][ceil(n_rows / block_rows)][ceil(n / 128)].
+ * scale = max |block| times fp32's 1 / 448, q = x / scale rounded to nearest
+ * (ties to even; a subnormal scale's quotients are cut off at 448).  A block of
+ * zeros has scale 0; one with a NaN or an infinity has scale NaN, and q 0.  Rows
+ * are ld apart, matrices mat_ld. */
+int ej_quantize_blocks(const void *x, int32_t dtype, int64_t n_mats, int64_t mat_ld,
+                       int64_t n_rows, int64_t ld, int32_t n, int32_t block_rows, uint8_t *q,
+                       float *scale, ej_stream_t stream);
 
 /* Gated products: with G | U = x[rows[s]] W_e, out[s] = act(G) U.  W holds 2 n
  * columns, the gate's n first (EJ_W_KN: rows of 2 n; EJ_W_NK: 2 n rows); the

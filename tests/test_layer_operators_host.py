@@ -82,3 +82,50 @@ def test_operands_must_be_on_the_gpu():
                  lambda: ej.gated_matmul_vjp(t, t, None, t)):
         with pytest.raises(TypeError, match="on the GPU"):
             call()
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(w_order=_lib.EJ_W_KN, w_stride=64), INVAL), (dict(out_dtype=_lib.EJ_E4M3), INVAL),
+    (dict(out_dtype=_lib.EJ_I8), INVAL), (dict(x_stride=63), INVAL), (dict(w_stride=63), INVAL),
+])
+def test_block_product_refusals(change, status):
+    d = desc(**{**dict(dtype=_lib.EJ_E4M3, w_order=_lib.EJ_W_NK, w_stride=64), **change})
+    lib = _lib.load()
+    args = (ctypes.byref(d), FAKE, None, FAKE, FAKE)
+    assert lib.ej_grouped_gemm(*args, FAKE, FAKE, FAKE, None, 0, None) == status
+    assert lib.ej_last_error()
+
+
+def test_block_product_arguments():
+    lib, n = _lib.load(), ctypes.c_size_t()
+    d = desc(dtype=_lib.EJ_E4M3, w_order=_lib.EJ_W_NK, w_stride=64)
+    args = (ctypes.byref(d), FAKE, None, FAKE, FAKE)
+    assert lib.ej_grouped_gemm(*args, None, FAKE, FAKE, None, 0, None) == INVAL
+    assert lib.ej_grouped_gemm(*args, FAKE, None, FAKE, None, 0, None) == INVAL
+    assert lib.ej_grouped_gemm_dw(*args, FAKE, None, 0, None) == INVAL
+    assert lib.ej_grouped_gemm_workspace_size(ctypes.byref(d), ctypes.byref(n)) == 0
+
+
+def test_quantize_blocks_arguments():
+    def quantize(x=FAKE, dtype=_lib.EJ_BF16, mats=1, rows=4, ld=8, n=8, block=1, q=FAKE, s=FAKE):
+        return _lib.load().ej_quantize_blocks(x, dtype, mats, 0, rows, ld, n, block, q, s, None)
+
+    assert quantize(dtype=_lib.EJ_I8) == INVAL
+    assert quantize(block=64) == INVAL
+    assert quantize(ld=7) == INVAL
+    assert quantize(rows=-1) == INVAL and quantize(mats=-1) == INVAL and quantize(n=-1) == INVAL
+    assert quantize(x=None) == INVAL and quantize(q=None) == INVAL and quantize(s=None) == INVAL
+    for empty in (dict(rows=0), dict(mats=0), dict(n=0)):
+        assert quantize(x=None, q=None, s=None, **empty) == 0
+    for large in (dict(rows=1 << 40), dict(mats=1 << 62), dict(mats=1 << 20, rows=1 << 20),
+                  dict(mats=1 << 40, rows=1 << 40), dict(rows=1 << 31, block=128),
+                  dict(n=(1 << 31) - 1, ld=1 << 31)):
+        assert quantize(**large) == UNSUPPORTED
+
+
+def test_8_bit_operands_must_be_on_the_gpu():
+    t = torch.zeros(4, 128)
+    q, s = t.to(torch.float8_e4m3fn), torch.zeros(4, 1)
+    for call in (lambda: ej.quantize_blocks(t), lambda: ej.fp8_matmul(q, s, q, s[:1])):
+        with pytest.raises(TypeError, match="on the GPU"):
+            call()
