@@ -14,6 +14,8 @@ libejhip.so (HIP kernels behind a C ABI, include/einjax_hip.h).
 from .autodiff import (
     combine_experts,
     combine_experts_vjp,
+    embed_tokens,
+    embed_tokens_vjp,
     gated_matmul,
     gated_matmul_vjp,
     grouped_matmul,
@@ -92,4 +94,5 @@ __all__ = [
     "grouped_matmul_vjp", "gated_matmul", "gated_matmul_vjp", "combine_experts",
     "combine_experts_vjp", "quantize_rows",
     "int8_matmul", "quantize_blocks", "fp8_matmul",
+    "embed_tokens", "embed_tokens_vjp",
 ]

@@ -177,6 +177,10 @@ SIGNATURES = {
     "ej_gated_gemm_workspace_size": (_i32, [ctypes.POINTER(GroupedDesc), _P_sz]),
     "ej_gated_gemm": (_i32, [ctypes.POINTER(GroupedDesc), _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                              _sz, _vp]),
+    "ej_embed": (_i32, [_vp, _i32, _i64, _i64, _i32, _vp, _i32, _i64, ctypes.c_float, _vp, _vp]),
+    "ej_embed_vjp_workspace_size": (_i32, [_i64, _i64, _i32, _P_sz]),
+    "ej_embed_vjp": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i32, ctypes.c_float, _vp, _vp,
+                            _sz, _vp]),
     "ej_gated_vjp": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _i32, _vp, _vp]),
 }
 

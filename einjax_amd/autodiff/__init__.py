@@ -17,7 +17,9 @@ from .experts import (
     route_experts,
     route_experts_vjp,
 )
+from .tokens import embed_tokens, embed_tokens_vjp
 
 __all__ = ["sparse_einsum", "sparse_einsum_raw", "sparse_einsum_raw_vjp", "route_experts",
            "route_experts_vjp", "grouped_matmul", "grouped_matmul_vjp", "gated_matmul",
-           "gated_matmul_vjp", "combine_experts", "combine_experts_vjp"]
+           "gated_matmul_vjp", "combine_experts", "combine_experts_vjp", "embed_tokens",
+           "embed_tokens_vjp"]

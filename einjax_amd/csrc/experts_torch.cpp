@@ -928,6 +928,96 @@ Tensor fp8_matmul(py::handle q, py::handle q_scale, py::handle w, py::handle w_s
   return run_scaled(a, out_type);
 }
 
+// ---- rows of a table for tokens ----------------------------------------------------------------
+
+Tensor run_embed(const Tensor &tokens, const Tensor &table_, double scale) {
+  no_tangents(table_);
+  const Tensor table = rows_of(table_);
+  const int64_t n = table.size(1);
+  Launch on(table);
+  std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+  shape.push_back(n);
+  Tensor out = at::empty(shape, table.options());
+  check(ej_embed(ptr(table), code_of(table.scalar_type()), table.size(0),
+                 std::max(row_stride(table), n), int32_of(n, "n"), ptr(tokens),
+                 tokens.scalar_type() == at::kInt ? EJ_I32 : EJ_I64, tokens.numel(),
+                 static_cast<float>(scale), mut(out), on.stream),
+        "ej_embed");
+  return out;
+}
+
+// grad [tokens..., n], in the table's type.
+Tensor run_embed_vjp(const Tensor &tokens, int64_t n_rows, const Tensor &grad_, double scale) {
+  at::NoGradGuard no_grad;
+  no_tangents(grad_);
+  const int64_t n = grad_.size(-1), count = tokens.numel();
+  const Tensor grad = rows_of(grad_.dim() == 2 ? grad_ : grad_.reshape({count, n}));
+  Launch on(grad);
+  Tensor out = at::empty({n_rows, n}, grad.options());
+  size_t bytes;
+  check(ej_embed_vjp_workspace_size(count, n_rows, int32_of(n, "n"), &bytes),
+        "ej_embed_vjp_workspace_size");
+  const Tensor ws = workspace(grad, bytes);
+  check(ej_embed_vjp(ptr(tokens), tokens.scalar_type() == at::kInt ? EJ_I32 : EJ_I64, count,
+                     ptr(grad), code_of(grad.scalar_type()), std::max(row_stride(grad), n), n_rows,
+                     static_cast<int32_t>(n), static_cast<float>(scale), mut(out), mut(ws), bytes,
+                     on.stream),
+        "ej_embed_vjp");
+  return out;
+}
+
+struct EmbedFunction : public Function<EmbedFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &table, const Tensor &tokens,
+                        double scale) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["n_rows"] = table.size(0);
+    ctx->saved_data["type"] = static_cast<int64_t>(table.scalar_type());
+    ctx->saved_data["scale"] = scale;
+    return run_embed(tokens, table, scale);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+    Tensor g = run_embed_vjp(s[0], ctx->saved_data["n_rows"].toInt(), grads[0].to(type),
+                             ctx->saved_data["scale"].toDouble());
+    return first_order({g, Tensor(), Tensor()});
+  }
+};
+
+struct EmbedArgs {
+  Tensor tokens, table;
+};
+
+EmbedArgs embed_args(py::handle tokens_, py::handle table_) {
+  EmbedArgs a;
+  a.table = on_gpu(table_, "table");
+  a.tokens = on_gpu_of(a.table, tokens_, "tokens");
+  value_code(a.table, "table");
+  if (a.table.dim() != 2)
+    throw py::value_error("table must be [rows, n], got shape " + str(a.table.sizes()));
+  if (a.tokens.scalar_type() != at::kInt && a.tokens.scalar_type() != at::kLong)
+    throw py::type_error("tokens must be int32 or int64, got " + name_of(a.tokens.scalar_type()));
+  a.tokens = a.tokens.contiguous();
+  return a;
+}
+
+Tensor embed_tokens(py::handle tokens, py::handle table, double scale) {
+  const EmbedArgs a = embed_args(tokens, table);
+  if (!wants_grad(a.table)) return run_embed(a.tokens, a.table, scale);
+  return EmbedFunction::apply(a.table, a.tokens, scale);
+}
+
+Tensor embed_tokens_vjp(py::handle tokens, py::handle table, py::handle grad_, double scale) {
+  const EmbedArgs a = embed_args(tokens, table);
+  const Tensor grad = on_gpu_of(a.table, grad_, "grad_out");
+  std::vector<int64_t> want(a.tokens.sizes().begin(), a.tokens.sizes().end());
+  want.push_back(a.table.size(1));
+  if (grad.sizes() != c10::IntArrayRef(want))
+    throw py::value_error("grad_out has shape " + str(grad.sizes()) + ", expected " + str(want));
+  at::NoGradGuard no_grad;
+  return run_embed_vjp(a.tokens, a.table.size(0), grad.to(a.table.scalar_type()), scale);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -952,6 +1042,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_matmul", &int8_matmul);
   m.def("quantize_blocks", &quantize_blocks);
   m.def("fp8_matmul", &fp8_matmul);
+  m.def("embed_tokens", &embed_tokens);
+  m.def("embed_tokens_vjp", &embed_tokens_vjp);
   m.def("rows_of", &rows_of);
   m.def("weight_order", [](const Tensor &w) {
     const Order o = weight_order(w);

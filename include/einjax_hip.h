@@ -42,7 +42,9 @@
  *                 relation of tokens and experts), ej_grouped_gemm /
  *                 ej_grouped_gemm_dw (products grouped by expert),
  *                 ej_expert_combine / ej_expert_combine_vjp (back to tokens),
- *                 ej_quantize_rows (8-bit rows for ej_grouped_gemm)
+ *                 ej_gated_gemm / ej_gated_vjp (gate and up projection in one),
+ *                 ej_quantize_rows / ej_quantize_blocks (8-bit operands for
+ *                 ej_grouped_gemm), ej_embed / ej_embed_vjp (tokens' rows)
  *                 (no counterpart in the reference)
  *
  * Conventions
@@ -803,6 +805,23 @@ int ej_gated_gemm(const ej_grouped_desc *desc, int32_t activation, const void *x
  * ej_grouped_gemm's of a product with 2 n columns whose gradient this is. */
 int ej_gated_vjp(const float *gate_up, const void *grad, int32_t dtype, int64_t n_rows, int32_t n,
                  int64_t grad_stride, int32_t activation, void *out, ej_stream_t stream);
+
+/* out[t] = scale table[tokens[t]]: rows of a table [n_rows][n] (EJ_F32, EJ_BF16
+ * or EJ_F16), ld apart, for tokens of EJ_I32 or EJ_I64, times scale in fp32 and
+ * rounded once; out [n_tokens][n].  A token outside [0, n_rows) gets zeros. */
+int ej_embed(const void *table, int32_t dtype, int64_t n_rows, int64_t ld, int32_t n,
+             const void *tokens, int32_t token_dtype, int64_t n_tokens, float scale, void *out,
+             ej_stream_t stream);
+
+/* Its gradient to the table: grad_table[v] = scale times the sum of grad[t] over
+ * the tokens t of row v, in fp32 in an order that the tokens alone set, rounded
+ * once; zeros for rows without tokens.  grad [n_tokens][n], rows grad_ld apart,
+ * and grad_table [n_rows][n] of `dtype`.  Tokens outside the table are left out.
+ * The workspace holds the sorted tokens and the parts of long sums. */
+int ej_embed_vjp_workspace_size(int64_t n_tokens, int64_t n_rows, int32_t n, size_t *bytes);
+int ej_embed_vjp(const void *tokens, int32_t token_dtype, int64_t n_tokens, const void *grad,
+                 int32_t dtype, int64_t grad_ld, int64_t n_rows, int32_t n, float scale,
+                 void *grad_table, void *workspace, size_t workspace_bytes, ej_stream_t stream);
 
 #ifdef __cplusplus
 }

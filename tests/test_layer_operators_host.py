@@ -129,3 +129,44 @@ def test_8_bit_operands_must_be_on_the_gpu():
     for call in (lambda: ej.quantize_blocks(t), lambda: ej.fp8_matmul(q, s, q, s[:1])):
         with pytest.raises(TypeError, match="on the GPU"):
             call()
+
+
+def test_embed_arguments():
+    lib, n = _lib.load(), ctypes.c_size_t()
+
+    def embed(table=FAKE, dtype=_lib.EJ_BF16, rows=9, ld=8, n=8, tokens=FAKE, kind=_lib.EJ_I64,
+              t=4, out=FAKE):
+        return lib.ej_embed(table, dtype, rows, ld, n, tokens, kind, t, 1.0, out, None)
+
+    def vjp(tokens=FAKE, kind=_lib.EJ_I64, t=4, grad=FAKE, dtype=_lib.EJ_BF16, ld=8, rows=9, n=8,
+            out=FAKE, ws=FAKE, size=1 << 20):
+        return lib.ej_embed_vjp(tokens, kind, t, grad, dtype, ld, rows, n, 1.0, out, ws, size,
+                                None)
+
+    for call in (embed, vjp):
+        assert call(dtype=_lib.EJ_I32) == INVAL and call(kind=_lib.EJ_F32) == INVAL
+        assert call(ld=7) == INVAL
+        assert call(t=-1) == INVAL and call(rows=-1) == INVAL and call(n=-1) == INVAL
+        assert call(tokens=None) == INVAL and call(out=None) == INVAL
+        assert call(rows=1 << 31) == UNSUPPORTED and call(t=1 << 31) == UNSUPPORTED
+        assert call(n=(1 << 31) - 1, ld=1 << 31) == UNSUPPORTED
+        assert call(n=0, ld=0, tokens=None, out=None) == 0
+    assert embed(table=None) == INVAL and vjp(grad=None) == INVAL
+    assert embed(t=0, tokens=None, out=None, table=None) == 0
+    assert vjp(rows=0, tokens=None, grad=None, out=None, ws=None, size=0) == 0
+    assert vjp(ws=None) == INVAL and vjp(size=1) == INVAL
+    assert b"workspace" in lib.ej_last_error()
+    # keys, places and the parts of long sums; above 16384 tokens the sort's room
+    sizes = []
+    for t in (0, 1, 16384, 16385):
+        assert lib.ej_embed_vjp_workspace_size(t, 9, 8, ctypes.byref(n)) == 0
+        sizes.append(n.value)
+    assert sizes[0] == 0 and 0 < sizes[1] < sizes[2] < sizes[3] - 16 * 16384
+    assert lib.ej_embed_vjp_workspace_size(4, 9, 8, None) == INVAL
+
+
+def test_tokens_must_be_on_the_gpu():
+    t, i = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: ej.embed_tokens(i, t), lambda: ej.embed_tokens_vjp(i, t, t)):
+        with pytest.raises(TypeError, match="on the GPU"):
+            call()
