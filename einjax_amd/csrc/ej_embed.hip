@@ -20,29 +20,24 @@ constexpr int kMaxBlocks = (1 << 24) - 1;  // of 256 threads in a launch
 template <class T>
 constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
 
-// A 16-byte piece of a row, anywhere in it; `there` of its values exist.
-template <class T>
+// N values of a row, from any element on.  A row is covered by whole pieces: the
+// last one begins N before its end, and what it shares with the one before is
+// computed twice.  (A branch for a short piece would have every load waited for
+// before the next one.)  Rows of fewer than 16 bytes go by single values.
+template <class T, int N>
 struct Piece {
-  T e[kPiece<T>];
-  __device__ inline void load(const T *p, int there) {
-    if (there >= kPiece<T>) {
-      __builtin_memcpy(e, __builtin_assume_aligned(p, alignof(T)), 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPiece<T>; ++i)
-        if (i < there) e[i] = p[i];
-    }
+  T e[N];
+  __device__ inline void load(const T *p) {
+    __builtin_memcpy(e, __builtin_assume_aligned(p, alignof(T)), sizeof(e));
   }
-  __device__ inline void store(T *p, int there) const {
-    if (there >= kPiece<T>) {
-      __builtin_memcpy(__builtin_assume_aligned(p, alignof(T)), e, 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPiece<T>; ++i)
-        if (i < there) p[i] = e[i];
-    }
+  __device__ inline void store(T *p) const {
+    __builtin_memcpy(__builtin_assume_aligned(p, alignof(T)), e, sizeof(e));
   }
 };
+template <int N>
+__device__ inline int32_t piece_at(int32_t col, int32_t n) {
+  return col <= n - N ? col : n - N;
+}
 
 // The row of a token, n_rows for those outside the table.
 __device__ inline uint32_t row_of(int64_t token, uint32_t n_rows) {
@@ -58,89 +53,162 @@ inline int row_threads(int64_t pieces) {
 
 // ---- the lookup -------------------------------------------------------------
 
-template <class T, class Token>
+// A thread takes one piece of R tokens' rows at a time, so that R rows are under
+// way together.
+template <class T, class Token, int N, int R>
 __global__ __launch_bounds__(kThreads) void embed_kernel(const T *table, uint32_t n_rows,
                                                          int64_t ld, int32_t n,
                                                          const Token *tokens, int64_t n_tokens,
                                                          float scale, int32_t across, T *out) {
-  constexpr int N = kPiece<T>;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / across) + threadIdx.x / across;
-  if (t >= n_tokens) return;
-  const uint32_t row = row_of(tokens[t], n_rows);
-  const bool held = row < n_rows;
-  const T *src = table + (held ? row : 0) * ld;
-  T *dst = out + t * n;
-#pragma unroll 2
-  for (int32_t c = (threadIdx.x & (across - 1)) * N; c < n; c += across * N) {
-    Piece<T> v;
-    if (held) v.load(src + c, n - c);
+  const int64_t step = kThreads / across;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * step * R + threadIdx.x / across;
+  uint32_t row[R];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      v.e[i] = held ? static_cast<T>(static_cast<float>(v.e[i]) * scale) : static_cast<T>(0.f);
-    v.store(dst + c, n - c);
+  for (int r = 0; r < R; ++r) {
+    const int64_t t = t0 + r * step;
+    row[r] = row_of(tokens[t < n_tokens ? t : n_tokens - 1], n_rows);
+  }
+  for (int32_t c = (threadIdx.x & (across - 1)) * N; c < n; c += across * N) {
+    const int32_t col = piece_at<N>(c, n);
+    Piece<T, N> v[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)  // row 0 for those outside: a table has one (n_rows 0: none is read)
+      if (n_rows) v[r].load(table + (row[r] < n_rows ? row[r] : 0) * ld + col);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t t = t0 + r * step;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[r].e[i] = row[r] < n_rows ? static_cast<T>(static_cast<float>(v[r].e[i]) * scale)
+                                    : static_cast<T>(0.f);
+      if (t < n_tokens) v[r].store(out + t * n + col);
+    }
   }
 }
 
 // ---- the order of the tokens -------------------------------------------------
 
-// Zeros, 16 bytes a thread: the workgroups of a launch from `first` on.
+// Zeros, 16 bytes a thread at a time: by the workgroups of a launch from `first` on.
 template <class T>
 __device__ inline void fill_zero(T *p, int64_t count, uint32_t first) {
   constexpr int N = kPiece<T>;
   const int64_t threads = static_cast<int64_t>(gridDim.x - first) * blockDim.x;
-  Piece<T> zero;
+  const int64_t mine = static_cast<int64_t>(blockIdx.x - first) * blockDim.x + threadIdx.x;
+  Piece<T, N> zero;
 #pragma unroll
   for (int i = 0; i < N; ++i) zero.e[i] = static_cast<T>(0.f);
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x - first) * blockDim.x + threadIdx.x) * N;
-       i < count; i += threads * N)
-    zero.store(p + i, count - i < N ? static_cast<int>(count - i) : N);
+  for (int64_t i = mine; i < count / N; i += threads) zero.store(p + i * N);
+  if (mine < count % N) p[count / N * N + mine] = static_cast<T>(0.f);
 }
 
-// Few tokens: each token's place is the number of tokens before it, by
-// comparison with every other one, in one launch.  A workgroup places 64 tokens,
-// one a lane; its 16 waves share out the tokens to compare with, which are
-// uniform and come through the scalar cache.  The workgroups behind those clear
-// the gradient meanwhile.
-constexpr int kRankWaves = 16;
-constexpr int64_t kRankTokens = 16384;
+// Few tokens: one workgroup sorts them in LDS, digit by digit, in one launch; the
+// workgroups behind it clear the gradient meanwhile.  Each of its 16 waves takes
+// a run of the sequence, 64 tokens at a time.  A pass counts every wave's digits,
+// scans the counts by digit and then by wave, and places the tokens in order:
+// those of a 64 with the same digit know each other by ballots of its bits.
+constexpr int kSortWaves = 16, kSortThreads = kSortWaves * 64;
+constexpr int kSortBits = 8, kSortDigits = 1 << kSortBits;
+constexpr int kSortTokens = 16384, kSortRows = kSortTokens / kSortThreads;
 
 template <class T, class Token>
-__global__ __launch_bounds__(kRankWaves * 64) void rank_kernel(
-    const Token *tokens, int32_t n_tokens, uint32_t n_rows, uint32_t *keys, int32_t *perm,
-    uint32_t rank_blocks, T *clear, int64_t clear_count) {
-  if (blockIdx.x >= rank_blocks) {
-    fill_zero(clear, clear_count, rank_blocks);
+__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(const Token *tokens,
+                                                                int32_t n_tokens, uint32_t n_rows,
+                                                                int32_t bits, uint32_t *keys,
+                                                                int32_t *perm, T *clear,
+                                                                int64_t clear_count) {
+  if (blockIdx.x > 0) {
+    fill_zero(clear, clear_count, 1);
     return;
   }
-  __shared__ int32_t counts[kRankWaves][64];
+  __shared__ uint32_t key_of[kSortTokens];
+  __shared__ uint16_t token_of[kSortTokens];
+  __shared__ int32_t place[kSortDigits * kSortWaves];
+  __shared__ int32_t wave_sum[kSortWaves];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int32_t first = blockIdx.x * 64, i = first + lane;
-  const uint32_t mine = i < n_tokens ? row_of(tokens[i], n_rows) : n_rows;
-  const auto *all = (const __attribute__((address_space(4))) Token *)(tokens);
-  const int32_t per = (n_tokens + kRankWaves - 1) / kRankWaves;
-  const int32_t lo = wave * per, hi = lo + per < n_tokens ? lo + per : n_tokens;
-  int32_t count = 0;
-  auto span = [&](int32_t a, int32_t b, uint32_t below) {
-    int32_t j = a;
-    for (; j + 16 <= b; j += 16)
+  // rows of 64 tokens for each wave
+  const int rows = (n_tokens + kSortThreads - 1) / kSortThreads;
+  const int32_t first = wave * rows * 64 + lane;
+  uint32_t key[kSortRows];
+  uint16_t token[kSortRows];
 #pragma unroll
-      for (int u = 0; u < 16; ++u) count += row_of(all[j + u], n_rows) < below;
-    for (; j < b; ++j) count += row_of(all[j], n_rows) < below;
-  };
-  // tokens before this workgroup's, equal ones counted; its own; those behind
-  span(lo, hi < first ? hi : first, mine + 1);
-  for (int32_t j = lo > first ? lo : first; j < hi && j < first + 64; ++j)
-    count += row_of(all[j], n_rows) < mine + (j < i ? 1 : 0);
-  span(lo > first + 64 ? lo : first + 64, hi, mine);
-  counts[wave][lane] = count;
-  __syncthreads();
-  if (wave == 0 && i < n_tokens) {
-    int32_t place = 0;
+  for (int r = 0; r < kSortRows; ++r) {
+    const int32_t i = first + r * 64;
+    if (r < rows && i < n_tokens) {
+      key[r] = row_of(tokens[i], n_rows);
+      token[r] = static_cast<uint16_t>(i);
+    }
+  }
+  for (int shift = 0; shift < bits; shift += kSortBits) {
+    if (shift > 0) {
 #pragma unroll
-    for (int w = 0; w < kRankWaves; ++w) place += counts[w][lane];
-    keys[place] = mine;
-    perm[place] = i;
+      for (int r = 0; r < kSortRows; ++r) {
+        const int32_t i = first + r * 64;
+        if (r < rows && i < n_tokens) {
+          key[r] = key_of[i];
+          token[r] = token_of[i];
+        }
+      }
+    }
+    for (int i = threadIdx.x; i < kSortDigits * kSortWaves; i += kSortThreads) place[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRows; ++r)
+      if (r < rows && first + r * 64 < n_tokens)
+        atomicAdd(&place[(key[r] >> shift & (kSortDigits - 1)) * kSortWaves + wave], 1);
+    __syncthreads();
+    // exclusive scan: four counts a thread
+    constexpr int kEach = kSortDigits * kSortWaves / kSortThreads;
+    int32_t v[kEach], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      v[i] = place[threadIdx.x * kEach + i];
+      mine += v[i];
+    }
+    int32_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int32_t below = __shfl_up(upto, d);
+      upto += lane >= d ? below : 0;
+    }
+    if (lane == 63) wave_sum[wave] = upto;
+    __syncthreads();
+    int32_t before = upto - mine;
+    for (int w = 0; w < wave; ++w) before += wave_sum[w];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      place[threadIdx.x * kEach + i] = before;
+      before += v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRows; ++r) {
+      if (r >= rows) break;
+      const bool there = first + r * 64 < n_tokens;
+      const uint32_t digit = key[r] >> shift & (kSortDigits - 1);
+      uint64_t same = __ballot(there);
+#pragma unroll
+      for (int b = 0; b < kSortBits; ++b) {
+        const uint64_t set = __ballot(digit >> b & 1);
+        same &= digit >> b & 1 ? set : ~set;
+      }
+      const int rank = __popcll(same & ((uint64_t{1} << lane) - 1));
+      int32_t *at = &place[digit * kSortWaves + wave];
+      const int32_t base = there ? *at : 0;
+      // every lane has read before the first of each digit moves it on
+      __builtin_amdgcn_wave_barrier();
+      if (there && rank == 0) *at = base + __popcll(same);
+      __builtin_amdgcn_wave_barrier();
+      if (there) {
+        key_of[base + rank] = key[r];
+        token_of[base + rank] = token[r];
+      }
+    }
+    __syncthreads();
+  }
+  for (int32_t i = threadIdx.x; i < n_tokens; i += kSortThreads) {
+    keys[i] = key_of[i];
+    perm[i] = token_of[i];
   }
 }
 
@@ -168,7 +236,8 @@ __global__ __launch_bounds__(kThreads) void narrow_keys_kernel(const uint64_t *f
 
 // ---- the sums -----------------------------------------------------------------
 
-// The sorted tokens in chunks of equal length.  A row whose tokens lie in one
+// The sorted tokens in chunks of equal length, so that a few tokens that make up
+// most of a batch do not leave the rest waiting.  A row whose tokens lie in one
 // chunk is written at once; of one that spans several, each chunk leaves its
 // part in fp32: `head` where the row began in an earlier chunk, `tail` where it
 // began in this one.
@@ -184,66 +253,58 @@ struct Sums {
   __device__ inline float *part(int64_t c, int tail) const { return parts + (c * 2 + tail) * n; }
 };
 
-template <class T>
+template <class T, int N>
 __device__ inline void put_row(const Sums &s, T *out, uint32_t row, int32_t col,
-                               const float (&sum)[kPiece<T>]) {
-  Piece<T> v;
+                               const float (&sum)[N]) {
+  Piece<T, N> v;
 #pragma unroll
-  for (int i = 0; i < kPiece<T>; ++i) v.e[i] = static_cast<T>(s.scale * sum[i]);
-  v.store(out + static_cast<int64_t>(row) * s.n + col, s.n - col);
+  for (int i = 0; i < N; ++i) v.e[i] = static_cast<T>(s.scale * sum[i]);
+  v.store(out + static_cast<int64_t>(row) * s.n + col);
 }
 
 template <int N>
-__device__ inline void put_part(float *p, int there, const float (&sum)[N]) {
-  if (there >= N) {
-    __builtin_memcpy(__builtin_assume_aligned(p, 4), sum, sizeof(sum));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < there) p[i] = sum[i];
-  }
-}
-template <int N>
-__device__ inline void add_part(const float *p, int there, float (&sum)[N]) {
-  float v[N] = {};
-  if (there >= N) {
-    __builtin_memcpy(v, __builtin_assume_aligned(p, 4), sizeof(v));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < there) v[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) sum[i] += v[i];
+__device__ inline void put_part(float *p, const float (&sum)[N]) {
+  __builtin_memcpy(__builtin_assume_aligned(p, 4), sum, sizeof(sum));
 }
 
-template <class T>
+template <class T, int N>
 __global__ __launch_bounds__(kThreads) void sum_chunks_kernel(Sums s, const T *grad, T *out) {
-  constexpr int N = kPiece<T>, kAhead = 8;
+  constexpr int kAhead = 8;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * (kThreads / s.across) +
                     threadIdx.x / s.across;
-  const int32_t col = (blockIdx.y * s.across + (threadIdx.x & (s.across - 1))) * N;
+  const int32_t first = (blockIdx.y * s.across + (threadIdx.x & (s.across - 1))) * N;
   const int64_t p0 = c * s.chunk;
-  if (p0 >= s.n_tokens || col >= s.n) return;
+  if (p0 >= s.n_tokens || first >= s.n) return;
+  const int32_t col = piece_at<N>(first, s.n);
   const int32_t p1 = p0 + s.chunk < s.n_tokens ? static_cast<int32_t>(p0) + s.chunk : s.n_tokens;
-  const int there = s.n - col;
   uint32_t row = s.keys[p0];
   bool head = p0 > 0 && s.keys[p0 - 1] == row;
   float sum[N] = {};
   auto finish = [&](bool goes_on) {
     if (row >= s.n_rows) return;
-    if (head) put_part(s.part(c, 0) + col, there, sum);
-    else if (goes_on) put_part(s.part(c, 1) + col, there, sum);
+    if (head) put_part(s.part(c, 0) + col, sum);
+    else if (goes_on) put_part(s.part(c, 1) + col, sum);
     else put_row(s, out, row, col, sum);
   };
-  for (int32_t p = static_cast<int32_t>(p0); p < p1; p += kAhead) {
-    uint32_t key[kAhead];
-    Piece<T> v[kAhead];
+  uint32_t key[kAhead], key_next[kAhead];
+  int32_t from_next[kAhead];
+  auto places = [&](int32_t p, uint32_t(&k)[kAhead], int32_t(&f)[kAhead]) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      key[u] = p + u < p1 ? s.keys[p + u] : s.n_rows;
-      if (key[u] < s.n_rows) v[u].load(grad + s.perm[p + u] * s.ld + col, there);
+      const int32_t at = p + u < p1 ? p + u : p1 - 1;
+      k[u] = s.keys[at];
+      f[u] = s.perm[at];
     }
+  };
+  places(static_cast<int32_t>(p0), key_next, from_next);
+  for (int32_t p = static_cast<int32_t>(p0); p < p1; p += kAhead) {
+    Piece<T, N> v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      key[u] = key_next[u];
+      v[u].load(grad + from_next[u] * s.ld + col);
+    }
+    places(p + kAhead, key_next, from_next);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (p + u >= p1) break;
@@ -264,32 +325,58 @@ __global__ __launch_bounds__(kThreads) void sum_chunks_kernel(Sums s, const T *g
 
 // Rows that span chunks: the tail of the chunk that a row began in and the heads
 // of the next ones, added in their order.
-template <class T>
+template <class T, int N>
 __global__ __launch_bounds__(kThreads) void join_chunks_kernel(Sums s, T *out) {
-  constexpr int N = kPiece<T>;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * (kThreads / s.across) +
                     threadIdx.x / s.across;
-  const int32_t col = (blockIdx.y * s.across + (threadIdx.x & (s.across - 1))) * N;
+  const int32_t first = (blockIdx.y * s.across + (threadIdx.x & (s.across - 1))) * N;
   const int64_t p0 = c * s.chunk, p1 = p0 + s.chunk;
-  if (p1 >= s.n_tokens || col >= s.n) return;
+  if (p1 >= s.n_tokens || first >= s.n) return;
+  const int32_t col = piece_at<N>(first, s.n);
   const uint32_t row = s.keys[p1 - 1];
   const bool began = s.keys[p0] != row || p0 == 0 || s.keys[p0 - 1] != row;
   if (row >= s.n_rows || !began || s.keys[p1] != row) return;
-  const int there = s.n - col;
-  float sum[N] = {};
-  add_part(s.part(c, 1) + col, there, sum);
-  for (int64_t next = c + 1; next * s.chunk < s.n_tokens && s.keys[next * s.chunk] == row;
-       ++next)
-    add_part(s.part(next, 0) + col, there, sum);
+  const int64_t chunks = (s.n_tokens + s.chunk - 1) / s.chunk;
+  // the chunk that the row ends in, kAhead looked at together
+  constexpr int kAhead = 8;
+  int64_t last = c;
+  for (int same = kAhead; same == kAhead; last += same) {
+    uint32_t key[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t next = last + 1 + u;
+      key[u] = s.keys[(next < chunks ? next : c) * s.chunk];
+      if (next >= chunks) key[u] = s.n_rows;
+    }
+    same = 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) same += same == u && key[u] == row;
+  }
+  float sum[N];
+  __builtin_memcpy(sum, __builtin_assume_aligned(s.part(c, 1) + col, 4), sizeof(sum));
+  for (int64_t next = c + 1; next <= last; next += kAhead) {
+    float v[kAhead][N];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      __builtin_memcpy(v[u], __builtin_assume_aligned(
+                                 s.part(next + u <= last ? next + u : last, 0) + col, 4),
+                       sizeof(v[u]));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum[i] += next + u <= last ? v[u][i] : 0.f;
+  }
   put_row(s, out, row, col, sum);
 }
 
 // ---- host ------------------------------------------------------------------------
 
-// Tokens of a chunk: 32, more where that gives above 2048 chunks (whose parts
-// one thread may have to add up).
-int32_t chunk_of(int64_t n_tokens) {
-  int64_t c = 32;
+// Tokens of a chunk: 8 to 32, as many as leave the chunks some 64 K threads (16384
+// tokens in 16 columns of bf16: 25 us in chunks of 32, 15 in 16), and more where
+// there would be above 2048 chunks, whose parts one thread may have to add up.
+int32_t chunk_of(int64_t n_tokens, int64_t n) {
+  int64_t c = 8;
+  while (c < 32 && n_tokens * ceil_div(n, 8) > c * 65536) c *= 2;
   while (ceil_div(n_tokens, c) > 2048) c *= 2;
   return static_cast<int32_t>(c);
 }
@@ -309,8 +396,8 @@ Plan carve(void *base, int64_t n_tokens, int64_t n) {
   Plan p = {};
   p.keys = c.take<uint32_t>(n_tokens);
   p.perm = c.take<int32_t>(n_tokens);
-  p.parts = c.take<float>(2 * n * ceil_div(n_tokens, chunk_of(n_tokens)));
-  if (n_tokens > kRankTokens) {
+  p.parts = c.take<float>(2 * n * ceil_div(n_tokens, chunk_of(n_tokens, n)));
+  if (n_tokens > kSortTokens) {
     p.keys64 = c.take<uint64_t>(n_tokens);
     p.keys_alt = c.take<uint64_t>(n_tokens);
     p.perm_alt = c.take<int32_t>(n_tokens);
@@ -373,15 +460,22 @@ extern "C" int ej_embed(const void *table, int32_t dtype, int64_t n_rows, int64_
     EJ_CHECK_ARG(ld >= n, "row stride %lld below n = %d", (long long)ld, n);
     if (n_tokens == 0 || n == 0) return EJ_OK;
     EJ_CHECK_ARG(tokens && out && (table || n_rows == 0), "null argument");
-    const int across = row_threads(ceil_div(n, kPiece<T>));
-    const int64_t blocks = ceil_div(n_tokens, kThreads / across);
-    if (blocks > kMaxBlocks) return too_many("tokens", n_tokens);
-    hipLaunchKernelGGL((embed_kernel<T, Token>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(kThreads), 0, as_stream(stream), static_cast<const T *>(table),
-                       static_cast<uint32_t>(n_rows), ld, n, static_cast<const Token *>(tokens),
-                       n_tokens, scale, across, static_cast<T *>(out));
-    EJ_LAUNCH_CHECK();
-    return EJ_OK;
+    constexpr int N = kPiece<T>;
+    const int across = row_threads(ceil_div(n, n < N ? 1 : N));
+    auto run = [&](auto kernel, int rows) {
+      const int64_t blocks = ceil_div(n_tokens, static_cast<int64_t>(kThreads / across) * rows);
+      if (blocks > kMaxBlocks) return too_many("tokens", n_tokens);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0,
+                         as_stream(stream), static_cast<const T *>(table),
+                         static_cast<uint32_t>(n_rows), ld, n, static_cast<const Token *>(tokens),
+                         n_tokens, scale, across, static_cast<T *>(out));
+      EJ_LAUNCH_CHECK();
+      return EJ_OK;
+    };
+    // several rows a thread where workgroups still fill the CUs
+    if (n < N) return run(embed_kernel<T, Token, 1, 1>, 1);
+    if (n_tokens >= 4096 * (kThreads / across)) return run(embed_kernel<T, Token, N, 4>, 4);
+    return run(embed_kernel<T, Token, N, 1>, 1);
   });
 }
 
@@ -415,18 +509,20 @@ extern "C" int ej_embed_vjp(const void *tokens, int32_t token_dtype, int64_t n_t
     const Plan p = n_tokens ? carve(workspace, n_tokens, n) : Plan{};
     EJ_CHECK_ARG(n_tokens == 0 || (workspace && workspace_bytes >= p.bytes),
                  "workspace of %zu bytes, expected %zu", workspace_bytes, p.bytes);
-    Sums s = {p.keys, p.perm, m, chunk_of(n_tokens), rows, n, 0, grad_ld, scale, p.parts};
-    s.across = row_threads(ceil_div(n, kPiece<T>));
+    Sums s = {p.keys, p.perm, m, chunk_of(n_tokens, n), rows, n, 0, grad_ld, scale, p.parts};
+    constexpr int N = kPiece<T>;
+    const int piece = n < N ? 1 : N;
+    s.across = row_threads(ceil_div(n, piece));
     const int64_t chunks = ceil_div(n_tokens, s.chunk);
-    const int64_t cols = ceil_div(n, static_cast<int64_t>(s.across) * kPiece<T>);
+    const int64_t cols = ceil_div(n, static_cast<int64_t>(s.across) * piece);
     const int64_t sum_blocks = ceil_div(chunks, kThreads / s.across);
     if (sum_blocks * cols > kMaxBlocks || cols > 65535) return too_many("columns", n);
-    if (n_tokens <= kRankTokens) {
-      constexpr int kT = kRankWaves * 64;
-      const int64_t blocks = ceil_div(n_tokens, 64);
-      hipLaunchKernelGGL((rank_kernel<T, Token>),
-                         dim3(static_cast<unsigned>(blocks + clear_blocks(bytes, kT))), dim3(kT), 0,
-                         stream, tok, m, rows, p.keys, p.perm, static_cast<uint32_t>(blocks), out,
+    int bits = 1;
+    while (n_rows >> bits) ++bits;  // keys up to n_rows
+    if (n_tokens <= kSortTokens) {
+      hipLaunchKernelGGL((sort_few_kernel<T, Token>),
+                         dim3(static_cast<unsigned>(1 + clear_blocks(bytes, kSortThreads))),
+                         dim3(kSortThreads), 0, stream, tok, m, rows, bits, p.keys, p.perm, out,
                          count);
       EJ_LAUNCH_CHECK();
     } else {
@@ -436,8 +532,6 @@ extern "C" int ej_embed_vjp(const void *tokens, int32_t token_dtype, int64_t n_t
                          dim3(kThreads), 0, stream, tok, m, rows, p.keys64, p.perm,
                          static_cast<uint32_t>(blocks), out, count);
       EJ_LAUNCH_CHECK();
-      int bits = 1;
-      while (n_rows >> bits) ++bits;  // keys up to n_rows
       EJ_TRY(sort_pairs_u64(p.keys64, p.perm, p.keys_alt, p.perm_alt, n_tokens, bits, p.sort,
                             stream, false, nullptr, false));
       hipLaunchKernelGGL(narrow_keys_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
@@ -446,13 +540,16 @@ extern "C" int ej_embed_vjp(const void *tokens, int32_t token_dtype, int64_t n_t
     }
     if (n_tokens == 0) return EJ_OK;
     const dim3 grid(static_cast<unsigned>(sum_blocks), static_cast<unsigned>(cols));
-    hipLaunchKernelGGL(sum_chunks_kernel<T>, grid, dim3(kThreads), 0, stream, s,
-                       static_cast<const T *>(grad), out);
-    EJ_LAUNCH_CHECK();
-    if (chunks > 1) {
-      hipLaunchKernelGGL(join_chunks_kernel<T>, grid, dim3(kThreads), 0, stream, s, out);
+    auto sums = [&](auto sum, auto join) {
+      hipLaunchKernelGGL(sum, grid, dim3(kThreads), 0, stream, s, static_cast<const T *>(grad),
+                         out);
       EJ_LAUNCH_CHECK();
-    }
-    return EJ_OK;
+      if (chunks == 1) return EJ_OK;
+      hipLaunchKernelGGL(join, grid, dim3(kThreads), 0, stream, s, out);
+      EJ_LAUNCH_CHECK();
+      return EJ_OK;
+    };
+    if (n < N) return sums(sum_chunks_kernel<T, 1>, join_chunks_kernel<T, 1>);
+    return sums(sum_chunks_kernel<T, N>, join_chunks_kernel<T, N>);
   });
 }
