@@ -26,6 +26,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef int i32v2_t __attribute__((ext_vector_type(2)));
 typedef int i32v4_t __attribute__((ext_vector_type(4)));
 typedef int i32v8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 // vectors at any element's alignment
 typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));

@@ -55,7 +55,12 @@ struct TileShape {
   static constexpr int kScales = kBlocks<Op> ? kThreads * 4 : 0;
   static_assert(!kBlocks<Op> || BM + BN <= kThreads, "a thread for each scale");
   static constexpr int kSlot = TA::kBytes + TB::kBytes + kScales;
-  static constexpr int kLds = NS == 0 ? 3 * TA::kBytes + 2 * TB::kBytes : NS * kSlot;
+  // NS == 0: the pipelined loops' rings
+  static constexpr int kPieces = LA::kLoads;  // of 64 rows (blocks): run_blocks
+  static constexpr int kLds = NS > 0           ? NS * kSlot
+                              : !kBlocks<Op> ? 3 * TA::kBytes + 2 * TB::kBytes
+                                             : (3 * kPieces - 1) * 8192 + 2 * TB::kBytes +
+                                                   4 * kScales;
   static constexpr int kLoads = LA::kLoads + LB::kLoads + (kBlocks<Op> ? 1 : 0);
 };
 
@@ -364,16 +369,17 @@ __device__ inline int gated_col(int i, int n0, int n, int *shift) {
   return n0 + i / WN * (WN / 2) + in % (WN / 2);
 }
 
-// The scales of a stage: thread t's is that of row t of the tile, or of column
-// t - rows.
+// The scales of a stage: thread t's is that of row row_of(t) of the tile, or of
+// column t - rows.
 struct ScaleLoader {
   const float *src;
   float held;
+  template <class RowOf>
   __device__ inline void init(const GroupedArgs &g, const RowBlock &r, int rows, int cols, int n0,
-                              int t, int st) {
+                              int t, int st, RowOf row_of) {
     const int64_t k_blocks = (g.k + 127) / 128;
     if (t < rows) {
-      const int s = r.lo + t < r.hi ? r.lo + t : r.hi - 1;
+      const int row = row_of(t), s = r.lo + row < r.hi ? r.lo + row : r.hi - 1;
       src = g.a_scale + slot_row(g.a_rows, g.n_a, s) * k_blocks + st;
     } else {
       int n = n0 + (t - rows < cols ? t - rows : cols - 1);
@@ -393,6 +399,143 @@ struct ScaleLoader {
     *reinterpret_cast<float *>(to + t * 4) = held;
   }
 };
+
+// Row of the tile whose scale is t-th among a stage's in run_blocks: a lane's two
+// of a pair of fragments lie side by side.
+template <class S>
+__device__ inline int blocks_row(int t) {
+  const int r = t % S::WM;
+  return t / S::WM * S::WM + (r / 32 * 2 + (r & 1)) * 16 + (r % 32) / 2;
+}
+
+// The pipelined loop of block-scaled products.  A wave takes its rows two
+// fragments (a pair) at a time, which it reads while the pair before is
+// multiplied; the fragments of its columns stay in registers for the stage:
+//   pairs but the last:  read the next pair; load most of A and the scales of
+//                        stage st + 2
+//   every wave has read stage st and stage st + 1 has landed: one barrier
+//   last pair:           read the first pair and, one by one as they become
+//                        free, the columns of stage st + 1; load B and the last
+//                        64 rows of A of stage st + 2
+// so that no fragment is waited for behind the barrier and loads are under way
+// all the time (see run_pipelined).  A lies in pieces of 64 rows in a ring of
+// one piece less than three stages, which leaves the room for the scales.
+template <class Op, class S>
+__device__ inline void run_blocks(f32x4_t (&acc)[S::FM][S::FN], unsigned char *ring, int stages,
+                                  int row0, int col0, int wave, int lane, typename S::LA &la,
+                                  typename S::LB &lb, ScaleLoader &scales, int k_left) {
+  constexpr int kPieces = S::kPieces, kSlots = 3 * kPieces - 1, kPiece = 8192;
+  constexpr int kB = kSlots * kPiece, kScale = kB + 2 * S::TB::kBytes;
+  constexpr int kPairs = S::FM / 2, kLate = kPieces;  // kPieces - 1 of A and the scales
+  static_assert(S::WM % 64 == 0 && S::FM % 4 == 0, "whole pieces of a wave");
+  if (stages == 0) return;
+  const uint32_t base = lds_address(ring);
+  typename S::FA fa;
+  typename S::FB fb;
+  fa.init(base, 0, lane);
+  fb.init(base + kB, col0, lane);
+  const uint32_t row_scale = base + kScale + row0 * 4 + (lane & 15) * 8;
+  const uint32_t col_scale = base + kScale + (S::kRows + col0) * 4;
+  const int piece0 = row0 / 64;
+  // slot of piece q of the stage whose first piece lies in slot `first`
+  auto slot_of = [&](int first, int q) {
+    const int s = first + q;
+    return s < kSlots ? s : s < 2 * kSlots ? s - kSlots : s - 2 * kSlots;
+  };
+  auto load_a = [&](int q, int st, int first) {
+    la.load(q, ring + (slot_of(first, q) - q) * kPiece, wave, k_left - st * 128, kRowB, true);
+  };
+  auto load_b = [&](int v, int st) {
+    lb.load(v, ring + kB + (st & 1) * S::TB::kBytes, wave, k_left - st * 128, kRowB, true);
+  };
+  auto load_scales = [&](int st) {
+    scales.load<true>(ring + kScale + (st & 3) * S::kScales, wave, st + 1 < stages ? 1 : 0);
+  };
+  BlockFragment<Op> a[2][2], b[S::FN];
+  f32x2_t as;
+  float bs;
+  auto read_pair = [&](int to, int first, int p) {
+    const uint32_t off = slot_of(first, piece0 + p / 2) * kPiece;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = p % 2 * 2 + h;
+      a[to][h].set(fa.read(off, i, 0), fa.read(off, i, 1));
+    }
+  };
+  auto read_b = [&](int j, int st) {
+    const uint32_t off = (st & 1) * S::TB::kBytes;
+    b[j].set(fb.read(off, j, 0), fb.read(off, j, 1));
+  };
+  auto multiply = [&](int p, int from, auto after) {
+    const f32x2_t s = as * bs;
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      const f32x4_t t0 = mma_block(b[j], a[from][0]), t1 = mma_block(b[j], a[from][1]);
+      after(j);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        acc[2 * p][j][c] = fmaf(t0[c], s[0], acc[2 * p][j][c]);
+        acc[2 * p + 1][j][c] = fmaf(t1[c], s[1], acc[2 * p + 1][j][c]);
+      }
+    }
+  };
+  auto read_scales = [&](int st, int p) {
+    as = *reinterpret_cast<const __attribute__((address_space(3))) f32x2_t *>(
+        (lds_u8 *)(size_t)(row_scale + (st & 3) * S::kScales + p * 128));
+    bs = ScalePlace::at(col_scale + (st & 3) * S::kScales);
+  };
+  // stages past the end are zeros, loaded from one cached line
+  int first = 0, first1 = kPieces;  // slots of the first pieces of stages st and st + 1
+#pragma unroll
+  for (int q = 0; q < kPieces; ++q) load_a(q, 0, first);
+#pragma unroll
+  for (int v = 0; v < S::LB::kLoads; ++v) load_b(v, 0);
+  load_scales(0);
+#pragma unroll
+  for (int q = 0; q < kPieces - 1; ++q) load_a(q, 1, first1);
+  load_scales(1);
+  load_a(kPieces - 1, 1, first1);
+#pragma unroll
+  for (int v = 0; v < S::LB::kLoads; ++v) load_b(v, 1);
+  wait_vm<kLate + 1 + S::LB::kLoads>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  read_pair(0, first, 0);
+#pragma unroll
+  for (int j = 0; j < S::FN; ++j) read_b(j, 0);
+  for (int st = 0; st < stages; ++st) {
+    const int first2 = slot_of(first1, kPieces);
+    read_scales(st, 0);
+#pragma unroll
+    for (int p = 0; p < kPairs - 1; ++p) {
+      // late loads of stage st + 2, spread over the pairs
+#pragma unroll
+      for (int l = p * kLate / (kPairs - 1); l < (p + 1) * kLate / (kPairs - 1); ++l) {
+        if (l < kPieces - 1) load_a(l, st + 2, first2);
+        else load_scales(st + 2);
+      }
+      multiply(p, p & 1, [&](int j) {
+        if (j == 0) read_pair(1 - (p & 1), first, p + 1);
+      });
+      read_scales(st, p + 1);
+    }
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLate) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    load_a(kPieces - 1, st + 2, first2);
+    multiply(kPairs - 1, (kPairs - 1) & 1, [&](int j) {
+      if (j == 0) read_pair(0, first1, 0);
+      if (j < S::LB::kLoads) load_b(j, st + 2);
+      read_b(j, st + 1);
+    });
+    static_assert(S::LB::kLoads <= S::FN && kPairs % 2 == 0, "loads and buffers of the last pair");
+    first = first1;
+    first1 = first2;
+  }
+  // no load may still be writing LDS when the workgroup ends
+  wait_vm<0>();
+}
 
 // C rows of one row block of a group times the BN columns from n0; GATED: the
 // BN / 2 gated columns from n0.
@@ -434,14 +577,18 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
   }
 
   ScaleLoader scales;
-  if constexpr (kBlocks<Op>) scales.init(g, r, BM, BN, n0, tid, st0);
+  if constexpr (kBlocks<Op>)
+    scales.init(g, r, BM, BN, n0, tid, st0, [](int t) { return NS == 0 ? blocks_row<S>(t) : t; });
 
   typename Op::acc acc[S::FM][S::FN];
 #pragma unroll
   for (int i = 0; i < S::FM; ++i)
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
-  run_stages<Op, S, DIRECT, NS>(
+  if constexpr (kBlocks<Op> && NS == 0) {
+    run_blocks<Op, S>(acc, ring, st1 - st0, row0, col0, wave, lane, la, lb, scales, ks);
+  } else
+    run_stages<Op, S, DIRECT, NS>(
       acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
         const int left = ks - st * kStep<Op>;
@@ -816,7 +963,8 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
   ScaleLoader scales;
-  if constexpr (kBlocks<Op>) scales.init(g, r, S::BM, BN, n0, lane, wave);
+  if constexpr (kBlocks<Op>)
+    scales.init(g, r, S::BM, BN, n0, lane, wave, [](int t) { return t; });
   auto load = [&](int i) {
     unsigned char *slot = ring + i % NS * S::kSlot;
     const int left = g.k - (wave + i * NW) * kStep<Op>;
