@@ -457,6 +457,18 @@ __device__ inline void load_word_to_lds(const float *src, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(src), "{m0}"(lds));
 #endif
 }
+// The same from a uniform address and 32 bits of offset for each lane, which take
+// no vector instruction to move on.
+__device__ inline void load_to_lds(const char *base, uint32_t off, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(lds));
+#endif
+}
+__device__ inline void load_word_to_lds(const char *base, uint32_t off, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "{m0}"(lds));
+#endif
+}
 __device__ inline uint32_t lds_address(const void *p) {
   return static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8 *)p));
 }

@@ -288,9 +288,12 @@ int pick_f8(const GroupedRows &r, hipStream_t stream) {
   if (few_rows(rows, tiles, 1)) return launch_skinny<Op, 32, 4, true, 2>(g, stream);
   if (rows <= 48 || tiles <= 576)
     return launch_rows<Op, 64, 64, 2, 2, true, true, 3>(g, stream);
+  // the large blocks' offsets of rows, in 32 bits
+  const bool near = g.ldb < (1 << 24) && g.lda < (1 << 24) &&
+                    (!g.a_rows || g.n_a <= (int64_t{1} << 32) / (g.lda > 128 ? g.lda : 128));
   if constexpr (__is_same(Op, OpF8)) {
     const double small = expected_tiles(g, 128, 128, groups) / 512;
-    if (large_rounds(expected_tiles(g, 256, 256, groups)) <= 0.8 * (small > 1 ? small : 1))
+    if (near && large_rounds(expected_tiles(g, 256, 256, groups)) <= 0.8 * (small > 1 ? small : 1))
       return launch_large<Op, true>(g, stream);
   }
   return launch_rows<Op, 128, 128, 2, 2, true, true, 2>(g, stream);

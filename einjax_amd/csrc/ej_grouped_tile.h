@@ -41,7 +41,7 @@ struct TileShape {
   using elem = typename Op::elem;
   static constexpr int kWaves = WR * WC;
   static constexpr int kThreads = kWaves * 64;
-  static constexpr int kRows = BM;
+  static constexpr int kRows = BM, kCols = BN;
   static constexpr int WM = BM / WR, WN = BN / WC;
   static constexpr int FM = WM / 16, FN = WN / 16;
   using TA = Tile<Op, BM, AKC>;
@@ -369,17 +369,16 @@ __device__ inline int gated_col(int i, int n0, int n, int *shift) {
   return n0 + i / WN * (WN / 2) + in % (WN / 2);
 }
 
-// The scales of a stage: thread t's is that of row row_of(t) of the tile, or of
-// column t - rows.
+// The scales of a stage: thread t's is that of row t of the tile, or of column
+// t - rows.
 struct ScaleLoader {
   const float *src;
   float held;
-  template <class RowOf>
   __device__ inline void init(const GroupedArgs &g, const RowBlock &r, int rows, int cols, int n0,
-                              int t, int st, RowOf row_of) {
+                              int t, int st) {
     const int64_t k_blocks = (g.k + 127) / 128;
     if (t < rows) {
-      const int row = row_of(t), s = r.lo + row < r.hi ? r.lo + row : r.hi - 1;
+      const int s = r.lo + t < r.hi ? r.lo + t : r.hi - 1;
       src = g.a_scale + slot_row(g.a_rows, g.n_a, s) * k_blocks + st;
     } else {
       int n = n0 + (t - rows < cols ? t - rows : cols - 1);
@@ -400,7 +399,39 @@ struct ScaleLoader {
   }
 };
 
-// Row of the tile whose scale is t-th among a stage's in run_blocks: a lane's two
+// Loads of a K tile's stages, and of the scales', at 32 bits from a uniform address.
+template <int ROWS, int NW>
+struct NearLoader {
+  static constexpr int kLoads = ROWS * kRowB / 1024 / NW;
+  static_assert(NW % 2 == 0, "one chunk of a row for each lane");
+  const char *base;
+  uint32_t off[kLoads];
+  int line;  // first k element of the lane's chunk
+  // row_off(i): offset of output row i from `from`
+  template <class RowOff>
+  __device__ inline void init(const char *from, int wave, int lane, RowOff row_off) {
+    base = from;
+#pragma unroll
+    for (int v = 0; v < kLoads; ++v) {
+      int row, chunk;
+      Tile<OpF8, ROWS, true>::at((v * NW + wave) * 64 + lane, &row, &chunk);
+      line = chunk * 16;
+      off[v] = row_off(row) + chunk * 16;
+    }
+  }
+  // Load v of stage st, of which `left` elements of k exist, to the tile at `lds`.
+  __device__ inline void load(int v, int st, uint32_t lds, int wave, int left, bool part) const {
+    const char *at = base + static_cast<int64_t>(st) * kRowB;
+    const uint32_t to = lds + (v * NW + wave) * 1024;
+    if (!part) {
+      load_to_lds(at, off[v], to);
+    } else {
+      load_to_lds(line < left ? at + off[v] : reinterpret_cast<const char *>(&grouped_zeros), to);
+    }
+  }
+};
+
+// Row of the tile whose scale is t-th among a stage's in blocks_256: a lane's two
 // of a pair of fragments lie side by side.
 template <class S>
 __device__ inline int blocks_row(int t) {
@@ -420,14 +451,42 @@ __device__ inline int blocks_row(int t) {
 // so that no fragment is waited for behind the barrier and loads are under way
 // all the time (see run_pipelined).  A lies in pieces of 64 rows in a ring of
 // one piece less than three stages, which leaves the room for the scales.
+// Its loads go by offsets of 32 bits: a pointer for each load in each lane would
+// take a fifth of the vector instructions' time, which scaling the sums needs.
 template <class Op, class S>
-__device__ inline void run_blocks(f32x4_t (&acc)[S::FM][S::FN], unsigned char *ring, int stages,
-                                  int row0, int col0, int wave, int lane, typename S::LA &la,
-                                  typename S::LB &lb, ScaleLoader &scales, int k_left) {
+__device__ inline void run_blocks(f32x4_t (&acc)[S::FM][S::FN], unsigned char *ring,
+                                  const GroupedArgs &g, const RowBlock &r, int n0, int row0,
+                                  int col0, int wave, int lane) {
   constexpr int kPieces = S::kPieces, kSlots = 3 * kPieces - 1, kPiece = 8192;
   constexpr int kB = kSlots * kPiece, kScale = kB + 2 * S::TB::kBytes;
   constexpr int kPairs = S::FM / 2, kLate = kPieces;  // kPieces - 1 of A and the scales
   static_assert(S::WM % 64 == 0 && S::FM % 4 == 0, "whole pieces of a wave");
+  const int stages = (g.k + 127) / 128, k_left = g.k;
+  NearLoader<S::kRows, S::kWaves> la;
+  NearLoader<S::kCols, S::kWaves> lb;
+  // rows that follow each other: from the block's first
+  const int64_t row_from = g.a_rows ? 0 : r.lo < g.n_a ? r.lo : g.n_a - 1;
+  auto near_row = [&](int i) {
+    const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
+    return static_cast<uint32_t>(slot_row(g.a_rows, g.n_a, s) - row_from);
+  };
+  auto near_col = [&](int i) { return static_cast<uint32_t>(n0 + i < g.n ? i : g.n - 1 - n0); };
+  la.init(g.a + row_from * g.lda, wave, lane,
+          [&](int i) { return near_row(i) * static_cast<uint32_t>(g.lda); });
+  lb.init(g.b + r.group * g.b_group + n0 * g.ldb, wave, lane,
+          [&](int i) { return near_col(i) * static_cast<uint32_t>(g.ldb); });
+  // scales of rows in the first waves, of columns in the others
+  const char *scale_base;
+  uint32_t scale_off;
+  if (wave * 64 < S::kRows) {
+    scale_base = reinterpret_cast<const char *>(g.a_scale + row_from * stages);
+    scale_off = near_row(blocks_row<S>(wave * 64 + lane)) * stages * 4;
+  } else {
+    const int64_t n_blocks = (g.n + 127) / 128;
+    const int i = wave * 64 + lane - S::kRows, n = n0 + (i < S::kCols ? i : 0);
+    scale_base = reinterpret_cast<const char *>(g.b_scale + (r.group * n_blocks) * stages);
+    scale_off = static_cast<uint32_t>((n < g.n ? n : g.n - 1) / 128) * stages * 4;
+  }
   if (stages == 0) return;
   const uint32_t base = lds_address(ring);
   typename S::FA fa;
@@ -442,97 +501,118 @@ __device__ inline void run_blocks(f32x4_t (&acc)[S::FM][S::FN], unsigned char *r
     const int s = first + q;
     return s < kSlots ? s : s < 2 * kSlots ? s - kSlots : s - 2 * kSlots;
   };
-  auto load_a = [&](int q, int st, int first) {
-    la.load(q, ring + (slot_of(first, q) - q) * kPiece, wave, k_left - st * 128, kRowB, true);
+  auto load_a = [&](int q, int st, int first, bool part) {
+    la.load(q, st, base + (slot_of(first, q) - q) * kPiece, wave, k_left - st * 128, part);
   };
-  auto load_b = [&](int v, int st) {
-    lb.load(v, ring + kB + (st & 1) * S::TB::kBytes, wave, k_left - st * 128, kRowB, true);
+  auto load_b = [&](int v, int st, bool part) {
+    lb.load(v, st, base + kB + (st & 1) * S::TB::kBytes, wave, k_left - st * 128, part);
   };
-  auto load_scales = [&](int st) {
-    scales.load<true>(ring + kScale + (st & 3) * S::kScales, wave, st + 1 < stages ? 1 : 0);
+  auto load_scales = [&](int st, bool part) {
+    const int there = !part || st < stages ? st : stages - 1;
+    load_word_to_lds(scale_base + there * 4ll, scale_off,
+                     base + kScale + (st & 3) * S::kScales + wave * 256);
   };
   BlockFragment<Op> a[2][2], b[S::FN];
-  f32x2_t as;
+  f32x2_t as[2] = {};
   float bs;
-  auto read_pair = [&](int to, int first, int p) {
+  auto read_a = [&](int first, int p, int h) {
     const uint32_t off = slot_of(first, piece0 + p / 2) * kPiece;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = p % 2 * 2 + h;
-      a[to][h].set(fa.read(off, i, 0), fa.read(off, i, 1));
-    }
+    const int i = p % 2 * 2 + h;
+    a[p & 1][h].set(fa.read(off, i, 0), fa.read(off, i, 1));
   };
   auto read_b = [&](int j, int st) {
     const uint32_t off = (st & 1) * S::TB::kBytes;
     b[j].set(fb.read(off, j, 0), fb.read(off, j, 1));
   };
-  auto multiply = [&](int p, int from, auto after) {
-    const f32x2_t s = as * bs;
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-      const f32x4_t t0 = mma_block(b[j], a[from][0]), t1 = mma_block(b[j], a[from][1]);
-      after(j);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        acc[2 * p][j][c] = fmaf(t0[c], s[0], acc[2 * p][j][c]);
-        acc[2 * p + 1][j][c] = fmaf(t1[c], s[1], acc[2 * p + 1][j][c]);
-      }
-    }
-  };
   auto read_scales = [&](int st, int p) {
-    as = *reinterpret_cast<const __attribute__((address_space(3))) f32x2_t *>(
+    as[p & 1] = *reinterpret_cast<const __attribute__((address_space(3))) f32x2_t *>(
         (lds_u8 *)(size_t)(row_scale + (st & 3) * S::kScales + p * 128));
-    bs = ScalePlace::at(col_scale + (st & 3) * S::kScales);
+    if (p == 0) bs = ScalePlace::at(col_scale + (st & 3) * S::kScales);
   };
   // stages past the end are zeros, loaded from one cached line
   int first = 0, first1 = kPieces;  // slots of the first pieces of stages st and st + 1
 #pragma unroll
-  for (int q = 0; q < kPieces; ++q) load_a(q, 0, first);
+  for (int q = 0; q < kPieces; ++q) load_a(q, 0, first, true);
 #pragma unroll
-  for (int v = 0; v < S::LB::kLoads; ++v) load_b(v, 0);
-  load_scales(0);
+  for (int v = 0; v < S::LB::kLoads; ++v) load_b(v, 0, true);
+  load_scales(0, true);
 #pragma unroll
-  for (int q = 0; q < kPieces - 1; ++q) load_a(q, 1, first1);
-  load_scales(1);
-  load_a(kPieces - 1, 1, first1);
+  for (int q = 0; q < kPieces - 1; ++q) load_a(q, 1, first1, true);
+  load_scales(1, true);
+  load_a(kPieces - 1, 1, first1, true);
 #pragma unroll
-  for (int v = 0; v < S::LB::kLoads; ++v) load_b(v, 1);
+  for (int v = 0; v < S::LB::kLoads; ++v) load_b(v, 1, true);
   wait_vm<kLate + 1 + S::LB::kLoads>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  read_pair(0, first, 0);
+  read_a(first, 0, 0);
+  read_a(first, 0, 1);
+  read_scales(0, 0);
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) read_b(j, 0);
-  for (int st = 0; st < stages; ++st) {
+  // steps of a stage: the matrix instructions of a pair and one fragment of
+  // columns; their sums are scaled and added up a step later, while the next
+  // ones are formed
+  constexpr int kSteps = kPairs * S::FN, kLastPair = kSteps - S::FN;
+  f32x4_t t[2][2] = {};
+  auto add_sums = [&](int step, int h) {
+    const int p = step / S::FN, j = step % S::FN;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      acc[2 * p + h][j][c] = fmaf(t[step & 1][h][c], as[p & 1][h], acc[2 * p + h][j][c]);
+  };
+  int st = 0;
+  auto stage = [&](auto kWhole) {
+    constexpr bool part = !decltype(kWhole)::value;
     const int first2 = slot_of(first1, kPieces);
-    read_scales(st, 0);
 #pragma unroll
-    for (int p = 0; p < kPairs - 1; ++p) {
-      // late loads of stage st + 2, spread over the pairs
-#pragma unroll
-      for (int l = p * kLate / (kPairs - 1); l < (p + 1) * kLate / (kPairs - 1); ++l) {
-        if (l < kPieces - 1) load_a(l, st + 2, first2);
-        else load_scales(st + 2);
+    for (int s = 0; s < kSteps; ++s) {
+      const int p = s / S::FN, j = s % S::FN;
+      if (s == kLastPair) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLate) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
       }
-      multiply(p, p & 1, [&](int j) {
-        if (j == 0) read_pair(1 - (p & 1), first, p + 1);
-      });
-      read_scales(st, p + 1);
+      // (of none yet: zeros)
+      constexpr int kEnd = kSteps - 1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        t[s & 1][h] = mma_block(b[j], a[p & 1][h]);
+        __builtin_amdgcn_sched_barrier(0);
+        add_sums(s > 0 ? s - 1 : kEnd, h);
+        if (h == 0) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (s < kLastPair) {
+        if (j < 2) read_a(first, p + 1, j);
+        if (j == 1) read_scales(st, p + 1);
+        // the late loads of stage st + 2
+        if (s % (kLastPair / kLate) == 0) {
+          constexpr int kEach = kLastPair / kLate;
+          if (s / kEach < kPieces - 1) load_a(s / kEach, st + 2, first2, part);
+          else if (s / kEach == kPieces - 1) load_scales(st + 2, part);
+        }
+      } else {
+        read_b(j, st + 1);
+        if (j < 2) read_a(first1, 0, j);
+        if (j == 1) read_scales(st + 1, 0);
+        if (j < S::LB::kLoads) load_b(j, st + 2, part);
+        if (j == 0) load_a(kPieces - 1, st + 2, first2, part);
+      }
+      if (j == 0) as[p & 1] *= bs;
+      __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLate) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    load_a(kPieces - 1, st + 2, first2);
-    multiply(kPairs - 1, (kPairs - 1) & 1, [&](int j) {
-      if (j == 0) read_pair(0, first1, 0);
-      if (j < S::LB::kLoads) load_b(j, st + 2);
-      read_b(j, st + 1);
-    });
-    static_assert(S::LB::kLoads <= S::FN && kPairs % 2 == 0, "loads and buffers of the last pair");
     first = first1;
     first1 = first2;
-  }
+    ++st;
+  };
+  static_assert(S::LB::kLoads <= S::FN && S::FN >= 2 && kPairs % 2 == 0 && kSteps % 2 == 0 &&
+                    kLastPair % kLate == 0,
+                "loads, buffers and reads of the steps");
+  while (st + 3 < stages) stage(std::true_type());
+  while (st < stages) stage(std::false_type());
+  add_sums(kSteps - 1, 0);
+  add_sums(kSteps - 1, 1);
   // no load may still be writing LDS when the workgroup ends
   wait_vm<0>();
 }
@@ -546,6 +626,23 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row0 = wave / WC * S::WM, col0 = wave % WC * S::WN;
+  typename Op::acc acc[S::FM][S::FN];
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
+  if constexpr (kBlocks<Op> && NS == 0) {
+    run_blocks<Op, S>(acc, ring, g, r, n0, row0, col0, wave, lane);
+    put_results<S>(
+        g, n0 + col0, lane,
+        [&](int i, int64_t *at) {
+          const int s = r.lo + row0 + i * 16 + (lane & 15);
+          *at = s * g.ldc;
+          return s < r.hi;
+        },
+        [&](int i, int j, int c) { return acc[i][j][c]; });
+    return;
+  }
   int st0, st1;
   part_of((g.k + kStep<Op> - 1) / kStep<Op>, blockIdx.y, g.splits, &st0, &st1);
   const int64_t k0 = static_cast<int64_t>(st0) * kStep<Op>;
@@ -577,18 +674,9 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
   }
 
   ScaleLoader scales;
-  if constexpr (kBlocks<Op>)
-    scales.init(g, r, BM, BN, n0, tid, st0, [](int t) { return NS == 0 ? blocks_row<S>(t) : t; });
+  if constexpr (kBlocks<Op>) scales.init(g, r, BM, BN, n0, tid, st0);
 
-  typename Op::acc acc[S::FM][S::FN];
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
-  if constexpr (kBlocks<Op> && NS == 0) {
-    run_blocks<Op, S>(acc, ring, st1 - st0, row0, col0, wave, lane, la, lb, scales, ks);
-  } else
-    run_stages<Op, S, DIRECT, NS>(
+  run_stages<Op, S, DIRECT, NS>(
       acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
         const int left = ks - st * kStep<Op>;
@@ -963,8 +1051,7 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
     b_step = kStep<Op> * g.ldb * kElem<Op>;
   }
   ScaleLoader scales;
-  if constexpr (kBlocks<Op>)
-    scales.init(g, r, S::BM, BN, n0, lane, wave, [](int t) { return t; });
+  if constexpr (kBlocks<Op>) scales.init(g, r, S::BM, BN, n0, lane, wave);
   auto load = [&](int i) {
     unsigned char *slot = ring + i % NS * S::kSlot;
     const int left = g.k - (wave + i * NW) * kStep<Op>;
