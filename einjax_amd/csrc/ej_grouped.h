@@ -26,6 +26,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef int i32v2_t __attribute__((ext_vector_type(2)));
 typedef int i32v4_t __attribute__((ext_vector_type(4)));
 typedef int i32v8_t __attribute__((ext_vector_type(8)));
+typedef int i32v4_any_t __attribute__((ext_vector_type(4), aligned(1)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 // vectors at any element's alignment
@@ -473,46 +474,51 @@ __device__ inline uint32_t lds_address(const void *p) {
   return static_cast<uint32_t>(reinterpret_cast<size_t>((lds_u8 *)p));
 }
 
-// 16 bytes from p on, at any element alignment, of which `valid` elements
-// exist (any number; the others come out zero).  Where fewer than a chunk do,
-// the last chunk of the row is loaded and shifted down: that needs rows of a
-// chunk at least (`whole`, uniform); shorter ones go element by element.
+// How tiles are loaded:
+//   kLoadDirect   16 bytes straight into LDS: rows 16-byte aligned, extents whole
+//                 chunks
+//   kLoadPieces   16 bytes into registers, at any element's alignment, stored to
+//                 LDS a stage later.  A chunk that a row ends in is loaded from
+//                 the row's last 16 bytes and shifted down when it is stored.
+//   kLoadElements the same, element by element: rows shorter than 16 bytes
+// In the first two no load stands behind a branch, which would have it waited
+// for before the next one.
+constexpr int kLoadPieces = 0, kLoadDirect = 1, kLoadElements = 2;
+
+// v moved down by n elements (0 to a chunk of them), zeros on top.
 template <class Op>
-__device__ inline i32v4_t load_chunk(const char *p, int valid, bool whole) {
+__device__ inline i32v4_t shift_down(const i32v4_t &v, int n) {
+  const int bits = n * kElem<Op> * 8;
+  uint64_t w[2];
+  __builtin_memcpy(w, &v, 16);
+  const uint64_t hi = bits < 64 ? w[1] >> bits : 0;
+  const uint64_t lo = bits == 0    ? w[0]
+                      : bits < 64  ? w[0] >> bits | w[1] << (64 - bits)
+                      : bits < 128 ? w[1] >> (bits - 64)
+                                   : 0;
+  w[0] = lo;
+  w[1] = hi;
+  i32v4_t r;
+  __builtin_memcpy(&r, w, 16);
+  return r;
+}
+
+// The first `valid` elements from p on (any number), zeros behind them.
+template <class Op>
+__device__ inline i32v4_t load_elements(const char *p, int valid) {
   using E = typename Op::elem;
-  constexpr int N = kChunk<Op>;
-  i32v4_t v = {0, 0, 0, 0};
-  if (whole) {
-    const int past = valid < N ? N - valid : 0;
-    __builtin_memcpy(&v, __builtin_assume_aligned(p - past * kElem<Op>, alignof(E)), 16);
-    if (__any(past > 0)) {
-      const int bits = past < N ? past * kElem<Op> * 8 : 128;
-      uint64_t w[2];
-      __builtin_memcpy(w, &v, 16);
-      const uint64_t down = bits < 64 ? w[1] >> bits : 0;
-      w[0] = bits == 0    ? w[0]
-             : bits < 64  ? w[0] >> bits | w[1] << (64 - bits)
-             : bits < 128 ? w[1] >> (bits - 64)
-                          : 0;
-      w[1] = down;
-      __builtin_memcpy(&v, w, 16);
-    }
-  } else {
-    E e[N] = {};
+  E e[kChunk<Op>] = {};
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < valid) e[i] = reinterpret_cast<const E *>(p)[i];
-    __builtin_memcpy(&v, e, 16);
-  }
+  for (int i = 0; i < kChunk<Op>; ++i)
+    if (i < valid) e[i] = reinterpret_cast<const E *>(p)[i];
+  i32v4_t v;
+  __builtin_memcpy(&v, e, 16);
   return v;
 }
 
 // One operand's loads of a stage, split over NW waves; lane positions are
-// fixed for the kernel, the sources advance stage by stage.  DIRECT: 16-byte
-// loads straight into LDS (rows 16-byte aligned, extents whole chunks);
-// otherwise loads into registers, at any alignment, stored to LDS a stage
-// later.
-template <class Op, int ROWS, bool KC, int NW, bool DIRECT>
+// fixed for the kernel, the sources advance stage by stage.
+template <class Op, int ROWS, bool KC, int NW, int LOADS>
 struct Loader {
   using T = Tile<Op, ROWS, KC>;
   static constexpr int kLoads = T::kBytes / 1024 / NW;  // load instructions per wave and stage
@@ -528,10 +534,11 @@ struct Loader {
 
   const char *src[kLoads];  // this lane's source in the next stage
   int line;                 // K: first k element of the lane's chunk; M: its k-row in load 0
-  int col[kCols];           // M: first column of the lane's chunk
-  int valid[kCols];         // M, not DIRECT: elements from the column to the extent
-  bool whole;               // not DIRECT: rows hold a chunk
-  i32v4_t reg[DIRECT ? 1 : kLoads];
+  int col[kCols];           // M: first column of the lane's chunk (in pieces: of what is loaded)
+  int valid[kCols];         // M, not direct: elements from the chunk's first column to the extent
+  bool edge;                // M, pieces: the tile reaches past the extent
+  int held_left;            // K, pieces: elements of k of the stage that is held
+  i32v4_t reg[LOADS == kLoadDirect ? 1 : kLoads];
 
   // k element (K) or k-row (M) of the lane's place in load v; in K tiles the
   // swizzle repeats every 16 rows, and differs by 4 between its halves.
@@ -542,8 +549,7 @@ struct Loader {
 
   // K tiles: row_at(i) is the address of output row i's first k element.
   template <class RowAt>
-  __device__ inline void init_k(int wave, int lane, int k, RowAt row_at) {
-    whole = k >= kChunk<Op>;
+  __device__ inline void init_k(int wave, int lane, RowAt row_at) {
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
       int row, chunk;
@@ -565,7 +571,7 @@ struct Loader {
   template <class ColAt>
   __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int ext,
                                 ColAt col_at) {
-    whole = ext >= kChunk<Op>;
+    edge = false;
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
       int krow, chunk;
@@ -573,15 +579,16 @@ struct Loader {
       if (v == 0) line = krow;
       if (v < kCols) {
         int shift, c = col_at(chunk * kChunk<Op>, &shift);
-        if constexpr (DIRECT) {
-          if (c > ext - kChunk<Op>) c = ext - kChunk<Op>;
-        } else {
-          valid[v] = ext - c;
+        valid[v] = ext - c;
+        if (LOADS != kLoadElements && c > ext - kChunk<Op>) {
+          c = ext - kChunk<Op>;
+          edge = true;
         }
         col[v] = c + shift;
       }
       src[v] = base + (line_at(v) * ld + col[v % kCols]) * kElem<Op>;
     }
+    if constexpr (LOADS == kLoadPieces) edge = __any(edge);
   }
 
   // Starts load v of the next stage, of which `left` elements of k exist
@@ -589,24 +596,45 @@ struct Loader {
   // part: the stage may end short of kStep elements.
   __device__ inline void load(int v, unsigned char *tile, int wave, int left, int64_t step,
                               bool part) {
-    if constexpr (DIRECT) {
-      const char *p = src[v];
-      if (part && left < kStep<Op>)
-        p = line_at(v) < left ? p : reinterpret_cast<const char *>(&grouped_zeros);
+    const char *zeros = reinterpret_cast<const char *>(&grouped_zeros), *p = src[v];
+    if constexpr (LOADS == kLoadDirect) {
+      if (part && left < kStep<Op>) p = line_at(v) < left ? p : zeros;
       load_to_lds(p, lds_address(tile) + (v * NW + wave) * 1024);
-    } else {
+    } else if constexpr (LOADS == kLoadPieces) {
+      const int there = left - line_at(v);
       if constexpr (KC) {
-        reg[v] = load_chunk<Op>(src[v], left - line_at(v), whole);
-      } else {
-        const bool there = line_at(v) < left;
-        reg[v] = load_chunk<Op>(there ? src[v] : reinterpret_cast<const char *>(&grouped_zeros),
-                                there ? valid[v % kCols] : whole ? kChunk<Op> : 0, whole);
+        p -= there < kChunk<Op> ? (kChunk<Op> - there) * kElem<Op> : 0;
+        held_left = left;
       }
+      p = there > 0 ? p : zeros;
+      // as global memory: a load that might be of LDS is waited for with the
+      // LDS reads
+      reg[v] = *(const __attribute__((address_space(1))) i32v4_any_t *)(p);
+    } else {
+      if constexpr (KC) reg[v] = load_elements<Op>(p, left - line_at(v));
+      else reg[v] = load_elements<Op>(p, line_at(v) < left ? valid[v % kCols] : 0);
     }
     src[v] += step;
   }
-  // Not DIRECT: what load() fetched, into the tile at `tile`.
+  // Not direct: what load() fetched, into the tile at `tile`.
   __device__ inline void store(unsigned char *tile, int wave, int lane) {
+    constexpr int N = kChunk<Op>;
+    if constexpr (LOADS == kLoadPieces && KC) {
+      if (held_left < kStep<Op>)
+#pragma unroll
+        for (int v = 0; v < kLoads; ++v) {
+          const int there = held_left - line_at(v);
+          reg[v] = shift_down<Op>(reg[v], there < N && there > 0 ? N - there : 0);
+        }
+    }
+    if constexpr (LOADS == kLoadPieces && !KC) {
+      if (edge)
+#pragma unroll
+        for (int v = 0; v < kLoads; ++v) {
+          const int there = valid[v % kCols];
+          reg[v] = shift_down<Op>(reg[v], there < N && there > 0 ? N - there : 0);
+        }
+    }
 #pragma unroll
     for (int v = 0; v < kLoads; ++v)
       *reinterpret_cast<i32v4_t *>(tile + ((v * NW + wave) * 64 + lane) * 16) = reg[v];

@@ -8,6 +8,12 @@
 
 namespace ej {
 
+// Whether rows of the operands are shorter than 16 bytes.
+template <class Op, bool BKC>
+bool short_rows(const GroupedArgs &g) {
+  return g.k < kChunk<Op> || (!BKC && g.n < kChunk<Op>);
+}
+
 inline int join_parts(const GroupedArgs &g, int64_t rows, int64_t m, bool skip_dead,
                       hipStream_t stream) {
   dim3 grid;
@@ -32,7 +38,7 @@ constexpr int result_cols(int bn) {
   return GATED ? bn / 2 : bn;
 }
 
-template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS,
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, int LOADS, int NS,
           bool GATED = false>
 int launch_rows(GroupedArgs g, hipStream_t stream) {
   const int64_t groups = g.n_groups < g.slots ? g.n_groups : g.slots;
@@ -42,7 +48,7 @@ int launch_rows(GroupedArgs g, hipStream_t stream) {
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks + kZeroBlocks,
                       WR * WC * 64, &grid));
   grid.y = g.splits;
-  hipLaunchKernelGGL((grouped_rows_kernel<Op, BM, BN, WR, WC, BKC, DIRECT, NS, GATED>), grid,
+  hipLaunchKernelGGL((grouped_rows_kernel<Op, BM, BN, WR, WC, BKC, LOADS, NS, GATED>), grid,
                      dim3(WR * WC * 64), 0, stream, g);
   EJ_LAUNCH_CHECK();
   if (g.splits == 1) return EJ_OK;
@@ -77,7 +83,7 @@ int launch_skinny(GroupedArgs g, hipStream_t stream) {
   return EJ_OK;
 }
 
-template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
+template <class Op, int BM, int BN, int WR, int WC, int LOADS, int NS, int GATHER>
 int launch_wgrad_as(GroupedArgs g, hipStream_t stream) {
   g.row_blocks = static_cast<uint32_t>(ceil_div(g.m, BM));
   g.col_blocks = static_cast<uint32_t>(ceil_div(g.n, BN));
@@ -85,18 +91,18 @@ int launch_wgrad_as(GroupedArgs g, hipStream_t stream) {
   EJ_TRY(grouped_grid(static_cast<int64_t>(g.row_blocks) * g.col_blocks * g.n_groups,
                       WR * WC * 64, &grid));
   grid.y = g.splits;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<Op, BM, BN, WR, WC, DIRECT, NS, GATHER>), grid,
+  hipLaunchKernelGGL((grouped_wgrad_kernel<Op, BM, BN, WR, WC, LOADS, NS, GATHER>), grid,
                      dim3(WR * WC * 64), 0, stream, g);
   EJ_LAUNCH_CHECK();
   return g.splits > 1 ? join_parts(g, static_cast<int64_t>(g.n_groups) * g.m, g.m, false, stream)
                       : EJ_OK;
 }
 
-template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS>
+template <class Op, int BM, int BN, int WR, int WC, int LOADS, int NS>
 int launch_wgrad(const GroupedArgs &g, hipStream_t stream) {
-  if (g.a_rows) return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 1>(g, stream);
-  if (g.b_rows) return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 2>(g, stream);
-  return launch_wgrad_as<Op, BM, BN, WR, WC, DIRECT, NS, 0>(g, stream);
+  if (g.a_rows) return launch_wgrad_as<Op, BM, BN, WR, WC, LOADS, NS, 1>(g, stream);
+  if (g.b_rows) return launch_wgrad_as<Op, BM, BN, WR, WC, LOADS, NS, 2>(g, stream);
+  return launch_wgrad_as<Op, BM, BN, WR, WC, LOADS, NS, 0>(g, stream);
 }
 
 template <class Op, int GATHER>
@@ -153,9 +159,11 @@ inline double large_rounds(double tiles) {
 template <class Op, bool BKC>
 int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
+  if (!r.direct && short_rows<Op, BKC>(g))
+    return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadElements, 2>(g, stream);
   if (g.splits > 1) {
-    if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
-    return launch_rows<Op, 64, 64, 2, 2, BKC, true, kElem<Op> == 4 ? 0 : 3>(g, stream);
+    if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, kElem<Op> == 4 ? 0 : 3>(g, stream);
   }
   const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
   const double rows = static_cast<double>(g.slots) / groups;
@@ -167,11 +175,11 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
     // groups 800 x 771 x 1283 f16 19, 18, 22; in 4 2000 x 255 x 333 fp32 13, 16,
     // 24, 8 bits 7 and 9 in 128 x 128
     if (tiles <= 512 || rows <= 128)
-      return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2>(g, stream);
+      return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2>(g, stream);
     if constexpr (kElem<Op> == 4)
-      return launch_rows<Op, 64, 128, 2, 4, BKC, false, 2>(g, stream);
+      return launch_rows<Op, 64, 128, 2, 4, BKC, kLoadPieces, 2>(g, stream);
     else
-      return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2>(g, stream);
+      return launch_rows<Op, 128, 128, 2, 4, BKC, kLoadPieces, 2>(g, stream);
   }
   // columns of a skinny block: 32, or what fills 128 bytes of a [k][n] row
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
@@ -181,18 +189,18 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
     // bound by the fp32 matrix instructions at any tile: the finest spreads
     // best (4096 x 1024 x 2048 in 8 groups 164 us, 212 with 128 x 128; equal
     // within 2% at 16384 x 2048 x 2048)
-    return launch_rows<Op, 64, 64, 2, 2, BKC, true, 0>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, 0>(g, stream);
   } else {
     // up to about two small tiles to a CU the finest spread best
     if (rows <= 48 || tiles <= 576)
-      return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3>(g, stream);
-    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, true, 3>(g, stream);
+      return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, 3>(g, stream);
+    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, kLoadDirect, 3>(g, stream);
     // rounds of large blocks against a fifth less time for a round of 512
     // quarter-size ones (two to a CU, which even out)
     const double small = expected_tiles(g, 128, 128, groups) / 512;
     if (large_rounds(expected_tiles(g, 256, 256, groups)) <= 0.8 * (small > 1 ? small : 1))
       return launch_large<Op, BKC>(g, stream);
-    return launch_rows<Op, 128, 128, 2, 2, BKC, true, 2>(g, stream);
+    return launch_rows<Op, 128, 128, 2, 2, BKC, kLoadDirect, 2>(g, stream);
   }
 }
 
@@ -218,20 +226,22 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
     return static_cast<double>(ceil_div(g.m, b) * ceil_div(g.n, b) * g.n_groups);
   };
   if (!direct) {
+    if (g.m < kChunk<Op> || g.n < kChunk<Op>)
+      return launch_wgrad<Op, 64, 64, 2, 2, kLoadElements, 2>(g, stream);
     if constexpr (kElem<Op> == 2) {
       if (g.splits == 1 && tiles(128) >= 512)
-        return launch_wgrad<Op, 128, 128, 2, 4, false, 2>(g, stream);
+        return launch_wgrad<Op, 128, 128, 2, 4, kLoadPieces, 2>(g, stream);
     }
-    return launch_wgrad<Op, 64, 64, 2, 2, false, 2>(g, stream);
+    return launch_wgrad<Op, 64, 64, 2, 2, kLoadPieces, 2>(g, stream);
   }
-  if (g.splits > 1) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
-  if (tiles(128) < 256) return launch_wgrad<Op, 64, 64, 2, 2, true, 3>(g, stream);
+  if (g.splits > 1) return launch_wgrad<Op, 64, 64, 2, 2, kLoadDirect, 3>(g, stream);
+  if (tiles(128) < 256) return launch_wgrad<Op, 64, 64, 2, 2, kLoadDirect, 3>(g, stream);
   if constexpr (kElem<Op> == 2) {
     const double small = tiles(128) / 512;
     if (large_rounds(tiles(256)) <= 0.55 * (small > 1 ? small : 1))
       return launch_wgrad_large<Op>(g, stream);
   }
-  return launch_wgrad<Op, 128, 128, 2, 2, true, 2>(g, stream);
+  return launch_wgrad<Op, 128, 128, 2, 2, kLoadDirect, 2>(g, stream);
 }
 
 // Gated rows: the same rules, with the columns of both projections for the
@@ -239,9 +249,11 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
 template <class Op, bool BKC>
 int pick_gated(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
+  if (!r.direct && short_rows<Op, BKC>(g))
+    return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadElements, 2, true>(g, stream);
   if (g.splits > 1) {
-    if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2, true>(g, stream);
-    return launch_rows<Op, 64, 64, 2, 2, BKC, true, kElem<Op> == 4 ? 0 : 3, true>(g, stream);
+    if (!r.direct) return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2, true>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, kElem<Op> == 4 ? 0 : 3, true>(g, stream);
   }
   const int64_t groups = g.n_groups < g.slots ? (g.n_groups > 0 ? g.n_groups : 1) : g.slots;
   const double rows = static_cast<double>(g.slots) / groups;
@@ -251,25 +263,25 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
   const double tiles = tiles_of(64, 64);
   if (!r.direct) {
     if (tiles <= 512 || rows <= 128)
-      return launch_rows<Op, 64, 64, 2, 2, BKC, false, 2, true>(g, stream);
+      return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2, true>(g, stream);
     if constexpr (kElem<Op> == 4)
-      return launch_rows<Op, 64, 128, 2, 4, BKC, false, 2, true>(g, stream);
+      return launch_rows<Op, 64, 128, 2, 4, BKC, kLoadPieces, 2, true>(g, stream);
     else
-      return launch_rows<Op, 128, 128, 2, 4, BKC, false, 2, true>(g, stream);
+      return launch_rows<Op, 128, 128, 2, 4, BKC, kLoadPieces, 2, true>(g, stream);
   }
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
   if (few_rows(rows, tiles, kElem<Op>))
     return launch_skinny<Op, kSkinny, 4, BKC, 2, true>(g, stream);
   if constexpr (kElem<Op> == 4) {
-    return launch_rows<Op, 64, 64, 2, 2, BKC, true, 0, true>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, 0, true>(g, stream);
   } else {
     if (rows <= 48 || tiles <= 576)
-      return launch_rows<Op, 64, 64, 2, 2, BKC, true, 3, true>(g, stream);
-    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, true, 3, true>(g, stream);
+      return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, 3, true>(g, stream);
+    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, kLoadDirect, 3, true>(g, stream);
     const double small = tiles_of(128, 128) / 512;
     if (large_rounds(tiles_of(256, 256)) <= 0.8 * (small > 1 ? small : 1))
       return launch_large<Op, BKC, true>(g, stream);
-    return launch_rows<Op, 128, 128, 2, 2, BKC, true, 2, true>(g, stream);
+    return launch_rows<Op, 128, 128, 2, 2, BKC, kLoadDirect, 2, true>(g, stream);
   }
 }
 
@@ -281,13 +293,15 @@ int pick_f8(const GroupedRows &r, hipStream_t stream) {
   const double rows = static_cast<double>(g.slots) / groups;
   const double tiles = expected_tiles(g, 64, 64, groups);
   if (!r.direct) {
+    if (short_rows<Op, true>(g))
+      return launch_rows<Op, 64, 64, 2, 2, true, kLoadElements, 2>(g, stream);
     if (tiles <= 512 || rows <= 128)
-      return launch_rows<Op, 64, 64, 2, 2, true, false, 2>(g, stream);
-    return launch_rows<Op, 128, 128, 2, 4, true, false, 2>(g, stream);
+      return launch_rows<Op, 64, 64, 2, 2, true, kLoadPieces, 2>(g, stream);
+    return launch_rows<Op, 128, 128, 2, 4, true, kLoadPieces, 2>(g, stream);
   }
   if (few_rows(rows, tiles, 1)) return launch_skinny<Op, 32, 4, true, 2>(g, stream);
   if (rows <= 48 || tiles <= 576)
-    return launch_rows<Op, 64, 64, 2, 2, true, true, 3>(g, stream);
+    return launch_rows<Op, 64, 64, 2, 2, true, kLoadDirect, 3>(g, stream);
   // the large blocks' offsets of rows, in 32 bits
   const bool near = g.ldb < (1 << 24) && g.lda < (1 << 24) &&
                     (!g.a_rows || g.n_a <= (int64_t{1} << 32) / (g.lda > 128 ? g.lda : 128));
@@ -296,7 +310,7 @@ int pick_f8(const GroupedRows &r, hipStream_t stream) {
     if (near && large_rounds(expected_tiles(g, 256, 256, groups)) <= 0.8 * (small > 1 ? small : 1))
       return launch_large<Op, true>(g, stream);
   }
-  return launch_rows<Op, 128, 128, 2, 2, true, true, 2>(g, stream);
+  return launch_rows<Op, 128, 128, 2, 2, true, kLoadDirect, 2>(g, stream);
 }
 
 }  // namespace ej

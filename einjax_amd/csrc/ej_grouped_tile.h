@@ -36,7 +36,7 @@ __device__ inline void band_pos(uint32_t lb, uint32_t rbs, uint32_t cbs, uint32_
   *cb = static_cast<int>(r / h);
 }
 
-template <class Op, int BM, int BN, int WR, int WC, bool AKC, bool BKC, bool DIRECT, int NS>
+template <class Op, int BM, int BN, int WR, int WC, bool AKC, bool BKC, int LOADS, int NS>
 struct TileShape {
   using elem = typename Op::elem;
   static constexpr int kWaves = WR * WC;
@@ -48,8 +48,8 @@ struct TileShape {
   using TB = Tile<Op, BN, BKC>;
   using FA = Fragments<Op, TA, AKC, FM>;
   using FB = Fragments<Op, TB, BKC, FN>;
-  using LA = Loader<Op, BM, AKC, kWaves, DIRECT>;
-  using LB = Loader<Op, BN, BKC, kWaves, DIRECT>;
+  using LA = Loader<Op, BM, AKC, kWaves, LOADS>;
+  using LB = Loader<Op, BN, BKC, kWaves, LOADS>;
   // scales of a stage, one a thread: the tile's rows', then its columns'
   static constexpr int kScaleAt = TA::kBytes + TB::kBytes;
   static constexpr int kScales = kBlocks<Op> ? kThreads * 4 : 0;
@@ -228,7 +228,7 @@ __device__ inline void run_pipelined(typename Op::acc (&acc)[S::FM][S::FN], unsi
 
 // The ring: load_stage(st, slot pointer) starts the loads of stage st,
 // store_stage(slot pointer) finishes them where they go through registers.
-template <class Op, class S, bool DIRECT, int NS, class Load, class Store>
+template <class Op, class S, int LOADS, int NS, class Load, class Store>
 __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigned char *ring,
                                   int stages, int row0, int col0, int lane, Load load_stage,
                                   Store store_stage) {
@@ -247,9 +247,9 @@ __device__ inline void run_stages(typename Op::acc (&acc)[S::FM][S::FN], unsigne
 #pragma unroll
     for (int v = 0; v < S::kLoads; ++v) load_stage(v, st, slot, true);
   };
-  if constexpr (DIRECT && NS == 0) {
+  if constexpr (LOADS == kLoadDirect && NS == 0) {
     run_pipelined<Op, S>(acc, ring, stages, fa, fb, load_stage);
-  } else if constexpr (DIRECT) {
+  } else if constexpr (LOADS == kLoadDirect) {
     int put = 0, get = 0;
     for (int st = 0; st < NS - 1 && st < stages; ++st) {
       load_all(st, ring + put * S::kSlot);
@@ -388,9 +388,9 @@ struct ScaleLoader {
     }
   }
   // The next stage's, `step` stages on from the one before.
-  template <bool DIRECT>
+  template <int LOADS>
   __device__ inline void load(unsigned char *to, int wave, int step) {
-    if constexpr (DIRECT) load_word_to_lds(src, lds_address(to) + wave * 256);
+    if constexpr (LOADS == kLoadDirect) load_word_to_lds(src, lds_address(to) + wave * 256);
     else held = *src;
     src += step;
   }
@@ -619,10 +619,10 @@ __device__ inline void run_blocks(f32x4_t (&acc)[S::FM][S::FN], unsigned char *r
 
 // C rows of one row block of a group times the BN columns from n0; GATED: the
 // BN / 2 gated columns from n0.
-template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS,
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, int LOADS, int NS,
           bool GATED = false>
 __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsigned char *ring) {
-  using S = TileShape<Op, BM, BN, WR, WC, true, BKC, DIRECT, NS>;
+  using S = TileShape<Op, BM, BN, WR, WC, true, BKC, LOADS, NS>;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row0 = wave / WC * S::WM, col0 = wave % WC * S::WN;
@@ -650,14 +650,14 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
 
   typename S::LA la;
   typename S::LB lb;
-  la.init_k(wave, lane, g.k, [&](int i) {
+  la.init_k(wave, lane, [&](int i) {
     const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
     return g.a + (slot_row(g.a_rows, g.n_a, s) * g.lda + k0) * kElem<Op>;
   });
   const char *bg = g.b + r.group * g.b_group * kElem<Op>;
   int64_t b_step;
   if constexpr (BKC) {
-    lb.init_k(wave, lane, g.k, [&](int i) {
+    lb.init_k(wave, lane, [&](int i) {
       int shift = 0, n = n0 + i;
       if constexpr (GATED) n = gated_col<S::WN>(i, n0, g.n, &shift);
       n = n < g.n ? n : g.n - 1;
@@ -676,7 +676,7 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
   ScaleLoader scales;
   if constexpr (kBlocks<Op>) scales.init(g, r, BM, BN, n0, tid, st0);
 
-  run_stages<Op, S, DIRECT, NS>(
+  run_stages<Op, S, LOADS, NS>(
       acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
         const int left = ks - st * kStep<Op>;
@@ -685,7 +685,7 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
         else if (v < S::LA::kLoads + S::LB::kLoads)
           lb.load(v - S::LA::kLoads, slot + S::TA::kBytes, wave, left, b_step, part);
         else
-          scales.load<DIRECT>(slot + S::kScaleAt, wave, 1);
+          scales.load<LOADS>(slot + S::kScaleAt, wave, 1);
       },
       [&](unsigned char *slot) {
         la.store(slot, wave, lane);
@@ -739,10 +739,10 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
 // registers: 33 us, 21 us at aligned extents; the rest are another column of
 // tiles and stage of k, and the unaligned loads, two lines for most of them.
 // Aligned loads with the bytes shifted into place afterwards took as long.
-template <class Op, int BM, int BN, int WR, int WC, bool BKC, bool DIRECT, int NS, bool GATED>
+template <class Op, int BM, int BN, int WR, int WC, bool BKC, int LOADS, int NS, bool GATED>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using S = TileShape<Op, BM, BN, WR, WC, true, BKC, DIRECT, NS>;
+  using S = TileShape<Op, BM, BN, WR, WC, true, BKC, LOADS, NS>;
   __shared__ __align__(1024) unsigned char ring[S::kLds];
   const uint32_t grid = g.row_blocks * g.col_blocks;
   if (blockIdx.x >= grid) {
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g
   if (blockIdx.x >= live) return;
   int rb, cb;
   band_pos(xcd_logical_block(live), rbs, g.col_blocks, 1024 / BM, &rb, &cb);
-  rows_block<Op, BM, BN, WR, WC, BKC, DIRECT, NS, GATED>(g, find_row_block(g, BM, rb),
+  rows_block<Op, BM, BN, WR, WC, BKC, LOADS, NS, GATED>(g, find_row_block(g, BM, rb),
                                                          cb * (GATED ? BN / 2 : BN), ring);
 #endif
 }
@@ -801,7 +801,7 @@ struct LargeUnit {
 template <class Op, bool BKC, bool GATED>
 __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using S = TileShape<Op, 256, 256, 2, 4, true, BKC, true, 0>;
+  using S = TileShape<Op, 256, 256, 2, 4, true, BKC, kLoadDirect, 0>;
   __shared__ __align__(1024) unsigned char ring[S::kLds];
   const uint32_t grid = g.row_blocks * g.col_blocks + kLargeExtra;
   if (blockIdx.x >= grid) {
@@ -818,20 +818,20 @@ __global__ __launch_bounds__(512) void grouped_large_kernel(GroupedArgs g) {
   const int n0 = (cb * 256 + u.col) / (GATED ? 2 : 1);
   if (r.lo >= r.hi || n0 >= g.n) return;
   if (u.parts == 4)
-    rows_block<Op, 128, 128, 2, 4, BKC, true, 0, GATED>(g, r, n0, ring);
+    rows_block<Op, 128, 128, 2, 4, BKC, kLoadDirect, 0, GATED>(g, r, n0, ring);
   else if (u.parts == 2 || r.hi - r.lo <= 128)
-    rows_block<Op, 128, 256, 2, 4, BKC, true, 0, GATED>(g, r, n0, ring);
+    rows_block<Op, 128, 256, 2, 4, BKC, kLoadDirect, 0, GATED>(g, r, n0, ring);
   else
-    rows_block<Op, 256, 256, 2, 4, BKC, true, 0, GATED>(g, r, n0, ring);
+    rows_block<Op, 256, 256, 2, 4, BKC, kLoadDirect, 0, GATED>(g, r, n0, ring);
 #endif
 }
 
 // D_e block: the BM columns of P from m0 (rows of the result) by the BN
 // columns of Q from n0, over the slots of a group; one without slots writes
 // zeros.  GATHER: 1 if P's rows go through an index, 2 if Q's do.
-template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
+template <class Op, int BM, int BN, int WR, int WC, int LOADS, int NS, int GATHER>
 __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, unsigned char *ring) {
-  using S = TileShape<Op, BM, BN, WR, WC, false, false, DIRECT, NS>;
+  using S = TileShape<Op, BM, BN, WR, WC, false, false, LOADS, NS>;
   int lo, hi;
   group_range(g, group, &lo, &hi);
   lo = __builtin_amdgcn_readfirstlane(lo);
@@ -868,7 +868,7 @@ __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, uns
   for (int i = 0; i < S::FM; ++i)
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) acc[i][j] = typename Op::acc{0, 0, 0, 0};
-  run_stages<Op, S, DIRECT, NS>(
+  run_stages<Op, S, LOADS, NS>(
       acc, ring, st1 - st0, row0, col0, lane,
       [&](int v, int st, unsigned char *slot, bool part) {
         const int left = hi - lo - st * kStep<Op>;
@@ -912,10 +912,10 @@ __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, uns
 
 // row_blocks x col_blocks covers one group's D; the grid holds n_groups of
 // them.
-template <class Op, int BM, int BN, int WR, int WC, bool DIRECT, int NS, int GATHER>
+template <class Op, int BM, int BN, int WR, int WC, int LOADS, int NS, int GATHER>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using S = TileShape<Op, BM, BN, WR, WC, false, false, DIRECT, NS>;
+  using S = TileShape<Op, BM, BN, WR, WC, false, false, LOADS, NS>;
   __shared__ __align__(1024) unsigned char ring[S::kLds];
   const uint32_t per = g.row_blocks * g.col_blocks;
   // runs of blocks dealt to the XCDs in turn: as one part each, the XCD of the
@@ -925,7 +925,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
   const uint32_t block = xcd_logical_block(gridDim.x, kXcdRun), group = block / per;
   int rb, cb;
   band_pos(block - group * per, g.row_blocks, g.col_blocks, 1024 / BM, &rb, &cb);
-  wgrad_block<Op, BM, BN, WR, WC, DIRECT, NS, GATHER>(g, group, rb * BM, cb * BN, ring);
+  wgrad_block<Op, BM, BN, WR, WC, LOADS, NS, GATHER>(g, group, rb * BM, cb * BN, ring);
 #endif
 }
 
@@ -937,7 +937,7 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 template <class Op, int GATHER>
 __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using S = TileShape<Op, 256, 256, 2, 4, false, false, true, 0>;
+  using S = TileShape<Op, 256, 256, 2, 4, false, false, kLoadDirect, 0>;
   __shared__ __align__(1024) unsigned char ring[S::kLds];
   const uint32_t per = g.row_blocks * g.col_blocks;
   LargeUnit u;
@@ -948,11 +948,11 @@ __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g)
   const int m0 = rb * 256 + u.row, n0 = cb * 256 + u.col;
   if (m0 >= g.m || n0 >= g.n) return;
   if (u.parts == 4)
-    wgrad_block<Op, 128, 128, 2, 4, true, 0, GATHER>(g, group, m0, n0, ring);
+    wgrad_block<Op, 128, 128, 2, 4, kLoadDirect, 0, GATHER>(g, group, m0, n0, ring);
   else if (u.parts == 2 || g.m - m0 <= 128)
-    wgrad_block<Op, 128, 256, 2, 4, true, 0, GATHER>(g, group, m0, n0, ring);
+    wgrad_block<Op, 128, 256, 2, 4, kLoadDirect, 0, GATHER>(g, group, m0, n0, ring);
   else
-    wgrad_block<Op, 256, 256, 2, 4, true, 0, GATHER>(g, group, m0, n0, ring);
+    wgrad_block<Op, 256, 256, 2, 4, kLoadDirect, 0, GATHER>(g, group, m0, n0, ring);
 #endif
 }
 
@@ -988,8 +988,8 @@ struct SkinnyShape {
   using TB = Tile<Op, BN, BKC>;
   using FA = Fragments<Op, TA, true, FM>;
   using FB = Fragments<Op, TB, BKC, FN>;
-  using LA = Loader<Op, BM, true, 1, true>;
-  using LB = Loader<Op, BN, BKC, 1, true>;
+  using LA = Loader<Op, BM, true, 1, kLoadDirect>;
+  using LB = Loader<Op, BN, BKC, 1, kLoadDirect>;
   static constexpr int kRows = BM;
   static constexpr int kScaleAt = TA::kBytes + TB::kBytes;
   static_assert(!kBlocks<Op> || BM + BN <= 64, "a lane for each scale");
@@ -1028,14 +1028,14 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
   const int stages = (g.k + kStep<Op> - 1) / kStep<Op>;
   const int mine = stages > wave ? (stages - wave + NW - 1) / NW : 0;
   const int64_t k0 = static_cast<int64_t>(wave) * kStep<Op>;
-  la.init_k(0, lane, g.k, [&](int i) {
+  la.init_k(0, lane, [&](int i) {
     const int s = r.lo + i < r.hi ? r.lo + i : r.hi - 1;
     return g.a + (slot_row(g.a_rows, g.n_a, s) * g.lda + k0) * kElem<Op>;
   });
   const char *bg = g.b + r.group * g.b_group * kElem<Op>;
   int64_t b_step;
   if constexpr (BKC) {
-    lb.init_k(0, lane, g.k, [&](int i) {
+    lb.init_k(0, lane, [&](int i) {
       int shift = 0, n = n0 + i;
       if constexpr (GATED) n = gated_col<BN>(i, n0, g.n, &shift);
       n = n < g.n ? n : g.n - 1;
@@ -1060,7 +1060,7 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
 #pragma unroll
     for (int v = 0; v < S::LB::kLoads; ++v)
       lb.load(v, slot + S::TA::kBytes, 0, left, NW * b_step, true);
-    if constexpr (kBlocks<Op>) scales.load<true>(slot + S::kScaleAt, 0, NW);
+    if constexpr (kBlocks<Op>) scales.load<kLoadDirect>(slot + S::kScaleAt, 0, NW);
   };
   typename S::FA fa;
   typename S::FB fb;
