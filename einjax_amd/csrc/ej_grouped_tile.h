@@ -853,12 +853,17 @@ __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, uns
   }
   la.init_m(wave, lane, g.a + (GATHER == 1 ? 0 : lo * g.lda * kElem<Op>), g.lda, m0, g.m);
   lb.init_m(wave, lane, g.b + (GATHER == 2 ? 0 : lo * g.ldb * kElem<Op>), g.ldb, n0, g.n);
-  // the gathered operand's rows of a stage, lane by lane, read a stage ahead
+  // The gathered operand's rows of a stage, lane by lane, read a stage ahead.
+  // Their bounds are checked when they are used: that waits for their load, and
+  // with it for the loads before it.
   const int32_t *rows = GATHER == 1 ? g.a_rows : g.b_rows;
   const int64_t n_rows = GATHER == 1 ? g.n_a : g.n_b;
   auto rows_of = [&](int st) {
     const int64_t s = lo + static_cast<int64_t>(st) * kStep<Op> + lane;
-    return static_cast<int>(slot_row(rows, n_rows, static_cast<int>(s < hi ? s : hi - 1)));
+    return rows[s < hi ? s : hi - 1];
+  };
+  auto in_bounds = [&](int r) {
+    return r < 0 ? 0 : r < n_rows ? r : static_cast<int>(n_rows - 1);
   };
   int row_now = 0, row_next = 0;
   if (GATHER && st1 > st0) row_next = rows_of(0);
@@ -877,7 +882,7 @@ __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, uns
         if (v < S::LA::kLoads) {
           if constexpr (GATHER == 1) {
             if (v == 0) {
-              row_now = row_next;
+              row_now = in_bounds(row_next);
               row_next = rows_of(st + 1);
               la.seek(g.a, g.lda, row_now);
             }
@@ -887,7 +892,7 @@ __device__ inline void wgrad_block(GroupedArgs g, int group, int m0, int n0, uns
           const int u = v - S::LA::kLoads;
           if constexpr (GATHER == 2) {
             if (u == 0) {
-              row_now = row_next;
+              row_now = in_bounds(row_next);
               row_next = rows_of(st + 1);
               lb.seek(g.b, g.ldb, row_now);
             }
@@ -930,10 +935,11 @@ __global__ __launch_bounds__(WR *WC * 64) void grouped_wgrad_kernel(GroupedArgs 
 }
 
 // The same in blocks of 256 x 256, cut as grouped_large_kernel's.  16384 rows
-// in 16 groups, 2048 x 4096 bf16: 272 us (1010 TFLOP/s), 306 with P gathered
-// (128 x 128: 350 and 442, 64 x 64: 522 and 721).  The bounds check of a row's
-// index, in rows_of, follows its load, and waiting for that is waiting for every
-// load in flight: each stage empties the ring that the others keep full.
+// in 16 groups, 2048 x 4096 bf16: 269 us (1020 TFLOP/s), 300 with P gathered
+// (bounds checked as soon as the index is loaded: 316).  A lane that uses an
+// index waits for its load, and with it for the loads of the other operand issued
+// before: each stage drains half of the ring.  Indices through the scalar cache
+// took 321 to 400: with scalar loads under way every wait for LDS is one for all.
 template <class Op, int GATHER>
 __global__ __launch_bounds__(512) void grouped_wgrad_large_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
