@@ -285,7 +285,21 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
   }
 }
 
-// Products of 8-bit floats with block scales.
+// Products of 8-bit floats with block scales.  Measured (us), 16-bit results:
+//   rows/group  groups     k x n      skinny  64 x 64  64 x 128  128 x 128  large
+//       48        1   4096 x 8192      11       19        26        26       23
+//      128        1   4096 x 4096      14       18        26        25       21
+//      256        1   4096 x 4096      25       19        26        26       21
+//       50       16   2048 x 2048      28       15        16        16       20
+//      100        8   2048 x 2048      28       13        17        16       16
+//      100       16   2048 x 2048      48       21        19        18       21
+//      200       16   2048 x 2048      88       35        34        26       23
+//      512       16   2048 x 2048     208       65        68        46       37
+//     1024        4   1024 x 1024      38       12        12        11       10
+// 128 x 128 in four waves 23 to 54 where eight take 16 to 46.  Results in fp32 (no
+// large blocks): 17 in 64 x 64 for 50 rows in 16 groups, 23 in 128 x 128; 28 and 25
+// for 100; 97 and 77 for 512.  Through registers (6 groups of 259, 1000 x 1283) 13
+// in 64 x 64 and in 128 x 128; 8 of 500, 1000 x 2000: 27 and 23.
 template <class Op>
 int pick_f8(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
@@ -295,22 +309,22 @@ int pick_f8(const GroupedRows &r, hipStream_t stream) {
   if (!r.direct) {
     if (short_rows<Op, true>(g))
       return launch_rows<Op, 64, 64, 2, 2, true, kLoadElements, 2>(g, stream);
-    if (tiles <= 512 || rows <= 128)
-      return launch_rows<Op, 64, 64, 2, 2, true, kLoadPieces, 2>(g, stream);
+    if (tiles <= 704) return launch_rows<Op, 64, 64, 2, 2, true, kLoadPieces, 2>(g, stream);
     return launch_rows<Op, 128, 128, 2, 4, true, kLoadPieces, 2>(g, stream);
   }
-  if (few_rows(rows, tiles, 1)) return launch_skinny<Op, 32, 4, true, 2>(g, stream);
-  if (rows <= 48 || tiles <= 576)
-    return launch_rows<Op, 64, 64, 2, 2, true, kLoadDirect, 3>(g, stream);
-  // the large blocks' offsets of rows, in 32 bits
-  const bool near = g.ldb < (1 << 24) && g.lda < (1 << 24) &&
-                    (!g.a_rows || g.n_a <= (int64_t{1} << 32) / (g.lda > 128 ? g.lda : 128));
+  if (rows <= 16 || (rows <= 128 && tiles <= 192))
+    return launch_skinny<Op, 32, 4, true, 2>(g, stream);
+  if (tiles <= 704) return launch_rows<Op, 64, 64, 2, 2, true, kLoadDirect, 2>(g, stream);
   if constexpr (__is_same(Op, OpF8)) {
+    // the large blocks' offsets of rows, in 32 bits
+    const bool near = g.ldb < (1 << 24) && g.lda < (1 << 24) &&
+                      (!g.a_rows || g.n_a <= (int64_t{1} << 32) / (g.lda > 128 ? g.lda : 128));
     const double small = expected_tiles(g, 128, 128, groups) / 512;
-    if (near && large_rounds(expected_tiles(g, 256, 256, groups)) <= 0.8 * (small > 1 ? small : 1))
+    if (near && rows > 128 &&
+        large_rounds(expected_tiles(g, 256, 256, groups)) <= (small > 1 ? small : 1))
       return launch_large<Op, true>(g, stream);
   }
-  return launch_rows<Op, 128, 128, 2, 2, true, kLoadDirect, 2>(g, stream);
+  return launch_rows<Op, 128, 128, 2, 4, true, kLoadDirect, 2>(g, stream);
 }
 
 }  // namespace ej
