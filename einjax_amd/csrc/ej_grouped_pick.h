@@ -170,10 +170,10 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const double tiles = expected_tiles(g, 64, 64, groups);
   if (!r.direct) {
     // (us) 64 x 64, 64 x 128 and 128 x 128; in 12 groups 3022 x 771 x 1283
-    // f16 38, 31, 33, fp32 120, 103, 130; in 4 groups 6000 x 1001 x 1001 fp32
-    // 157, 126, 157; in 6 3000 x 517 x 2051 f16 31, 32, 25; few tiles: in 8
-    // groups 800 x 771 x 1283 f16 19, 18, 22; in 4 2000 x 255 x 333 fp32 13, 16,
-    // 24, 8 bits 7 and 9 in 128 x 128
+    // f16 38, 31, 31, fp32 85, 90, 115; in 4 groups 6000 x 1001 x 1001 f16 45,
+    // 35, 36, fp32 139, 115, 146; in 6 3000 x 517 x 2051 f16 31, 30, 25; few
+    // tiles: in 8 groups 800 x 771 x 1283 f16 17, 18, 21; in 4 2000 x 255 x 333
+    // fp32 11, 14, 22, 8 bits 7 and 9 in 128 x 128
     if (tiles <= 512 || rows <= 128)
       return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2>(g, stream);
     if constexpr (kElem<Op> == 4)
@@ -216,10 +216,9 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
 //   16384    16   2048 x 4096   522/721    350/442   273/308
 // fp32: 4096 rows, 8 groups, 1024 x 2048: 128 x 128 153, 64 x 64 173; 1200
 // rows, 5 groups, 320 x 520: 32 and 13.  Through registers, f16, 64 x 64 and 128
-// x 128: 16384 rows, 8 groups, 1023 x 2047 267/294 and 182/200; 4096, 4, 771 x
-// 1283 52/56 and 43/49; 5820, 7, 512 x 1477 43/51 and 43/47, in very
-// unequal groups 16 more (few tiles of the longest one); fp32 4096, 4, 771 x
-// 1283 153 and 200.
+// x 128: 16384 rows, 8 groups, 1023 x 2047 219/222 and 131/136; 4096, 4, 771 x
+// 1283 41/44 and 35/37; 5820, 7, 512 x 1477 33/34 and 29/29; fp32 4096, 4, 771
+// x 1283 109 and 140.
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
   auto tiles = [&](int b) {
@@ -229,7 +228,7 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
     if (g.m < kChunk<Op> || g.n < kChunk<Op>)
       return launch_wgrad<Op, 64, 64, 2, 2, kLoadElements, 2>(g, stream);
     if constexpr (kElem<Op> == 2) {
-      if (g.splits == 1 && tiles(128) >= 512)
+      if (g.splits == 1 && tiles(128) >= 256)
         return launch_wgrad<Op, 128, 128, 2, 4, kLoadPieces, 2>(g, stream);
     }
     return launch_wgrad<Op, 64, 64, 2, 2, kLoadPieces, 2>(g, stream);
@@ -262,12 +261,15 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
   };
   const double tiles = tiles_of(64, 64);
   if (!r.direct) {
+    // (us) 64 x 64, 64 x 128, 128 x 128 in waves of 64 x 32 and of 32 x 64: 3022
+    // picks in 12 groups, 771 x 2566 f16 67, 54, 50, 48, [n][k] 50, 47, 44, 44;
+    // 12000 in 4, 1023 x 2042 182, 130, 105, 100; few: 600 in 12 23, 22, 28, 28
     if (tiles <= 512 || rows <= 128)
       return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2, true>(g, stream);
     if constexpr (kElem<Op> == 4)
       return launch_rows<Op, 64, 128, 2, 4, BKC, kLoadPieces, 2, true>(g, stream);
     else
-      return launch_rows<Op, 128, 128, 2, 4, BKC, kLoadPieces, 2, true>(g, stream);
+      return launch_rows<Op, 128, 128, 4, 2, BKC, kLoadPieces, 2, true>(g, stream);
   }
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
   if (few_rows(rows, tiles, kElem<Op>))
