@@ -101,6 +101,12 @@ __device__ inline void fill_zero(T *p, int64_t count, uint32_t first) {
   if (mine < count % N) p[count / N * N + mine] = static_cast<T>(0.f);
 }
 
+// LDS accesses of the wave's lanes before and behind stay in this order.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Few tokens: one workgroup sorts them in LDS, digit by digit, in one launch; the
 // workgroups behind it clear the gradient meanwhile.  Each of its 16 waves takes
 // a run of the sequence, 64 tokens at a time.  A pass counts every wave's digits,
@@ -196,9 +202,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_few_kernel(const Token *tok
       int32_t *at = &place[digit * kSortWaves + wave];
       const int32_t base = there ? *at : 0;
       // every lane has read before the first of each digit moves it on
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
       if (there && rank == 0) *at = base + __popcll(same);
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
       if (there) {
         key_of[base + rank] = key[r];
         token_of[base + rank] = token[r];
