@@ -90,14 +90,24 @@ int split_parts(double tiles, int64_t contraction, int elem, bool whole, double 
   return saved > 5 + parts * sums * 8 / 4e6 ? static_cast<int>(parts) : 1;
 }
 
-// n: columns of W
-int rows_parts(const ej_grouped_desc *d, int64_t n) {
+// n: columns of W.
+//
+// A few rows' gated products with W [k][n]: 32 columns of each projection are half a
+// line, so blocks of twice the columns would be wanted and leave CUs idle; with k
+// in parts instead (us, bf16, without / with 4 parts, weights from memory): 1 x
+// 2048 x 4096 18/16, 1 x 4096 x 22016 54/45, 8 x 4096 x 8192 33/25, 40 x 4096 x
+// 8192 33/27, 2 x 2048 x 4096 in 2 groups 19/16; 16 x 1024 x 8192 12/13, 32 x 2048
+// x 4096 in 16 groups 62/68.
+int rows_parts(const ej_grouped_desc *d, int64_t n, bool gated = false) {
   if (scaled_8(d->dtype) || d->n_groups == 0 || d->n_slots == 0) return 1;
   const int64_t groups = d->n_groups < d->n_slots ? d->n_groups : d->n_slots;
   const double rows = static_cast<double>(d->n_slots) / groups;
   const double tiles = (rows / 64 + 0.5) * groups * ceil_div(n, 64);
   const int elem = elem_size(d->dtype);
   const bool whole = whole_chunks(d);
+  if (gated && whole && elem == 2 && d->w_order == EJ_W_KN && few_rows(rows, tiles, elem) &&
+      tiles <= 256 && d->k >= 2048)
+    return 4;
   // the kernel for few rows splits k by itself
   if (whole && few_rows(rows, tiles, elem) && (rows <= 16 || tiles > 64)) return 1;
   return split_parts(tiles, d->k, elem, whole, static_cast<double>(d->n_slots) * n);
@@ -266,7 +276,7 @@ extern "C" int ej_gated_gemm_workspace_size(const ej_grouped_desc *d, size_t *by
   EJ_TRY(check_gated(d));
   EJ_CHECK_ARG(bytes, "null bytes");
   const int64_t n2 = 2 * static_cast<int64_t>(d->n);
-  const int parts = rows_parts(d, n2);
+  const int parts = rows_parts(d, n2, true);
   *bytes = parts > 1 ? sizeof(float) * parts * d->n_slots * n2 : 0;
   return EJ_OK;
 }
@@ -287,7 +297,7 @@ extern "C" int ej_gated_gemm(const ej_grouped_desc *d, int32_t activation, const
   GroupedRows r = rows_args(d, x, rows, offsets, w, out);
   r.g.gate_up = gate_up;
   r.g.activation = activation;
-  EJ_TRY(check_workspace(rows_parts(d, n2), d->n_slots * n2, workspace, workspace_bytes, &r.g));
+  EJ_TRY(check_workspace(rows_parts(d, n2, true), d->n_slots * n2, workspace, workspace_bytes, &r.g));
   switch (d->dtype) {
     case EJ_BF16: return gated_rows_bf16(r, as_stream(stream));
     case EJ_F16: return gated_rows_f16(r, as_stream(stream));

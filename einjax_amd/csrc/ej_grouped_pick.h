@@ -243,8 +243,22 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
   return launch_wgrad<Op, 128, 128, 2, 2, kLoadDirect, 2>(g, stream);
 }
 
-// Gated rows: the same rules, with the columns of both projections for the
-// tiles' (each tile's epilogue gives half as many results).
+// Gated rows, by the columns of both projections.  Measured (us), bf16, W [n][k] /
+// [k][n], n both projections', weights from memory in the first five lines:
+//   rows/group  groups     k x n      skinny  64 x 64  64 x 128  128 x 128  large
+//        16        1   4096 x 8192    15/34   29/36     34/38      61/60    50/56
+//         8        8   1024 x 1024     6/11   10/11     12/12      18/19    15/17
+//         2       16   2048 x 4096    44/49   60/57     56/48      59/46    60/51
+//        16       16   2048 x 4096    55/70   63/61     63/53      67/55    69/54
+//        32       16   2048 x 4096    79/100  65/64     63/54      67/56    69/54
+//        50        8   2048 x 2048    21/27   15/16     19/19      25/25    20/23
+//        50       16   2048 x 2048    40/50   27/28     26/28      27/27    28/30
+//       100       16   2048 x 2048    67/80   37/38     33/31      27/28    28/30
+//       200       16   2048 x 2048   126/142  55/77     46/48      36/34    33/33
+//       512       16   2048 x 2048           115/147  102/101     86/86    75/77
+//      8192        1   4096 x 8192           869/1137 720/748    522/530  391/388
+// [k][n] in 64 columns takes half a line of each projection, so with many tiles 128
+// are better from the first row on.
 template <class Op, bool BKC>
 int pick_gated(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
@@ -272,14 +286,15 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
       return launch_rows<Op, 128, 128, 4, 2, BKC, kLoadPieces, 2, true>(g, stream);
   }
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
-  if (few_rows(rows, tiles, kElem<Op>))
+  const bool wide = !BKC && kElem<Op> == 2 && rows <= 48 && tiles > 512;
+  if (!wide && few_rows(rows, tiles, kElem<Op>))
     return launch_skinny<Op, kSkinny, 4, BKC, 2, true>(g, stream);
   if constexpr (kElem<Op> == 4) {
     return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, 0, true>(g, stream);
   } else {
-    if (rows <= 48 || tiles <= 576)
+    if (!wide && (rows <= 48 || tiles <= 576))
       return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadDirect, 3, true>(g, stream);
-    if (rows <= 100) return launch_rows<Op, 64, 128, 2, 2, BKC, kLoadDirect, 3, true>(g, stream);
+    if (rows <= 64) return launch_rows<Op, 64, 128, 2, 2, BKC, kLoadDirect, 3, true>(g, stream);
     const double small = tiles_of(128, 128) / 512;
     if (large_rounds(tiles_of(256, 256)) <= 0.8 * (small > 1 ? small : 1))
       return launch_large<Op, BKC, true>(g, stream);
