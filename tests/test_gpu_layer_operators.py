@@ -3,6 +3,7 @@ gated product, the second product and the sum, forward and backward, in a graph,
 and the same in 8-bit floating point."""
 
 import runpy
+import threading
 from pathlib import Path
 
 import pytest
@@ -185,3 +186,106 @@ def test_gated_layer_example(gpu):
             for p, g in zip(params, grads):
                 p.sub_(g, alpha=sign * step)
     assert abs((ends[0] - ends[1]) / (2 * step) / size - 1) < 0.02
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_nothing_to_do(gpu, dtype):
+    """No experts, no tokens, no rows, no columns: empty results, or zeros."""
+    def new(*shape):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+    none = ej.group_by_expert(torch.full((5, 2), -1, device="cuda"), 3)
+    for offsets in (torch.zeros(1, dtype=torch.int32, device="cuda"), none):
+        e = 0 if offsets is not none else 3
+        x, w = torch.ones_like(new(10, 16)), torch.ones_like(new(e, 16, 24))
+        h = ej.gated_matmul(x, w, offsets)
+        assert h.shape == (10, 12) and not h.any()
+        gx, gw = ej.gated_matmul_vjp(x, w, offsets, torch.ones_like(h))
+        assert gx.shape == x.shape and gw.shape == w.shape and not gx.any() and not gw.any()
+        (q, qs), (p, ps) = ej.quantize_blocks(x), ej.quantize_blocks(w, block_rows=128)
+        got = ej.fp8_matmul(q, qs, p.transpose(1, 2).contiguous(), ps, offsets)
+        assert got.shape == (10, 24) and not got.any()
+    no_tokens = torch.zeros(0, dtype=torch.int64, device="cuda")
+    table = torch.ones_like(new(4, 8))
+    assert ej.embed_tokens(no_tokens, table).shape == (0, 8)
+    grad = ej.embed_tokens_vjp(no_tokens, table, new(0, 8))
+    assert grad.shape == (4, 8) and not grad.any()
+    tokens = torch.arange(3, device="cuda")
+    out = ej.embed_tokens(tokens, new(0, 8))
+    assert out.shape == (3, 8) and not out.any()
+    assert ej.embed_tokens_vjp(tokens, new(0, 8), new(3, 8)).shape == (0, 8)
+    assert ej.embed_tokens_vjp(tokens, new(4, 0), new(3, 0)).shape == (4, 0)
+
+
+def test_two_graphs_of_one_pool(gpu):
+    """Graphs that share their memory, replayed in turn on new inputs: split
+    contractions, the sorts of few and of many tokens, sums in parts."""
+    g = rng(12)
+    x, w = randn(g, 12, 2048, dtype=BF16), randn(g, 2048, 1024, dtype=BF16, scale=2048 ** -0.5)
+    cot = randn(g, 12, 512, dtype=BF16)
+    tokens = make_tokens(20000, 300, "zipf", 1)
+    few = tokens[:700].clone()
+    table, grad = randn(g, 300, 96, dtype=BF16), randn(g, 20000, 96, dtype=BF16)
+
+    def first():
+        return (ej.gated_matmul(x, w), *ej.gated_matmul_vjp(x, w, None, cot),
+                ej.embed_tokens_vjp(few, table, grad[:700]))
+
+    def second():
+        (q, qs), (p, ps) = ej.quantize_blocks(x), ej.quantize_blocks(w.t(), block_rows=128)
+        return (ej.fp8_matmul(q, qs, p, ps), ej.embed_tokens(tokens, table),
+                ej.embed_tokens_vjp(tokens, table, grad))
+
+    first(), second()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for step in (first, second):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(step())
+        graphs.append(graph)
+    for i in range(4):
+        x.copy_(randn(g, 12, 2048, dtype=BF16))
+        tokens.copy_(make_tokens(20000, 300, "zipf", i + 2))
+        few.copy_(tokens[:700])
+        for graph, step, out in zip(graphs, (first, second), outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_calls_of_two_threads(gpu):
+    """Two threads, a stream each: the same results as one call after the other."""
+    cases = [layer_case(500, 40, 128, 64, 4, BF16), layer_case(90, 60, 77, 131, 5, F16)]
+
+    def work(c):
+        leaves = [c[n].clone().requires_grad_() for n in ("table", "w_in", "w_out")]
+        _, y = run_layer(c, leaves)
+        grads = torch.autograd.grad(y, leaves, c["cot"])
+        q, qs = ej.quantize_blocks(y)
+        w, ws = ej.quantize_blocks(c["w_in"].transpose(1, 2)[0], block_rows=128)
+        return (y.detach(), *grads, ej.fp8_matmul(q, qs, w, ws))
+
+    want = [work(c) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i].append(work(cases[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as error:  # shown by the assertion below
+            errors.append(error)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, runs in zip(want, got):
+        assert len(runs) == 5
+        for b in runs:
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
