@@ -27,7 +27,6 @@ typedef int i32v2_t __attribute__((ext_vector_type(2)));
 typedef int i32v4_t __attribute__((ext_vector_type(4)));
 typedef int i32v8_t __attribute__((ext_vector_type(8)));
 typedef int i32v4_any_t __attribute__((ext_vector_type(4), aligned(1)));
-typedef int word_any_t __attribute__((aligned(1)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 // vectors at any element's alignment
@@ -479,13 +478,8 @@ __device__ inline uint32_t lds_address(const void *p) {
 //   kLoadDirect   16 bytes straight into LDS: rows 16-byte aligned, extents whole
 //                 chunks
 //   kLoadPieces   16 bytes into registers, at any element's alignment, stored to
-//                 LDS a stage later.  Loads off 4 bytes take three times as long
-//                 (18 bytes a cycle from L2, 56 at any multiple of 4), so elements
-//                 of fewer than 4 bytes are loaded from the word that the chunk
-//                 begins in and moved into place when they are stored; the word
-//                 that is missing at the end is the next lane's first.  1511 x 2
-//                 picks, 771 x 2566 f16: 45 us, 51 before.  A chunk that a row
-//                 ends in is loaded from the row's last 16 bytes and shifted down.
+//                 LDS a stage later.  A chunk that a row ends in is loaded from
+//                 the row's last 16 bytes and shifted down when it is stored.
 //   kLoadElements the same, element by element: rows shorter than 16 bytes
 // In the first two no load stands behind a branch, which would have it waited
 // for before the next one.
@@ -545,73 +539,43 @@ struct Loader {
   bool edge;                // M, pieces: the tile reaches past the extent
   int held_left;            // K, pieces: elements of k of the stage that is held
   i32v4_t reg[LOADS == kLoadDirect ? 1 : kLoads];
-  // Pieces of elements of fewer than 4 bytes: the last word of the last chunk of
-  // `run` that follow each other, which the next lane does not have.
-  static constexpr bool kWords = LOADS == kLoadPieces && kElem<Op> < 4;
-  static_assert(!kWords || 16 % T::kChunks == 0, "a line's lanes lie in a row of 16");
-  int last_word[kWords ? kLoads : 1];
-  int run;
-  bool off_words;  // whether any of the wave's sources lies off 4 bytes
-  __device__ inline void look_at_words() {
-    size_t bits = 0;
-#pragma unroll
-    for (int v = 0; v < kLoads; ++v) bits |= reinterpret_cast<size_t>(src[v]);
-    off_words = __any((bits & 3) != 0);
-  }
-
-  // Line and chunk of the lane's place in load v.  Through registers the lanes
-  // follow each other along a line, and the swizzle is in the address they store to.
-  __device__ static inline void place(int v, int wave, int lane, int *at_line, int *chunk) {
-    const int pos = (v * NW + wave) * 64 + lane;
-    if constexpr (LOADS == kLoadDirect) {
-      T::at(pos, at_line, chunk);
-    } else {
-      *at_line = pos / T::kChunks;
-      *chunk = pos % T::kChunks;
-    }
-  }
-  __device__ inline bool last_of_run(int lane) const { return (lane & (run - 1)) == run - 1; }
 
   // k element (K) or k-row (M) of the lane's place in load v; in K tiles the
   // swizzle repeats every 16 rows, and differs by 4 between its halves.
   __device__ inline int line_at(int v) const {
-    if constexpr (KC)
-      return LOADS != kLoadDirect || NW % 2 == 0 || v % 2 == 0 ? line : line ^ (4 * kChunk<Op>);
+    if constexpr (KC) return NW % 2 == 0 || v % 2 == 0 ? line : line ^ (4 * kChunk<Op>);
     else return line + v * kApart;
   }
 
   // K tiles: row_at(i) is the address of output row i's first k element.
   template <class RowAt>
   __device__ inline void init_k(int wave, int lane, RowAt row_at) {
-    run = T::kChunks;
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
       int row, chunk;
-      place(v, wave, lane, &row, &chunk);
+      T::at((v * NW + wave) * 64 + lane, &row, &chunk);
       if (v == 0) line = chunk * kChunk<Op>;
       src[v] = row_at(row) + chunk * 16;
     }
-    if constexpr (kWords) look_at_words();
   }
   // M tiles: column col0 + i of the operand is output row i; extent `ext`.
   __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int col0,
                                 int ext) {
-    init_m(wave, lane, base, ld, ext, ROWS, [&](int i, int *shift) {
+    init_m(wave, lane, base, ld, ext, [&](int i, int *shift) {
       *shift = 0;
       return col0 + i;
     });
   }
   // M tiles: output row i is column col_at(i, &shift) of an extent `ext` that
-  // begins at column shift; `cols` columns (a power of two) follow each other.
+  // begins at column shift; a chunk's columns follow each other.
   template <class ColAt>
-  __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int ext, int cols,
+  __device__ inline void init_m(int wave, int lane, const char *base, int64_t ld, int ext,
                                 ColAt col_at) {
-    run = cols / kChunk<Op>;
     edge = false;
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) {
       int krow, chunk;
-      place(v, wave, lane, &krow, &chunk);
+      T::at((v * NW + wave) * 64 + lane, &krow, &chunk);
       if (v == 0) line = krow;
       if (v < kCols) {
         int shift, c = col_at(chunk * kChunk<Op>, &shift);
@@ -625,7 +589,6 @@ struct Loader {
       src[v] = base + (line_at(v) * ld + col[v % kCols]) * kElem<Op>;
     }
     if constexpr (LOADS == kLoadPieces) edge = __any(edge);
-    if constexpr (kWords) look_at_words();
   }
 
   // Starts load v of the next stage, of which `left` elements of k exist
@@ -644,14 +607,6 @@ struct Loader {
         held_left = left;
       }
       p = there > 0 ? p : zeros;
-      if constexpr (kWords) {
-        const bool words = off_words && (KC ? left >= kStep<Op> : !edge);
-        // the word's alignment is the address's, in any address space
-        const int off = words ? static_cast<int>(reinterpret_cast<size_t>(p) & 3) : 0;
-        if (words && last_of_run(threadIdx.x & 63))
-          last_word[v] = *(const __attribute__((address_space(1))) word_any_t *)(p + 12);
-        p -= off;
-      }
       // as global memory: a load that might be of LDS is waited for with the
       // LDS reads
       reg[v] = *(const __attribute__((address_space(1))) i32v4_any_t *)(p);
@@ -664,21 +619,6 @@ struct Loader {
   // Not direct: what load() fetched, into the tile at `tile`.
   __device__ inline void store(unsigned char *tile, int wave, int lane) {
     constexpr int N = kChunk<Op>;
-    if constexpr (kWords) {
-      if (off_words && (KC ? held_left >= kStep<Op> : !edge))
-#pragma unroll
-        for (int v = 0; v < kLoads; ++v) {
-          // a stage's step is a multiple of 4 bytes: the offset is still the source's
-          const int off = static_cast<int>(reinterpret_cast<size_t>(src[v]) & 3);
-          const int next = __builtin_amdgcn_update_dpp(0, reg[v][0], 0x101, 0xf, 0xf, false);
-          i32v4_t w;
-#pragma unroll
-          for (int i = 0; i < 3; ++i) w[i] = __builtin_amdgcn_alignbyte(reg[v][i + 1], reg[v][i], off);
-          const int end = __builtin_amdgcn_alignbyte(next, reg[v][3], off);
-          w[3] = last_of_run(lane) ? last_word[v] : end;
-          reg[v] = w;
-        }
-    }
     if constexpr (LOADS == kLoadPieces && KC) {
       if (held_left < kStep<Op>)
 #pragma unroll
@@ -696,12 +636,8 @@ struct Loader {
         }
     }
 #pragma unroll
-    for (int v = 0; v < kLoads; ++v) {
-      int at_line, chunk;
-      place(v, wave, lane, &at_line, &chunk);
-      chunk ^= KC ? swz_k(at_line) : swz_m<Op, T::kChunks>(at_line);
-      *reinterpret_cast<i32v4_t *>(tile + (at_line * T::kChunks + chunk) * 16) = reg[v];
-    }
+    for (int v = 0; v < kLoads; ++v)
+      *reinterpret_cast<i32v4_t *>(tile + ((v * NW + wave) * 64 + lane) * 16) = reg[v];
   }
 
   // M tiles of gathered rows (weight gradient): the sources of the stage whose
@@ -712,7 +648,6 @@ struct Loader {
     for (int v = 0; v < kLoads; ++v) r[v] = __shfl(row, line_at(v));
 #pragma unroll
     for (int v = 0; v < kLoads; ++v) src[v] = base + (r[v] * ld + col[v % kCols]) * kElem<Op>;
-    if constexpr (kWords) look_at_words();
   }
 };
 

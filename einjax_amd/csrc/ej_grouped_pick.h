@@ -170,9 +170,9 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
   const double tiles = expected_tiles(g, 64, 64, groups);
   if (!r.direct) {
     // (us) 64 x 64, 64 x 128 and 128 x 128; in 12 groups 3022 x 771 x 1283
-    // f16 38, 31, 31, fp32 85, 90, 115; in 4 groups 6000 x 1001 x 1001 f16 45,
-    // 35, 36, fp32 139, 115, 146; in 6 3000 x 517 x 2051 f16 31, 30, 25; few
-    // tiles: in 8 groups 800 x 771 x 1283 f16 17, 18, 21; in 4 2000 x 255 x 333
+    // f16 34, 30, 29, fp32 85, 88, 113; in 4 groups 6000 x 1001 x 1001 f16 45,
+    // 33, 34, fp32 135, 112, 145; in 6 3000 x 517 x 2051 f16 29, 28, 23; few
+    // tiles: in 8 groups 800 x 771 x 1283 f16 14, 15, 19; in 4 2000 x 255 x 333
     // fp32 11, 14, 22, 8 bits 7 and 9 in 128 x 128
     if (tiles <= 512 || rows <= 128)
       return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2>(g, stream);
@@ -216,9 +216,9 @@ int pick_rows(const GroupedRows &r, hipStream_t stream) {
 //   16384    16   2048 x 4096   522/721    350/442   273/308
 // fp32: 4096 rows, 8 groups, 1024 x 2048: 128 x 128 153, 64 x 64 173; 1200
 // rows, 5 groups, 320 x 520: 32 and 13.  Through registers, f16, 64 x 64 and 128
-// x 128: 16384 rows, 8 groups, 1023 x 2047 219/222 and 131/136; 4096, 4, 771 x
-// 1283 41/44 and 35/37; 5820, 7, 512 x 1477 33/34 and 29/29; fp32 4096, 4, 771
-// x 1283 109 and 140.
+// x 128: 16384 rows, 8 groups, 1023 x 2047 209/205 and 122/125; 4096, 4, 771 x
+// 1283 36/39 and 30/34; 5820, 7, 512 x 1477 29/31 and 25/27; fp32 4096, 4, 771 x
+// 1283 108 and 138.
 template <class Op>
 int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
   auto tiles = [&](int b) {
@@ -275,15 +275,23 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
   };
   const double tiles = tiles_of(64, 64);
   if (!r.direct) {
-    // (us) 64 x 64, 64 x 128, 128 x 128 in waves of 64 x 32 and of 32 x 64: 3022
-    // picks in 12 groups, 771 x 2566 f16 67, 54, 50, 48, [n][k] 50, 47, 44, 44;
-    // 12000 in 4, 1023 x 2042 182, 130, 105, 100; few: 600 in 12 23, 22, 28, 28
-    if (tiles <= 512 || rows <= 128)
-      return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2, true>(g, stream);
-    if constexpr (kElem<Op> == 4)
+    if constexpr (kElem<Op> == 4) {
+      if (tiles <= 512 || rows <= 128)
+        return launch_rows<Op, 64, 64, 2, 2, BKC, kLoadPieces, 2, true>(g, stream);
       return launch_rows<Op, 64, 128, 2, 4, BKC, kLoadPieces, 2, true>(g, stream);
-    else
+    } else {
+      // The columns of a wave lie in two runs, which its loads of [k][n] take one by
+      // one: longer runs, fewer lines.  (us) 64 x 64 in 2 x 2 and 4 x 1 waves, 64 x
+      // 128 in 4 x 2, 128 x 128 in 2 x 4 and 4 x 2, f16: 3022 picks in 12 groups, 771
+      // x 2566 71, 56, 44, 53, 44, [n][k] 48, 48, 42, 42, 42; 12000 in 4, 1023 x 2042
+      // 212, 155, 121, 117, 92; 600 in 12 26, 23, 20, 35, 25; 200 in 12, [n][k]
+      // 16, 15, 16, 19, 19
+      if (tiles <= 512)
+        return launch_rows<Op, 64, 64, 4, 1, BKC, kLoadPieces, 2, true>(g, stream);
+      if (rows <= 128)
+        return launch_rows<Op, 64, 128, 4, 2, BKC, kLoadPieces, 2, true>(g, stream);
       return launch_rows<Op, 128, 128, 4, 2, BKC, kLoadPieces, 2, true>(g, stream);
+    }
   }
   constexpr int kSkinny = BKC || kElem<Op> == 4 ? 32 : 64;
   const bool wide = !BKC && kElem<Op> == 2 && rows <= 48 && tiles > 512;
@@ -315,8 +323,9 @@ int pick_gated(const GroupedRows &r, hipStream_t stream) {
 //     1024        4   1024 x 1024      38       12        12        11       10
 // 128 x 128 in four waves 23 to 54 where eight take 16 to 46.  Results in fp32 (no
 // large blocks): 17 in 64 x 64 for 50 rows in 16 groups, 23 in 128 x 128; 28 and 25
-// for 100; 97 and 77 for 512.  Through registers (6 groups of 259, 1000 x 1283) 13
-// in 64 x 64 and in 128 x 128; 8 of 500, 1000 x 2000: 27 and 23.
+// for 100; 97 and 77 for 512.  Through registers 64 x 64 in four waves and in
+// eight, 128 x 128: 6 groups of 259, 1000 x 1283 14, 14, 14; 8 of 500, 1000 x 2000
+// 29, 31, 27; 1 of 16, 4090 x 4096 24, 22, 36; 4 of 150, 4001 x 1000 32, 31, 48.
 template <class Op>
 int pick_f8(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
@@ -326,6 +335,7 @@ int pick_f8(const GroupedRows &r, hipStream_t stream) {
   if (!r.direct) {
     if (short_rows<Op, true>(g))
       return launch_rows<Op, 64, 64, 2, 2, true, kLoadElements, 2>(g, stream);
+    if (tiles <= 256) return launch_rows<Op, 64, 64, 4, 2, true, kLoadPieces, 2>(g, stream);
     if (tiles <= 704) return launch_rows<Op, 64, 64, 2, 2, true, kLoadPieces, 2>(g, stream);
     return launch_rows<Op, 128, 128, 2, 4, true, kLoadPieces, 2>(g, stream);
   }

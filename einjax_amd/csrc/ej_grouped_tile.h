@@ -673,7 +673,7 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
     b_step = kRowB;
   } else {
     if constexpr (GATED)
-      lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, g.n, S::WN / 2,
+      lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, g.n,
                 [&](int i, int *shift) { return gated_col<S::WN>(i, n0, g.n, shift); });
     else
       lb.init_m(wave, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
@@ -743,8 +743,10 @@ __device__ inline void rows_block(GroupedArgs g, const RowBlock &r, int n0, unsi
 // instructions (fp32).  4096 rows in 8 groups, k = 1024, n = 2048 in fp32, 64 x
 // 64: 154 us (111 TFLOP/s, of 128 that a large fp32 product reaches).  Rows off
 // 16 bytes (3022 rows in 12 groups, k = 771, n = 1283, f16), 128 x 128 through
-// registers: 31 us, 21 us at aligned extents; the rest are another column of
-// tiles and stage of k, and the loads off 16 bytes, two lines for most of them.
+// registers: 29 us, 21 us at aligned extents; the rest are another column of
+// tiles and stage of k, and the unaligned loads, two lines for most of them.
+// Loads at words with the bytes moved into place when they are stored, the last
+// word from the next lane, took 31.
 template <class Op, int BM, int BN, int WR, int WC, bool BKC, int LOADS, int NS, bool GATED>
 __global__ __launch_bounds__(WR *WC * 64) void grouped_rows_kernel(GroupedArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -1056,7 +1058,7 @@ __global__ __launch_bounds__(NW * 64) void grouped_skinny_kernel(GroupedArgs g) 
     b_step = kRowB;
   } else {
     if constexpr (GATED)
-      lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, g.n, BN / 2,
+      lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, g.n,
                 [&](int i, int *shift) { return gated_col<BN>(i, n0, g.n, shift); });
     else
       lb.init_m(0, lane, bg + k0 * g.ldb * kElem<Op>, g.ldb, n0, g.n);
