@@ -196,7 +196,8 @@ extern "C" int ej_quantize_blocks(const void *x, int32_t dtype, int64_t n_mats, 
   EJ_CHECK_ARG(x && q && scale, "null argument");
   EJ_CHECK_ARG(ld >= n, "row stride %lld below n = %d", (long long)ld, n);
   // a launch holds fewer than 2^32 threads
-  const int64_t k_blocks = (static_cast<int64_t>(n) + 127) / 128, most = (int64_t{1} << 32) / kThreads;
+  const int64_t k_blocks = (static_cast<int64_t>(n) + 127) / 128;
+  const int64_t most = (int64_t{1} << 32) / kThreads;
   const int64_t per_mat = block_rows == 1 ? n_rows : ceil_div(n_rows, 128);
   const int64_t held = (block_rows == 1 ? kThreads / 16 : 1) * (most - 1);
   if (n > INT32_MAX - 256 || n_rows > held || n_mats > held || per_mat > held / k_blocks / n_mats) {

@@ -297,7 +297,8 @@ extern "C" int ej_gated_gemm(const ej_grouped_desc *d, int32_t activation, const
   GroupedRows r = rows_args(d, x, rows, offsets, w, out);
   r.g.gate_up = gate_up;
   r.g.activation = activation;
-  EJ_TRY(check_workspace(rows_parts(d, n2, true), d->n_slots * n2, workspace, workspace_bytes, &r.g));
+  EJ_TRY(check_workspace(rows_parts(d, n2, true), d->n_slots * n2, workspace, workspace_bytes,
+                         &r.g));
   switch (d->dtype) {
     case EJ_BF16: return gated_rows_bf16(r, as_stream(stream));
     case EJ_F16: return gated_rows_f16(r, as_stream(stream));
