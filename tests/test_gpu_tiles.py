@@ -12,7 +12,9 @@ import torch
 import einjax_amd as ej
 from test_gpu_experts import (BF16, F16, F32, TINY, UNIT, assert_within, product64, randn, rng,
                               sum_bound)
-from test_gpu_fp8 import (LARGE_F8, assert_product, blocks, fp8_64, operands, scales)
+from test_gpu_fp8 import LARGE_F8, assert_product, blocks, fp8_64, operands, scales
+from test_gpu_gated import gated64
+from test_gpu_unaligned_rows import at_offset
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +57,95 @@ def test_fp8_large_blocks_without_groups(gpu, m, k, n, out_dtype):
     got = ej.fp8_matmul(q, qs, w, ws, out_dtype=out_dtype)
     want, size = fp8_64(q, qs, w[None], ws[None], None, None, m)
     assert_product(got, want, size, k, out_dtype)
+
+
+# ---- a middling number of rows a group ------------------------------------------------
+
+# rows of each group, slots of no group, k, n of a plain product
+MIDDLE = [([70, 0, 61, 100, 3, 64, 129, 53], 4, 136, 3336), ([60] * 16, 0, 64, 2048),
+          ([99, 1, 128, 172], 0, 200, 8000)]
+# the same for gated ones, whose n is that of the results: 49 to 64 rows, and
+# fewer with many columns of W [k][n]
+MIDDLE_GATED = [([70, 0, 61, 100, 3, 64, 129, 53], 4, 136, 1640), ([16, 0, 33, 5, 20, 17, 1, 40],
+                                                                   0, 72, 2728),
+                ([16] * 16, 3, 264, 1024)]
+
+
+def product_operands(sizes, dead, k, n, dtype, order):
+    g, slots = rng(k + n), sum(sizes) + dead
+    x = randn(g, slots, k, dtype=dtype)
+    w = randn(g, len(sizes), k, n, dtype=dtype, scale=k ** -0.5)
+    if order == "nk":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    x[slots - dead:] = float("nan")
+    return g, slots, x, w
+
+
+def shuffled(sizes, dead, seed):
+    """The relation of rows in a shuffled order, `dead` of them of no group."""
+    g = torch.Generator().manual_seed(seed)
+    picks = torch.repeat_interleave(torch.arange(len(sizes)), torch.tensor(sizes))
+    picks = torch.cat([picks, torch.full((dead,), -1)])
+    return ej.group_by_expert(picks[torch.randperm(len(picks), generator=g)].cuda()[:, None],
+                              len(sizes))
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("sizes,dead,k,n", MIDDLE)
+def test_grouped_matmul_of_some_rows_a_group(gpu, sizes, dead, k, n, dtype, order):
+    g, slots, x, w = product_operands(sizes, dead, k, n, dtype, order)
+    offsets, live = ends_of(sizes), sum(sizes)
+    got, wide = ej.grouped_matmul(x, w, offsets), ej.grouped_matmul(x, w, offsets, out_dtype=F32)
+    x[live:] = 0
+    want, mag = product64(x, None, offsets, w, slots)
+    assert_within(got, want, sum_bound(want, mag, k, dtype))
+    assert_within(wide, want, sum_bound(want, mag, k, F32))
+    r = shuffled(sizes, dead, n)
+    got = ej.grouped_matmul(x, w, r, gather=True)
+    want, mag = product64(x, r.rows, r.offsets, w, slots)
+    assert_within(got, want, sum_bound(want, mag, k, dtype))
+    assert bool((got[live:] == 0).all())
+
+
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("sizes,dead,k,n", MIDDLE_GATED)
+def test_gated_matmul_of_some_rows_a_group(gpu, sizes, dead, k, n, dtype, order):
+    g, slots, x, w = product_operands(sizes, dead, k, 2 * n, dtype, order)
+    offsets, live = ends_of(sizes), sum(sizes)
+    got = ej.gated_matmul(x, w, offsets)
+    leaf = x.detach().requires_grad_()
+    assert torch.equal(got, ej.gated_matmul(leaf, w, offsets).detach())  # keeps both projections
+    x[live:] = 0
+    h, eh, *_ = gated64(x, None, offsets, w, slots, "silu")
+    assert_within(got, h, eh + UNIT[dtype] * (h.abs() + eh) + TINY[dtype])
+    r = shuffled(sizes, dead, n)
+    got = ej.gated_matmul(x, w, r, activation="gelu_tanh", gather=True)
+    h, eh, *_ = gated64(x, r.rows, r.offsets, w, slots, "gelu_tanh")
+    assert_within(got, h, eh + UNIT[dtype] * (h.abs() + eh) + TINY[dtype])
+    assert bool((got[live:] == 0).all())
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3, 4])
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("k,n", [(77, 1283), (260, 1090)])
+def test_gated_matmul_of_some_unaligned_rows_a_group(gpu, k, n, dtype, order, shift):
+    sizes, dead = [100, 0, 128, 64, 200, 1, 90, 217], 5
+    g, slots, x, w = product_operands(sizes, dead, k, 2 * n, dtype, order)
+    x = at_offset(x, shift)
+    if order == "nk":
+        w = at_offset(w.transpose(1, 2), (shift + 1) % 8).transpose(1, 2)
+    else:
+        w = at_offset(w, (shift + 1) % 8)
+    offsets, live = ends_of(sizes), sum(sizes)
+    got = ej.gated_matmul(x, w, offsets)
+    x[live:] = 0
+    h, eh, *_ = gated64(x, None, offsets, w, slots, "silu")
+    assert_within(got, h, eh + UNIT[dtype] * (h.abs() + eh) + TINY[dtype])
+    r = shuffled(sizes, dead, n)
+    got = ej.gated_matmul(x, w, r, activation="gelu", gather=True)
+    h, eh, *_ = gated64(x, r.rows, r.offsets, w, slots, "gelu")
+    assert_within(got, h, eh + UNIT[dtype] * (h.abs() + eh) + TINY[dtype])
+    assert bool((got[live:] == 0).all())
