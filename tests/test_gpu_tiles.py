@@ -149,3 +149,43 @@ def test_gated_matmul_of_some_unaligned_rows_a_group(gpu, k, n, dtype, order, sh
     h, eh, *_ = gated64(x, r.rows, r.offsets, w, slots, "gelu")
     assert_within(got, h, eh + UNIT[dtype] * (h.abs() + eh) + TINY[dtype])
     assert bool((got[live:] == 0).all())
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("sizes,dead,k,n", [
+    ([100] * 16, 0, 272, 1409), ([128, 90, 0, 200, 7, 64, 150, 99, 100, 33], 6, 400, 2050),
+    ([300, 0, 250, 120, 7, 100], 3, 200, 1300), ([150] * 4, 0, 131, 1500)])
+def test_fp8_matmul_of_some_rows_a_group(gpu, sizes, dead, k, n, out_dtype):
+    g, live, e = rng(k + n), sum(sizes), len(sizes)
+    slots = live + dead
+    w, ws = operands(g, n, k, (e,)), scales(g, e, blocks(n), blocks(k)) * 1e-4
+    q, qs = operands(g, slots, k), scales(g, slots, blocks(k)) * 1e-2
+    qs[live:] = float("nan")
+    got = ej.fp8_matmul(q, qs, w, ws, ends_of(sizes), out_dtype=out_dtype)
+    want, size = fp8_64(q, torch.nan_to_num(qs), w, ws, None, ends_of(sizes), slots)
+    assert_product(got, want, size, k, out_dtype)
+    qs[live:] = 1.0
+    r = shuffled(sizes, dead, n)
+    got = ej.fp8_matmul(q, qs, w, ws, r, gather=True, out_dtype=out_dtype)
+    want, size = fp8_64(q, qs, w, ws, r.rows, r.offsets, slots)
+    assert_product(got, want, size, k, out_dtype)
+    assert bool((got[live:] == 0).all())
+
+
+@pytest.mark.parametrize("sizes,dead,k,n", [([70, 0, 61, 100, 3, 64, 129, 53], 4, 144, 3336),
+                                            ([60] * 16, 0, 64, 2049)])
+def test_int8_matmul_of_some_rows_a_group(gpu, sizes, dead, k, n):
+    g, live, e = rng(k + n), sum(sizes), len(sizes)
+    slots = live + dead
+    q = torch.randint(-128, 128, (slots, k), generator=g, device="cuda").to(torch.int8)
+    w = torch.randint(-128, 128, (e, n, k), generator=g, device="cuda").to(torch.int8)
+    one, ones = torch.ones(slots, device="cuda"), torch.ones(e, n, device="cuda")
+    r = shuffled(sizes, dead, n)
+    for gather, groups in ((False, ends_of(sizes)), (True, r)):
+        got = ej.int8_matmul(q, one, w, ones, groups, gather=gather, out_dtype=F32)
+        x = q[r.rows.long()] if gather else q
+        ends = ends_of(sizes).tolist()
+        for i, (a, b) in enumerate(zip(ends, ends[1:])):
+            # below 2^24: exact
+            assert torch.equal(got[a:b].double(), x[a:b].double() @ w[i].double().T)
+        assert bool((got[live:] == 0).all())
