@@ -14,6 +14,7 @@ from test_gpu_experts import (BF16, F16, F32, TINY, UNIT, assert_within, product
                               sum_bound)
 from test_gpu_fp8 import LARGE_F8, assert_product, blocks, fp8_64, operands, scales
 from test_gpu_gated import gated64
+from test_gpu_tokens import check_gradient, make_tokens
 from test_gpu_unaligned_rows import at_offset
 
 pytestmark = pytest.mark.gpu
@@ -189,3 +190,60 @@ def test_int8_matmul_of_some_rows_a_group(gpu, sizes, dead, k, n):
             # below 2^24: exact
             assert torch.equal(got[a:b].double(), x[a:b].double() @ w[i].double().T)
         assert bool((got[live:] == 0).all())
+
+
+# ---- rows shorter than 16 bytes ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k,n", [(3, 70), (70, 3), (2, 5), (3, 2), (7, 7), (130, 1)])
+def test_products_of_short_rows(gpu, k, n, dtype):
+    """k or n of less than 16 bytes in either order of W, with the gradients,
+    of gathered rows and of rows as they lie."""
+    sizes, dead = [40, 0, 131, 3, 66], 4
+    live = sum(sizes)
+    for order in ("kn", "nk"):
+        g, slots, x, w = product_operands(sizes, dead, k, 2 * n, dtype, order)
+        x[live:] = 0
+        r = shuffled(sizes, dead, n)
+        ends = r.offsets.tolist()
+        grad = randn(g, slots, 2 * n, dtype=dtype)
+        grad[live:] = float("nan")
+        for gather in (False, True):
+            rows = r.rows if gather else None
+            got = ej.grouped_matmul(x, w, r, gather=gather)
+            want, mag = product64(x, rows, r.offsets, w, slots)
+            assert_within(got, want, sum_bound(want, mag, k, dtype))
+            got = ej.gated_matmul(x, w, r, gather=gather)
+            h, eh, *_ = gated64(x, rows, r.offsets, w, slots, "silu")
+            assert_within(got, h, eh + UNIT[dtype] * (h.abs() + eh) + TINY[dtype])
+            gx, gw = ej.grouped_matmul_vjp(x, w, r, grad, gather=gather)
+            slot_x = torch.zeros(slots, k, dtype=torch.double, device="cuda")
+            slot_mag = torch.zeros_like(slot_x)
+            for i, (a, b) in enumerate(zip(ends, ends[1:])):
+                xe = (x[r.rows[a:b].long()] if gather else x[a:b]).double()
+                ge, we = grad[a:b].double(), w[i].double()
+                assert_within(gw[i], xe.T @ ge,
+                              sum_bound(xe.T @ ge, xe.abs().T @ ge.abs(), b - a, dtype))
+                slot_x[a:b], slot_mag[a:b] = ge @ we.T, ge.abs() @ we.abs().T
+            if gather:  # one slot a row
+                want, mag = torch.zeros_like(slot_x), torch.zeros_like(slot_x)
+                at = r.rows[:live].long()
+                want[at], mag[at] = slot_x[:live], slot_mag[:live]
+            else:
+                want, mag = slot_x, slot_mag
+            assert_within(gx, want, sum_bound(want, mag, 2 * n, dtype))
+
+
+# rows of a table shorter than 16 bytes whose sums span chunks of the tokens
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,v,n,kind", [(3000, 3, 1, "zipf"), (3000, 5, 3, "padded"),
+                                        (20000, 4, 2, "one"), (40000, 6000, 3, "zipf"),
+                                        (16384, 300, 3, "runs")])
+def test_table_gradients_of_narrow_rows(gpu, t, v, n, kind, dtype, index):
+    g = rng(t + n)
+    tokens, cot = make_tokens(t, v, kind, 1, index), randn(g, t, n, dtype=dtype)
+    table = randn(g, v, n, dtype=dtype)
+    got = ej.embed_tokens_vjp(tokens, table, cot, scale=1.5)
+    check_gradient(got, tokens, v, cot, 1.5, dtype)
