@@ -12,7 +12,8 @@ import torch
 import einjax_amd as ej
 from test_gpu_experts import (BF16, F16, F32, TINY, UNIT, assert_within, product64, randn, rng,
                               sum_bound)
-from test_gpu_fp8 import LARGE_F8, assert_product, blocks, fp8_64, operands, scales
+from test_gpu_fp8 import (LARGE_F8, QUANTIZED, assert_product, blocks, fp8_64, operands,
+                          plain_blocks, scales)
 from test_gpu_gated import gated64
 from test_gpu_tokens import check_gradient, make_tokens
 from test_gpu_unaligned_rows import at_offset
@@ -247,3 +248,37 @@ def test_table_gradients_of_narrow_rows(gpu, t, v, n, kind, dtype, index):
     table = randn(g, v, n, dtype=dtype)
     got = ej.embed_tokens_vjp(tokens, table, cot, scale=1.5)
     check_gradient(got, tokens, v, cot, 1.5, dtype)
+
+
+# ---- quantization of matrices ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n", QUANTIZED)
+def test_blocks_of_128_rows_reach_the_largest_value(gpu, m, n, dtype):
+    """Every finite 128 x 128 block that is not zero has a value of 448: its
+    largest over the scale is 448 within three roundings.  (Some of float16's
+    pass its range: their blocks have scale NaN and values of 0.)"""
+    g = rng(m * n)
+    x = (randn(g, m, n) * torch.exp(3 * randn(g, m, 1))).to(dtype)
+    x[m // 2:, : n // 2] = 0
+    q, scale = ej.quantize_blocks(x, block_rows=128)
+    padded = torch.nn.functional.pad(q.float().abs(), (0, -n % 128, 0, -m % 128))
+    most = padded.reshape(padded.shape[0] // 128, 128, blocks(n), 128).amax((1, 3))
+    plain = torch.nn.functional.pad(x.float().abs(), (0, -n % 128, 0, -m % 128))
+    top = plain.reshape(most.shape[0], 128, blocks(n), 128).amax((1, 3))
+    live = (top > 0) & torch.isfinite(top)
+    assert torch.equal(scale > 0, live) and torch.equal(torch.isnan(scale), torch.isinf(top))
+    assert torch.equal(most, torch.where(live, 448.0, 0.0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantize_blocks_of_matrices_that_lie_apart(gpu, rows, dtype):
+    g = rng(12)
+    wide = (randn(g, 5, 140, 400) * torch.exp(3 * randn(g, 5, 140, 1))).to(dtype)
+    for x in (wide[:, :130], wide[:, 3:, 1:301], wide[::2, ::2, :7], wide[:, :1, 5:],
+              wide[:1].expand(4, 140, 400)):
+        q, scale = ej.quantize_blocks(x, block_rows=rows)
+        want, by = plain_blocks(x, rows)
+        assert torch.equal(scale, by) and torch.equal(q.float(), want)
