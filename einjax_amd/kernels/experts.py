@@ -142,8 +142,10 @@ def fp8_matmul(q, q_scale, w, w_scale, groups=None, *, gather: bool = False,
     not pass), is added up in float32 and rounded once to out_dtype (float32,
     bfloat16 or float16).  For 16-bit results the 8-bit matrix instructions form
     the blocks' sums: of 8 consecutive k they drop what lies below 2^-13 of the
-    largest product.  For float32 ones the sums are formed in float32, at half
-    the rate.
+    largest product, at most 7 2^-13 of the sum of the largest magnitudes.  Where
+    products do not cancel, that is below bfloat16's rounding; float16's it may
+    pass if they are far apart.  For float32 results the sums are formed in
+    float32, at half the rate.
 
     Without groups: w [n, k] or [1, n, k], w_scale [ceil(n / 128),
     ceil(k / 128)] or with a leading 1, the dense product [m, n].  With groups
