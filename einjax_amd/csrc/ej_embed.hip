@@ -105,6 +105,10 @@ __device__ inline void wave_sync() {
 // those of a 64 with the same digit know each other by ballots of its bits.  16384
 // tokens of 50000 rows: 40 us with a gradient of 64 columns, where the sort counts
 // alone, 59 with one of 4096 (410 MB, whose clearing alone takes 58); 2000 tokens 10.
+// 16384 tokens, a power of two, take 112 of the CU's 160 KB.  The whole gradient (us),
+// 50000 rows of bf16: 4096 columns 150 and, by the radix sort, 157 for one token more;
+// 64 columns, where nothing hides the sort, 50 and 32 (8192 tokens 33, 2000 18): so
+// narrow tables lose here from some 8000 tokens on.
 constexpr int kSortWaves = 16, kSortThreads = kSortWaves * 64;
 constexpr int kSortBits = 8, kSortDigits = 1 << kSortBits;
 constexpr int kSortTokens = 16384, kSortRows = kSortTokens / kSortThreads;
@@ -374,6 +378,9 @@ __global__ __launch_bounds__(kThreads) void join_chunks_kernel(Sums s, T *out) {
 // Tokens of a chunk: 8 to 32, as many as leave the chunks some 64 K threads (16384
 // tokens in 16 columns of bf16: 25 us in chunks of 32, 15 in 16), and more where
 // there would be above 2048 chunks, whose parts one thread may have to add up.
+// Many tokens of a narrow table then have few threads, 2048 for each 16 bytes of
+// its rows: the gradient of 131072 tokens in 64 columns of bf16 takes 60 us, of
+// 2^21 tokens 324 (their bytes 55).
 int32_t chunk_of(int64_t n_tokens, int64_t n) {
   int64_t c = 8;
   while (c < 32 && n_tokens * ceil_div(n, 8) > c * 65536) c *= 2;
