@@ -258,7 +258,17 @@ int pick_wgrad(const GroupedArgs &g, bool direct, hipStream_t stream) {
 //       512       16   2048 x 2048           115/147  102/101     86/86    75/77
 //      8192        1   4096 x 8192           869/1137 720/748    522/530  391/388
 // [k][n] in 64 columns takes half a line of each projection, so with many tiles 128
-// are better from the first row on.
+// are better from the first row on.  fp32 (128 x 128 as the pipelined loop):
+//        16       16   2048 x 4096   105/135  156/160
+//        24       16   2048 x 4096   130/176  156/161
+//        32       16   2048 x 4096   134/181  159/160
+//        64       16   1024 x 2048             46/45     42/42      70/73
+//       100        8   1024 x 2048             40/42     38/40      67/72
+//       512        8   1024 x 4096            278/278   262/270   255/262
+//      8192        1   2048 x 4096           1065/1065 1011/1028  979/1006
+// The choice, skinny up to 24 rows and 64 x 64 above, is within 9% of the best but at
+// 32 rows of [n][k]: the matrix instructions bound all tiles (8192 rows: 129
+// TFLOP/s in 64 x 64, 140 in 128 x 128).
 template <class Op, bool BKC>
 int pick_gated(const GroupedRows &r, hipStream_t stream) {
   const GroupedArgs &g = r.g;
