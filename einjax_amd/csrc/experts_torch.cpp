@@ -53,10 +53,14 @@ std::string str(c10::IntArrayRef s) {
   return r + ")";
 }
 
+// What a view of the negatives (the imaginary part of a conjugate) stands for; any
+// other tensor as it is.
+Tensor as_values(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 Tensor on_gpu(py::handle h, const char *what) {
   if (!THPVariable_Check(h.ptr()) || !THPVariable_Unpack(h.ptr()).is_cuda())
     throw py::type_error(std::string(what) + " must be a torch tensor on the GPU");
-  return THPVariable_Unpack(h.ptr());
+  return as_values(THPVariable_Unpack(h.ptr()));
 }
 
 Tensor on_gpu_of(const Tensor &ref, py::handle h, const char *what) {
@@ -109,8 +113,9 @@ Tensor index(Tensor t, c10::IntArrayRef shape, const char *what) {
 }
 
 // t [n, m] with unit stride along its rows and rows that do not overlap
-// (itself if it is so already).
-Tensor rows_of(const Tensor &t) {
+// (itself if it is so already).  Cotangents from autograd come here as they are.
+Tensor rows_of(const Tensor &given) {
+  const Tensor t = as_values(given);
   if (t.is_contiguous()) return t;
   const int64_t n = t.size(0), m = t.size(1);
   if ((m <= 1 || t.stride(1) == 1) && (n <= 1 || t.stride(0) >= m)) return t;
@@ -225,7 +230,7 @@ Tensor run_route_vjp(const Tensor &given, const Tensor &experts, const Tensor &g
   no_tangents(given, grad);
   const Tensor logits = rows_of(given);
   const int64_t T = logits.size(0), E = logits.size(1), k = experts.size(1);
-  const Tensor g = grad.to(at::kFloat).contiguous();
+  const Tensor g = as_values(grad.to(at::kFloat).contiguous());
   Launch on(logits);
   Tensor out = at::empty({T, E}, logits.options());
   check(ej_expert_route_vjp(ptr(logits), code, T, int32_of(E, "experts"),
