@@ -123,7 +123,8 @@ def quantize_blocks(x, *, block_rows: int = 1) -> tuple:
     [..., m, n] has one for every 128 x 128 block of a matrix, scale
     [..., ceil(m / 128), ceil(n / 128)].  Blocks at the ends may be smaller.
 
-    scale = max |block| / 448, q = x / scale rounded to nearest (ties to even).
+    scale = max |block| times float32's 1 / 448, q = x / scale rounded to nearest
+    (ties to even).
     A block of zeros has scale 0; a block that holds a NaN or an infinity has
     scale NaN, so that every product with it is NaN.
     Not differentiable: q and scale are constants to torch.autograd."""
